@@ -98,6 +98,26 @@ typedef struct vmlm_sparse_conn_w {
     float *act;
 } vmlm_sparse_conn_w;
 
+/* A KV cache held in 4 bits (no reference counterpart). Each 32 channels of a
+ * position's head share a bf16 scale and a bf16 minimum; a value stands for
+ * min + scale * u, u = rint((x - min) / scale) in 0 .. 15, where min is the lowest
+ * of the 32 rounded down and scale (highest - min) / 15 rounded up (ties of u
+ * to even; difference and quotients in f32): off by at most scale / 2. 32 values
+ * among which one is a NaN or an infinity, or whose range leaves f32, read as NaN.
+ *   k       [batch][n_kv_heads][cap][head_dim / 2], channels 2i (low nibble) and
+ *           2i + 1 in byte i
+ *   v       [batch][n_kv_heads][cap / 32][head_dim][16], positions 2i and 2i + 1
+ *           of a 32-position block in byte i
+ *   k_meta, v_meta  [batch][n_kv_heads][cap][head_dim / 32], the scale's bf16 bits
+ *           in the low half, the minimum's in the high half
+ * A nibble is u ^ 8. head_dim is 32, 64, 128 or 256, cap a multiple of 32; k and v
+ * are 16-byte aligned. Positions that nothing was appended to may hold anything. */
+typedef struct vmlm_kv4_cache {
+    uint8_t *k, *v;
+    uint32_t *k_meta, *v_meta;
+    size_t batch, n_kv_heads, cap, head_dim;
+} vmlm_kv4_cache;
+
 /* ================================================================ layer 1
  * Host pointers, synchronous. Each replaces the vmlm-ops function cited. */
 
@@ -213,6 +233,22 @@ int vmlm_attention_decode_split(const float *q, const float *k_new, const float 
                                 size_t head_dim, size_t cap, size_t pos, float theta,
                                 float scale, int split);
 
+/* The 4-bit operators over host arrays (no reference counterparts; the contracts
+ * are at their device forms below). Rows are contiguous: ldq = n_heads * head_dim
+ * and so on; the cache's four arrays are copied in and, where they change, back. */
+int vmlm_gemm_nt_int4(const float *a, const uint8_t *q, const float *scale, float *c, size_t m,
+                      size_t n, size_t k, size_t group);
+int vmlm_qk_norm_rope(float *q_out, float *k_out, const float *q, const float *k, const float *gq,
+                      const float *gk, const int32_t *pos, size_t rows, size_t n_heads,
+                      size_t n_kv_heads, size_t head_dim, float eps, float theta);
+int vmlm_kv4_append(const vmlm_kv4_cache *cache, const float *k, const float *v,
+                    const int32_t *pos0, const int32_t *count, size_t S);
+int vmlm_kv4_read(const vmlm_kv4_cache *cache, float *k, float *v, const int32_t *pos0,
+                  const int32_t *count, size_t S);
+int vmlm_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, const float *k_new,
+                              const float *v_new, const int32_t *pos, float *out, size_t n_heads,
+                              float scale);
+
 /* ================================================================ layer 2
  * Device pointers, asynchronous on `stream`. Same semantics as layer 1.
  * The result of the f32, int8 and bf16 weight GEMMs may lie over their operands (C
@@ -286,6 +322,60 @@ int vmlm_hip_attention_decode_split(const float *q, const float *k_new, const fl
                                     float *kcache, float *vcache, float *out, size_t n_heads,
                                     size_t head_dim, size_t cap, size_t pos, float theta,
                                     float scale, int split, void *stream);
+
+/* ---- a decode layer in 4 bits (no reference counterparts). These five launch
+ * kernels only, so they can be captured, and they refuse (9) overlapping operands
+ * that a kernel would read after writing them. The library's GPU must be the
+ * calling thread's current device. */
+
+/* C[m][j] = sum over groups g of scale[j][g] * (A[m] . Q[j] over the group):
+ * q [n][k / 2] signed 4-bit weights, byte i of a row holding k = 2i (low nibble) and
+ * 2i + 1 in two's complement, any alignment; scale [n][ceil(k / group)]. k is a
+ * multiple of 32, group 32, 64 or a multiple of 128 (the last group may be short).
+ * The rows of A are split exactly into int8 terms, 24 bits below the largest of
+ * 128 neighbours, and the products summed in integers within a group, so results
+ * are as near as f32 sums are; rows with a NaN or an infinity are summed in f32. */
+int vmlm_hip_gemm_nt_int4(const float *a, const uint8_t *q, const float *scale, float *c,
+                          size_t m, size_t n, size_t k, size_t group, void *stream);
+/* RMSNorm of each head of q [rows][ldq] (n_heads heads) and k [rows][ldk]
+ * (n_kv_heads heads) with the gains gq, gk [head_dim], then the pairs (i, i +
+ * head_dim / 2) rotated by pos[row] * theta^(-2i / head_dim), the angle formed in 64 bits
+ * (vmlm_hip_rope keeps the reference's 32-bit steps). pos null: the norm
+ * alone; rows with pos < 0 are left as they are. Outputs have strides of their own
+ * and may be the inputs (same address and stride). Either side may be absent (0
+ * heads). head_dim is a multiple of 8 up to 512. */
+int vmlm_hip_qk_norm_rope(float *q_out, size_t ldqo, float *k_out, size_t ldko, const float *q,
+                          size_t ldq, const float *k, size_t ldk, const float *gq,
+                          const float *gk, const int32_t *pos, size_t rows, size_t n_heads,
+                          size_t n_kv_heads, size_t head_dim, float eps, float theta,
+                          void *stream);
+/* Stores rows k [batch][S][ldk] and v [batch][S][ldv] (n_kv_heads * head_dim values
+ * each): row (b, t) at position pos0[b] + t, for t < count[b] (count null: all S). Sequences
+ * with pos0 < 0 are idle. Rows from cap on are dropped and reported by the
+ * next vmlm_hip_check_guards() as status 9. */
+int vmlm_hip_kv4_append(const vmlm_kv4_cache *cache, const float *k, size_t ldk, const float *v,
+                        size_t ldv, const int32_t *pos0, const int32_t *count, size_t S,
+                        void *stream);
+/* The other way: the same rows as the f32 values that the cache holds. Rows of idle
+ * sequences, from count[b] on and from cap on are left as they are. */
+int vmlm_hip_kv4_read(const vmlm_kv4_cache *cache, float *k, size_t ldk, float *v, size_t ldv,
+                      const int32_t *pos0, const int32_t *count, size_t S, void *stream);
+/* One token a sequence: k_new, v_new [batch][ldkv] (both null: nothing) are stored
+ * at pos[b] as kv4_append stores them, then each head of q [batch][ldq] attends
+ * positions 0 .. pos[b] of the cache of its group (head h reads kv head h / (n_heads /
+ * n_kv_heads)): out [batch][ldo]. q and k_new come rotated (vmlm_hip_qk_norm_rope).
+ * Sequences with pos < 0 are idle: their cache and output row stay as they are; pos >=
+ * cap trips the device guard and is treated so. A query head with a NaN or an
+ * infinity gives NaN. n_heads is a multiple of n_kv_heads, up to 16 times it.
+ * `work`: vmlm_hip_attention_decode_kv4_work() bytes, 16-byte aligned, used by one
+ * call at a time; null: the stream's own workspace, which a call under stream capture may
+ * not use (9), since graphs that run at once would share it. */
+int vmlm_hip_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, size_t ldq,
+                                  const float *k_new, const float *v_new, size_t ldkv,
+                                  const int32_t *pos, float *out, size_t ldo, size_t n_heads,
+                                  float scale, void *work, size_t work_bytes, void *stream);
+int vmlm_hip_attention_decode_kv4_work(const vmlm_kv4_cache *cache, size_t n_heads,
+                                       size_t *bytes);
 
 /* ================================================================ layer 3 */
 

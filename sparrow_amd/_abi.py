@@ -31,6 +31,12 @@ class Backend(C.Structure):
                 ("scale_mul", C.CFUNCTYPE(None, P, P, F, SZ))]
 
 
+class Kv4Cache(C.Structure):
+    """The 4-bit KV cache, vmlm_kv4_cache."""
+    _fields_ = [("k", P), ("v", P), ("k_meta", P), ("v_meta", P), ("batch", SZ),
+                ("n_kv_heads", SZ), ("cap", SZ), ("head_dim", SZ)]
+
+
 class DecoderCfg(C.Structure):
     _fields_ = [("n_layers", U32), ("hidden", U32), ("n_heads", U32), ("head_dim", U32),
                 ("inter", U32), ("vocab", U32), ("batch", U32), ("cap", U32),
@@ -94,6 +100,11 @@ SIGNATURES = {
     "vmlm_attention_prefill": (I, [P, P, P, P, SZ, SZ, SZ, F, U16, F, B]),
     "vmlm_attention_decode": (I, [P, P, P, P, P, P, SZ, SZ, SZ, SZ, F, F]),
     "vmlm_attention_decode_split": (I, [P, P, P, P, P, P, SZ, SZ, SZ, SZ, F, F, I]),
+    "vmlm_gemm_nt_int4": (I, [P, P, P, P, SZ, SZ, SZ, SZ]),
+    "vmlm_qk_norm_rope": (I, [P, P, P, P, P, P, P, SZ, SZ, SZ, SZ, F, F]),
+    "vmlm_kv4_append": (I, [C.POINTER(Kv4Cache), P, P, P, P, SZ]),
+    "vmlm_kv4_read": (I, [C.POINTER(Kv4Cache), P, P, P, P, SZ]),
+    "vmlm_attention_decode_kv4": (I, [C.POINTER(Kv4Cache), P, P, P, P, P, SZ, F]),
     # layer 2
     "vmlm_hip_gemm_nt_int8": (I, [P, P, P, P, SZ, SZ, SZ, P]),
     "vmlm_hip_gemm_nt_int8_noalloc": (I, [P, P, P, P, SZ, SZ, SZ, P]),
@@ -122,6 +133,13 @@ SIGNATURES = {
     "vmlm_hip_attention_prefill": (I, [P, P, P, P, SZ, SZ, SZ, F, U16, F, B, P]),
     "vmlm_hip_attention_decode": (I, [P, P, P, P, P, P, SZ, SZ, SZ, SZ, F, F, P]),
     "vmlm_hip_attention_decode_split": (I, [P, P, P, P, P, P, SZ, SZ, SZ, SZ, F, F, I, P]),
+    "vmlm_hip_gemm_nt_int4": (I, [P, P, P, P, SZ, SZ, SZ, SZ, P]),
+    "vmlm_hip_qk_norm_rope": (I, [P, SZ, P, SZ, P, SZ, P, SZ, P, P, P, SZ, SZ, SZ, SZ, F, F, P]),
+    "vmlm_hip_kv4_append": (I, [C.POINTER(Kv4Cache), P, SZ, P, SZ, P, P, SZ, P]),
+    "vmlm_hip_kv4_read": (I, [C.POINTER(Kv4Cache), P, SZ, P, SZ, P, P, SZ, P]),
+    "vmlm_hip_attention_decode_kv4": (I, [C.POINTER(Kv4Cache), P, SZ, P, P, SZ, P, P, SZ, SZ, F,
+                                          P, SZ, P]),
+    "vmlm_hip_attention_decode_kv4_work": (I, [C.POINTER(Kv4Cache), SZ, C.POINTER(SZ)]),
     # layer 3
     "vmlm_decoder_create": (I, [C.POINTER(DecoderCfg), C.POINTER(P)]),
     "vmlm_decoder_destroy": (I, [P]),

@@ -5,6 +5,7 @@
 // synchronises (serialised by a mutex). Layer 2 (vmlm_hip_*): device pointers,
 // asynchronous. Both validate like the reference interpreter's guards and
 // return its exit codes instead of exiting.
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <cstring>
@@ -67,6 +68,7 @@ static void setup_scratch(int device) {
 static std::once_flag g_once;
 static int g_init_status = -1;
 static std::atomic<bool> g_ready{false};
+static int g_device = 0;
 static hipStream_t g_stream = nullptr;
 static int *g_guard = nullptr;
 static std::mutex g_host_mutex;
@@ -105,6 +107,7 @@ static void do_init(int device) {
         return;
     }
     setup_scratch(device);
+    g_device = device;
     g_init_status = VMLM_OK;
     g_ready.store(true, std::memory_order_release);
 }
@@ -1008,6 +1011,263 @@ int vmlm_hip_attention_decode_split(const float *q, const float *k_new, const fl
     return launch_attention_decode(a, 1, out, (int)(n_heads * head_dim), nullptr, 0, 0, st, work);
 }
 
+// ---------------------------------------------------------------- 4-bit operators
+// Arguments are checked before the library is initialised: a call that is refused is
+// refused without a GPU too. Kernels go to the calling thread's current device: refused on another than the
+// library's, whose memory and streams they would be given.
+static int on_library_device() {
+    int d = -1;
+    VMLM_HIP_CHECK(hipGetDevice(&d));
+    VMLM_GUARD(d == g_device, "the current device is %d, the library's is %d", d, g_device);
+    return VMLM_OK;
+}
+
+constexpr size_t DIM_MAX = (size_t)1 << 30;  // of one dimension: int arithmetic with room
+
+// Whether rows of wp floats at p and of wq at q, at strides ldp and ldq, share a float.
+static bool rows_overlap(const float *p, size_t ldp, size_t wp, const float *q, size_t ldq,
+                         size_t wq, size_t rows) {
+    if (rows == 0 || wp == 0 || wq == 0) return false;
+    if (!overlap(p, ((rows - 1) * ldp + wp) * 4, q, ((rows - 1) * ldq + wq) * 4)) return false;
+    if (rows == 1 || ldp != ldq) return true;
+    // columns of one matrix, as the parts of a fused q / k / v row
+    const uintptr_t d = (uintptr_t)q - (uintptr_t)p, ld = ldp * 4;
+    const uintptr_t off = (uintptr_t)q >= (uintptr_t)p ? d % ld : (ld - (0 - d) % ld) % ld;
+    return off < wp * 4 || off + wq * 4 > ld;
+}
+
+// The descriptor (host arrays: of any alignment).
+static int check_kv4(const vmlm_kv4_cache *c, Kv4View *v, bool device = true) {
+    VMLM_GUARD(c != nullptr, "kv4: null cache");
+    VMLM_GUARD(c->head_dim == 32 || c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256,
+               "kv4: head_dim %zu unsupported (32, 64, 128, 256)", c->head_dim);
+    VMLM_GUARD(c->cap % 32 == 0 && c->cap <= DIM_MAX, "kv4: cap %zu is no multiple of 32 (or over 2^30)",
+               c->cap);
+    VMLM_GUARD(c->batch <= 65535 && c->n_kv_heads <= 65535, "kv4: batch %zu or n_kv_heads %zu over 65535",
+               c->batch, c->n_kv_heads);
+    v->k = c->k;
+    v->v = c->v;
+    v->km = c->k_meta;
+    v->vm = c->v_meta;
+    v->B = (int)c->batch;
+    v->Hkv = (int)c->n_kv_heads;
+    v->cap = (int)c->cap;
+    v->hd = (int)c->head_dim;
+    if (v->B == 0 || v->Hkv == 0 || v->cap == 0) return VMLM_OK;
+    VMLM_GUARD(v->k && v->v && v->km && v->vm, "kv4: null cache array");
+    VMLM_GUARD(!device || ((((uintptr_t)v->k | (uintptr_t)v->v) & 15) == 0 &&
+                           (((uintptr_t)v->km | (uintptr_t)v->vm) & 3) == 0),
+               "kv4: k and v must be 16-byte aligned, k_meta and v_meta 4-byte");
+    return VMLM_OK;
+}
+
+static int check_int4(const float *a, const uint8_t *q, const float *scale, const float *c,
+                      size_t m, size_t n, size_t k, size_t group) {
+    VMLM_GUARD(k % 32 == 0, "int4 gemm: k=%zu is no multiple of 32", k);
+    VMLM_GUARD(group == 32 || group == 64 || (group > 0 && group % 128 == 0),
+               "int4 gemm: group=%zu is not 32, 64 or a multiple of 128", group);
+    VMLM_GUARD(m <= DIM_MAX && n <= DIM_MAX && k <= (size_t)1 << 24,
+               "int4 gemm: m=%zu n=%zu k=%zu (limits 2^30, 2^30, 2^24)", m, n, k);
+    if (m == 0 || n == 0) return VMLM_OK;
+    VMLM_GUARD(c, "int4 gemm: null result");
+    VMLM_GUARD(k == 0 || (a && q && scale), "int4 gemm: null operand");
+    return VMLM_OK;
+}
+
+int vmlm_hip_gemm_nt_int4(const float *a, const uint8_t *q, const float *scale, float *c,
+                          size_t m, size_t n, size_t k, size_t group, void *stream) {
+    int rc = check_int4(a, q, scale, c, m, n, k, group);
+    if (rc || m == 0 || n == 0) return rc;
+    const size_t cb = m * n * 4;
+    VMLM_GUARD(k == 0 || (!overlap(c, cb, a, m * k * 4) && !overlap(c, cb, q, n * (k / 2)) &&
+                          !overlap(c, cb, scale, n * cdiv(k, group) * 4)),
+               "int4 gemm: the result lies over an operand");
+    INIT_OR_RETURN();
+    if ((rc = on_library_device())) return rc;
+    hipStream_t st = as_stream(stream);
+    if (k == 0) return launch_fill_zero(c, cb, st);
+    Int4Args x;
+    x.A = a;
+    x.Q = q;
+    x.scale = scale;
+    x.C = c;
+    x.M = (int)m;
+    x.N = (int)n;
+    x.K = (int)k;
+    // groups beyond the row are one group of it
+    x.G = (int)std::min(group, (k + 127) / 128 * 128);
+    return launch_gemm_int4(x, st);
+}
+
+static int check_headnorm(const HeadNormArgs &a, size_t rows, size_t H, size_t Hkv, size_t hd) {
+    VMLM_GUARD(hd >= 8 && hd % 8 == 0 && hd <= HEADNORM_MAX_HD,
+               "qk_norm_rope: head_dim %zu is no multiple of 8 up to %d", hd, HEADNORM_MAX_HD);
+    VMLM_GUARD(a.theta > 0.0f && a.theta < __builtin_inff(), "ROPE: theta must be > 0");
+    VMLM_GUARD(a.eps >= 0.0f && a.eps < __builtin_inff(), "qk_norm_rope: eps must be >= 0");
+    VMLM_GUARD(rows <= DIM_MAX && H <= 65535 && Hkv <= 65535,
+               "qk_norm_rope: rows %zu over 2^30, or n_heads %zu, n_kv_heads %zu over 65535", rows, H,
+               Hkv);
+    if (rows == 0) return VMLM_OK;
+    const size_t wq = H * hd, wk = Hkv * hd;
+    VMLM_GUARD(H == 0 || (a.q && a.qo && a.gq), "qk_norm_rope: null query rows or gain");
+    VMLM_GUARD(Hkv == 0 || (a.k && a.ko && a.gk), "qk_norm_rope: null key rows or gain");
+    VMLM_GUARD(rows == 1 || ((H == 0 || (a.ldq >= wq && a.ldqo >= wq)) &&
+                             (Hkv == 0 || (a.ldk >= wk && a.ldko >= wk))),
+               "qk_norm_rope: a row stride is below the row's width");
+    const bool same_q = a.qo == a.q && a.ldqo == a.ldq, same_k = a.ko == a.k && a.ldko == a.ldk;
+    VMLM_GUARD((same_q || !rows_overlap(a.qo, a.ldqo, wq, a.q, a.ldq, wq, rows)) &&
+                   (same_k || !rows_overlap(a.ko, a.ldko, wk, a.k, a.ldk, wk, rows)) &&
+                   !rows_overlap(a.qo, a.ldqo, wq, a.k, a.ldk, wk, rows) &&
+                   !rows_overlap(a.ko, a.ldko, wk, a.q, a.ldq, wq, rows) &&
+                   !rows_overlap(a.qo, a.ldqo, wq, a.ko, a.ldko, wk, rows),
+               "qk_norm_rope: an output lies over another operand (only its own input may be it)");
+    for (const float *g : {a.gq, a.gk})
+        VMLM_GUARD(!rows_overlap(g, hd, hd, a.qo, (rows - 1) * a.ldqo + wq,
+                                 H ? (rows - 1) * a.ldqo + wq : 0, 1) &&
+                       !rows_overlap(g, hd, hd, a.ko, (rows - 1) * a.ldko + wk,
+                                     Hkv ? (rows - 1) * a.ldko + wk : 0, 1),
+                   "qk_norm_rope: an output lies over a gain");
+    return VMLM_OK;
+}
+
+int vmlm_hip_qk_norm_rope(float *q_out, size_t ldqo, float *k_out, size_t ldko, const float *q,
+                          size_t ldq, const float *k, size_t ldk, const float *gq,
+                          const float *gk, const int32_t *pos, size_t rows, size_t n_heads,
+                          size_t n_kv_heads, size_t head_dim, float eps, float theta,
+                          void *stream) {
+    HeadNormArgs a;
+    a.q = q;
+    a.k = k;
+    a.gq = gq;
+    a.gk = gk;
+    a.qo = q_out;
+    a.ko = k_out;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldqo = ldqo;
+    a.ldko = ldko;
+    a.pos = pos;
+    a.eps = eps;
+    a.theta = theta;
+    int rc = check_headnorm(a, rows, n_heads, n_kv_heads, head_dim);
+    if (rc || rows == 0 || n_heads + n_kv_heads == 0) return rc;
+    INIT_OR_RETURN();
+    if ((rc = on_library_device())) return rc;
+    a.rows = (int)rows;
+    a.H = (int)n_heads;
+    a.Hkv = (int)n_kv_heads;
+    a.hd = (int)head_dim;
+    return launch_headnorm(a, as_stream(stream));
+}
+
+// Rows [B][S] of the cache's width beside it.
+static int check_kv4_rows(const Kv4View &c, const float *k, size_t ldk, const float *v, size_t ldv,
+                          const int32_t *pos0, size_t S) {
+    VMLM_GUARD(S <= DIM_MAX, "kv4: %zu rows a sequence (limit 2^30)", S);
+    if (c.B == 0 || c.Hkv == 0 || S == 0) return VMLM_OK;
+    VMLM_GUARD(c.cap > 0, "kv4: capacity 0");
+    VMLM_GUARD(k && v && pos0, "kv4: null rows or positions");
+    const size_t w = (size_t)c.Hkv * c.hd;
+    VMLM_GUARD((size_t)c.B * S == 1 || (ldk >= w && ldv >= w),
+               "kv4: row strides %zu, %zu are below the row's width %zu", ldk, ldv, w);
+    return VMLM_OK;
+}
+
+int vmlm_hip_kv4_append(const vmlm_kv4_cache *cache, const float *k, size_t ldk, const float *v,
+                        size_t ldv, const int32_t *pos0, const int32_t *count, size_t S,
+                        void *stream) {
+    Kv4View c;
+    int rc = check_kv4(cache, &c);
+    if (!rc) rc = check_kv4_rows(c, k, ldk, v, ldv, pos0, S);
+    if (rc || c.B == 0 || c.Hkv == 0 || S == 0) return rc;
+    INIT_OR_RETURN();
+    if ((rc = on_library_device())) return rc;
+    return launch_kv4_append(c, k, ldk, v, ldv, pos0, count, (int)S, as_stream(stream));
+}
+
+int vmlm_hip_kv4_read(const vmlm_kv4_cache *cache, float *k, size_t ldk, float *v, size_t ldv,
+                      const int32_t *pos0, const int32_t *count, size_t S, void *stream) {
+    Kv4View c;
+    int rc = check_kv4(cache, &c);
+    if (!rc) rc = check_kv4_rows(c, k, ldk, v, ldv, pos0, S);
+    if (rc || c.B == 0 || c.Hkv == 0 || S == 0) return rc;
+    const size_t w = (size_t)c.Hkv * c.hd;
+    VMLM_GUARD(!rows_overlap(k, ldk, w, v, ldv, w, (size_t)c.B * S),
+               "kv4_read: k and v lie over each other");
+    INIT_OR_RETURN();
+    if ((rc = on_library_device())) return rc;
+    return launch_kv4_read(c, k, ldk, v, ldv, pos0, count, (int)S, as_stream(stream));
+}
+
+static int check_attn4(const vmlm_kv4_cache *cache, const Kv4View &c, size_t n_heads) {
+    VMLM_GUARD(c.Hkv > 0 && n_heads % c.Hkv == 0 && n_heads / c.Hkv <= 16,
+               "kv4 attention: %zu heads over %d kv heads (a multiple, up to 16 times)", n_heads,
+               c.Hkv);
+    return VMLM_OK;
+}
+
+int vmlm_hip_attention_decode_kv4_work(const vmlm_kv4_cache *cache, size_t n_heads,
+                                       size_t *bytes) {
+    VMLM_GUARD(bytes, "kv4 attention: null size");
+    Kv4View c;
+    int rc = check_kv4(cache, &c);
+    if (!rc) rc = check_attn4(cache, c, n_heads);
+    if (!rc) *bytes = attn4_work_floats(c, (int)n_heads) * 4;
+    return rc;
+}
+
+int vmlm_hip_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, size_t ldq,
+                                  const float *k_new, const float *v_new, size_t ldkv,
+                                  const int32_t *pos, float *out, size_t ldo, size_t n_heads,
+                                  float scale, void *work, size_t work_bytes, void *stream) {
+    Attn4Args a;
+    int rc = check_kv4(cache, &a.c);
+    if (!rc) rc = check_attn4(cache, a.c, n_heads);
+    if (rc || a.c.B == 0 || n_heads == 0) return rc;
+    const size_t B = a.c.B, w = n_heads * a.c.hd, wk = (size_t)a.c.Hkv * a.c.hd;
+    VMLM_GUARD(a.c.cap > 0, "kv4 attention: capacity 0");
+    VMLM_GUARD(q && pos && out, "kv4 attention: null queries, positions or output");
+    VMLM_GUARD((k_new == nullptr) == (v_new == nullptr),
+               "kv4 attention: k_new and v_new are given together or not at all");
+    VMLM_GUARD(B == 1 || (ldq >= w && ldo >= w && (!k_new || ldkv >= wk)),
+               "kv4 attention: a row stride is below the row's width");
+    VMLM_GUARD(scale - scale == 0.0f, "kv4 attention: the score scale is not finite");
+    VMLM_GUARD(!rows_overlap(out, ldo, w, q, ldq, w, B) &&
+                   (!k_new || (!rows_overlap(out, ldo, w, k_new, ldkv, wk, B) &&
+                               !rows_overlap(out, ldo, w, v_new, ldkv, wk, B))),
+               "kv4 attention: the output lies over its input");
+    INIT_OR_RETURN();
+    if ((rc = on_library_device())) return rc;
+    hipStream_t st = as_stream(stream);
+    a.q = q;
+    a.ldq = ldq;
+    a.k_new = k_new;
+    a.v_new = v_new;
+    a.ldkv = ldkv;
+    a.pos = pos;
+    a.out = out;
+    a.ldo = ldo;
+    a.H = (int)n_heads;
+    a.scale = scale;
+    const size_t wf = attn4_work_floats(a.c, a.H);
+    if (wf == 0) return launch_attn4(a, st);
+    if (work) {
+        VMLM_GUARD(work_bytes >= wf * 4 && ((uintptr_t)work & 15) == 0,
+                   "kv4 attention: workspace of %zu bytes, %zu needed (16-byte aligned)",
+                   work_bytes, wf * 4);
+        a.work = (float *)work;
+        return launch_attn4(a, st);
+    }
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    VMLM_HIP_CHECK(hipStreamIsCapturing(st, &cs));
+    VMLM_GUARD(cs == hipStreamCaptureStatusNone,
+               "kv4 attention: a captured call needs a workspace of its own (%zu bytes)", wf * 4);
+    Stage stg(st);
+    a.work = stg.alloc<float>(wf);
+    STAGE_OK(stg);
+    return launch_attn4(a, st);
+}
+
 // ================================================================ layer 1
 int vmlm_gemm_nt_int8(const float *a, const int8_t *q, const float *scale, float *c, size_t m,
                       size_t n, size_t k) {
@@ -1421,6 +1681,155 @@ int vmlm_attention_decode_split(const float *q, const float *k_new, const float 
         if (!rc) rc = download(out, dout, w * sizeof(float), st);
         if (!rc) rc = download(kcache, dkc, cn * sizeof(float), st);
         if (!rc) rc = download(vcache, dvc, cn * sizeof(float), st);
+        if (rc) return rc;
+    }
+    FINISH(st);
+}
+
+// ---------------------------------------------------------------- 4-bit operators
+int vmlm_gemm_nt_int4(const float *a, const uint8_t *q, const float *scale, float *c, size_t m,
+                      size_t n, size_t k, size_t group) {
+    int rc = check_int4(a, q, scale, c, m, n, k, group);
+    if (rc || m == 0 || n == 0) return rc;
+    HOST_CALL_BEGIN();
+    {
+        Stage stg(st);
+        float *da = stg.upload(a, m * k), *dc = stg.alloc<float>(m * n);
+        uint8_t *dq = stg.upload(q, n * (k / 2));
+        float *ds = stg.upload(scale, n * cdiv(k, group));
+        STAGE_OK(stg);
+        rc = vmlm_hip_gemm_nt_int4(da, dq, ds, dc, m, n, k, group, st);
+        if (!rc) rc = download(c, dc, m * n * sizeof(float), st);
+        if (rc) return rc;
+    }
+    FINISH(st);
+}
+
+int vmlm_qk_norm_rope(float *q_out, float *k_out, const float *q, const float *k, const float *gq,
+                      const float *gk, const int32_t *pos, size_t rows, size_t n_heads,
+                      size_t n_kv_heads, size_t head_dim, float eps, float theta) {
+    HeadNormArgs h;
+    h.q = q;
+    h.k = k;
+    h.gq = gq;
+    h.gk = gk;
+    h.qo = q_out;
+    h.ko = k_out;
+    const size_t wq = n_heads * head_dim, wk = n_kv_heads * head_dim;
+    h.ldq = h.ldqo = wq;
+    h.ldk = h.ldko = wk;
+    h.eps = eps;
+    h.theta = theta;
+    int rc = check_headnorm(h, rows, n_heads, n_kv_heads, head_dim);
+    if (rc || rows == 0) return rc;
+    HOST_CALL_BEGIN();
+    {
+        Stage stg(st);
+        float *dq = stg.upload(q, rows * wq), *dk = stg.upload(k, rows * wk);
+        float *dgq = stg.upload(gq, n_heads ? head_dim : 0);
+        float *dgk = stg.upload(gk, n_kv_heads ? head_dim : 0);
+        int32_t *dp = pos ? stg.upload(pos, rows) : nullptr;
+        // idle rows come back as they are
+        float *dqo = q_out == q ? dq : stg.upload((const float *)q_out, rows * wq);
+        float *dko = k_out == k ? dk : stg.upload((const float *)k_out, rows * wk);
+        STAGE_OK(stg);
+        rc = vmlm_hip_qk_norm_rope(dqo, wq, dko, wk, dq, wq, dk, wk, dgq, dgk, dp, rows, n_heads,
+                                   n_kv_heads, head_dim, eps, theta, st);
+        if (!rc) rc = download(q_out, dqo, rows * wq * sizeof(float), st);
+        if (!rc) rc = download(k_out, dko, rows * wk * sizeof(float), st);
+        if (rc) return rc;
+    }
+    FINISH(st);
+}
+
+// A host cache's arrays on the device, and their bytes.
+struct Kv4Staged {
+    vmlm_kv4_cache d;
+    size_t code = 0, meta = 0;
+    Kv4Staged(Stage &stg, const vmlm_kv4_cache &h) : d(h) {
+        const size_t vals = h.batch * h.n_kv_heads * h.cap * h.head_dim;
+        code = vals / 2;
+        meta = vals / 32;
+        d.k = stg.upload((const uint8_t *)h.k, code);
+        d.v = stg.upload((const uint8_t *)h.v, code);
+        d.k_meta = stg.upload((const uint32_t *)h.k_meta, meta);
+        d.v_meta = stg.upload((const uint32_t *)h.v_meta, meta);
+    }
+    int back(const vmlm_kv4_cache &h, hipStream_t st) const {
+        int rc = download(h.k, d.k, code, st);
+        if (!rc) rc = download(h.v, d.v, code, st);
+        if (!rc) rc = download(h.k_meta, d.k_meta, meta * 4, st);
+        return rc ? rc : download(h.v_meta, d.v_meta, meta * 4, st);
+    }
+};
+
+int vmlm_kv4_append(const vmlm_kv4_cache *cache, const float *k, const float *v,
+                    const int32_t *pos0, const int32_t *count, size_t S) {
+    Kv4View c;
+    int rc = check_kv4(cache, &c, false);
+    const size_t w = rc ? 0 : (size_t)c.Hkv * c.hd, rows = rc ? 0 : c.B * S;
+    if (!rc) rc = check_kv4_rows(c, k, w, v, w, pos0, S);
+    if (rc || rows == 0 || w == 0) return rc;
+    HOST_CALL_BEGIN();
+    {
+        Stage stg(st);
+        Kv4Staged dc(stg, *cache);
+        float *dk = stg.upload(k, rows * w), *dv = stg.upload(v, rows * w);
+        int32_t *dp = stg.upload(pos0, c.B), *dn = count ? stg.upload(count, c.B) : nullptr;
+        STAGE_OK(stg);
+        rc = vmlm_hip_kv4_append(&dc.d, dk, w, dv, w, dp, dn, S, st);
+        if (!rc) rc = dc.back(*cache, st);
+        if (rc) return rc;
+    }
+    FINISH(st);
+}
+
+int vmlm_kv4_read(const vmlm_kv4_cache *cache, float *k, float *v, const int32_t *pos0,
+                  const int32_t *count, size_t S) {
+    Kv4View c;
+    int rc = check_kv4(cache, &c, false);
+    const size_t w = rc ? 0 : (size_t)c.Hkv * c.hd, rows = rc ? 0 : c.B * S;
+    if (!rc) rc = check_kv4_rows(c, k, w, v, w, pos0, S);
+    if (rc || rows == 0 || w == 0) return rc;
+    HOST_CALL_BEGIN();
+    {
+        Stage stg(st);
+        Kv4Staged dc(stg, *cache);
+        float *dk = stg.upload((const float *)k, rows * w), *dv = stg.upload((const float *)v, rows * w);
+        int32_t *dp = stg.upload(pos0, c.B), *dn = count ? stg.upload(count, c.B) : nullptr;
+        STAGE_OK(stg);
+        rc = vmlm_hip_kv4_read(&dc.d, dk, w, dv, w, dp, dn, S, st);
+        if (!rc) rc = download(k, dk, rows * w * sizeof(float), st);
+        if (!rc) rc = download(v, dv, rows * w * sizeof(float), st);
+        if (rc) return rc;
+    }
+    FINISH(st);
+}
+
+int vmlm_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, const float *k_new,
+                              const float *v_new, const int32_t *pos, float *out, size_t n_heads,
+                              float scale) {
+    Kv4View c;
+    int rc = check_kv4(cache, &c, false);
+    if (!rc) rc = check_attn4(cache, c, n_heads);
+    if (rc || c.B == 0 || n_heads == 0) return rc;
+    VMLM_GUARD(c.cap > 0 && q && pos && out && (k_new == nullptr) == (v_new == nullptr),
+               "kv4 attention: capacity 0, null queries, positions or output, or one of k_new and "
+               "v_new alone");
+    HOST_CALL_BEGIN();
+    {
+        const size_t B = c.B, w = n_heads * c.hd, wk = (size_t)c.Hkv * c.hd;
+        Stage stg(st);
+        Kv4Staged dc(stg, *cache);
+        float *dq = stg.upload(q, B * w), *dout = stg.upload((const float *)out, B * w);
+        float *dk = k_new ? stg.upload(k_new, B * wk) : nullptr;
+        float *dv = v_new ? stg.upload(v_new, B * wk) : nullptr;
+        int32_t *dp = stg.upload(pos, B);
+        STAGE_OK(stg);
+        rc = vmlm_hip_attention_decode_kv4(&dc.d, dq, w, dk, dv, wk, dp, dout, w, n_heads, scale,
+                                           nullptr, 0, st);
+        if (!rc) rc = download(out, dout, B * w * sizeof(float), st);
+        if (!rc && k_new) rc = dc.back(*cache, st);
         if (rc) return rc;
     }
     FINISH(st);

@@ -494,6 +494,62 @@ size_t attention_decode_work_floats(const DecodeArgs &a, int B);
 int launch_attention_decode(const DecodeArgs &a, int B, float *out, int ldo, uint16_t *terms,
                             int T, int ldt, hipStream_t st, float *work = nullptr);
 
+// GEMM over 4-bit weights with group scales (k_int4.hip): Q [N][K/2] two's
+// complement nibbles, k even in the low one; scale [N][ceil(K/G)]. K % 32 == 0, G 32,
+// 64 or a multiple of 128.
+struct Int4Args {
+    const float *A = nullptr;  // [M][K]
+    const uint8_t *Q = nullptr;
+    const float *scale = nullptr;
+    float *C = nullptr;  // [M][N]
+    int M = 0, N = 0, K = 0, G = 0;
+};
+int launch_gemm_int4(const Int4Args &a, hipStream_t st);
+
+// RMSNorm of each query and key head and the position rotation in one pass
+// (k_headnorm.hip). hd % 8 == 0, hd <= HEADNORM_MAX_HD; pos null: no rotation;
+// rows with pos < 0 are left as they are.
+constexpr int HEADNORM_MAX_HD = 512;
+struct HeadNormArgs {
+    const float *q = nullptr, *k = nullptr, *gq = nullptr, *gk = nullptr;
+    float *qo = nullptr, *ko = nullptr;
+    size_t ldq = 0, ldk = 0, ldqo = 0, ldko = 0;
+    const int32_t *pos = nullptr;
+    int rows = 0, H = 0, Hkv = 0, hd = 0;
+    float eps = 0.0f, theta = 0.0f;
+};
+int launch_headnorm(const HeadNormArgs &a, hipStream_t st);
+
+// The 4-bit KV cache (format: kv4.hpp). hd 32, 64, 128 or 256, cap % 32 == 0.
+constexpr int KV4_MAX_HD = 256;
+struct Kv4View {
+    uint8_t *k = nullptr, *v = nullptr;
+    uint32_t *km = nullptr, *vm = nullptr;
+    int B = 0, Hkv = 0, cap = 0, hd = 0;
+};
+// Row (b, t) of k / v [B][S][ld] is position pos0[b] + t, t < count[b] (null: all S);
+// sequences with pos0 < 0 and positions from cap on are left out (the latter trip
+// the device guard).
+int launch_kv4_append(const Kv4View &c, const float *k, size_t ldk, const float *v, size_t ldv,
+                      const int32_t *pos0, const int32_t *count, int S, hipStream_t st);
+int launch_kv4_read(const Kv4View &c, float *k, size_t ldk, float *v, size_t ldv,
+                    const int32_t *pos0, const int32_t *count, int S, hipStream_t st);
+// Decode attention over it (k_attn4.hip): k_new / v_new (or null) are stored at
+// pos[b], then q attends positions 0 .. pos[b]. `work`: attn4_work_floats() floats.
+struct Attn4Args {
+    Kv4View c;
+    const float *q = nullptr, *k_new = nullptr, *v_new = nullptr;
+    size_t ldq = 0, ldkv = 0;
+    const int32_t *pos = nullptr;
+    float *out = nullptr;
+    size_t ldo = 0;
+    int H = 0;
+    float scale = 0.0f;
+    float *work = nullptr;
+};
+size_t attn4_work_floats(const Kv4View &c, int H);
+int launch_attn4(const Attn4Args &a, hipStream_t st);
+
 // B1 gather forward over source-major activations.
 int launch_b1_forward(const float *w, const uint32_t *src, int n, int k0, const float *xt,
                       size_t t8, int n_tokens, float *yt, int mode, int act, hipStream_t st);

@@ -1,0 +1,67 @@
+// kv4.hpp -- the KV cache in 4 bits, as its kernels see it (vmlm_kv4_cache).
+//
+// 32 channels of one position's head share (min, scale), two bf16 in one dword
+// (scale in the low half): min is their lowest value rounded down, scale a
+// fifteenth of the way to their highest rounded up, so that the 16 steps reach
+// both. A value is held as u = rint((x - min) / scale) in 0..15 and stands for
+// min + scale * u; the nibble is u ^ 8, the two's complement of u - 8, which an
+// int8 matrix product reads with one mask. The difference and both quotients are
+// f32, correctly rounded. 5 bits a value.
+//
+// K codes lie by position ([hd/2] bytes: channels 2i and 2i + 1 in byte i): the
+// scores' products run over channels. V codes lie in blocks of 32 positions
+// ([hd][16] bytes: positions 2i and 2i + 1 of a channel): the output's run over
+// positions, and a lane's 16-byte load is 32 positions of one channel.
+#pragma once
+
+#include "internal.hpp"
+
+namespace vmlm {
+
+constexpr int KV4_BLOCK = 32;
+
+// The meta of 32 values with lowest lo and highest hi; NaN twice where one of
+// them is not finite (`bad`) or their range leaves f32.
+__device__ __forceinline__ uint32_t kv4_meta(float lo, float hi, bool bad) {
+    const uint32_t b = __float_as_uint(lo);
+    const uint32_t mn = ((b >> 31) ? b + 0xffffu : b) & 0xffff0000u;
+    const float q = (hi - __uint_as_float(mn)) / 15.0f;
+    const uint32_t sc = (__float_as_uint(q) + 0xffffu) & 0xffff0000u;
+    const bool ok = !bad && (mn & 0x7f800000u) != 0x7f800000u && (sc & 0x7f800000u) != 0x7f800000u;
+    return ok ? mn | (sc >> 16) : 0x7fc07fc0u;
+}
+__device__ __forceinline__ float kv4_scale(uint32_t meta) { return __uint_as_float(meta << 16); }
+__device__ __forceinline__ float kv4_min(uint32_t meta) {
+    return __uint_as_float(meta & 0xffff0000u);
+}
+// the nibble of x
+__device__ __forceinline__ uint32_t kv4_code(float x, float mn, float sc) {
+    const float u = sc > 0.0f ? fminf(fmaxf(rintf((x - mn) / sc), 0.0f), 15.0f) : 0.0f;
+    return (uint32_t)u ^ 8u;
+}
+// the value of a nibble (in the low four bits)
+__device__ __forceinline__ float kv4_value(uint32_t nib, float mn, float sc) {
+    return sc * (float)((nib & 15u) ^ 8u) + mn;
+}
+
+// Minimum, maximum and non-finite flag of 32 values held by 8 neighbouring
+// lanes, four each; the same in all eight.
+__device__ __forceinline__ uint32_t kv4_meta8(const float (&x)[4]) {
+    float lo = x[0], hi = x[0];
+    int bad = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        lo = fminf(lo, x[e]);
+        hi = fmaxf(hi, x[e]);
+        bad |= !(fabsf(x[e]) <= 3.40282347e38f);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o *= 2) {
+        lo = fminf(lo, __shfl_xor(lo, o, 64));
+        hi = fmaxf(hi, __shfl_xor(hi, o, 64));
+        bad |= __shfl_xor(bad, o, 64);
+    }
+    return kv4_meta(lo, hi, bad != 0);
+}
+
+}  // namespace vmlm

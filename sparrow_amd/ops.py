@@ -258,3 +258,105 @@ def attention_decode(q, k_new, v_new, kcache, vcache, pos, theta=10000.0, scale=
                                             _p(vcache), _p(out), H, hd, cap, int(pos),
                                             float(theta), float(scale), int(split)))
     return out
+
+
+# ---------------------------------------------------------------- 4-bit operators
+def quantize_int4(w, group=128):
+    """f32 weights [n, k] as the 4-bit rows and group scales that gemm_nt_int4
+    takes: scale = max|w| / 7 over a group, q = rint(w / scale) in -7 .. 7."""
+    w = _c(w, np.float32)
+    n, k = w.shape
+    ng = -(-k // group)
+    g = np.zeros((n, ng, group), np.float32)
+    g.reshape(n, -1)[:, :k] = w
+    s = np.abs(g).max(-1) / np.float32(7)
+    q = np.rint(g / np.where(s > 0, s, 1)[..., None]).astype(np.int8).reshape(n, -1)[:, :k]
+    u = (q & 15).astype(np.uint8)
+    return u[:, 0::2] | (u[:, 1::2] << 4), s
+
+
+def gemm_nt_int4(a, q, scale, group):
+    """C = A . W^T over 4-bit weights [n, k / 2] (two's complement nibbles, even k
+    low) with scales [n, ceil(k / group)]."""
+    a, q, s = _c(a, np.float32), _c(q, np.uint8), _c(scale, np.float32)
+    m, k = a.shape
+    n = q.shape[0]
+    assert q.shape[1] * 2 == k and group > 0 and s.shape == (n, -(-k // group))
+    c = np.empty((m, n), np.float32)
+    check(lib().vmlm_gemm_nt_int4(_p(a), _p(q), _p(s), _p(c), m, n, k, int(group)))
+    return c
+
+
+def qk_norm_rope(q, k, gq, gk, pos, head_dim, eps=1e-5, theta=10000.0):
+    """RMSNorm of every head of q [rows, H * head_dim] and k [rows, Hkv * head_dim],
+    rotated to `pos` [rows] (None: not rotated). Rows with pos < 0 give zeros."""
+    q, k = _c(q, np.float32), _c(k, np.float32)
+    gq, gk = _c(gq, np.float32), _c(gk, np.float32)
+    rows = q.shape[0]
+    assert k.shape[0] == rows and gq.size == head_dim and gk.size == head_dim
+    assert q.shape[1] % head_dim == 0 and k.shape[1] % head_dim == 0
+    pos = None if pos is None else _c(pos, np.int32)
+    assert pos is None or pos.size == rows
+    qo, ko = np.zeros_like(q), np.zeros_like(k)
+    check(lib().vmlm_qk_norm_rope(_p(qo), _p(ko), _p(q), _p(k), _p(gq), _p(gk),
+                                  None if pos is None else _p(pos), rows, q.shape[1] // head_dim,
+                                  k.shape[1] // head_dim, head_dim, float(eps), float(theta)))
+    return qo, ko
+
+
+class Kv4Cache:
+    """A KV cache in 4 bits over host arrays (vmlm_kv4_cache), empty."""
+
+    def __init__(self, batch, n_kv_heads, cap, head_dim):
+        self.batch, self.n_kv_heads, self.cap, self.head_dim = batch, n_kv_heads, cap, head_dim
+        bh = (batch, n_kv_heads)
+        self.k = np.zeros((*bh, cap, head_dim // 2), np.uint8)
+        self.v = np.zeros((*bh, cap // 32, head_dim, 16), np.uint8)
+        self.k_meta = np.zeros((*bh, cap, head_dim // 32), np.uint32)
+        self.v_meta = np.zeros((*bh, cap, head_dim // 32), np.uint32)
+
+    def descriptor(self):
+        return _abi.Kv4Cache(k=_p(self.k), v=_p(self.v), k_meta=_p(self.k_meta),
+                             v_meta=_p(self.v_meta), batch=self.batch,
+                             n_kv_heads=self.n_kv_heads, cap=self.cap, head_dim=self.head_dim)
+
+    def _rows(self, pos0, count):
+        pos0 = _c(pos0, np.int32)
+        count = None if count is None else _c(count, np.int32)
+        assert pos0.size == self.batch and (count is None or count.size == self.batch)
+        return pos0, count
+
+    def append(self, k, v, pos0, count=None):
+        """Rows [batch, S, n_kv_heads * head_dim] at positions pos0[b] + t, t < count[b]."""
+        k, v = _c(k, np.float32), _c(v, np.float32)
+        pos0, count = self._rows(pos0, count)
+        assert k.shape == v.shape == (self.batch, k.shape[1], self.n_kv_heads * self.head_dim)
+        check(lib().vmlm_kv4_append(self.descriptor(), _p(k), _p(v), _p(pos0),
+                                    None if count is None else _p(count), k.shape[1]))
+
+    def read(self, pos0, S, count=None):
+        """(k, v): the rows as the values the cache holds; zeros where there are none."""
+        pos0, count = self._rows(pos0, count)
+        k = np.zeros((self.batch, S, self.n_kv_heads * self.head_dim), np.float32)
+        v = np.zeros_like(k)
+        check(lib().vmlm_kv4_read(self.descriptor(), _p(k), _p(v), _p(pos0),
+                                  None if count is None else _p(count), S))
+        return k, v
+
+    def attention_decode(self, q, pos, k_new=None, v_new=None, scale=None):
+        """Stores k_new, v_new [batch, n_kv_heads * head_dim] (if given) at pos [batch] and
+        attends q [batch, n_heads * head_dim] over positions 0 .. pos. Zeros where pos < 0."""
+        q = _c(q, np.float32)
+        n_heads = q.shape[1] // self.head_dim
+        pos, _ = self._rows(pos, None)
+        assert q.shape == (self.batch, n_heads * self.head_dim)
+        new = [None if x is None else _c(x, np.float32) for x in (k_new, v_new)]
+        for x in new:
+            assert x is None or x.shape == (self.batch, self.n_kv_heads * self.head_dim)
+        if scale is None:
+            scale = float(np.float32(1.0 / np.sqrt(self.head_dim)))
+        out = np.zeros_like(q)
+        check(lib().vmlm_attention_decode_kv4(self.descriptor(), _p(q),
+                                              *(None if x is None else _p(x) for x in new),
+                                              _p(pos), _p(out), n_heads, float(scale)))
+        return out
