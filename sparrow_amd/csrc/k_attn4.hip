@@ -1,83 +1,548 @@
 // k_attn4.hip -- decode attention over the 4-bit KV cache
 // (vmlm_hip_attention_decode_kv4); the format is in kv4.hpp.
+//
+// For each head, s_p = scale * q . k_p over positions 0 .. pos and
+// o = sum_p exp(s_p - m) v_p / sum_p exp(s_p - m).
+//
+// Bound by the cache's bytes: 5 bits a value, read once for all query heads of a
+// group. What keeps the arithmetic out of the way is that both products run on int8
+// matrix instructions over the nibbles as they lie:
+//  * A nibble in the high half of a byte is 16 (u - 8) as a signed byte, so a
+//    16-byte load becomes two int8 operands (low and high nibbles) with 12
+//    operations. q, and for the output the weights, are 31-bit fixed-point numbers
+//    below their largest value, as four signed bytes: with 16 (u - 8) every product
+//    and sum is exact in int32, and four conversions and three FMAs put the terms
+//    together. 32-bit sums, then, at 8-bit rates. (Three bytes left the many small
+//    weights 2^-22 of the largest: 1.4e-6 off where f32 sums are 4e-7.)
+//  * Scores: a wave takes 128 positions. Lane (row kb, column n) loads the 32
+//    channels of group kb mod NG at one position. The A operand has a row (j, t) for
+//    each kb = j and term t that is zero outside kb = j, so D's rows 4 kb + t at column n
+//    -- the registers of that very lane -- hold its own 32 channels' product, and
+//    the lane applies the scale and minimum that it loaded beside them. The groups of a
+//    position meet by lane swaps.
+//  * Output: o[c] = sum_p (P_p scale_p,g) 16 (u - 8) / 16 + sum_p P_p (min + 8 scale)_p,g.
+//    The lanes that hold (p, g) write P_p scale_p,g as four bytes to LDS, from where
+//    they are the A operand (rows: head, term) against V's nibbles, which lie along
+//    positions; the second sum is a lane's own.
+//  * The maximum and sum of the softmax run along in the wave; the waves of a
+//    workgroup meet in LDS, the workgroups of a split head in a second launch.
+// The new token's row is quantised by the wave that holds its position, put into
+// its registers and stored from there: no read back, no second launch.
+#include <algorithm>
+
 #include "kv4.hpp"
 
 namespace vmlm {
 namespace {
 
-// One workgroup per (query head, sequence): 256 positions at a time, a running
-// maximum and sum.
-__global__ __launch_bounds__(256) void attn4_simple(Kv4View c, const float *q, size_t ldq,
-                                                    const int32_t *posp, float *out, size_t ldo,
-                                                    int H, float scale, int *guard) {
-    __shared__ float qs[KV4_MAX_HD], ps[256], red[4], os[256];
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, hd = c.hd, ng = hd / 32;
-    const int pos = posp[b], kvh = h / (H / c.Hkv);
-    if (pos < 0) return;
-    if (pos >= c.cap) {
-        if (h == 0 && tid == 0) atomicOr(guard, 1);
+typedef float f32x4a __attribute__((ext_vector_type(4), aligned(4)));
+typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
+
+// Positions of a wave at a time: what the registers hold.
+constexpr int attn4_ch(int hd) { return hd <= 128 ? 128 : 64; }
+constexpr int A4_MAX_GH = 4;   // query heads of a workgroup (rows of the A operand / 4)
+constexpr int A4_MAX_W = 8;    // waves of a workgroup
+
+struct Attn4Params {
+    Kv4View c;
+    const float *q, *k_new, *v_new;
+    size_t ldq, ldkv, ldo;
+    const int32_t *pos;
+    float *out, *work;
+    int H, G, nsplit, ch;
+    int parts;  // workgroups that share a kv head's queries
+    float scale2;  // score scale * log2(e)
+    int *guard;
+};
+
+__device__ __forceinline__ float swap16(float v, float (*f)(float, float)) {
+    const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    return f(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+__device__ __forceinline__ float swap32(float v, float (*f)(float, float)) {
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    return f(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+__device__ __forceinline__ float add_f(float a, float b) { return a + b; }
+__device__ __forceinline__ float max_f(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float row16_max(float v) {
+    v = fmaxf(v, dpp_mov<0xB1>(v));
+    v = fmaxf(v, dpp_mov<0x4E>(v));
+    v = fmaxf(v, dpp_mov<0x124>(v));
+    return fmaxf(v, dpp_mov<0x128>(v));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+    v += dpp_mov<0xB1>(v);
+    v += dpp_mov<0x4E>(v);
+    v += dpp_mov<0x124>(v);
+    return v + dpp_mov<0x128>(v);
+}
+// over the rows of lanes that hold other positions of the same group
+template <int GR>
+__device__ __forceinline__ float rows_red(float v, float (*f)(float, float)) {
+    if (GR == 1) v = swap16(v, f);
+    if (GR <= 2) v = swap32(v, f);
+    return v;
+}
+
+__device__ __forceinline__ i32x4 nib_lo(u32x4 w) {
+    return __builtin_bit_cast(i32x4, (w << 4) & 0xf0f0f0f0u);
+}
+__device__ __forceinline__ i32x4 nib_hi(u32x4 w) {
+    return __builtin_bit_cast(i32x4, w & 0xf0f0f0f0u);
+}
+// An integer as four signed bytes, b3 2^24 + b2 2^16 + b1 2^8 + b0 (|x| < 2^30).
+__device__ __forceinline__ uint32_t digits(int x) {
+    return ((uint32_t)x + 0x808080u) ^ 0x808080u;
+}
+// and their sums, highest first, put together again
+__device__ __forceinline__ float undigits(const i32x4 &d) {
+    float f = (float)d[0];
+#pragma unroll
+    for (int t = 1; t < 4; ++t) f = __builtin_fmaf(f, 256.0f, (float)d[t]);
+    return f;
+}
+// The power of two that brings values up to mx below 2^30 (0 for none).
+__device__ __forceinline__ int fixed_exp(float mx) {
+    return mx > 0.0f && mx <= 3.40282347e38f ? 29 - ilogbf(mx) : 0;
+}
+
+// A lane's V codes of one channel: CH / 4 positions, and their product with the
+// weights' bytes. at(p): the byte of position p among those of a term.
+template <int CH>
+struct VCodes {  // 128: 32 positions, low nibbles (even ones), then high ones
+    u32x4 w;
+    __device__ __forceinline__ void load(const uint8_t *v) { w = *(const u32x4 *)v; }
+    static __device__ __forceinline__ int at(int p) {
+        return (p & 1) * 64 + (p >> 5) * 16 + (p & 31) / 2;
+    }
+    __device__ __forceinline__ i32x4 product(const uint8_t *a) const {
+        i32x4 d = {0, 0, 0, 0};
+        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4 *)a, nib_lo(w), d, 0, 0, 0);
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4 *)(a + 64), nib_hi(w), d, 0, 0, 0);
+    }
+};
+typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2;
+template <>
+struct VCodes<64> {  // 16 positions: both nibbles in one operand
+    u32x2 w;
+    __device__ __forceinline__ void load(const uint8_t *v) { w = *(const u32x2 *)v; }
+    static __device__ __forceinline__ int at(int p) {
+        return (p >> 4) * 16 + (p & 1) * 8 + (p & 15) / 2;
+    }
+    __device__ __forceinline__ i32x4 product(const uint8_t *a) const {
+        const u32x2 lo = (w << 4) & 0xf0f0f0f0u, hi = w & 0xf0f0f0f0u;
+        const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4 *)a, __builtin_bit_cast(i32x4, v),
+                                                     i32x4{0, 0, 0, 0}, 0, 0, 0);
+    }
+};
+
+struct Split {
+    int c0, c1;  // chunks of this split
+};
+__device__ __forceinline__ Split split_of(int pos, int ch, int nsplit, int s) {
+    const int nc = pos / ch + 1, per = (nc + nsplit - 1) / nsplit;
+    return {s * per, min(nc, (s + 1) * per)};
+}
+
+// LDS of a workgroup: the query terms [head][term][group][32], their factors and group
+// sums, the new token's codes and meta, the V offsets of each wave, and one region
+// that holds the waves' weight terms, then their results.
+template <int HD, int HEADS>
+struct Lds {
+    static constexpr int NG = HD / 32;
+    static constexpr int Q = 0;
+    static constexpr int F = Q + HEADS * 4 * HD;
+    static constexpr int S = F + HEADS * 4;
+    static constexpr int NK = (S + HEADS * NG * 4 + 15) / 16 * 16;
+    static constexpr int NV = NK + HD / 2;
+    static constexpr int NM = NV + HD;
+    static constexpr int OFF = NM + 2 * NG * 4;
+    static constexpr int R0 = OFF + A4_MAX_W * HEADS * NG * 4;
+    static constexpr int R = (R0 + 15) / 16 * 16;
+};
+
+// GH query heads of one kv head.
+template <int HD, int GH>
+__global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
+    constexpr int NG = HD / 32, GR = NG < 4 ? NG : 4, GL = NG / GR, PS = 64 / GR;
+    constexpr int CH = attn4_ch(HD), NS = CH / PS, CT = HD / 16, TB = CH;  // bytes of a term
+    using M = Lds<HD, GH>;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, w = tid >> 6, W = blockDim.x >> 6, lane = tid & 63;
+    const int kb = lane >> 4, n = lane & 15, g0 = kb % GR, prow = kb / GR;
+    // the parts of a kv head lie 8 workgroups apart: on one XCD, whose L2 then gives
+    // the later ones the cache
+    const int x8 = blockIdx.x / 8, kvh = (x8 / p.parts) * 8 + (int)(blockIdx.x % 8);
+    const int part = x8 % p.parts, b = blockIdx.z;
+    if (kvh >= p.c.Hkv) return;
+    const int h0 = part * GH, G = min(GH, p.G - h0);  // of the kv head's queries
+    const int pos = p.pos[b];
+    if (pos < 0) return;  // an idle sequence
+    if (pos >= p.c.cap) {
+        if (tid == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(p.guard, 1);
         return;
     }
-    const size_t head = (size_t)b * c.Hkv + kvh;
-    if (tid < hd) qs[tid] = q[b * ldq + (size_t)h * hd + tid] * scale;
+    const Split sp = split_of(pos, CH, p.nsplit, blockIdx.y);
+    if (sp.c0 >= sp.c1) return;
+    const size_t head = (size_t)b * p.c.Hkv + kvh, row0 = head * p.c.cap;
+    const int last = pos / CH;
+
+    // 1. the query heads as fixed-point terms
+    float *qf = (float *)(lds + M::F), *qs = (float *)(lds + M::S);
+    for (int h = w; h < GH; h += W) {
+        const float *q = p.q + b * p.ldq + ((size_t)kvh * p.G + h0 + min(h, G - 1)) * HD;
+        constexpr int CL = (HD + 63) / 64;
+        float x[CL], mx = 0.0f;
+        int bad = 0;
+#pragma unroll
+        for (int i = 0; i < CL; ++i) {
+            const int c = i * 64 + lane;
+            x[i] = c < HD ? q[c] : 0.0f;
+            mx = fmaxf(mx, fabsf(x[i]));
+            bad |= !(fabsf(x[i]) <= 3.40282347e38f);
+        }
+        mx = wave_max(mx);
+        bad = __any(bad);
+        const int e = fixed_exp(mx);
+#pragma unroll
+        for (int i = 0; i < CL; ++i) {
+            const int c = i * 64 + lane;
+            float s = x[i];
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) s += __shfl_xor(s, o, 64);
+            if (c >= HD) continue;
+            const uint32_t d = digits(bad ? 0 : (int)rintf(ldexpf(x[i], e)));
+            uint8_t *t = lds + M::Q + ((h * 4) * NG + c / 32) * 32 + (c & 1) * 16 + c % 32 / 2;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k * NG * 32] = (uint8_t)(d >> (24 - 8 * k));
+            if ((c & 31) == 0) qs[h * NG + c / 32] = s * p.scale2;
+        }
+        if (lane == 0)
+            qf[h] = bad ? __builtin_nanf("") : ldexpf(p.scale2, -e - 4);
+    }
     __syncthreads();
-    float m = -__builtin_inff(), L = 0.0f, o = 0.0f;
-    const int parts = 256 / hd, ch = tid % hd, part = tid / hd;
-    for (int p0 = 0; p0 <= pos; p0 += 256) {
-        const int p = p0 + tid;
-        float s = -__builtin_inff();
-        if (p <= pos) {
-            s = 0.0f;
-            const uint8_t *kr = c.k + (head * c.cap + p) * (size_t)(hd / 2);
-            for (int g = 0; g < ng; ++g) {
-                const uint32_t mt = c.km[(head * c.cap + p) * ng + g];
-                for (int i = 0; i < 32; ++i)
-                    s = __builtin_fmaf(qs[g * 32 + i],
-                                       kv4_value(kr[(g * 32 + i) / 2] >> (4 * (i & 1)),
-                                                 kv4_min(mt), kv4_scale(mt)), s);
+
+    // the A operand of head h: row (j, t), nonzero where kb = j
+    const bool mine = n >> 2 == kb;
+    const int term = n & 3;
+    auto qa = [&](int h, int e, int par) {
+        const i32x4 a = *(const i32x4 *)(lds + M::Q + ((h * 4 + term) * NG + g0 + 4 * e) * 32 +
+                                         par * 16);
+        return mine ? a : i32x4{0, 0, 0, 0};
+    };
+
+    float m[GH], l[GH], off[GH][GL], O[CT];
+#pragma unroll
+    for (int h = 0; h < GH; ++h) {
+        m[h] = -__builtin_inff();
+        l[h] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < GL; ++e) off[h][e] = 0.0f;
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) O[ct] = 0.0f;
+    uint8_t *pb = lds + M::R + w * (GH * NG * 4 * TB);
+
+    for (int ch = sp.c0 + w; ch < sp.c1; ch += W) {
+        const int p0 = ch * CH;
+        // 2. everything of the CH positions; past the last one, that one again
+        u32x4 kc[NS][GL];
+        VCodes<CH> vc[CT];
+        uint32_t km[NS][GL], vm[NS][GL];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const size_t row = row0 + min(p0 + i * PS + prow * 16 + n, pos);
+#pragma unroll
+            for (int e = 0; e < GL; ++e) {
+                kc[i][e] = *(const u32x4 *)(p.c.k + row * (HD / 2) + (g0 + 4 * e) * 16);
+                km[i][e] = p.c.km[row * NG + g0 + 4 * e];
+                vm[i][e] = p.c.vm[row * NG + g0 + 4 * e];
             }
         }
-        float mx = wave_max(s);
-        if ((tid & 63) == 0) red[tid >> 6] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float mn = fmaxf(m, mx), corr = __expf(m - mn);
-        const float pr = p <= pos ? expf(s - mn) : 0.0f;
-        ps[tid] = pr;
-        __syncthreads();
-        o *= corr;
-        L *= corr;
-        m = mn;
-        const int n = min(256, pos + 1 - p0);
-        for (int i = 0; i < n; ++i) L += ps[i];
-        for (int i = part; i < n; i += parts) {
-            const size_t at = p0 + i;
-            const uint32_t mt = c.vm[(head * c.cap + at) * ng + ch / 32];
-            const uint8_t vb = c.v[((head * (c.cap / 32) + at / 32) * hd + ch) * 16 + at % 32 / 2];
-            o = __builtin_fmaf(ps[i], kv4_value(vb >> (4 * (at & 1)), kv4_min(mt), kv4_scale(mt)),
-                               o);
+        // lane (kb, n): the kb-th quarter of the positions, channel 16 ct + n
+        const int vblk = min((p0 + kb * (CH / 4)) / KV4_BLOCK, pos / KV4_BLOCK);
+        uint8_t *vb = p.c.v + ((head * (p.c.cap / KV4_BLOCK) + vblk) * HD + n) * 16 +
+                      (CH == 128 ? 0 : (kb & 1) * 8);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) vc[ct].load(vb + ct * 256);
+
+        if (p.k_new && ch == last) {  // 3. the new token: quantised, stored, put in place
+            uint32_t *nm = (uint32_t *)(lds + M::NM);
+            const int c4 = min(lane, HD / 4 - 1) * 4;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const float *src = (v ? p.v_new : p.k_new) + b * p.ldkv + (size_t)kvh * HD;
+                const f32x4a r = *(const f32x4a *)(src + c4);
+                const float x[4] = {r[0], r[1], r[2], r[3]};
+                const uint32_t mt = kv4_meta8(x);
+                uint32_t c[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[e] = kv4_code(x[e], kv4_min(mt), kv4_scale(mt));
+                if (lane < HD / 4) {
+                    if (v)
+                        *(uint32_t *)(lds + M::NV + c4) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+                    else
+                        *(uint16_t *)(lds + M::NK + c4 / 2) =
+                            (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
+                    if ((lane & 7) == 0) nm[v * NG + lane / 8] = mt;
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                if (p0 + i * PS + prow * 16 + n != pos) continue;
+#pragma unroll
+                for (int e = 0; e < GL; ++e) {
+                    const int g = g0 + 4 * e;
+                    const size_t row = row0 + pos;
+                    kc[i][e] = *(const u32x4 *)(lds + M::NK + g * 16);
+                    km[i][e] = nm[g];
+                    vm[i][e] = nm[NG + g];
+                    if (part) continue;
+                    *(u32x4 *)(p.c.k + row * (HD / 2) + g * 16) = kc[i][e];
+                    p.c.km[row * NG + g] = km[i][e];
+                    p.c.vm[row * NG + g] = vm[i][e];
+                }
+            }
+            if ((p0 + kb * (CH / 4)) / (CH / 4) == pos / (CH / 4)) {
+                const int d = pos % (CH / 4) / 8, sh = pos % 8 * 4;
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    const uint32_t nib = (uint32_t)lds[M::NV + ct * 16 + n] << sh;
+#pragma unroll
+                    for (int x = 0; x < CH / 32; ++x)
+                        if (x == d) {
+                            vc[ct].w[x] = (vc[ct].w[x] & ~(15u << sh)) | nib;
+                            if (part == 0) *(uint32_t *)(vb + ct * 256 + x * 4) = vc[ct].w[x];
+                        }
+                }
+            }
         }
-        __syncthreads();
+
+        // 4. V's scales (none past the last position) and the fixed point of each group
+        float vs[NS][GL], vo[NS][GL];
+        int ev[GL];
+#pragma unroll
+        for (int e = 0; e < GL; ++e) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const bool in = p0 + i * PS + prow * 16 + n <= pos;
+                vs[i][e] = in ? kv4_scale(vm[i][e]) : 0.0f;
+                vo[i][e] = in ? __builtin_fmaf(8.0f, vs[i][e], kv4_min(vm[i][e])) : 0.0f;
+                mx = fmaxf(mx, vs[i][e]);
+            }
+            ev[e] = fixed_exp(rows_red<GR>(row16_max(mx), max_f));
+        }
+
+        float corr[GH];
+#pragma unroll
+        for (int h = 0; h < GH; ++h) {
+            // 5. scores of the lane's positions, in powers of two
+            float s[NS], mx = -__builtin_inff();
+            const float f = qf[h];
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                s[i] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < GL; ++e) {
+                    i32x4 d = {0, 0, 0, 0};
+                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 0), nib_lo(kc[i][e]), d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 1), nib_hi(kc[i][e]), d, 0, 0, 0);
+                    const float sc = kv4_scale(km[i][e]);
+                    const float mid = __builtin_fmaf(8.0f, sc, kv4_min(km[i][e]));
+                    s[i] = __builtin_fmaf(undigits(d) * f, sc,
+                                          __builtin_fmaf(mid, qs[h * NG + g0 + 4 * e], s[i]));
+                }
+                if (GR >= 2) s[i] = swap16(s[i], add_f);
+                if (GR == 4) s[i] = swap32(s[i], add_f);
+                if (p0 + i * PS + prow * 16 + n > pos) s[i] = -__builtin_inff();
+                mx = fmaxf(mx, s[i]);
+            }
+            // 6. the running maximum, the weights and their bytes
+            mx = fmaxf(m[h], rows_red<GR>(row16_max(mx), max_f));
+            corr[h] = __builtin_amdgcn_exp2f(m[h] - mx);
+            m[h] = mx;
+            l[h] *= corr[h];
+#pragma unroll
+            for (int e = 0; e < GL; ++e) off[h][e] *= corr[h];
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const float P = __builtin_amdgcn_exp2f(s[i] - mx);
+                l[h] += P;
+                const int at = i * PS + prow * 16 + n;  // position in the chunk
+#pragma unroll
+                for (int e = 0; e < GL; ++e) {
+                    off[h][e] = __builtin_fmaf(P, vo[i][e], off[h][e]);
+                    const uint32_t d = digits((int)rintf(ldexpf(P * vs[i][e], ev[e])));
+                    uint8_t *o = pb + ((h * NG + g0 + 4 * e) * 4) * TB + VCodes<CH>::at(at);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[k * TB] = (uint8_t)(d >> (24 - 8 * k));
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        // 7. the output's product over the positions
+        float cq = corr[0];
+#pragma unroll
+        for (int h = 1; h < GH; ++h) cq = kb == h ? corr[h] : cq;
+        const int hq = min(n >> 2, GH - 1);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            const int g = ct / 2;
+            const i32x4 d = vc[ct].product(pb + ((hq * NG + g) * 4 + term) * TB + kb * 16);
+            const int eg = __builtin_amdgcn_readlane(ev[g / 4], (g % GR) * 16);
+            O[ct] = __builtin_fmaf(O[ct], cq, ldexpf(undigits(d), -eg - 4));
+        }
+        __builtin_amdgcn_wave_barrier();
     }
-    os[tid] = o;
+
+    // 8. the waves' results
+    float *offl = (float *)(lds + M::OFF) + w * GH * NG;
+#pragma unroll
+    for (int h = 0; h < GH; ++h) {
+        l[h] = rows_red<GR>(row16_sum(l[h]), add_f);
+#pragma unroll
+        for (int e = 0; e < GL; ++e) {
+            const float o = rows_red<GR>(row16_sum(off[h][e]), add_f);
+            if (n == 0 && kb < GR) offl[h * NG + kb + 4 * e] = o;
+        }
+    }
+    __syncthreads();  // the weights' bytes are read; the region is the results' now
+    float *mo = (float *)(lds + M::R), *ml = mo + W * GH * HD;
+    if (kb < G) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+            mo[(w * GH + kb) * HD + ct * 16 + n] = O[ct] + offl[kb * NG + ct / 2];
+    }
+#pragma unroll
+    for (int h = 0; h < GH; ++h)
+        if (lane == 0) {
+            ml[(w * GH + h) * 2] = m[h];
+            ml[(w * GH + h) * 2 + 1] = l[h];
+        }
     __syncthreads();
-    if (tid < hd) {
-        for (int i = 1; i < parts; ++i) o += os[tid + i * hd];
-        out[b * ldo + (size_t)h * hd + tid] = o / L;
+    const size_t oh = (size_t)b * p.H + (size_t)kvh * p.G + h0;
+    for (int i = tid; i < G * HD; i += blockDim.x) {
+        const int h = i / HD, c = i % HD;
+        float mx = -__builtin_inff(), L = 0.0f, o = 0.0f;
+        for (int x = 0; x < W; ++x) mx = fmaxf(mx, ml[(x * GH + h) * 2]);
+        for (int x = 0; x < W; ++x) {
+            const float mw = ml[(x * GH + h) * 2];
+            // a wave without a chunk has no maximum
+            const float f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - mx);
+            L = __builtin_fmaf(f, ml[(x * GH + h) * 2 + 1], L);
+            o = __builtin_fmaf(f, mo[(x * GH + h) * HD + c], o);
+        }
+        if (p.nsplit == 1) {
+            p.out[b * p.ldo + ((size_t)kvh * p.G + h0 + h) * HD + c] = o / L;
+        } else {
+            float *pw = p.work + ((oh + h) * p.nsplit + blockIdx.y) * (HD + 4);
+            pw[c] = o;
+            if (c == 0) {
+                pw[HD] = mx;
+                pw[HD + 1] = L;
+            }
+        }
     }
+}
+
+// The splits of a head, in order.
+__global__ __launch_bounds__(KV4_MAX_HD) void attn4_merge_kernel(Attn4Params p) {
+    const int h = blockIdx.x, b = blockIdx.y, c = threadIdx.x, hd = p.c.hd;
+    const int pos = p.pos[b];
+    if (pos < 0 || pos >= p.c.cap || c >= hd) return;
+    const float *pw = p.work + ((size_t)b * p.H + h) * p.nsplit * (hd + 4);
+    int live = 0;
+    while (live < p.nsplit && split_of(pos, p.ch, p.nsplit, live).c0 < split_of(pos, p.ch, p.nsplit, live).c1)
+        ++live;
+    float mx = -__builtin_inff(), L = 0.0f, o = 0.0f;
+    for (int s = 0; s < live; ++s) mx = fmaxf(mx, pw[s * (hd + 4) + hd]);
+    for (int s = 0; s < live; ++s) {
+        const float f = __builtin_amdgcn_exp2f(pw[s * (hd + 4) + hd] - mx);
+        L = __builtin_fmaf(f, pw[s * (hd + 4) + hd + 1], L);
+        o = __builtin_fmaf(f, pw[s * (hd + 4) + c], o);
+    }
+    p.out[b * p.ldo + (size_t)h * hd + c] = o / L;
+}
+
+struct Attn4Plan {
+    int W, nsplit, parts;
+};
+Attn4Plan attn4_plan(const Kv4View &c, int H) {
+    const int ch = attn4_ch(c.hd), chunks = (c.cap + ch - 1) / ch;
+    Attn4Plan pl;
+    pl.parts = (H / c.Hkv + A4_MAX_GH - 1) / A4_MAX_GH;
+    const long long pairs = (long long)c.B * c.Hkv * pl.parts;
+    pl.W = std::min(A4_MAX_W, chunks);
+    const long long want = 2048 / (pairs * pl.W);
+    pl.nsplit = (int)std::max(1LL, std::min(want, (long long)chunks / pl.W));
+    return pl;
+}
+
+template <int HD, int GH>
+int launch_t(const Attn4Params &p, int W, hipStream_t st) {
+    using M = Lds<HD, GH>;
+    // a wave's weight terms, or its results
+    constexpr size_t region = std::max(GH * M::NG * 4 * attn4_ch(HD), GH * (HD + 2) * 4);
+    const size_t bytes = M::R + W * region;
+    int rc = allow_lds((const void *)attn4_kernel<HD, GH>, bytes, M::R + A4_MAX_W * region);
+    if (rc) return rc;
+    const dim3 grid(cdiv((size_t)p.c.Hkv, 8) * 8 * p.parts, (unsigned)p.nsplit, (unsigned)p.c.B);
+    attn4_kernel<HD, GH><<<grid, 64 * W, bytes, st>>>(p);
+    VMLM_HIP_CHECK(hipGetLastError());
+    return VMLM_OK;
+}
+
+template <int HD>
+int launch_hd(const Attn4Params &p, int W, hipStream_t st) {
+    if (p.G == 1) return launch_t<HD, 1>(p, W, st);
+    if (p.G == 2) return launch_t<HD, 2>(p, W, st);
+    return launch_t<HD, A4_MAX_GH>(p, W, st);
 }
 
 }  // namespace
 
-size_t attn4_work_floats(const Kv4View &c, int H) { return 0; }
+size_t attn4_work_floats(const Kv4View &c, int H) {
+    if (c.B == 0 || c.Hkv == 0 || c.cap == 0 || H == 0) return 0;
+    const Attn4Plan pl = attn4_plan(c, H);
+    return pl.nsplit == 1 ? 0 : (size_t)c.B * H * pl.nsplit * (c.hd + 4);
+}
 
 int launch_attn4(const Attn4Args &a, hipStream_t st) {
-    if (a.k_new) {
-        int rc = launch_kv4_append(a.c, a.k_new, a.ldkv, a.v_new, a.ldkv, a.pos, nullptr, 1, st);
-        if (rc) return rc;
+    const Attn4Plan pl = attn4_plan(a.c, a.H);
+    Attn4Params p;
+    p.c = a.c;
+    p.q = a.q;
+    p.k_new = a.k_new;
+    p.v_new = a.v_new;
+    p.ldq = a.ldq;
+    p.ldkv = a.ldkv;
+    p.ldo = a.ldo;
+    p.pos = a.pos;
+    p.out = a.out;
+    p.work = a.work;
+    p.H = a.H;
+    p.G = a.H / a.c.Hkv;
+    p.nsplit = pl.nsplit;
+    p.parts = pl.parts;
+    p.ch = attn4_ch(a.c.hd);
+    p.scale2 = a.scale * 1.44269504088896340736f;
+    p.guard = guard_flag_ptr();
+    VMLM_GUARD(p.nsplit == 1 || p.work, "kv4 attention: split positions need a workspace");
+    int rc;
+    switch (a.c.hd) {
+    case 32: rc = launch_hd<32>(p, pl.W, st); break;
+    case 64: rc = launch_hd<64>(p, pl.W, st); break;
+    case 128: rc = launch_hd<128>(p, pl.W, st); break;
+    default: rc = launch_hd<256>(p, pl.W, st); break;
     }
-    attn4_simple<<<dim3((unsigned)a.H, (unsigned)a.c.B), 256, 0, st>>>(
-        a.c, a.q, a.ldq, a.pos, a.out, a.ldo, a.H, a.scale, guard_flag_ptr());
+    if (rc || p.nsplit == 1) return rc;
+    attn4_merge_kernel<<<dim3((unsigned)p.H, (unsigned)p.c.B), std::max(64, p.c.hd), 0, st>>>(p);
     VMLM_HIP_CHECK(hipGetLastError());
     return VMLM_OK;
 }

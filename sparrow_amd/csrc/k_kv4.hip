@@ -1,5 +1,7 @@
 // k_kv4.hip -- rows into the 4-bit KV cache and out of it
 // (vmlm_hip_kv4_append, vmlm_hip_kv4_read); the format is in kv4.hpp.
+#include <algorithm>
+
 #include "kv4.hpp"
 
 namespace vmlm {
