@@ -503,7 +503,11 @@ struct Int4Args {
     const float *scale = nullptr;
     float *C = nullptr;  // [M][N]
     int M = 0, N = 0, K = 0, G = 0;
+    // gemm_int4_work_bytes() bytes for the activations as byte planes, or null: each
+    // workgroup then splits the rows itself, with the same result
+    void *work = nullptr;
 };
+size_t gemm_int4_work_bytes(int M, int N, int K);
 int launch_gemm_int4(const Int4Args &a, hipStream_t st);
 
 // RMSNorm of each query and key head and the position rotation in one pass
