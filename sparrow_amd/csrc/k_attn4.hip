@@ -280,8 +280,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
                 const float x[4] = {r[0], r[1], r[2], r[3]};
                 const uint32_t mt = kv4_meta8(x);
                 uint32_t c[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) c[e] = kv4_code(x[e], kv4_min(mt), kv4_scale(mt));
+                kv4_codes(x, mt, c);
                 if (lane < HD / 4) {
                     if (v)
                         *(uint32_t *)(lds + M::NV + c4) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;

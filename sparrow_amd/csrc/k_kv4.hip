@@ -39,82 +39,134 @@ __device__ __forceinline__ bool kv4_rows(const Kv4Params &p, int b, int blk, int
     return *t0 < *t1;
 }
 
+// Four bytes of four dwords transposed: byte e of out[k] is byte k of v[e].
+__device__ __forceinline__ void transpose_bytes(const uint32_t (&v)[4], uint32_t (&out)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);
+    const uint32_t b = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
+    const uint32_t d = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    out[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
 // One workgroup per (32-position block, head, sequence). Eight lanes quantise 32
 // channels of a position; V's codes cross LDS to be packed along positions, and a
-// block's bytes that hold other positions keep their nibbles.
+// block's bytes that hold other positions keep their nibbles. Bound by the f32 rows;
+// all of a thread's loads are issued before the first is used.
+template <int HD>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Params p) {
-    __shared__ uint8_t codes[KV4_BLOCK * KV4_MAX_HD];
-    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, hd = p.c.hd, ng = hd / 32;
+    constexpr int NG = HD / 32, LD = HD + 4;  // bytes of a position in LDS
+    __shared__ __align__(4) uint8_t codes[KV4_BLOCK * LD];
+    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
     int first, pos0, t0, t1;
     if (!kv4_rows(p, b, blockIdx.x, &first, &pos0, &t0, &t1)) return;
     const size_t head = (size_t)b * p.c.Hkv + h;
     const int l = tid & 7;
-    for (int task = tid >> 3; task < KV4_BLOCK * ng; task += 32) {
-        const int o = task / ng, g = task - o * ng, t = first + o - pos0;
+    f32x4a rk[NG], rv[NG];
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const int task = (tid >> 3) + i * 32, o = task / NG, g = task % NG;
+        const int t = min(max(first + o - pos0, t0), t1 - 1);
+        const size_t row = (size_t)b * p.S + t, at = (size_t)h * HD + g * 32 + 4 * l;
+        rk[i] = *(const f32x4a *)(p.k + row * p.ldk + at);
+        rv[i] = *(const f32x4a *)(p.v + row * p.ldv + at);
+    }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const int task = (tid >> 3) + i * 32, o = task / NG, g = task % NG;
+        const int t = first + o - pos0, ch = g * 32 + 4 * l;
         if (t < t0 || t >= t1) continue;  // the same for the eight lanes
-        const size_t row = (size_t)b * p.S + t, pos = head * p.c.cap + first + o;
-        const int ch = g * 32 + 4 * l;
-        float x[4];
-        f32x4a r = *(const f32x4a *)(p.k + row * p.ldk + (size_t)h * hd + ch);
-        for (int e = 0; e < 4; ++e) x[e] = r[e];
-        uint32_t m = kv4_meta8(x);
-        float mn = kv4_min(m), sc = kv4_scale(m);
+        const size_t pos = head * p.c.cap + first + o;
+        const float k[4] = {rk[i][0], rk[i][1], rk[i][2], rk[i][3]};
+        const float v[4] = {rv[i][0], rv[i][1], rv[i][2], rv[i][3]};
+        const uint32_t mk = kv4_meta8(k), mv = kv4_meta8(v);
         uint32_t c[4];
-        for (int e = 0; e < 4; ++e) c[e] = kv4_code(x[e], mn, sc);
-        *(uint16_t *)(p.c.k + pos * (hd / 2) + ch / 2) =
+        kv4_codes(k, mk, c);
+        *(uint16_t *)(p.c.k + pos * (HD / 2) + ch / 2) =
             (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
-        if (l == 0) p.c.km[pos * ng + g] = m;
-        r = *(const f32x4a *)(p.v + row * p.ldv + (size_t)h * hd + ch);
-        for (int e = 0; e < 4; ++e) x[e] = r[e];
-        m = kv4_meta8(x);
-        mn = kv4_min(m);
-        sc = kv4_scale(m);
-        for (int e = 0; e < 4; ++e) c[e] = kv4_code(x[e], mn, sc);
-        *(uint32_t *)(codes + o * hd + ch) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-        if (l == 0) p.c.vm[pos * ng + g] = m;
+        kv4_codes(v, mv, c);
+        *(uint32_t *)(codes + o * LD + ch) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+        if (l == 0) {
+            p.c.km[pos * NG + g] = mk;
+            p.c.vm[pos * NG + g] = mv;
+        }
     }
     __syncthreads();
     const int o0 = pos0 + t0 - first, o1 = pos0 + t1 - first;  // offsets that are new
     uint32_t *vb = (uint32_t *)(p.c.v + (head * (p.c.cap / KV4_BLOCK) + first / KV4_BLOCK) *
-                                            (size_t)(hd * 16));
-    for (int i = tid; i < hd * 4; i += 256) {  // dword: channel i / 4, offsets 8 (i % 4) ..
-        const int ch = i >> 2, base = (i & 3) * 8;
-        uint32_t w = 0, mask = 0;
-        for (int e = 0; e < 8; ++e) {
-            const int o = base + e;
-            if (o >= o0 && o < o1) {
-                w |= (uint32_t)codes[o * hd + ch] << (4 * e);
-                mask |= 15u << (4 * e);
-            }
-        }
-        if (mask == 0) continue;
-        if (mask != 0xffffffffu) w |= vb[i] & ~mask;
-        vb[i] = w;
+                                            (size_t)(HD * 16));
+    if (tid >= HD) return;
+    // four channels, eight positions: byte e of a dword holds 2e and 2e + 1
+    const int ch = tid / 4 * 4, base = (tid & 3) * 8;
+    uint32_t w[4], out[4], mask = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint8_t *a = codes + (base + 2 * e) * LD + ch;
+        // (positions without a new row hold anything)
+        w[e] = (*(const uint32_t *)a & 0x0f0f0f0fu) |
+               (*(const uint32_t *)(a + LD) << 4 & 0xf0f0f0f0u);
+    }
+    transpose_bytes(w, out);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (base + e >= o0 && base + e < o1) mask |= 15u << (4 * e);
+    if (mask == 0) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        uint32_t *at = vb + (ch + k) * 4 + (tid & 3);
+        *at = mask == 0xffffffffu ? out[k] : (out[k] & mask) | (*at & ~mask);
     }
 }
 
+// The block's codes and meta through LDS, then four channels of a position a thread.
+template <int HD>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Params p) {
-    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, hd = p.c.hd, ng = hd / 32;
+    constexpr int NG = HD / 32, KD = HD * 4, LV = 20;  // dwords of codes; LDS bytes of a V channel
+    __shared__ uint32_t kc[KD], km[KV4_BLOCK * NG], vm[KV4_BLOCK * NG];
+    __shared__ __align__(4) uint8_t vc[HD * LV];
+    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
     int first, pos0, t0, t1;
     if (!kv4_rows(p, b, blockIdx.x, &first, &pos0, &t0, &t1)) return;
-    const size_t head = (size_t)b * p.c.Hkv + h;
-    const uint8_t *vb = p.c.v + (head * (p.c.cap / KV4_BLOCK) + first / KV4_BLOCK) *
-                                    (size_t)(hd * 16);
-    for (int i = tid; i < KV4_BLOCK * hd / 4; i += 256) {
-        const int o = i / (hd / 4), ch = (i - o * (hd / 4)) * 4, t = first + o - pos0;
-        if (t < t0 || t >= t1) continue;
-        const size_t row = (size_t)b * p.S + t, pos = head * p.c.cap + first + o;
-        const uint32_t km = p.c.km[pos * ng + ch / 32], vm = p.c.vm[pos * ng + ch / 32];
-        const uint32_t kc = *(const uint16_t *)(p.c.k + pos * (hd / 2) + ch / 2);
-        f32x4a k, v;
-        for (int e = 0; e < 4; ++e) {
-            k[e] = kv4_value(kc >> (4 * e), kv4_min(km), kv4_scale(km));
-            v[e] = kv4_value((uint32_t)vb[(ch + e) * 16 + o / 2] >> (4 * (o & 1)), kv4_min(vm),
-                             kv4_scale(vm));
-        }
-        *(f32x4a *)(p.ko + row * p.ldk + (size_t)h * hd + ch) = k;
-        *(f32x4a *)(p.vo + row * p.ldv + (size_t)h * hd + ch) = v;
+    const size_t head = (size_t)b * p.c.Hkv + h, pos = head * p.c.cap + first;
+    const uint32_t *kb = (const uint32_t *)(p.c.k + pos * (HD / 2));
+    const uint32_t *vb = (const uint32_t *)(p.c.v + pos * (HD / 2));  // a block is as long
+#pragma unroll
+    for (int i = tid; i < KD; i += 256) {
+        kc[i] = kb[i];
+        *(uint32_t *)(vc + i / 4 * LV + i % 4 * 4) = vb[i];
     }
+    if (tid < KV4_BLOCK * NG) {
+        km[tid] = p.c.km[pos * NG + tid];
+        vm[tid] = p.c.vm[pos * NG + tid];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const int x = tid + i * 256, o = x / (HD / 4), ch = x % (HD / 4) * 4, t = first + o - pos0;
+        if (t < t0 || t >= t1) continue;
+        const size_t row = (size_t)b * p.S + t;
+        const uint32_t mk = km[o * NG + ch / 32], mv = vm[o * NG + ch / 32];
+        const uint32_t c = ((const uint16_t *)kc)[x];
+        f32x4a k, v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            k[e] = kv4_value(c >> (4 * e), kv4_min(mk), kv4_scale(mk));
+            v[e] = kv4_value((uint32_t)vc[(ch + e) * LV + o / 2] >> (4 * (o & 1)), kv4_min(mv),
+                             kv4_scale(mv));
+        }
+        *(f32x4a *)(p.ko + row * p.ldk + (size_t)h * HD + ch) = k;
+        *(f32x4a *)(p.vo + row * p.ldv + (size_t)h * HD + ch) = v;
+    }
+}
+
+template <int HD>
+void launch_hd(const Kv4Params &p, dim3 grid, hipStream_t st) {
+    if (p.k)
+        kv4_append_kernel<HD><<<grid, 256, 0, st>>>(p);
+    else
+        kv4_read_kernel<HD><<<grid, 256, 0, st>>>(p);
 }
 
 dim3 kv4_grid(const Kv4View &c, int S) {
@@ -123,22 +175,30 @@ dim3 kv4_grid(const Kv4View &c, int S) {
     return dim3((unsigned)blocks, (unsigned)c.Hkv, (unsigned)c.B);
 }
 
-}  // namespace
-
-int launch_kv4_append(const Kv4View &c, const float *k, size_t ldk, const float *v, size_t ldv,
-                      const int32_t *pos0, const int32_t *count, int S, hipStream_t st) {
-    Kv4Params p{c, k, v, nullptr, nullptr, ldk, ldv, pos0, count, S, guard_flag_ptr()};
-    kv4_append_kernel<<<kv4_grid(c, S), 256, 0, st>>>(p);
+int launch_kv4(const Kv4Params &p, hipStream_t st) {
+    const dim3 grid = kv4_grid(p.c, p.S);
+    switch (p.c.hd) {
+    case 32: launch_hd<32>(p, grid, st); break;
+    case 64: launch_hd<64>(p, grid, st); break;
+    case 128: launch_hd<128>(p, grid, st); break;
+    default: launch_hd<256>(p, grid, st); break;
+    }
     VMLM_HIP_CHECK(hipGetLastError());
     return VMLM_OK;
 }
 
+}  // namespace
+
+int launch_kv4_append(const Kv4View &c, const float *k, size_t ldk, const float *v, size_t ldv,
+                      const int32_t *pos0, const int32_t *count, int S, hipStream_t st) {
+    return launch_kv4(Kv4Params{c, k, v, nullptr, nullptr, ldk, ldv, pos0, count, S,
+                                guard_flag_ptr()}, st);
+}
+
 int launch_kv4_read(const Kv4View &c, float *k, size_t ldk, float *v, size_t ldv,
                     const int32_t *pos0, const int32_t *count, int S, hipStream_t st) {
-    Kv4Params p{c, nullptr, nullptr, k, v, ldk, ldv, pos0, count, S, guard_flag_ptr()};
-    kv4_read_kernel<<<kv4_grid(c, S), 256, 0, st>>>(p);
-    VMLM_HIP_CHECK(hipGetLastError());
-    return VMLM_OK;
+    return launch_kv4(Kv4Params{c, nullptr, nullptr, k, v, ldk, ldv, pos0, count, S,
+                                guard_flag_ptr()}, st);
 }
 
 }  // namespace vmlm

@@ -20,48 +20,63 @@ namespace vmlm {
 
 constexpr int KV4_BLOCK = 32;
 
-// The meta of 32 values with lowest lo and highest hi; NaN twice where one of
-// them is not finite (`bad`) or their range leaves f32.
-__device__ __forceinline__ uint32_t kv4_meta(float lo, float hi, bool bad) {
+// The meta of 32 values with lowest lo and highest hi (NaN among them gives both
+// NaN); NaN twice where one of them is not finite or their range leaves f32.
+__device__ __forceinline__ uint32_t kv4_meta(float lo, float hi) {
     const uint32_t b = __float_as_uint(lo);
     const uint32_t mn = ((b >> 31) ? b + 0xffffu : b) & 0xffff0000u;
     const float q = (hi - __uint_as_float(mn)) / 15.0f;
     const uint32_t sc = (__float_as_uint(q) + 0xffffu) & 0xffff0000u;
-    const bool ok = !bad && (mn & 0x7f800000u) != 0x7f800000u && (sc & 0x7f800000u) != 0x7f800000u;
+    const bool ok = (mn & 0x7f800000u) != 0x7f800000u && (sc & 0x7f800000u) != 0x7f800000u;
     return ok ? mn | (sc >> 16) : 0x7fc07fc0u;
 }
 __device__ __forceinline__ float kv4_scale(uint32_t meta) { return __uint_as_float(meta << 16); }
 __device__ __forceinline__ float kv4_min(uint32_t meta) {
     return __uint_as_float(meta & 0xffff0000u);
 }
-// the nibble of x
+// the nibble of x, by the definition's quotient
 __device__ __forceinline__ uint32_t kv4_code(float x, float mn, float sc) {
     const float u = sc > 0.0f ? fminf(fmaxf(rintf((x - mn) / sc), 0.0f), 15.0f) : 0.0f;
     return (uint32_t)u ^ 8u;
+}
+// The nibbles of four values. A product with 1 / scale is within 2^-22 of the quotient
+// relative to it, 2^-18 in all, so it decides every code whose quotient is not
+// nearer than 2^-16 to a half; the wave takes the quotients themselves where one is,
+// or where the scale is so small or large that its reciprocal is not normal.
+__device__ __forceinline__ void kv4_codes(const float (&x)[4], uint32_t meta, uint32_t (&c)[4]) {
+    const float mn = kv4_min(meta), sc = kv4_scale(meta), r = __builtin_amdgcn_rcpf(sc);
+    bool near = !(sc > 1e-36f && sc < 1e36f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float q = (x[e] - mn) * r, n = rintf(q);
+        near |= !(fabsf(q - n) < 0.5f - 0x1p-16f);
+        c[e] = (uint32_t)(int)fminf(fmaxf(n, 0.0f), 15.0f) ^ 8u;
+    }
+    if (__builtin_expect(__any(near), 0)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = kv4_code(x[e], mn, sc);
+    }
 }
 // the value of a nibble (in the low four bits)
 __device__ __forceinline__ float kv4_value(uint32_t nib, float mn, float sc) {
     return sc * (float)((nib & 15u) ^ 8u) + mn;
 }
 
-// Minimum, maximum and non-finite flag of 32 values held by 8 neighbouring
-// lanes, four each; the same in all eight.
+// The meta of 32 values held by 8 neighbouring lanes, four each; the same in all
+// eight. (Minimum and maximum that keep a NaN; lanes swapped within a quad, then the
+// half row mirrored.)
 __device__ __forceinline__ uint32_t kv4_meta8(const float (&x)[4]) {
-    float lo = x[0], hi = x[0];
-    int bad = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
-        bad |= !(fabsf(x[e]) <= 3.40282347e38f);
-    }
-#pragma unroll
-    for (int o = 1; o < 8; o *= 2) {
-        lo = fminf(lo, __shfl_xor(lo, o, 64));
-        hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-        bad |= __shfl_xor(bad, o, 64);
-    }
-    return kv4_meta(lo, hi, bad != 0);
+    float lo = __builtin_elementwise_minimum(__builtin_elementwise_minimum(x[0], x[1]),
+                                             __builtin_elementwise_minimum(x[2], x[3]));
+    float hi = __builtin_elementwise_maximum(__builtin_elementwise_maximum(x[0], x[1]),
+                                             __builtin_elementwise_maximum(x[2], x[3]));
+    lo = __builtin_elementwise_minimum(lo, dpp_mov<0xB1>(lo));
+    hi = __builtin_elementwise_maximum(hi, dpp_mov<0xB1>(hi));
+    lo = __builtin_elementwise_minimum(lo, dpp_mov<0x4E>(lo));
+    hi = __builtin_elementwise_maximum(hi, dpp_mov<0x4E>(hi));
+    lo = __builtin_elementwise_minimum(lo, dpp_mov<0x141>(lo));
+    hi = __builtin_elementwise_maximum(hi, dpp_mov<0x141>(hi));
+    return kv4_meta(lo, hi);
 }
 
 }  // namespace vmlm
