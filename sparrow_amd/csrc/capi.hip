@@ -1043,7 +1043,7 @@ static int check_kv4(const vmlm_kv4_cache *c, Kv4View *v, bool device = true) {
                "kv4: head_dim %zu unsupported (32, 64, 128, 256)", c->head_dim);
     VMLM_GUARD(c->cap % 32 == 0 && c->cap <= DIM_MAX, "kv4: cap %zu is no multiple of 32 (or over 2^30)",
                c->cap);
-    VMLM_GUARD(c->batch <= 65535 && c->n_kv_heads <= 65535, "kv4: batch %zu or n_kv_heads %zu over 65535",
+    VMLM_GUARD(c->batch <= 65535 && c->n_kv_heads <= 32767, "kv4: batch %zu over 65535 or n_kv_heads %zu over 32767",
                c->batch, c->n_kv_heads);
     v->k = c->k;
     v->v = c->v;

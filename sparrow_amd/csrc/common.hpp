@@ -172,6 +172,22 @@ __device__ __forceinline__ uint32_t pack_i8x4(int a, int b, int c, int d) {
            ((uint32_t)(d & 0xff) << 24);
 }
 
+// Four dwords' bytes transposed: byte e of out[k] is byte k of v[e].
+__device__ __forceinline__ void transpose_bytes(const uint32_t (&v)[4], uint32_t (&out)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);  // v0.0 v1.0 v0.1 v1.1
+    const uint32_t b = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);  // v0.2 v1.2 v0.3 v1.3
+    const uint32_t d = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    out[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+// An integer as four signed bytes, b3 2^24 + b2 2^16 + b1 2^8 + b0 (|x| < 2^30).
+__device__ __forceinline__ uint32_t signed_bytes(int x) {
+    return ((uint32_t)x + 0x808080u) ^ 0x808080u;
+}
+
 // ------------------------------------------------------------------ math
 // Device ports of the reference's scalar math, operation for operation, so
 // that elementwise kernels are bitwise equal to the CPU kernels.

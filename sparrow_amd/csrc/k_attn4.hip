@@ -11,7 +11,7 @@
 //    16-byte load becomes two int8 operands (low and high nibbles) with 12
 //    operations. q, and for the output the weights, are 31-bit fixed-point numbers
 //    below their largest value, as four signed bytes: with 16 (u - 8) every product
-//    and sum is exact in int32, and four conversions and three FMAs put the terms
+//    and sum is exact in int32, and two conversions and an FMA put the terms
 //    together. 32-bit sums, then, at 8-bit rates. (Three bytes left the many small
 //    weights 2^-22 of the largest: 1.4e-6 off where f32 sums are 4e-7.)
 //  * Scores: a wave takes 128 positions. Lane (row kb, column n) loads the 32
@@ -19,7 +19,8 @@
 //    each kb = j and term t that is zero outside kb = j, so D's rows 4 kb + t at column n
 //    -- the registers of that very lane -- hold its own 32 channels' product, and
 //    the lane applies the scale and minimum that it loaded beside them. The groups of a
-//    position meet by lane swaps.
+//    position meet by lane swaps that leave each position's sum, and its exponential,
+//    to one lane.
 //  * Output: o[c] = sum_p (P_p scale_p,g) 16 (u - 8) / 16 + sum_p P_p (min + 8 scale)_p,g.
 //    The lanes that hold (p, g) write P_p scale_p,g as four bytes to LDS, from where
 //    they are the A operand (rows: head, term) against V's nibbles, which lie along
@@ -29,6 +30,7 @@
 // The new token's row is quantised by the wave that holds its position, put into
 // its registers and stored from there: no read back, no second launch.
 #include <algorithm>
+#include <cstdlib>
 
 #include "kv4.hpp"
 
@@ -36,12 +38,14 @@ namespace vmlm {
 namespace {
 
 typedef float f32x4a __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4m __attribute__((ext_vector_type(4), aligned(4)));
 typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
 
 // Positions of a wave at a time: what the registers hold.
 constexpr int attn4_ch(int hd) { return hd <= 128 ? 128 : 64; }
 constexpr int A4_MAX_GH = 4;   // query heads of a workgroup (rows of the A operand / 4)
 constexpr int A4_MAX_W = 8;    // waves of a workgroup
+constexpr int A4_MAX_SPLIT = 64;
 
 struct Attn4Params {
     Kv4View c;
@@ -93,16 +97,10 @@ __device__ __forceinline__ i32x4 nib_lo(u32x4 w) {
 __device__ __forceinline__ i32x4 nib_hi(u32x4 w) {
     return __builtin_bit_cast(i32x4, w & 0xf0f0f0f0u);
 }
-// An integer as four signed bytes, b3 2^24 + b2 2^16 + b1 2^8 + b0 (|x| < 2^30).
-__device__ __forceinline__ uint32_t digits(int x) {
-    return ((uint32_t)x + 0x808080u) ^ 0x808080u;
-}
-// and their sums, highest first, put together again
+// Sums of an integer's four bytes, highest first, put together again.
 __device__ __forceinline__ float undigits(const i32x4 &d) {
-    float f = (float)d[0];
-#pragma unroll
-    for (int t = 1; t < 4; ++t) f = __builtin_fmaf(f, 256.0f, (float)d[t]);
-    return f;
+    // each is below 2^22: two of them fit an int32
+    return __builtin_fmaf((float)(d[0] * 256 + d[1]), 65536.0f, (float)(d[2] * 256 + d[3]));
 }
 // The power of two that brings values up to mx below 2^30 (0 for none).
 __device__ __forceinline__ int fixed_exp(float mx) {
@@ -110,14 +108,11 @@ __device__ __forceinline__ int fixed_exp(float mx) {
 }
 
 // A lane's V codes of one channel: CH / 4 positions, and their product with the
-// weights' bytes. at(p): the byte of position p among those of a term.
+// weights' bytes.
 template <int CH>
 struct VCodes {  // 128: 32 positions, low nibbles (even ones), then high ones
     u32x4 w;
     __device__ __forceinline__ void load(const uint8_t *v) { w = *(const u32x4 *)v; }
-    static __device__ __forceinline__ int at(int p) {
-        return (p & 1) * 64 + (p >> 5) * 16 + (p & 31) / 2;
-    }
     __device__ __forceinline__ i32x4 product(const uint8_t *a) const {
         i32x4 d = {0, 0, 0, 0};
         d = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4 *)a, nib_lo(w), d, 0, 0, 0);
@@ -129,9 +124,6 @@ template <>
 struct VCodes<64> {  // 16 positions: both nibbles in one operand
     u32x2 w;
     __device__ __forceinline__ void load(const uint8_t *v) { w = *(const u32x2 *)v; }
-    static __device__ __forceinline__ int at(int p) {
-        return (p >> 4) * 16 + (p & 1) * 8 + (p & 15) / 2;
-    }
     __device__ __forceinline__ i32x4 product(const uint8_t *a) const {
         const u32x2 lo = (w << 4) & 0xf0f0f0f0u, hi = w & 0xf0f0f0f0u;
         const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
@@ -139,6 +131,133 @@ struct VCodes<64> {  // 16 positions: both nibbles in one operand
                                                      i32x4{0, 0, 0, 0}, 0, 0, 0);
     }
 };
+
+// Sums over the GR rows of lanes that hold a position's groups; of each GR steps a
+// row keeps its own (GR = 4: row kb of step 4 j + kb; 2: row g of step 2 j + g).
+template <int GR, int NS>
+__device__ __forceinline__ void sum_groups(const float (&x)[NS], float (&s)[NS / GR]) {
+    auto pair16 = [](float a, float b) {
+        const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false,
+                                                        false);
+        return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+    };
+    auto pair32 = [](float a, float b) {
+        const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false,
+                                                        false);
+        return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+    };
+#pragma unroll
+    for (int j = 0; j < NS / GR; ++j) {
+        if constexpr (GR == 4)
+            s[j] = pair16(pair32(x[4 * j], x[4 * j + 2]), pair32(x[4 * j + 1], x[4 * j + 3]));
+        else if constexpr (GR == 2)
+            s[j] = pair16(x[2 * j], x[2 * j + 1]);
+        else
+            s[j] = x[j];
+    }
+}
+// The way back: every step's value in all of its rows.
+template <int GR, int NO, int NS>
+__device__ __forceinline__ void to_groups(const float (&s)[NO], float (&x)[NS]) {
+#pragma unroll
+    for (int j = 0; j < NO; ++j) {
+        const uint32_t v = __float_as_uint(s[j]);
+        if constexpr (GR == 4) {
+            const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+            const auto a = __builtin_amdgcn_permlane16_swap(t[0], t[0], false, false);
+            const auto b = __builtin_amdgcn_permlane16_swap(t[1], t[1], false, false);
+            x[4 * j] = __uint_as_float(a[0]);
+            x[4 * j + 1] = __uint_as_float(a[1]);
+            x[4 * j + 2] = __uint_as_float(b[0]);
+            x[4 * j + 3] = __uint_as_float(b[1]);
+        } else if constexpr (GR == 2) {
+            const auto t = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+            x[2 * j] = __uint_as_float(t[0]);
+            x[2 * j + 1] = __uint_as_float(t[1]);
+        } else {
+            x[j] = s[j];
+        }
+    }
+}
+
+// 4 x 4 dwords transposed over the four rows of lanes: r[i] of row k becomes r[k] of row i.
+__device__ __forceinline__ void transpose_rows(uint32_t (&r)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const auto t = __builtin_amdgcn_permlane32_swap(r[i], r[i + 2], false, false);
+        r[i] = t[0];
+        r[i + 2] = t[1];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const auto t = __builtin_amdgcn_permlane16_swap(r[i], r[i + 1], false, false);
+        r[i] = t[0];
+        r[i + 1] = t[1];
+    }
+}
+
+// The meta dwords of the lane's positions: 16 bytes a load, its neighbours in the
+// other rows of lanes given theirs by a transpose. Past `pos`: of positions up to it.
+template <int HD, int NS, int GL>
+__device__ __forceinline__ void load_meta(const uint32_t *m, int p0, int n, int kb, int pos,
+                                          uint32_t (&out)[NS][GL]) {
+    constexpr int NG = HD / 32, PN = attn4_ch(HD) / 16;
+    if constexpr (NG == 1) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            out[i][0] = m[min(p0 + n * PN + 2 * ((kb >> 1) * NS + i) + (kb & 1), pos)];
+    } else {
+        // row kb loads what step kb (of each parity, HD = 128; of each half, 256) needs
+#pragma unroll
+        for (int s = 0; s < NS * GL / 4; ++s) {
+            size_t at;
+            if (NG == 2)
+                at = (size_t)min(p0 + n * PN + 2 * kb, pos & ~1) * 2;  // both parities' groups
+            else if (NG == 4)
+                at = (size_t)min(p0 + n * PN + 2 * kb + s, pos) * 4;
+            else
+                at = (size_t)min(p0 + n * PN + 2 * (kb & 1) + (kb >> 1), pos) * 8 + 4 * s;
+            const u32x4m v = *(const u32x4m *)(m + at);
+            uint32_t r[4] = {v[0], v[1], v[2], v[3]};
+            transpose_rows(r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (NG == 8)
+                    out[i][s] = r[i];
+                else
+                    out[s * 4 + i][0] = r[i];
+            }
+        }
+    }
+}
+
+// The bytes of the lane's weights into the terms (highest first, TB bytes each).
+template <int HD, int NS>
+__device__ __forceinline__ void store_terms(uint8_t *o, int n, int kb, const uint32_t (&d)[NS]) {
+    constexpr int TB = attn4_ch(HD);
+    if constexpr (HD == 64 || HD == 128) {  // four of one parity
+#pragma unroll
+        for (int s = 0; s < NS / 4; ++s) {
+            uint32_t t[4];
+            transpose_bytes({d[s * 4], d[s * 4 + 1], d[s * 4 + 2], d[s * 4 + 3]}, t);
+            uint8_t *at = o + (HD == 128 ? s : kb >> 1) * 64 + n * 4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) *(uint32_t *)(at + k * TB) = t[3 - k];
+        }
+    } else {  // two
+#pragma unroll
+        for (int s = 0; s < NS / 2; ++s) {
+            const uint32_t a = __builtin_amdgcn_perm(d[s * 2 + 1], d[s * 2], 0x07030602u);
+            const uint32_t b = __builtin_amdgcn_perm(d[s * 2 + 1], d[s * 2], 0x05010400u);
+            uint8_t *at = HD == 32 ? o + (kb & 1) * 64 + n * 4 + (kb >> 1) * 2
+                                   : o + (n >> 2) * 16 + s * 8 + (n & 3) * 2;
+            *(uint16_t *)at = (uint16_t)(a >> 16);
+            *(uint16_t *)(at + TB) = (uint16_t)a;
+            *(uint16_t *)(at + 2 * TB) = (uint16_t)(b >> 16);
+            *(uint16_t *)(at + 3 * TB) = (uint16_t)b;
+        }
+    }
+}
 
 struct Split {
     int c0, c1;  // chunks of this split
@@ -148,14 +267,15 @@ __device__ __forceinline__ Split split_of(int pos, int ch, int nsplit, int s) {
     return {s * per, min(nc, (s + 1) * per)};
 }
 
-// LDS of a workgroup: the query terms [head][term][group][32], their factors and group
+// LDS of a workgroup: the query terms [head][term][group][32], zeros, their factors and group
 // sums, the new token's codes and meta, the V offsets of each wave, and one region
 // that holds the waves' weight terms, then their results.
 template <int HD, int HEADS>
 struct Lds {
     static constexpr int NG = HD / 32;
     static constexpr int Q = 0;
-    static constexpr int F = Q + HEADS * 4 * HD;
+    static constexpr int Z = Q + HEADS * 4 * HD;  // as many zeros
+    static constexpr int F = Z + HEADS * 4 * HD;
     static constexpr int S = F + HEADS * 4;
     static constexpr int NK = (S + HEADS * NG * 4 + 15) / 16 * 16;
     static constexpr int NV = NK + HD / 2;
@@ -168,12 +288,13 @@ struct Lds {
 // GH query heads of one kv head.
 template <int HD, int GH>
 __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
-    constexpr int NG = HD / 32, GR = NG < 4 ? NG : 4, GL = NG / GR, PS = 64 / GR;
-    constexpr int CH = attn4_ch(HD), NS = CH / PS, CT = HD / 16, TB = CH;  // bytes of a term
+    constexpr int NG = HD / 32, GR = NG < 4 ? NG : 4, GL = NG / GR;
+    constexpr int CH = attn4_ch(HD), PN = CH / 16, NS = PN * GR / 4, CT = HD / 16;
+    constexpr int TB = CH;  // bytes of a term
     using M = Lds<HD, GH>;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, w = tid >> 6, W = blockDim.x >> 6, lane = tid & 63;
-    const int kb = lane >> 4, n = lane & 15, g0 = kb % GR, prow = kb / GR;
+    const int kb = lane >> 4, n = lane & 15, g0 = kb % GR;
     // the parts of a kv head lie 8 workgroups apart: on one XCD, whose L2 then gives
     // the later ones the cache
     const int x8 = blockIdx.x / 8, kvh = (x8 / p.parts) * 8 + (int)(blockIdx.x % 8);
@@ -192,6 +313,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
     const int last = pos / CH;
 
     // 1. the query heads as fixed-point terms
+    for (int i = tid; i < GH * HD / 4; i += W * 64) ((u32x4 *)(lds + M::Z))[i] = u32x4{0, 0, 0, 0};
     float *qf = (float *)(lds + M::F), *qs = (float *)(lds + M::S);
     for (int h = w; h < GH; h += W) {
         const float *q = p.q + b * p.ldq + ((size_t)kvh * p.G + h0 + min(h, G - 1)) * HD;
@@ -211,28 +333,41 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
 #pragma unroll
         for (int i = 0; i < CL; ++i) {
             const int c = i * 64 + lane;
-            float s = x[i];
+            const int f = bad ? 0 : (int)rintf(ldexpf(x[i], e));
+            float s = (float)f;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) s += __shfl_xor(s, o, 64);
             if (c >= HD) continue;
-            const uint32_t d = digits(bad ? 0 : (int)rintf(ldexpf(x[i], e)));
+            const uint32_t d = signed_bytes(f);
             uint8_t *t = lds + M::Q + ((h * 4) * NG + c / 32) * 32 + (c & 1) * 16 + c % 32 / 2;
 #pragma unroll
             for (int k = 0; k < 4; ++k) t[k * NG * 32] = (uint8_t)(d >> (24 - 8 * k));
-            if ((c & 31) == 0) qs[h * NG + c / 32] = s * p.scale2;
+            if ((c & 31) == 0) qs[h * NG + c / 32] = 16.0f * s;
         }
         if (lane == 0)
-            qf[h] = bad ? __builtin_nanf("") : ldexpf(p.scale2, -e - 4);
+            qf[h] = bad ? __builtin_nanf("") : ldexpf(p.scale2, 30 - e);  // 2^34 of it is in K's scales
     }
     __syncthreads();
 
     // the A operand of head h: row (j, t), nonzero where kb = j
-    const bool mine = n >> 2 == kb;
     const int term = n & 3;
+    const uint8_t *qt = lds + (n >> 2 == kb ? M::Q + (term * NG + g0) * 32 : M::Z);
     auto qa = [&](int h, int e, int par) {
-        const i32x4 a = *(const i32x4 *)(lds + M::Q + ((h * 4 + term) * NG + g0 + 4 * e) * 32 +
-                                         par * 16);
-        return mine ? a : i32x4{0, 0, 0, 0};
+        return *(const i32x4 *)(qt + (h * 4 * NG + 4 * e) * 32 + par * 16);
+    };
+    // Column n of the scores is PN neighbouring positions, and the lane's are NS of them,
+    // of one parity (or, with a group each for the four kb, first the even ones, then the
+    // odd ones): their bytes lie side by side in the weights' terms.
+    auto place = [&](int i) {
+        if (GR == 4) return n * PN + 2 * (i % (PN / 2)) + i / (PN / 2);
+        if (GR == 2) return n * PN + 2 * i + (kb >> 1);
+        return n * PN + 2 * ((kb >> 1) * NS + i) + (kb & 1);
+    };
+    // the positions whose score is summed here (sum_groups)
+    auto own_place = [&](int j) {
+        if (GR == 4) return n * PN + 2 * ((j * 4 + kb) % (PN / 2)) + (j * 4 + kb) / (PN / 2);
+        if (GR == 2) return n * PN + 2 * (j * 2 + (kb & 1)) + (kb >> 1);
+        return place(j);
     };
 
     float m[GH], l[GH], off[GH][GL], O[CT];
@@ -255,14 +390,13 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
         uint32_t km[NS][GL], vm[NS][GL];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const size_t row = row0 + min(p0 + i * PS + prow * 16 + n, pos);
+            const size_t row = row0 + min(p0 + place(i), pos);
 #pragma unroll
-            for (int e = 0; e < GL; ++e) {
+            for (int e = 0; e < GL; ++e)
                 kc[i][e] = *(const u32x4 *)(p.c.k + row * (HD / 2) + (g0 + 4 * e) * 16);
-                km[i][e] = p.c.km[row * NG + g0 + 4 * e];
-                vm[i][e] = p.c.vm[row * NG + g0 + 4 * e];
-            }
         }
+        load_meta<HD>(p.c.km + row0 * NG, p0, n, kb, pos, km);
+        load_meta<HD>(p.c.vm + row0 * NG, p0, n, kb, pos, vm);
         // lane (kb, n): the kb-th quarter of the positions, channel 16 ct + n
         const int vblk = min((p0 + kb * (CH / 4)) / KV4_BLOCK, pos / KV4_BLOCK);
         uint8_t *vb = p.c.v + ((head * (p.c.cap / KV4_BLOCK) + vblk) * HD + n) * 16 +
@@ -293,7 +427,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                if (p0 + i * PS + prow * 16 + n != pos) continue;
+                if (p0 + place(i) != pos) continue;
 #pragma unroll
                 for (int e = 0; e < GL; ++e) {
                     const int g = g0 + 4 * e;
@@ -322,66 +456,73 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             }
         }
 
-        // 4. V's scales (none past the last position) and the fixed point of each group
-        float vs[NS][GL], vo[NS][GL];
+        // 4. scales and middles, V's (none past the last position) in its group's fixed point
+        float ks[NS][GL], ko[NS][GL], vs[NS][GL], vo[NS][GL];
         int ev[GL];
 #pragma unroll
         for (int e = 0; e < GL; ++e) {
             float mx = 0.0f;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                const bool in = p0 + i * PS + prow * 16 + n <= pos;
+                const bool in = p0 + place(i) <= pos;
+                ks[i][e] = kv4_scale(km[i][e]) * 0x1p-34f;
+                ko[i][e] = __builtin_fmaf(8.0f, ks[i][e], kv4_min(km[i][e]) * 0x1p-34f);
                 vs[i][e] = in ? kv4_scale(vm[i][e]) : 0.0f;
                 vo[i][e] = in ? __builtin_fmaf(8.0f, vs[i][e], kv4_min(vm[i][e])) : 0.0f;
                 mx = fmaxf(mx, vs[i][e]);
             }
             ev[e] = fixed_exp(rows_red<GR>(row16_max(mx), max_f));
+#pragma unroll
+            for (int i = 0; i < NS; ++i) vs[i][e] = ldexpf(vs[i][e], ev[e]);
         }
 
         float corr[GH];
 #pragma unroll
         for (int h = 0; h < GH; ++h) {
-            // 5. scores of the lane's positions, in powers of two
-            float s[NS], mx = -__builtin_inff();
-            const float f = qf[h];
+            // 5. scores in powers of two, each position's in one of the lanes that hold it
+            float part_s[NS], s[NS / GR], mx = m[h];
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                s[i] = 0.0f;
+                part_s[i] = 0.0f;
 #pragma unroll
                 for (int e = 0; e < GL; ++e) {
                     i32x4 d = {0, 0, 0, 0};
                     d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 0), nib_lo(kc[i][e]), d, 0, 0, 0);
                     d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 1), nib_hi(kc[i][e]), d, 0, 0, 0);
-                    const float sc = kv4_scale(km[i][e]);
-                    const float mid = __builtin_fmaf(8.0f, sc, kv4_min(km[i][e]));
-                    s[i] = __builtin_fmaf(undigits(d) * f, sc,
-                                          __builtin_fmaf(mid, qs[h * NG + g0 + 4 * e], s[i]));
+                    part_s[i] = __builtin_fmaf(ko[i][e], qs[h * NG + g0 + 4 * e], part_s[i]);
+                    part_s[i] = __builtin_fmaf(undigits(d), ks[i][e], part_s[i]);
                 }
-                if (GR >= 2) s[i] = swap16(s[i], add_f);
-                if (GR == 4) s[i] = swap32(s[i], add_f);
-                if (p0 + i * PS + prow * 16 + n > pos) s[i] = -__builtin_inff();
-                mx = fmaxf(mx, s[i]);
+            }
+            sum_groups<GR>(part_s, s);
+#pragma unroll
+            for (int j = 0; j < NS / GR; ++j) {
+                s[j] = p0 + own_place(j) <= pos ? s[j] * qf[h] : -__builtin_inff();
+                mx = fmaxf(mx, s[j]);
             }
             // 6. the running maximum, the weights and their bytes
-            mx = fmaxf(m[h], rows_red<GR>(row16_max(mx), max_f));
+            mx = swap32(swap16(row16_max(mx), max_f), max_f);
             corr[h] = __builtin_amdgcn_exp2f(m[h] - mx);
             m[h] = mx;
             l[h] *= corr[h];
 #pragma unroll
-            for (int e = 0; e < GL; ++e) off[h][e] *= corr[h];
+            for (int j = 0; j < NS / GR; ++j) {
+                s[j] = __builtin_amdgcn_exp2f(s[j] - mx);
+                l[h] += s[j];
+            }
+            float P[NS];
+            to_groups<GR>(s, P);
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                const float P = __builtin_amdgcn_exp2f(s[i] - mx);
-                l[h] += P;
-                const int at = i * PS + prow * 16 + n;  // position in the chunk
+            for (int e = 0; e < GL; ++e) {
+                off[h][e] *= corr[h];
+                uint32_t d[NS];
 #pragma unroll
-                for (int e = 0; e < GL; ++e) {
-                    off[h][e] = __builtin_fmaf(P, vo[i][e], off[h][e]);
-                    const uint32_t d = digits((int)rintf(ldexpf(P * vs[i][e], ev[e])));
-                    uint8_t *o = pb + ((h * NG + g0 + 4 * e) * 4) * TB + VCodes<CH>::at(at);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) o[k * TB] = (uint8_t)(d >> (24 - 8 * k));
+                for (int i = 0; i < NS; ++i) {
+                    off[h][e] = __builtin_fmaf(P[i], vo[i][e], off[h][e]);
+                    // signed_bytes of the product (below 2^30), the sum rounded to an integer
+                    // (or to f32's 24 bits)
+                    d[i] = (uint32_t)__builtin_fmaf(P[i], vs[i][e], (float)0x808080) ^ 0x808080u;
                 }
+                store_terms<HD>(pb + (h * NG + g0 + 4 * e) * 4 * TB, n, kb, d);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -404,7 +545,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
     float *offl = (float *)(lds + M::OFF) + w * GH * NG;
 #pragma unroll
     for (int h = 0; h < GH; ++h) {
-        l[h] = rows_red<GR>(row16_sum(l[h]), add_f);
+        l[h] = rows_red<1>(row16_sum(l[h]), add_f);
 #pragma unroll
         for (int e = 0; e < GL; ++e) {
             const float o = rows_red<GR>(row16_sum(off[h][e]), add_f);
@@ -450,23 +591,37 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
     }
 }
 
-// The splits of a head, in order.
+// The splits of a head, in order: the lanes of the first wave take a split's maximum
+// and sum each, the threads four of its partial rows at a time.
 __global__ __launch_bounds__(KV4_MAX_HD) void attn4_merge_kernel(Attn4Params p) {
-    const int h = blockIdx.x, b = blockIdx.y, c = threadIdx.x, hd = p.c.hd;
+    __shared__ float weight[A4_MAX_SPLIT], sum;
+    const int h = blockIdx.x, b = blockIdx.y, c = threadIdx.x, hd = p.c.hd, ld = hd + 4;
     const int pos = p.pos[b];
-    if (pos < 0 || pos >= p.c.cap || c >= hd) return;
-    const float *pw = p.work + ((size_t)b * p.H + h) * p.nsplit * (hd + 4);
-    int live = 0;
-    while (live < p.nsplit && split_of(pos, p.ch, p.nsplit, live).c0 < split_of(pos, p.ch, p.nsplit, live).c1)
-        ++live;
-    float mx = -__builtin_inff(), L = 0.0f, o = 0.0f;
-    for (int s = 0; s < live; ++s) mx = fmaxf(mx, pw[s * (hd + 4) + hd]);
-    for (int s = 0; s < live; ++s) {
-        const float f = __builtin_amdgcn_exp2f(pw[s * (hd + 4) + hd] - mx);
-        L = __builtin_fmaf(f, pw[s * (hd + 4) + hd + 1], L);
-        o = __builtin_fmaf(f, pw[s * (hd + 4) + c], o);
+    if (pos < 0 || pos >= p.c.cap) return;
+    const float *pw = p.work + ((size_t)b * p.H + h) * p.nsplit * ld;
+    const int nc = pos / p.ch + 1, per = (nc + p.nsplit - 1) / p.nsplit;
+    const int live = (nc + per - 1) / per;  // the splits that have a chunk
+    if (c < 64) {
+        const int s = min(c, live - 1);
+        const float m = pw[s * ld + hd], l = pw[s * ld + hd + 1];
+        const float mx = wave_max(m), e = __builtin_amdgcn_exp2f(m - mx);
+        const float f = c < live ? e : 0.0f;
+        weight[c] = f;
+        const float t = wave_sum(c < live ? f * l : 0.0f);
+        if (c == 0) sum = t;
     }
-    p.out[b * p.ldo + (size_t)h * hd + c] = o / L;
+    __syncthreads();
+    if (c >= hd) return;
+    float o = 0.0f;
+    for (int s = 0; s < live; s += 4) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = pw[min(s + i, live - 1) * ld + c];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o = s + i < live ? __builtin_fmaf(weight[s + i], x[i], o) : o;
+    }
+    p.out[b * p.ldo + (size_t)h * hd + c] = o / sum;
 }
 
 struct Attn4Plan {
@@ -478,8 +633,8 @@ Attn4Plan attn4_plan(const Kv4View &c, int H) {
     pl.parts = (H / c.Hkv + A4_MAX_GH - 1) / A4_MAX_GH;
     const long long pairs = (long long)c.B * c.Hkv * pl.parts;
     pl.W = std::min(A4_MAX_W, chunks);
-    const long long want = 2048 / (pairs * pl.W);
-    pl.nsplit = (int)std::max(1LL, std::min(want, (long long)chunks / pl.W));
+    const long long want = (getenv("A4W") ? atoi(getenv("A4W")) : 3072) / (pairs * pl.W);
+    pl.nsplit = (int)std::max(1LL, std::min({want, (long long)chunks / pl.W, (long long)A4_MAX_SPLIT}));
     return pl;
 }
 

@@ -8,7 +8,7 @@
 // of a row becomes two int8 operands (even and odd k) with 12 operations and no
 // conversion. The activations of a run of 128 k are 31-bit fixed-point numbers
 // below the row's largest value there, as four signed bytes, so every product and
-// sum over a group is exact in int32 and four conversions, three FMAs and one scale make
+// sum over a group is exact in int32 and two conversions, an FMA and two products make
 // an f32 of it: errors are those of K/128 f32 additions.
 //
 // D = A . B^T per v_mfma_i32_16x16x64_i8, B the nibbles of 16 weight rows, the 16
@@ -134,18 +134,6 @@ __device__ __forceinline__ size_t plane_at(int runs, int m, int r) {
     return ((size_t)(m >> 2) * runs + r) * 2048 + (m & 3) * 64;
 }
 
-// Four integers' bytes transposed: byte i of out[t] is digit t (highest first) of v[i].
-__device__ __forceinline__ void digit_planes(const uint32_t (&v)[4], uint32_t (&out)[4]) {
-    const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);  // v0.0 v1.0 v0.1 v1.1
-    const uint32_t b = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
-    const uint32_t c = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);  // v0.2 v1.2 v0.3 v1.3
-    const uint32_t d = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
-    out[3] = __builtin_amdgcn_perm(b, a, 0x05040100u);
-    out[2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-    out[1] = __builtin_amdgcn_perm(d, c, 0x05040100u);
-    out[0] = __builtin_amdgcn_perm(d, c, 0x07060302u);
-}
-
 __device__ __forceinline__ float row16_max(float v) {
     v = fmaxf(v, dpp_mov<0xB1>(v));
     v = fmaxf(v, dpp_mov<0x4E>(v));
@@ -175,9 +163,9 @@ __device__ __forceinline__ float split8(const float *row, int k, int K, uint32_t
     uint32_t d[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-        d[e] = ((uint32_t)(ok ? (int)rintf(ldexpf(x[e], e2)) : 0) + 0x808080u) ^ 0x808080u;
-    digit_planes({d[0], d[2], d[4], d[6]}, ev);
-    digit_planes({d[1], d[3], d[5], d[7]}, od);
+        d[e] = signed_bytes(ok ? (int)rintf(ldexpf(x[e], e2)) : 0);
+    transpose_bytes({d[0], d[2], d[4], d[6]}, ev);
+    transpose_bytes({d[1], d[3], d[5], d[7]}, od);
     // 2^-4 for the nibble's place in its byte
     return ok ? ldexpf(1.0f, -e2 - 4) : __builtin_nanf("");
 }
@@ -194,8 +182,8 @@ __global__ __launch_bounds__(256) void int4_planes_kernel(const float *A, int M,
     uint8_t *o = planes + plane_at(runs, m, r) + (l >> 2) * 256 + (l & 3) * 4;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        *(uint32_t *)(o + t * 16) = ev[t];
-        *(uint32_t *)(o + 1024 + t * 16) = od[t];
+        *(uint32_t *)(o + t * 16) = ev[3 - t];
+        *(uint32_t *)(o + 1024 + t * 16) = od[3 - t];
     }
     if (l == 0) fac[(size_t)r * rows + m] = f;
 }
@@ -331,8 +319,8 @@ __global__ __launch_bounds__(TN == 4 ? 256 : 1024) void gemm_int4_kernel(Int4Par
                     uint8_t *o = buf + x % (CR * ROWS) * 512 + n * 4;
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
-                        *(uint32_t *)(o + t * 128) = ev[t];
-                        *(uint32_t *)(o + t * 128 + 64) = od[t];
+                        *(uint32_t *)(o + t * 128) = ev[3 - t];
+                        *(uint32_t *)(o + t * 128 + 64) = od[3 - t];
                     }
                     if (n == 0) fac[rr * ROWS + mr] = f;
                 }

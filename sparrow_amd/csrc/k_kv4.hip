@@ -39,39 +39,29 @@ __device__ __forceinline__ bool kv4_rows(const Kv4Params &p, int b, int blk, int
     return *t0 < *t1;
 }
 
-// Four bytes of four dwords transposed: byte e of out[k] is byte k of v[e].
-__device__ __forceinline__ void transpose_bytes(const uint32_t (&v)[4], uint32_t (&out)[4]) {
-    const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);
-    const uint32_t b = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
-    const uint32_t c = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
-    const uint32_t d = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
-    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
-    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-    out[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
-    out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
-}
-
-// One workgroup per (32-position block, head, sequence). Eight lanes quantise 32
+// One workgroup per (32-position block, head, K or V, sequence). Eight lanes quantise 32
 // channels of a position; V's codes cross LDS to be packed along positions, and a
 // block's bytes that hold other positions keep their nibbles. Bound by the f32 rows;
-// all of a thread's loads are issued before the first is used.
+// all of a thread's loads are issued before the first is used. (K and V in one
+// workgroup: 7.0 us instead of 6.1 for 3 x 333 rows of 8 heads of 128.)
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Params p) {
     constexpr int NG = HD / 32, LD = HD + 4;  // bytes of a position in LDS
     __shared__ __align__(4) uint8_t codes[KV4_BLOCK * LD];
-    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+    const int b = blockIdx.z, h = blockIdx.y >> 1, isv = blockIdx.y & 1, tid = threadIdx.x;
     int first, pos0, t0, t1;
     if (!kv4_rows(p, b, blockIdx.x, &first, &pos0, &t0, &t1)) return;
     const size_t head = (size_t)b * p.c.Hkv + h;
+    const float *src = isv ? p.v : p.k;
+    const size_t ld = isv ? p.ldv : p.ldk;
+    uint32_t *meta = isv ? p.c.vm : p.c.km;
     const int l = tid & 7;
-    f32x4a rk[NG], rv[NG];
+    f32x4a row[NG];
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
         const int task = (tid >> 3) + i * 32, o = task / NG, g = task % NG;
         const int t = min(max(first + o - pos0, t0), t1 - 1);
-        const size_t row = (size_t)b * p.S + t, at = (size_t)h * HD + g * 32 + 4 * l;
-        rk[i] = *(const f32x4a *)(p.k + row * p.ldk + at);
-        rv[i] = *(const f32x4a *)(p.v + row * p.ldv + at);
+        row[i] = *(const f32x4a *)(src + ((size_t)b * p.S + t) * ld + (size_t)h * HD + g * 32 + 4 * l);
     }
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
@@ -79,20 +69,18 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Params p) {
         const int t = first + o - pos0, ch = g * 32 + 4 * l;
         if (t < t0 || t >= t1) continue;  // the same for the eight lanes
         const size_t pos = head * p.c.cap + first + o;
-        const float k[4] = {rk[i][0], rk[i][1], rk[i][2], rk[i][3]};
-        const float v[4] = {rv[i][0], rv[i][1], rv[i][2], rv[i][3]};
-        const uint32_t mk = kv4_meta8(k), mv = kv4_meta8(v);
+        const float x[4] = {row[i][0], row[i][1], row[i][2], row[i][3]};
+        const uint32_t m = kv4_meta8(x);
         uint32_t c[4];
-        kv4_codes(k, mk, c);
-        *(uint16_t *)(p.c.k + pos * (HD / 2) + ch / 2) =
-            (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
-        kv4_codes(v, mv, c);
-        *(uint32_t *)(codes + o * LD + ch) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-        if (l == 0) {
-            p.c.km[pos * NG + g] = mk;
-            p.c.vm[pos * NG + g] = mv;
-        }
+        kv4_codes(x, m, c);
+        if (isv)
+            *(uint32_t *)(codes + o * LD + ch) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+        else
+            *(uint16_t *)(p.c.k + pos * (HD / 2) + ch / 2) =
+                (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
+        if (l == 0) meta[pos * NG + g] = m;
     }
+    if (!isv) return;
     __syncthreads();
     const int o0 = pos0 + t0 - first, o1 = pos0 + t1 - first;  // offsets that are new
     uint32_t *vb = (uint32_t *)(p.c.v + (head * (p.c.cap / KV4_BLOCK) + first / KV4_BLOCK) *
@@ -123,41 +111,41 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Params p) {
 // The block's codes and meta through LDS, then four channels of a position a thread.
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Params p) {
-    constexpr int NG = HD / 32, KD = HD * 4, LV = 20;  // dwords of codes; LDS bytes of a V channel
-    __shared__ uint32_t kc[KD], km[KV4_BLOCK * NG], vm[KV4_BLOCK * NG];
-    __shared__ __align__(4) uint8_t vc[HD * LV];
-    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+    constexpr int NG = HD / 32, LV = 20;  // LDS bytes of a V channel
+    __shared__ __align__(4) uint8_t codes[HD * LV];
+    __shared__ uint32_t meta[KV4_BLOCK * NG];
+    const int b = blockIdx.z, h = blockIdx.y >> 1, isv = blockIdx.y & 1, tid = threadIdx.x;
     int first, pos0, t0, t1;
     if (!kv4_rows(p, b, blockIdx.x, &first, &pos0, &t0, &t1)) return;
     const size_t head = (size_t)b * p.c.Hkv + h, pos = head * p.c.cap + first;
-    const uint32_t *kb = (const uint32_t *)(p.c.k + pos * (HD / 2));
-    const uint32_t *vb = (const uint32_t *)(p.c.v + pos * (HD / 2));  // a block is as long
+    // a V block is as long as its positions' K rows
+    const uint32_t *cb = (const uint32_t *)((isv ? p.c.v : p.c.k) + pos * (HD / 2));
+    const uint32_t *mb = (isv ? p.c.vm : p.c.km) + pos * NG;
 #pragma unroll
-    for (int i = tid; i < KD; i += 256) {
-        kc[i] = kb[i];
-        *(uint32_t *)(vc + i / 4 * LV + i % 4 * 4) = vb[i];
-    }
-    if (tid < KV4_BLOCK * NG) {
-        km[tid] = p.c.km[pos * NG + tid];
-        vm[tid] = p.c.vm[pos * NG + tid];
-    }
+    for (int i = tid; i < HD * 4; i += 256)
+        *(uint32_t *)(codes + (isv ? i / 4 * LV + i % 4 * 4 : i * 4)) = cb[i];
+    if (tid < KV4_BLOCK * NG) meta[tid] = mb[tid];
     __syncthreads();
+    float *dst = isv ? p.vo : p.ko;
+    const size_t ld = isv ? p.ldv : p.ldk;
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
         const int x = tid + i * 256, o = x / (HD / 4), ch = x % (HD / 4) * 4, t = first + o - pos0;
         if (t < t0 || t >= t1) continue;
-        const size_t row = (size_t)b * p.S + t;
-        const uint32_t mk = km[o * NG + ch / 32], mv = vm[o * NG + ch / 32];
-        const uint32_t c = ((const uint16_t *)kc)[x];
-        f32x4a k, v;
+        const uint32_t m = meta[o * NG + ch / 32];
+        uint32_t c;
+        if (isv) {
+            c = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            k[e] = kv4_value(c >> (4 * e), kv4_min(mk), kv4_scale(mk));
-            v[e] = kv4_value((uint32_t)vc[(ch + e) * LV + o / 2] >> (4 * (o & 1)), kv4_min(mv),
-                             kv4_scale(mv));
+            for (int e = 0; e < 4; ++e)
+                c |= ((uint32_t)codes[(ch + e) * LV + o / 2] >> (4 * (o & 1)) & 15u) << (4 * e);
+        } else {
+            c = ((const uint16_t *)codes)[x];
         }
-        *(f32x4a *)(p.ko + row * p.ldk + (size_t)h * HD + ch) = k;
-        *(f32x4a *)(p.vo + row * p.ldv + (size_t)h * HD + ch) = v;
+        f32x4a y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = kv4_value(c >> (4 * e), kv4_min(m), kv4_scale(m));
+        *(f32x4a *)(dst + ((size_t)b * p.S + t) * ld + (size_t)h * HD + ch) = y;
     }
 }
 
@@ -172,7 +160,7 @@ void launch_hd(const Kv4Params &p, dim3 grid, hipStream_t st) {
 dim3 kv4_grid(const Kv4View &c, int S) {
     // the blocks that S rows can touch, from any position of the first
     const size_t blocks = std::min((size_t)c.cap / KV4_BLOCK, ((size_t)S + 30) / KV4_BLOCK + 1);
-    return dim3((unsigned)blocks, (unsigned)c.Hkv, (unsigned)c.B);
+    return dim3((unsigned)blocks, 2 * (unsigned)c.Hkv, (unsigned)c.B);
 }
 
 int launch_kv4(const Kv4Params &p, hipStream_t st) {
