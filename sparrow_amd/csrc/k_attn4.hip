@@ -30,7 +30,6 @@
 // The new token's row is quantised by the wave that holds its position, put into
 // its registers and stored from there: no read back, no second launch.
 #include <algorithm>
-#include <cstdlib>
 
 #include "kv4.hpp"
 
@@ -45,7 +44,7 @@ typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
 constexpr int attn4_ch(int hd) { return hd <= 128 ? 128 : 64; }
 constexpr int A4_MAX_GH = 4;   // query heads of a workgroup (rows of the A operand / 4)
 constexpr int A4_MAX_W = 8;    // waves of a workgroup
-constexpr int A4_MAX_SPLIT = 64;
+constexpr int A4_MAX_SPLIT = 64;  // shares of a sequence
 
 struct Attn4Params {
     Kv4View c;
@@ -53,7 +52,8 @@ struct Attn4Params {
     size_t ldq, ldkv, ldo;
     const int32_t *pos;
     float *out, *work;
-    int H, G, nsplit, ch;
+    int H, G, ch, W;
+    int shares;  // of a split launch (0: one workgroup a pair of head and sequence)
     int parts;  // workgroups that share a kv head's queries
     float scale2;  // score scale * log2(e)
     int *guard;
@@ -197,39 +197,50 @@ __device__ __forceinline__ void transpose_rows(uint32_t (&r)[4]) {
 }
 
 // The meta dwords of the lane's positions: 16 bytes a load, its neighbours in the
-// other rows of lanes given theirs by a transpose. Past `pos`: of positions up to it.
+// other rows of lanes given theirs by a transpose when they are used (it waits for
+// the loads). Past `pos`: of positions up to it.
 template <int HD, int NS, int GL>
-__device__ __forceinline__ void load_meta(const uint32_t *m, int p0, int n, int kb, int pos,
-                                          uint32_t (&out)[NS][GL]) {
-    constexpr int NG = HD / 32, PN = attn4_ch(HD) / 16;
-    if constexpr (NG == 1) {
+struct Meta {
+    static constexpr int NG = HD / 32, PN = attn4_ch(HD) / 16, L = NG == 1 ? NS : NS * GL / 4;
+    uint32_t raw[L][NG == 1 ? 1 : 4];
+    __device__ __forceinline__ void load(const uint32_t *m, int p0, int n, int kb, int pos) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
-            out[i][0] = m[min(p0 + n * PN + 2 * ((kb >> 1) * NS + i) + (kb & 1), pos)];
-    } else {
-        // row kb loads what step kb (of each parity, HD = 128; of each half, 256) needs
-#pragma unroll
-        for (int s = 0; s < NS * GL / 4; ++s) {
-            size_t at;
-            if (NG == 2)
-                at = (size_t)min(p0 + n * PN + 2 * kb, pos & ~1) * 2;  // both parities' groups
-            else if (NG == 4)
-                at = (size_t)min(p0 + n * PN + 2 * kb + s, pos) * 4;
-            else
-                at = (size_t)min(p0 + n * PN + 2 * (kb & 1) + (kb >> 1), pos) * 8 + 4 * s;
-            const u32x4m v = *(const u32x4m *)(m + at);
-            uint32_t r[4] = {v[0], v[1], v[2], v[3]};
-            transpose_rows(r);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (NG == 8)
-                    out[i][s] = r[i];
+        for (int s = 0; s < L; ++s) {
+            if constexpr (NG == 1) {
+                raw[s][0] = m[min(p0 + n * PN + 2 * ((kb >> 1) * NS + s) + (kb & 1), pos)];
+            } else {
+                // row kb loads what step kb (of each parity, HD = 128; of each half, 256) needs
+                size_t at;
+                if (NG == 2)
+                    at = (size_t)min(p0 + n * PN + 2 * kb, pos & ~1) * 2;  // both parities' groups
+                else if (NG == 4)
+                    at = (size_t)min(p0 + n * PN + 2 * kb + s, pos) * 4;
                 else
-                    out[s * 4 + i][0] = r[i];
+                    at = (size_t)min(p0 + n * PN + 2 * (kb & 1) + (kb >> 1), pos) * 8 + 4 * s;
+                const u32x4m v = *(const u32x4m *)(m + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[s][i] = v[i];
             }
         }
     }
-}
+    __device__ __forceinline__ void spread(uint32_t (&out)[NS][GL]) {
+#pragma unroll
+        for (int s = 0; s < L; ++s) {
+            if constexpr (NG == 1) {
+                out[s][0] = raw[s][0];
+            } else {
+                transpose_rows(raw[s]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (NG == 8)
+                        out[i][s] = raw[s][i];
+                    else
+                        out[s * 4 + i][0] = raw[s][i];
+                }
+            }
+        }
+    }
+};
 
 // The bytes of the lane's weights into the terms (highest first, TB bytes each).
 template <int HD, int NS>
@@ -259,12 +270,59 @@ __device__ __forceinline__ void store_terms(uint8_t *o, int n, int kb, const uin
     }
 }
 
-struct Split {
-    int c0, c1;  // chunks of this split
+// Shares of a split launch. The positions are known on the device alone and differ
+// between sequences: every workgroup works out from all of them how many chunks a share
+// takes so that about `shares` of them cover all sequences, and which one is its own.
+// A sequence has one share for every `each` chunks, at most A4_MAX_SPLIT.
+struct Shares {
+    int each;
+    int b, pos, count, first;  // a sequence, its shares and the number of the first
 };
-__device__ __forceinline__ Split split_of(int pos, int ch, int nsplit, int s) {
-    const int nc = pos / ch + 1, per = (nc + nsplit - 1) / nsplit;
-    return {s * per, min(nc, (s + 1) * per)};
+__device__ __forceinline__ int chunks_of(const Attn4Params &p, int b, int *pos) {
+    *pos = b < p.c.B ? p.pos[b] : -1;
+    if (*pos >= p.c.cap) {
+        atomicOr(p.guard, 1);
+        return 0;
+    }
+    return *pos < 0 ? 0 : *pos / p.ch + 1;
+}
+// The sequence of share number `at`, or (want_b >= 0) that sequence; count 0: there is none.
+// Called by whole waves.
+__device__ __forceinline__ Shares shares_of(const Attn4Params &p, int at, int want_b) {
+    const int lane = threadIdx.x & 63;
+    int pos;
+    float all = 0.0f, most = 0.0f;
+    for (int b0 = 0; b0 < p.c.B; b0 += 64) {
+        const float n = (float)chunks_of(p, b0 + lane, &pos);
+        all += wave_sum(n);
+        most = fmaxf(most, wave_max(n));
+    }
+    Shares r;
+    const int want = max((int)ceilf(all / (float)p.shares), (int)ceilf(most / A4_MAX_SPLIT));
+    r.each = __builtin_amdgcn_readfirstlane(max(1, (want + p.W - 1) / p.W)) * p.W;
+    r.count = 0;
+    int before = 0;
+    for (int b0 = 0; b0 < p.c.B; b0 += 64) {
+        const int n = chunks_of(p, b0 + lane, &pos), mine = (n + r.each - 1) / r.each;
+        int to = mine;  // shares up to this lane's sequence
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int v = __shfl_up(to, o, 64);
+            to += lane >= o ? v : 0;
+        }
+        const unsigned long long hit =
+            __ballot(want_b >= 0 ? b0 + lane == want_b : before + to > at);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            r.b = b0 + l;
+            r.pos = __builtin_amdgcn_readlane(pos, l);
+            r.count = __builtin_amdgcn_readlane(mine, l);
+            r.first = before + __builtin_amdgcn_readlane(to, l) - r.count;
+            return r;
+        }
+        before += __builtin_amdgcn_readlane(to, 63);
+    }
+    return r;
 }
 
 // LDS of a workgroup: the query terms [head][term][group][32], zeros, their factors and group
@@ -295,24 +353,61 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, w = tid >> 6, W = blockDim.x >> 6, lane = tid & 63;
     const int kb = lane >> 4, n = lane & 15, g0 = kb % GR;
-    // the parts of a kv head lie 8 workgroups apart: on one XCD, whose L2 then gives
-    // the later ones the cache
-    const int x8 = blockIdx.x / 8, kvh = (x8 / p.parts) * 8 + (int)(blockIdx.x % 8);
-    const int part = x8 % p.parts, b = blockIdx.z;
+    // The parts of a kv head lie 8 workgroups apart: on one XCD, whose L2 then gives the
+    // later ones the cache. (Single ones go round the XCDs: 36 heads bound to them are
+    // five on four of them.)
+    int kvh = blockIdx.x, part = 0;
+    if (p.parts > 1) {
+        const int x8 = blockIdx.x / 8;
+        kvh = x8 / p.parts * 8 + (int)(blockIdx.x % 8);
+        part = x8 % p.parts;
+    }
     if (kvh >= p.c.Hkv) return;
     const int h0 = part * GH, G = min(GH, p.G - h0);  // of the kv head's queries
-    const int pos = p.pos[b];
-    if (pos < 0) return;  // an idle sequence
-    if (pos >= p.c.cap) {
-        if (tid == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(p.guard, 1);
-        return;
+    int b = blockIdx.y, pos = 0, c0 = 0, c1 = 0, count = 1;
+    if (p.shares) {
+        const Shares sh = shares_of(p, blockIdx.y, -1);
+        if (sh.count == 0) return;
+        const int n = sh.pos / CH + 1, s = (int)blockIdx.y - sh.first;
+        b = sh.b;
+        pos = sh.pos;
+        count = sh.count;
+        c0 = (int)((long long)s * n / count);
+        c1 = (int)((long long)(s + 1) * n / count);
+    } else {
+        pos = p.pos[b];
+        if (pos < 0) return;  // an idle sequence
+        if (pos >= p.c.cap) {
+            if (tid == 0 && blockIdx.x == 0) atomicOr(p.guard, 1);
+            return;
+        }
+        c1 = pos / CH + 1;
     }
-    const Split sp = split_of(pos, CH, p.nsplit, blockIdx.y);
-    if (sp.c0 >= sp.c1) return;
     const size_t head = (size_t)b * p.c.Hkv + kvh, row0 = head * p.c.cap;
     const int last = pos / CH;
 
-    // 1. the query heads as fixed-point terms
+    // 1. the new token's codes, by the wave that will put them in place; the query heads as
+    // fixed-point terms
+    if (p.k_new && last < c1 && (last - c0) % W == w) {
+        uint32_t *nm = (uint32_t *)(lds + M::NM);
+        const int c4 = min(lane, HD / 4 - 1) * 4;
+        const size_t at = b * p.ldkv + (size_t)kvh * HD + c4;
+        const f32x4a rk = *(const f32x4a *)(p.k_new + at), rv = *(const f32x4a *)(p.v_new + at);
+        const float k[4] = {rk[0], rk[1], rk[2], rk[3]}, v[4] = {rv[0], rv[1], rv[2], rv[3]};
+        const uint32_t mk = kv4_meta8(k), mv = kv4_meta8(v);
+        uint32_t ck[4], cv[4];
+        kv4_codes(k, mk, ck);
+        kv4_codes(v, mv, cv);
+        if (lane < HD / 4) {
+            *(uint16_t *)(lds + M::NK + c4 / 2) =
+                (uint16_t)(ck[0] | ck[1] << 4 | ck[2] << 8 | ck[3] << 12);
+            *(uint32_t *)(lds + M::NV + c4) = cv[0] | cv[1] << 8 | cv[2] << 16 | cv[3] << 24;
+            if ((lane & 7) == 0) {
+                nm[lane / 8] = mk;
+                nm[NG + lane / 8] = mv;
+            }
+        }
+    }
     for (int i = tid; i < GH * HD / 4; i += W * 64) ((u32x4 *)(lds + M::Z))[i] = u32x4{0, 0, 0, 0};
     float *qf = (float *)(lds + M::F), *qs = (float *)(lds + M::S);
     for (int h = w; h < GH; h += W) {
@@ -370,6 +465,16 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
         return place(j);
     };
 
+    // the new token's meta, from LDS, in the lanes that hold its position
+    auto new_meta = [&](uint32_t (&m)[NS][GL], int at) {
+        const uint32_t *nm = (const uint32_t *)(lds + M::NM) + at;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int e = 0; e < GL; ++e)
+                if (last * CH + place(i) == pos) m[i][e] = nm[g0 + 4 * e];
+    };
+
     float m[GH], l[GH], off[GH][GL], O[CT];
 #pragma unroll
     for (int h = 0; h < GH; ++h) {
@@ -382,12 +487,13 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
     for (int ct = 0; ct < CT; ++ct) O[ct] = 0.0f;
     uint8_t *pb = lds + M::R + w * (GH * NG * 4 * TB);
 
-    for (int ch = sp.c0 + w; ch < sp.c1; ch += W) {
+    for (int ch = c0 + w; ch < c1; ch += W) {
         const int p0 = ch * CH;
-        // 2. everything of the CH positions; past the last one, that one again
+        // 2. everything of the CH positions; past the last one, that one again. (K a chunk
+        // ahead gained nothing: the loads of the CU's other waves fill the time.)
         u32x4 kc[NS][GL];
+        Meta<HD, NS, GL> kmeta, vmeta;
         VCodes<CH> vc[CT];
-        uint32_t km[NS][GL], vm[NS][GL];
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const size_t row = row0 + min(p0 + place(i), pos);
@@ -395,36 +501,18 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             for (int e = 0; e < GL; ++e)
                 kc[i][e] = *(const u32x4 *)(p.c.k + row * (HD / 2) + (g0 + 4 * e) * 16);
         }
-        load_meta<HD>(p.c.km + row0 * NG, p0, n, kb, pos, km);
-        load_meta<HD>(p.c.vm + row0 * NG, p0, n, kb, pos, vm);
+        kmeta.load(p.c.km + row0 * NG, p0, n, kb, pos);
         // lane (kb, n): the kb-th quarter of the positions, channel 16 ct + n
         const int vblk = min((p0 + kb * (CH / 4)) / KV4_BLOCK, pos / KV4_BLOCK);
         uint8_t *vb = p.c.v + ((head * (p.c.cap / KV4_BLOCK) + vblk) * HD + n) * 16 +
                       (CH == 128 ? 0 : (kb & 1) * 8);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) vc[ct].load(vb + ct * 256);
+        vmeta.load(p.c.vm + row0 * NG, p0, n, kb, pos);
 
-        if (p.k_new && ch == last) {  // 3. the new token: quantised, stored, put in place
-            uint32_t *nm = (uint32_t *)(lds + M::NM);
-            const int c4 = min(lane, HD / 4 - 1) * 4;
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const float *src = (v ? p.v_new : p.k_new) + b * p.ldkv + (size_t)kvh * HD;
-                const f32x4a r = *(const f32x4a *)(src + c4);
-                const float x[4] = {r[0], r[1], r[2], r[3]};
-                const uint32_t mt = kv4_meta8(x);
-                uint32_t c[4];
-                kv4_codes(x, mt, c);
-                if (lane < HD / 4) {
-                    if (v)
-                        *(uint32_t *)(lds + M::NV + c4) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-                    else
-                        *(uint16_t *)(lds + M::NK + c4 / 2) =
-                            (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
-                    if ((lane & 7) == 0) nm[v * NG + lane / 8] = mt;
-                }
-            }
-            __builtin_amdgcn_wave_barrier();
+        const bool put = p.k_new && ch == last;
+        if (put) {  // 3. the new token: put in place and stored
+            const uint32_t *nm = (const uint32_t *)(lds + M::NM);
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 if (p0 + place(i) != pos) continue;
@@ -433,12 +521,10 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
                     const int g = g0 + 4 * e;
                     const size_t row = row0 + pos;
                     kc[i][e] = *(const u32x4 *)(lds + M::NK + g * 16);
-                    km[i][e] = nm[g];
-                    vm[i][e] = nm[NG + g];
                     if (part) continue;
                     *(u32x4 *)(p.c.k + row * (HD / 2) + g * 16) = kc[i][e];
-                    p.c.km[row * NG + g] = km[i][e];
-                    p.c.vm[row * NG + g] = vm[i][e];
+                    p.c.km[row * NG + g] = nm[g];
+                    p.c.vm[row * NG + g] = nm[NG + g];
                 }
             }
             if ((p0 + kb * (CH / 4)) / (CH / 4) == pos / (CH / 4)) {
@@ -456,8 +542,44 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             }
         }
 
-        // 4. scales and middles, V's (none past the last position) in its group's fixed point
-        float ks[NS][GL], ko[NS][GL], vs[NS][GL], vo[NS][GL];
+        // 4. scores in powers of two, each position's in one of the lanes that hold it
+        float s[GH][NS / GR];
+        {
+            uint32_t km[NS][GL];
+            kmeta.spread(km);
+            if (put) new_meta(km, 0);
+            float ks[NS][GL], ko[NS][GL];
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int e = 0; e < GL; ++e) {
+                    ks[i][e] = kv4_scale(km[i][e]) * 0x1p-34f;
+                    ko[i][e] = __builtin_fmaf(8.0f, ks[i][e], kv4_min(km[i][e]) * 0x1p-34f);
+                }
+#pragma unroll
+            for (int h = 0; h < GH; ++h) {
+                float part_s[NS];
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    part_s[i] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < GL; ++e) {
+                        i32x4 d = {0, 0, 0, 0};
+                        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 0), nib_lo(kc[i][e]), d, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 1), nib_hi(kc[i][e]), d, 0, 0, 0);
+                        part_s[i] = __builtin_fmaf(ko[i][e], qs[h * NG + g0 + 4 * e], part_s[i]);
+                        part_s[i] = __builtin_fmaf(undigits(d), ks[i][e], part_s[i]);
+                    }
+                }
+                sum_groups<GR>(part_s, s[h]);
+            }
+        }
+
+        uint32_t vm[NS][GL];
+        vmeta.spread(vm);
+        if (put) new_meta(vm, NG);
+        // 5. V's scales and middles (none past the last position) in their group's fixed point
+        float vs[NS][GL], vo[NS][GL];
         int ev[GL];
 #pragma unroll
         for (int e = 0; e < GL; ++e) {
@@ -465,8 +587,6 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 const bool in = p0 + place(i) <= pos;
-                ks[i][e] = kv4_scale(km[i][e]) * 0x1p-34f;
-                ko[i][e] = __builtin_fmaf(8.0f, ks[i][e], kv4_min(km[i][e]) * 0x1p-34f);
                 vs[i][e] = in ? kv4_scale(vm[i][e]) : 0.0f;
                 vo[i][e] = in ? __builtin_fmaf(8.0f, vs[i][e], kv4_min(vm[i][e])) : 0.0f;
                 mx = fmaxf(mx, vs[i][e]);
@@ -479,38 +599,24 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
         float corr[GH];
 #pragma unroll
         for (int h = 0; h < GH; ++h) {
-            // 5. scores in powers of two, each position's in one of the lanes that hold it
-            float part_s[NS], s[NS / GR], mx = m[h];
-#pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                part_s[i] = 0.0f;
-#pragma unroll
-                for (int e = 0; e < GL; ++e) {
-                    i32x4 d = {0, 0, 0, 0};
-                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 0), nib_lo(kc[i][e]), d, 0, 0, 0);
-                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 1), nib_hi(kc[i][e]), d, 0, 0, 0);
-                    part_s[i] = __builtin_fmaf(ko[i][e], qs[h * NG + g0 + 4 * e], part_s[i]);
-                    part_s[i] = __builtin_fmaf(undigits(d), ks[i][e], part_s[i]);
-                }
-            }
-            sum_groups<GR>(part_s, s);
+            // 6. the running maximum, the weights and their bytes
+            float mx = m[h];
 #pragma unroll
             for (int j = 0; j < NS / GR; ++j) {
-                s[j] = p0 + own_place(j) <= pos ? s[j] * qf[h] : -__builtin_inff();
-                mx = fmaxf(mx, s[j]);
+                s[h][j] = p0 + own_place(j) <= pos ? s[h][j] * qf[h] : -__builtin_inff();
+                mx = fmaxf(mx, s[h][j]);
             }
-            // 6. the running maximum, the weights and their bytes
             mx = swap32(swap16(row16_max(mx), max_f), max_f);
             corr[h] = __builtin_amdgcn_exp2f(m[h] - mx);
             m[h] = mx;
             l[h] *= corr[h];
 #pragma unroll
             for (int j = 0; j < NS / GR; ++j) {
-                s[j] = __builtin_amdgcn_exp2f(s[j] - mx);
-                l[h] += s[j];
+                s[h][j] = __builtin_amdgcn_exp2f(s[h][j] - mx);
+                l[h] += s[h][j];
             }
             float P[NS];
-            to_groups<GR>(s, P);
+            to_groups<GR>(s[h], P);
 #pragma unroll
             for (int e = 0; e < GL; ++e) {
                 off[h][e] *= corr[h];
@@ -566,7 +672,6 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             ml[(w * GH + h) * 2 + 1] = l[h];
         }
     __syncthreads();
-    const size_t oh = (size_t)b * p.H + (size_t)kvh * p.G + h0;
     for (int i = tid; i < G * HD; i += blockDim.x) {
         const int h = i / HD, c = i % HD;
         float mx = -__builtin_inff(), L = 0.0f, o = 0.0f;
@@ -578,10 +683,10 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             L = __builtin_fmaf(f, ml[(x * GH + h) * 2 + 1], L);
             o = __builtin_fmaf(f, mo[(x * GH + h) * HD + c], o);
         }
-        if (p.nsplit == 1) {
+        if (count == 1) {
             p.out[b * p.ldo + ((size_t)kvh * p.G + h0 + h) * HD + c] = o / L;
         } else {
-            float *pw = p.work + ((oh + h) * p.nsplit + blockIdx.y) * (HD + 4);
+            float *pw = p.work + ((size_t)blockIdx.y * p.H + (size_t)kvh * p.G + h0 + h) * (HD + 4);
             pw[c] = o;
             if (c == 0) {
                 pw[HD] = mx;
@@ -591,16 +696,16 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
     }
 }
 
-// The splits of a head, in order: the lanes of the first wave take a split's maximum
-// and sum each, the threads four of its partial rows at a time.
+// The shares of a head, in order: the lanes of the first wave take one's maximum and sum
+// each, the threads eight of their rows at a time.
 __global__ __launch_bounds__(KV4_MAX_HD) void attn4_merge_kernel(Attn4Params p) {
     __shared__ float weight[A4_MAX_SPLIT], sum;
-    const int h = blockIdx.x, b = blockIdx.y, c = threadIdx.x, hd = p.c.hd, ld = hd + 4;
-    const int pos = p.pos[b];
-    if (pos < 0 || pos >= p.c.cap) return;
-    const float *pw = p.work + ((size_t)b * p.H + h) * p.nsplit * ld;
-    const int nc = pos / p.ch + 1, per = (nc + p.nsplit - 1) / p.nsplit;
-    const int live = (nc + per - 1) / per;  // the splits that have a chunk
+    const int h = blockIdx.x, c = threadIdx.x, hd = p.c.hd;
+    const Shares sh = shares_of(p, 0, blockIdx.y);
+    const int live = sh.count, b = sh.b;
+    if (live <= 1) return;  // idle, or written already
+    const size_t ld = (size_t)p.H * (hd + 4);
+    const float *pw = p.work + (size_t)sh.first * ld + (size_t)h * (hd + 4);
     if (c < 64) {
         const int s = min(c, live - 1);
         const float m = pw[s * ld + hd], l = pw[s * ld + hd + 1];
@@ -613,50 +718,63 @@ __global__ __launch_bounds__(KV4_MAX_HD) void attn4_merge_kernel(Attn4Params p) 
     __syncthreads();
     if (c >= hd) return;
     float o = 0.0f;
-    for (int s = 0; s < live; s += 4) {
-        float x[4];
+    for (int s = 0; s < live; s += 8) {
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = pw[min(s + i, live - 1) * ld + c];
+        for (int i = 0; i < 8; ++i) x[i] = pw[min(s + i, live - 1) * ld + c];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
             o = s + i < live ? __builtin_fmaf(weight[s + i], x[i], o) : o;
     }
     p.out[b * p.ldo + (size_t)h * hd + c] = o / sum;
 }
 
+// Where the sequences can be long and the pairs of head and sequence are fewer than
+// the workgroups that the chip holds, the pairs are split into about as many shares: 512
+// of eight waves where a wave keeps to 128 registers, else of four. Short ones: a wave a
+// chunk, up to eight, and no second launch.
 struct Attn4Plan {
-    int W, nsplit, parts;
+    int W, parts, shares;
 };
 Attn4Plan attn4_plan(const Kv4View &c, int H) {
-    const int ch = attn4_ch(c.hd), chunks = (c.cap + ch - 1) / ch;
+    const int ch = attn4_ch(c.hd), chunks = (c.cap + ch - 1) / ch, per = H / c.Hkv;
     Attn4Plan pl;
-    pl.parts = (H / c.Hkv + A4_MAX_GH - 1) / A4_MAX_GH;
-    const long long pairs = (long long)c.B * c.Hkv * pl.parts;
+    pl.parts = (per + A4_MAX_GH - 1) / A4_MAX_GH;
     pl.W = std::min(A4_MAX_W, chunks);
-    const long long want = (getenv("A4W") ? atoi(getenv("A4W")) : 3072) / (pairs * pl.W);
-    pl.nsplit = (int)std::max(1LL, std::min({want, (long long)chunks / pl.W, (long long)A4_MAX_SPLIT}));
+    pl.shares = 0;
+    const long long heads = (long long)c.Hkv * pl.parts;
+    const long long room = 512 / heads;
+    if (chunks > A4_MAX_W && room > c.B) {
+        // a sequence's last share is half one in the mean
+        pl.shares = (int)(room - c.B / 2);
+        pl.W = c.hd <= 64 && per == 1 ? 8 : 4;
+    }
     return pl;
 }
+// The shares that there can be: `each` is at least their part of the chunks, and a
+// sequence has one more for what is left.
+int attn4_rows(const Attn4Plan &pl, int B) { return pl.shares + B + 1; }
 
 template <int HD, int GH>
-int launch_t(const Attn4Params &p, int W, hipStream_t st) {
+int launch_t(const Attn4Params &p, int W, int rows, hipStream_t st) {
     using M = Lds<HD, GH>;
     // a wave's weight terms, or its results
     constexpr size_t region = std::max(GH * M::NG * 4 * attn4_ch(HD), GH * (HD + 2) * 4);
     const size_t bytes = M::R + W * region;
     int rc = allow_lds((const void *)attn4_kernel<HD, GH>, bytes, M::R + A4_MAX_W * region);
     if (rc) return rc;
-    const dim3 grid(cdiv((size_t)p.c.Hkv, 8) * 8 * p.parts, (unsigned)p.nsplit, (unsigned)p.c.B);
+    const dim3 grid(p.parts > 1 ? cdiv((size_t)p.c.Hkv, 8) * 8 * p.parts : (unsigned)p.c.Hkv,
+                    (unsigned)rows);
     attn4_kernel<HD, GH><<<grid, 64 * W, bytes, st>>>(p);
     VMLM_HIP_CHECK(hipGetLastError());
     return VMLM_OK;
 }
 
 template <int HD>
-int launch_hd(const Attn4Params &p, int W, hipStream_t st) {
-    if (p.G == 1) return launch_t<HD, 1>(p, W, st);
-    if (p.G == 2) return launch_t<HD, 2>(p, W, st);
-    return launch_t<HD, A4_MAX_GH>(p, W, st);
+int launch_hd(const Attn4Params &p, int W, int rows, hipStream_t st) {
+    if (p.G == 1) return launch_t<HD, 1>(p, W, rows, st);
+    if (p.G == 2) return launch_t<HD, 2>(p, W, rows, st);
+    return launch_t<HD, A4_MAX_GH>(p, W, rows, st);
 }
 
 }  // namespace
@@ -664,7 +782,7 @@ int launch_hd(const Attn4Params &p, int W, hipStream_t st) {
 size_t attn4_work_floats(const Kv4View &c, int H) {
     if (c.B == 0 || c.Hkv == 0 || c.cap == 0 || H == 0) return 0;
     const Attn4Plan pl = attn4_plan(c, H);
-    return pl.nsplit == 1 ? 0 : (size_t)c.B * H * pl.nsplit * (c.hd + 4);
+    return pl.shares ? (size_t)attn4_rows(pl, c.B) * H * (c.hd + 4) : 0;
 }
 
 int launch_attn4(const Attn4Args &a, hipStream_t st) {
@@ -682,20 +800,22 @@ int launch_attn4(const Attn4Args &a, hipStream_t st) {
     p.work = a.work;
     p.H = a.H;
     p.G = a.H / a.c.Hkv;
-    p.nsplit = pl.nsplit;
+    p.shares = pl.shares;
+    p.W = pl.W;
     p.parts = pl.parts;
     p.ch = attn4_ch(a.c.hd);
     p.scale2 = a.scale * 1.44269504088896340736f;
     p.guard = guard_flag_ptr();
-    VMLM_GUARD(p.nsplit == 1 || p.work, "kv4 attention: split positions need a workspace");
+    VMLM_GUARD(!p.shares || p.work, "kv4 attention: split positions need a workspace");
+    const int rows = p.shares ? attn4_rows(pl, a.c.B) : a.c.B;
     int rc;
     switch (a.c.hd) {
-    case 32: rc = launch_hd<32>(p, pl.W, st); break;
-    case 64: rc = launch_hd<64>(p, pl.W, st); break;
-    case 128: rc = launch_hd<128>(p, pl.W, st); break;
-    default: rc = launch_hd<256>(p, pl.W, st); break;
+    case 32: rc = launch_hd<32>(p, pl.W, rows, st); break;
+    case 64: rc = launch_hd<64>(p, pl.W, rows, st); break;
+    case 128: rc = launch_hd<128>(p, pl.W, rows, st); break;
+    default: rc = launch_hd<256>(p, pl.W, rows, st); break;
     }
-    if (rc || p.nsplit == 1) return rc;
+    if (rc || !p.shares) return rc;
     attn4_merge_kernel<<<dim3((unsigned)p.H, (unsigned)p.c.B), std::max(64, p.c.hd), 0, st>>>(p);
     VMLM_HIP_CHECK(hipGetLastError());
     return VMLM_OK;
