@@ -1096,7 +1096,7 @@ int vmlm_hip_gemm_nt_int4(const float *a, const uint8_t *q, const float *scale, 
     x.K = (int)k;
     // groups beyond the row are one group of it
     x.G = (int)std::min(group, (k + 127) / 128 * 128);
-    const size_t wb = gemm_int4_work_bytes(x.M, x.N, x.K);
+    const size_t wb = gemm_int4_work_bytes(x.M, x.N, x.K, x.G);
     hipStreamCaptureStatus cs = hipStreamCaptureStatusActive;
     if (wb) VMLM_HIP_CHECK(hipStreamIsCapturing(st, &cs));
     // graphs that run at once would share the stream's workspace: a captured call

@@ -507,7 +507,7 @@ struct Int4Args {
     // workgroup then splits the rows itself, with the same result
     void *work = nullptr;
 };
-size_t gemm_int4_work_bytes(int M, int N, int K);
+size_t gemm_int4_work_bytes(int M, int N, int K, int G);
 int launch_gemm_int4(const Int4Args &a, hipStream_t st);
 
 // RMSNorm of each query and key head and the position rotation in one pass

@@ -24,6 +24,7 @@
 // from the rows, 16 neighbouring lanes want 16 rows, and the address unit, which takes
 // them line by line, was what the time went to (LM head 47 us so, 37 this way).
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.hpp"
 
@@ -134,11 +135,12 @@ __device__ __forceinline__ size_t plane_at(int runs, int m, int r) {
     return ((size_t)(m >> 2) * runs + r) * 2048 + (m & 3) * 64;
 }
 
-__device__ __forceinline__ float row16_max(float v) {
-    v = fmaxf(v, dpp_mov<0xB1>(v));
-    v = fmaxf(v, dpp_mov<0x4E>(v));
-    v = fmaxf(v, dpp_mov<0x124>(v));
-    return fmaxf(v, dpp_mov<0x128>(v));
+// over each row of 16 lanes; a NaN stays
+__device__ __forceinline__ float row16_maximum(float v) {
+    v = __builtin_elementwise_maximum(v, dpp_mov<0xB1>(v));
+    v = __builtin_elementwise_maximum(v, dpp_mov<0x4E>(v));
+    v = __builtin_elementwise_maximum(v, dpp_mov<0x124>(v));
+    return __builtin_elementwise_maximum(v, dpp_mov<0x128>(v));
 }
 
 // Eight neighbouring values of a run's row, 16 lanes a row, as digit planes of the
@@ -147,30 +149,45 @@ __device__ __forceinline__ float row16_max(float v) {
 __device__ __forceinline__ float split8(const float *row, int k, int K, uint32_t (&ev)[4],
                                         uint32_t (&od)[4]) {
     const float *a = row + min(k, K - 8);
+    const bool in = k < K;
     const f32x4a x0 = *(const f32x4a *)a, x1 = *(const f32x4a *)(a + 4);
-    float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-    float mx = 0.0f;
-    if (k >= K) {
+    const float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+    float mx = 0.0f;  // a NaN stays
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, q8_mag(x[e]));
-    mx = row16_max(mx);
+    for (int e = 0; e < 8; ++e) mx = __builtin_elementwise_maximum(mx, fabsf(x[e]));
+    mx = row16_maximum(in ? mx : 0.0f);
     const bool ok = mx <= 3.40282347e38f;
     // (below 2^-112 the factor's range leaves fewer bits)
     const int e2 = ok && mx > 0.0f ? min(29 - ilogbf(mx), 141) : 0;
+    const int es = in && ok ? e2 : -1000;  // none behind K, nor of a row without a factor
     uint32_t d[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        d[e] = signed_bytes(ok ? (int)rintf(ldexpf(x[e], e2)) : 0);
+    for (int e = 0; e < 8; ++e)  // signed_bytes, the sum rounded to an integer or f32's 24 bits
+        d[e] = (uint32_t)(int)(ldexpf(x[e], es) + (float)0x808080) ^ 0x808080u;
     transpose_bytes({d[0], d[2], d[4], d[6]}, ev);
     transpose_bytes({d[1], d[3], d[5], d[7]}, od);
     // 2^-4 for the nibble's place in its byte
     return ok ? ldexpf(1.0f, -e2 - 4) : __builtin_nanf("");
 }
 
-// The rows' planes and factors [runs][rows]; 16 lanes a (row, run).
+// 4 x 4 dwords transposed over four neighbouring lanes: r[i] of lane k becomes r[k] of
+// lane i.
+__device__ __forceinline__ void transpose_quad(uint32_t (&r)[4], int lane) {
+    auto swap = [&](uint32_t &a, uint32_t &b, auto ctrl, bool odd) {
+        const uint32_t give = odd ? a : b;
+        const uint32_t got = __float_as_uint(dpp_mov<decltype(ctrl)::value>(__uint_as_float(give)));
+        (odd ? a : b) = got;
+    };
+    using Xor1 = std::integral_constant<int, 0xB1>;
+    using Xor2 = std::integral_constant<int, 0x4E>;
+    swap(r[0], r[1], Xor1{}, lane & 1);
+    swap(r[2], r[3], Xor1{}, lane & 1);
+    swap(r[0], r[2], Xor2{}, lane & 2);
+    swap(r[1], r[3], Xor2{}, lane & 2);
+}
+
+// The rows' planes and factors [runs][rows]; 16 lanes a (row, run), four of them 64
+// bytes of a plane.
 __global__ __launch_bounds__(256) void int4_planes_kernel(const float *A, int M, int K, int runs,
                                                           int rows, uint8_t *planes, float *fac) {
     const int rb = (runs + 15) / 16, m = blockIdx.x / rb;
@@ -179,12 +196,11 @@ __global__ __launch_bounds__(256) void int4_planes_kernel(const float *A, int M,
     const int k = r * I4_RUN + l * 8;
     uint32_t ev[4], od[4];
     const float f = split8(A + (size_t)m * K, k, K, ev, od);
-    uint8_t *o = planes + plane_at(runs, m, r) + (l >> 2) * 256 + (l & 3) * 4;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        *(uint32_t *)(o + t * 16) = ev[3 - t];
-        *(uint32_t *)(o + 1024 + t * 16) = od[3 - t];
-    }
+    transpose_quad(ev, l);  // byte l & 3 (lowest first) of 16 k
+    transpose_quad(od, l);
+    uint8_t *o = planes + plane_at(runs, m, r) + (l >> 2) * 256 + (3 - (l & 3)) * 16;
+    *(u32x4 *)o = u32x4{ev[0], ev[1], ev[2], ev[3]};
+    *(u32x4 *)(o + 1024) = u32x4{od[0], od[1], od[2], od[3]};
     if (l == 0) fac[(size_t)r * rows + m] = f;
 }
 
@@ -480,14 +496,19 @@ template <int GM, int MT>
 int launch_mt(const Int4Params &p, hipStream_t st) {
     const size_t slabs = cdiv((size_t)p.M, GM / 32 * MT);
     const size_t tiles = cdiv((size_t)p.N, 16) * slabs;
+    // Up to a tile a CU each for itself (2304 columns, one row: 4.8 us against 5.2 with two
+    // together); more share the rows' split (5760 columns, one row 6.0 and 5.2, 16 rows 17.4 and
+    // 10.2); with many, loads run ahead in long workgroups (24 x 20000 45 and 42).
     if (tiles >= 2048) return launch_t<GM, MT, 4>(p, st);
-    if (tiles >= 1024) return launch_t<GM, MT, 2>(p, st);
+    if (tiles > 256) return launch_t<GM, MT, 2>(p, st);
     return launch_t<GM, MT, 1>(p, st);
 }
 
 template <int GM>
 int launch_gm(const Int4Params &p, hipStream_t st) {
-    if (p.planes) return launch_rows<GM>(p, st);
+    if constexpr (GM > 32) {  // (no planes for groups of 32)
+        if (p.planes) return launch_rows<GM>(p, st);
+    }
     const int tiles = cdiv((size_t)p.M, GM / 32);
     if (tiles == 1) return launch_mt<GM, 1>(p, st);
     if (tiles == 2) return launch_mt<GM, 2>(p, st);
@@ -499,8 +520,13 @@ size_t plane_rows(int M) { return ((size_t)M + I4_SLAB - 1) / I4_SLAB * I4_SLAB;
 
 }  // namespace
 
-size_t gemm_int4_work_bytes(int M, int N, int K) {
-    if (M <= 16) return 0;
+// Planes cost a launch and their bytes, splitting in place the split again in every
+// workgroup (K = 2304, group 128, in place and from planes, us): 16 rows of 2304 columns 9.5
+// and 10.5, of 5760 10.2 and 10.6, of 20000 27 and 18.4; 64 rows 18.8 and 11.3, 25.6 and
+// 17.6, 61.7 and 37.7; 8 rows of 20000 17.4 and 17.2. With groups of 32 a slab is four rows
+// either way: 64 rows of 2304 21.7 and 21.9, of 20000 113 and 122.
+size_t gemm_int4_work_bytes(int M, int N, int K, int G) {
+    if (G == 32 || M <= 8 || (M <= 16 && N <= 5760)) return 0;
     const size_t runs = cdiv((size_t)K, 2 * I4_RUN) * 2;
     return plane_rows(M) * runs * (512 + 4);
 }
