@@ -498,7 +498,7 @@ int launch_mt(const Int4Params &p, hipStream_t st) {
     const size_t tiles = cdiv((size_t)p.N, 16) * slabs;
     // Up to a tile a CU each for itself (2304 columns, one row: 4.8 us against 5.2 with two
     // together); more share the rows' split (5760 columns, one row 6.0 and 5.2, 16 rows 17.4 and
-    // 10.2); with many, loads run ahead in long workgroups (24 x 20000 45 and 42).
+    // 10.2); with many, loads run ahead in long workgroups (24 rows of 20000 45 and 42).
     if (tiles >= 2048) return launch_t<GM, MT, 4>(p, st);
     if (tiles > 256) return launch_t<GM, MT, 2>(p, st);
     return launch_t<GM, MT, 1>(p, st);
@@ -520,13 +520,14 @@ size_t plane_rows(int M) { return ((size_t)M + I4_SLAB - 1) / I4_SLAB * I4_SLAB;
 
 }  // namespace
 
-// Planes cost a launch and their bytes, splitting in place the split again in every
-// workgroup (K = 2304, group 128, in place and from planes, us): 16 rows of 2304 columns 9.5
-// and 10.5, of 5760 10.2 and 10.6, of 20000 27 and 18.4; 64 rows 18.8 and 11.3, 25.6 and
-// 17.6, 61.7 and 37.7; 8 rows of 20000 17.4 and 17.2. With groups of 32 a slab is four rows
-// either way: 64 rows of 2304 21.7 and 21.9, of 20000 113 and 122.
+// Planes cost a launch and their bytes, splitting in place the split again for every
+// 16 to 64 columns (K = 2304, planes and in place, us; group 128: 16 rows of 5760 columns 10.2 and
+// 8.7, 20 rows 10.7 and 15.6, 32 rows of 2304 10.4 and 8.7, 64 rows 10.9 and 15.8, 6 rows of
+// 20000 16.8 and 16.9, 12 rows 17.4 and 21.6; group 64: 8 rows of 5760 9.3 and 7.0, 12 rows 9.7
+// and 12.2, 20 rows of 2304 9.5 and 7.0, 32 rows 9.6 and 12.0). With groups of 32 a slab is
+// four rows either way: 64 rows of 2304 21.9 and 21.7, of 20000 122 and 113.
 size_t gemm_int4_work_bytes(int M, int N, int K, int G) {
-    if (G == 32 || M <= 8 || (M <= 16 && N <= 5760)) return 0;
+    if (G == 32 || M <= 4 || (size_t)M * N <= (G == 64 ? 60000 : 100000)) return 0;
     const size_t runs = cdiv((size_t)K, 2 * I4_RUN) * 2;
     return plane_rows(M) * runs * (512 + 4);
 }
