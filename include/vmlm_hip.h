@@ -332,9 +332,11 @@ int vmlm_hip_attention_decode_split(const float *q, const float *k_new, const fl
  * q [n][k / 2] signed 4-bit weights, byte i of a row holding k = 2i (low nibble) and
  * 2i + 1 in two's complement, any alignment; scale [n][ceil(k / group)]. k is a
  * multiple of 32, group 32, 64 or a multiple of 128 (the last group may be short).
- * The rows of A are split exactly into int8 terms, 24 bits below the largest of
- * 128 neighbours, and the products summed in integers within a group, so results
- * are as near as f32 sums are; rows with a NaN or an infinity are summed in f32. */
+ * The rows of A become fixed-point numbers of 31 bits below the largest of 128
+ * neighbours, as four int8 terms, and the products are summed in integers within a
+ * group: results are as near as f32 sums are (values below 2^-7 of that largest one
+ * keep fewer bits than f32's 24). Rows with a NaN or an infinity are summed in f32.
+ * Many rows go through the stream's workspace, in a captured call through none. */
 int vmlm_hip_gemm_nt_int4(const float *a, const uint8_t *q, const float *scale, float *c,
                           size_t m, size_t n, size_t k, size_t group, void *stream);
 /* RMSNorm of each head of q [rows][ldq] (n_heads heads) and k [rows][ldk]

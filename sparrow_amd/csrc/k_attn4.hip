@@ -294,8 +294,8 @@ __device__ __forceinline__ Shares shares_of(const Attn4Params &p, int at, int wa
     float all = 0.0f, most = 0.0f;
     for (int b0 = 0; b0 < p.c.B; b0 += 64) {
         const float n = (float)chunks_of(p, b0 + lane, &pos);
-        all += wave_sum(n);
-        most = fmaxf(most, wave_max(n));
+        all += wave_sum_dpp(n);
+        most = fmaxf(most, wave_max_nonneg(n));
     }
     Shares r;
     const int want = max((int)ceilf(all / (float)p.shares), (int)ceilf(most / A4_MAX_SPLIT));
@@ -706,25 +706,29 @@ __global__ __launch_bounds__(KV4_MAX_HD) void attn4_merge_kernel(Attn4Params p) 
     if (live <= 1) return;  // idle, or written already
     const size_t ld = (size_t)p.H * (hd + 4);
     const float *pw = p.work + (size_t)sh.first * ld + (size_t)h * (hd + 4);
+    const int cc = min(c, hd - 1);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = pw[min(i, live - 1) * ld + cc];
     if (c < 64) {
         const int s = min(c, live - 1);
         const float m = pw[s * ld + hd], l = pw[s * ld + hd + 1];
-        const float mx = wave_max(m), e = __builtin_amdgcn_exp2f(m - mx);
-        const float f = c < live ? e : 0.0f;
+        const float mx = swap32(swap16(row16_max(m), max_f), max_f);
+        const float e = __builtin_amdgcn_exp2f(m - mx), f = c < live ? e : 0.0f;
         weight[c] = f;
-        const float t = wave_sum(c < live ? f * l : 0.0f);
+        const float t = wave_sum_dpp(c < live ? f * l : 0.0f);
         if (c == 0) sum = t;
     }
     __syncthreads();
     if (c >= hd) return;
     float o = 0.0f;
     for (int s = 0; s < live; s += 8) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = pw[min(s + i, live - 1) * ld + c];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             o = s + i < live ? __builtin_fmaf(weight[s + i], x[i], o) : o;
+        if (s + 8 >= live) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = pw[min(s + 8 + i, live - 1) * ld + c];
     }
     p.out[b * p.ldo + (size_t)h * hd + c] = o / sum;
 }

@@ -213,7 +213,9 @@ def test_int4_two_streams(dev):
     """Calls at once on streams of their own give what they give alone."""
     rng = np.random.default_rng(5)
     jobs = []
-    for m, n, k, group in ((1, 2304, 2304, 128), (16, 5760, 2304, 64)):
+    # (the last one's rows go through the stream's workspace)
+    for m, n, k, group in ((1, 2304, 2304, 128), (16, 5760, 2304, 64), (70, 2304, 1024, 128),
+                           (70, 2400, 1000 // 32 * 32, 64)):
         a, q, s = int4_case(rng, m, n, k, group)
         jobs.append((dev.stream(), dev.up(a), dev.up(q), dev.up(s),
                      [dev.zeros(m, n) for _ in range(20)], (m, n, k, group)))
@@ -228,6 +230,34 @@ def test_int4_two_streams(dev):
         int4_check(one, a.get(), q.get(), s.get(), dims[3])
         for x in c[1:]:
             assert np.array_equal(x.get(), one)
+
+
+@pytest.mark.parametrize("m,n,group", [(3, 500, 32), (16, 700, 128), (40, 5000, 128), (70, 3000, 64)])
+def test_int4_captured(dev, m, n, group):
+    """Captured calls take no workspace (two graphs may run at once) and agree with the
+    definition on every replay, with eager calls of the same stream between them."""
+    rng = np.random.default_rng(6)
+    a, q, s = int4_case(rng, m, n, 416, group)
+    da, dq, ds, dc, de = dev.up(a), dev.up(q), dev.up(s), dev.zeros(m, n), dev.zeros(m, n)
+    st, graph = dev.stream(), C.c_void_p()
+
+    def call(c):
+        dev.check(dev.L.vmlm_hip_gemm_nt_int4(da.ptr, dq.ptr, ds.ptr, c.ptr, m, n, 416, group, st))
+    call(dc)
+    dev.check(dev.L.vmlm_hip_capture_begin(st))
+    call(dc)
+    dev.check(dev.L.vmlm_hip_capture_end(st, C.byref(graph)))
+    for i in range(3):
+        a = rng.standard_normal(a.shape, dtype=np.float32)
+        dev.sync()
+        da.put(a)
+        dc.put(np.zeros((m, n)))
+        dev.check(dev.L.vmlm_hip_graph_launch(graph, st))
+        call(de)
+        dev.sync()
+        int4_check(dc.get(), a, q, s, group)
+        int4_check(de.get(), a, q, s, group)
+    dev.check(dev.L.vmlm_hip_graph_destroy(graph))
 
 
 # ------------------------------------------------------------------ qk_norm_rope
@@ -506,7 +536,11 @@ ATTN = [(1, 1, 1, 32, 32, [0]), (1, 1, 1, 64, 32, [31]), (1, 36, 36, 64, 128, [1
         (4, 4, 4, 64, 256, [0, 1, 130, -1]), (2, 6, 2, 128, 320, [319, 127]),
         (3, 8, 1, 64, 192, [31, 32, 190]), (2, 16, 1, 256, 160, [77, 159]),
         (1, 15, 3, 32, 544, [543]), (2, 14, 2, 64, 96, [95, 5]), (1, 24, 2, 128, 1056, [1040]),
-        (1, 2, 1, 64, 4128, [4100]), (1, 2, 2, 64, 8192, [8191]), (2, 5, 1, 128, 5120, [5000, 3])]
+        (1, 2, 1, 64, 4128, [4100]), (1, 2, 2, 64, 8192, [8191]), (2, 5, 1, 128, 5120, [5000, 3]),
+        (1, 3, 3, 32, 4096, [4000]), (3, 2, 1, 256, 1600, [1599, 700, -1]), (2, 9, 1, 64, 2080, [5, 2079]),
+        # more sequences than a wave has lanes, some idle, most of them short
+        (70, 1, 1, 64, 1152, [-1, 1151, 0, 64, 700, -1, 127, 128, 1000, 3] * 7),
+        (130, 2, 1, 32, 1056, ([-1] * 60 + [1055, 31, 90, 500, 0]) * 2)]
 
 
 @pytest.mark.parametrize("B,H,Hkv,hd,cap,pos", ATTN)
@@ -598,6 +632,61 @@ def test_attention_position_past_the_capacity(ops):
             c.attention_decode(q, [p, 63], q, q)
         assert e.value.code == 9
     assert np.isfinite(c.attention_decode(q, [63, 63])).all()
+
+
+def test_attention_split_position_past_the_capacity(ops):
+    """The same where the sequences are split."""
+    from sparrow_amd import VmlmError
+    rng = np.random.default_rng(15)
+    c, m = filled(ops, rng, 2, 1, 2048, 64, [2048, 2048])
+    q = rng.standard_normal((2, 64), dtype=np.float32)
+    for p in (2048, 2 ** 31 - 1):
+        with pytest.raises(VmlmError) as e:
+            c.attention_decode(q, [2047, p])
+        assert e.value.code == 9
+    out = c.attention_decode(q, [2047, 1500])
+    ref, tol = attn_ref(m, q, [2047, 1500], 1, 64, 0.125)
+    assert (np.abs(out - ref) <= tol).all()
+
+
+def test_offsets_past_32_bits(dev):
+    """The last of five sequences whose caches are 1 GB of codes each: its rows lie
+    past 2^32 bytes in every array of codes."""
+    from sparrow_amd import _abi
+    B, H, cap, hd, S = 5, 8, 1 << 20, 256, 6
+    ptrs = []
+    for n in [B * H * cap * hd // 2] * 2 + [B * H * cap * hd // 8] * 2:
+        p = C.c_void_p()
+        dev.check(dev.L.vmlm_hip_malloc(C.byref(p), n))
+        dev.bufs.append(p.value)
+        ptrs.append(p.value)
+    d = _abi.Kv4Cache(*ptrs, B, H, cap, hd)
+    rng = np.random.default_rng(16)
+    k, v = rng.standard_normal((2, B, S, H * hd), dtype=np.float32)
+    q = rng.standard_normal((B, H * hd), dtype=np.float32)
+    dk, dv, dq = dev.up(k), dev.up(v), dev.up(q)
+    rk, rv, out = dev.zeros(*k.shape), dev.zeros(*v.shape), dev.zeros(*q.shape)
+    need = C.c_size_t()
+    dev.check(dev.L.vmlm_hip_attention_decode_kv4_work(d, H, C.byref(need)))
+    work = dev.zeros(max(need.value, 16), dtype=np.uint8)
+    w = H * hd
+    for first in (cap - S, 0):
+        pos = dev.up(np.array([-1] * (B - 1) + [first], np.int32))
+        dev.check(dev.L.vmlm_hip_kv4_append(d, dk.ptr, w, dv.ptr, w, pos.ptr, None, S, None))
+        dev.check(dev.L.vmlm_hip_kv4_read(d, rk.ptr, w, rv.ptr, w, pos.ptr, None, S, None))
+        dev.sync()
+        for got, x in ((rk.get(), k), (rv.get(), v)):
+            assert not got[:-1].any() and np.array_equal(got[-1], held(x[-1])[2])
+    pos = np.array([-1] * (B - 1) + [S - 1], np.int32)
+    dp = dev.up(pos)
+    dev.check(dev.L.vmlm_hip_attention_decode_kv4(d, dq.ptr, w, None, None, 0, dp.ptr, out.ptr, w, H,
+                                                  0.0625, work.ptr, work.nbytes, None))
+    dev.check(dev.L.vmlm_hip_check_guards())
+    dev.sync()
+    m = new_model(B, H, 32, hd)
+    put(m, k[-1], v[-1], B - 1, 0, S, H)
+    ref, tol = attn_ref(m, q, pos, H, hd, 0.0625)
+    assert (np.abs(out.get() - ref) <= tol).all()
 
 
 def device_cache(dev, c):
