@@ -1054,11 +1054,22 @@ static int check_kv4(const vmlm_kv4_cache *c, Kv4View *v, bool device = true) {
     v->cap = (int)c->cap;
     v->hd = (int)c->head_dim;
     if (v->B == 0 || v->Hkv == 0 || v->cap == 0) return VMLM_OK;
+    // (of more, products of sizes would leave 64 bits)
+    VMLM_GUARD(c->batch * c->n_kv_heads <= ((size_t)1 << 42) / (c->cap * c->head_dim),
+               "kv4: batch %zu, n_kv_heads %zu, cap %zu, head_dim %zu: over 2^42 values", c->batch,
+               c->n_kv_heads, c->cap, c->head_dim);
     VMLM_GUARD(v->k && v->v && v->km && v->vm, "kv4: null cache array");
     VMLM_GUARD(!device || ((((uintptr_t)v->k | (uintptr_t)v->v) & 15) == 0 &&
                            (((uintptr_t)v->km | (uintptr_t)v->vm) & 3) == 0),
                "kv4: k and v must be 16-byte aligned, k_meta and v_meta 4-byte");
     return VMLM_OK;
+}
+
+// Whether `rows` rows of w floats at stride ld lie over one of the cache's arrays.
+static bool over_cache(const Kv4View &c, const float *p, size_t ld, size_t w, size_t rows) {
+    const size_t vals = (size_t)c.B * c.Hkv * c.cap * c.hd, bytes = ((rows - 1) * ld + w) * 4;
+    return overlap(p, bytes, c.k, vals / 2) || overlap(p, bytes, c.v, vals / 2) ||
+           overlap(p, bytes, c.km, vals / 8) || overlap(p, bytes, c.vm, vals / 8);
 }
 
 static int check_int4(const float *a, const uint8_t *q, const float *scale, const float *c,
@@ -1179,6 +1190,10 @@ static int check_kv4_rows(const Kv4View &c, const float *k, size_t ldk, const fl
     const size_t w = (size_t)c.Hkv * c.hd;
     VMLM_GUARD((size_t)c.B * S == 1 || (ldk >= w && ldv >= w),
                "kv4: row strides %zu, %zu are below the row's width %zu", ldk, ldv, w);
+    const size_t rows = (size_t)c.B * S, most = std::max(w, rows > 1 ? std::max(ldk, ldv) : 0);
+    VMLM_GUARD(rows <= ((size_t)1 << 50) / most, "kv4: %zu rows of %zu values (limit 2^50)", rows, most);
+    VMLM_GUARD(!over_cache(c, k, ldk, w, rows) && !over_cache(c, v, ldv, w, rows),
+               "kv4: rows lie over the cache");
     return VMLM_OK;
 }
 
@@ -1245,6 +1260,17 @@ int vmlm_hip_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, s
                    (!k_new || (!rows_overlap(out, ldo, w, k_new, ldkv, wk, B) &&
                                !rows_overlap(out, ldo, w, v_new, ldkv, wk, B))),
                "kv4 attention: the output lies over its input");
+    VMLM_GUARD(!over_cache(a.c, out, ldo, w, B), "kv4 attention: the output lies over the cache");
+    const size_t wf = attn4_work_floats(a.c, (int)n_heads);
+    if (wf && work) {
+        VMLM_GUARD(work_bytes >= wf * 4 && ((uintptr_t)work & 15) == 0,
+                   "kv4 attention: workspace of %zu bytes, %zu needed (16-byte aligned)",
+                   work_bytes, wf * 4);
+        VMLM_GUARD(!overlap(work, wf * 4, out, ((B - 1) * ldo + w) * 4) &&
+                       !overlap(work, wf * 4, q, ((B - 1) * ldq + w) * 4) &&
+                       !over_cache(a.c, (float *)work, wf, wf, 1),
+                   "kv4 attention: the workspace lies over an operand");
+    }
     INIT_OR_RETURN();
     if ((rc = on_library_device())) return rc;
     hipStream_t st = as_stream(stream);
@@ -1258,12 +1284,7 @@ int vmlm_hip_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, s
     a.ldo = ldo;
     a.H = (int)n_heads;
     a.scale = scale;
-    const size_t wf = attn4_work_floats(a.c, a.H);
-    if (wf == 0) return launch_attn4(a, st);
-    if (work) {
-        VMLM_GUARD(work_bytes >= wf * 4 && ((uintptr_t)work & 15) == 0,
-                   "kv4 attention: workspace of %zu bytes, %zu needed (16-byte aligned)",
-                   work_bytes, wf * 4);
+    if (wf == 0 || work) {
         a.work = (float *)work;
         return launch_attn4(a, st);
     }

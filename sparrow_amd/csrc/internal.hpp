@@ -504,7 +504,7 @@ struct Int4Args {
     float *C = nullptr;  // [M][N]
     int M = 0, N = 0, K = 0, G = 0;
     // gemm_int4_work_bytes() bytes for the activations as byte planes, or null: each
-    // workgroup then splits the rows itself, with the same result
+    // workgroup then splits the rows itself, the same numbers added in another order
     void *work = nullptr;
 };
 size_t gemm_int4_work_bytes(int M, int N, int K, int G);

@@ -30,8 +30,8 @@ struct HeadNormParams {
     int rows, H, Hkv, hd;
     int per;  // heads a wave carries
     float eps;
-    // theta^(-2i/hd) / 2 pi = coarse[i / 16] * fine[i % 16] (256 bytes of arguments: the
-    // table itself, 2 KB of them, took 0.@ us of each call)
+    // theta^(-2i/hd) / 2 pi = coarse[i / 16] * fine[i % 16] (256 bytes of arguments: with the
+    // table itself, 2 KB of them, a call of one row took 6.2 us instead of 5.0)
     double coarse[HEADNORM_MAX_HD / 32], fine[16];
 };
 

@@ -134,11 +134,42 @@ def test_attention_refused(L):
     assert attend(L, cache(), H=0) == 0
 
 
+def test_rows_over_the_cache_refused(L):
+    """An output among the codes or the meta would be read back as them."""
+    ends = (A, A + 8192 - 4, Q + 64, S, S + 4, S + 0x1000000 + 2048 - 4)  # 2 * 2 * 64 * 64 values
+    for at in ends:
+        for fn in ("vmlm_hip_kv4_append", "vmlm_hip_kv4_read"):
+            assert rows(L, fn, cache(), k=at) == 9, hex(at)
+            assert rows(L, fn, cache(), v=at) == 9, hex(at)
+            assert "lie over the cache" in message(L)
+        assert attend(L, cache(), out=at) == 9, hex(at)
+        assert "over the cache" in message(L)
+
+
+def test_sizes_past_64_bits_refused(L):
+    """Products of sizes, each within its own limit, that would wrap."""
+    huge = cache(batch=65535, n_kv_heads=32767, cap=2 ** 30, head_dim=256)
+    assert rows(L, "vmlm_hip_kv4_append", huge, ldk=2 ** 23, ldv=2 ** 23) == 9
+    assert attend(L, huge, H=32767, ldq=2 ** 23, ldo=2 ** 23) == 9
+    assert L.vmlm_kv4_read(huge, A, Q, S, None, 1) == 9
+    wide = cache(batch=65535, n_kv_heads=2, cap=32, head_dim=32)
+    assert rows(L, "vmlm_hip_kv4_read", wide, S=2 ** 30) == 9
+
+
 def test_attention_workspace(L):
     n = C.c_size_t(1)
     assert L.vmlm_hip_attention_decode_kv4_work(cache(), 4, None) == 9
     assert L.vmlm_hip_attention_decode_kv4_work(cache(), 3, C.byref(n)) == 9
     assert L.vmlm_hip_attention_decode_kv4_work(cache(cap=65536, batch=1), 4, C.byref(n)) == 0
+    assert n.value > 0
+    long, out = cache(cap=65536, batch=1), Y + 0x100000
+    work = Z + 0x1000000
+    for bad in (dict(work=work, nbytes=n.value - 1), dict(work=work + 4, nbytes=n.value),
+                dict(work=out, nbytes=n.value), dict(work=out + 4 * 256 - 16, nbytes=n.value),
+                dict(work=Y, nbytes=n.value), dict(work=A, nbytes=n.value),
+                dict(work=S, nbytes=n.value)):
+        assert attend(L, long, out=out, **bad) == 9, bad
+        assert "workspace" in message(L)
 
 
 def test_host_forms_refuse_before_any_copy(L):
