@@ -10,6 +10,9 @@
 // sines and cosines in registers and carries 64 / LH of the row's heads at a
 // time through them.
 //
+// Bound by the rows' bytes, read once and written once: 2048 rows of 36 + 36 heads of 64
+// take 14.6 us, 5.2 TB/s (a large copy 5.1). One row takes 2.8 us, a launch and a latency.
+//
 // Angles: pos * theta^(-2i/hd) / 2 pi is formed in 64 bits and its whole turns
 // dropped there; a 32-bit product would be off by 2^-24 of the angle itself (0.006 at
 // position 100000), more than the values' own rounding from a few positions on.

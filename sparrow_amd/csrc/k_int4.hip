@@ -22,7 +22,12 @@
 // Codes and scales come in pairs of runs, eight lanes to 128 bytes of a row, and take
 // their places for the B operand through LDS that belongs to the wave: read straight
 // from the rows, 16 neighbouring lanes want 16 rows, and the address unit, which takes
-// them line by line, was what the time went to (LM head 47 us so, 37 this way).
+// them line by line, was what the time went to (LM head 47 us so, 36.5 this way).
+//
+// Bound, and measured (kernel times): one row of 122753 x 2304 in groups of 64 takes 36.5
+// us, 4.4 TB/s of codes and scales against 5.1 of a large copy. Up to a tile a CU the
+// launch and one latency through the K / 256 pairs are the time: 1 x 2304 x 2304 in 5 us,
+// where a call's issue takes 3.8. Many rows: see gemm_int4_rows_kernel.
 #include <algorithm>
 #include <type_traits>
 
@@ -187,7 +192,8 @@ __device__ __forceinline__ void transpose_quad(uint32_t (&r)[4], int lane) {
 }
 
 // The rows' planes and factors [runs][rows]; 16 lanes a (row, run), four of them 64
-// bytes of a plane.
+// bytes of a plane. One pass: 4 bytes read and 4 written a value; 100 x 5760 in 4.5 us, most
+// of it a launch and one latency.
 __global__ __launch_bounds__(256) void int4_planes_kernel(const float *A, int M, int K, int runs,
                                                           int rows, uint8_t *planes, float *fac) {
     const int rb = (runs + 15) / 16, m = blockIdx.x / rb;
@@ -375,7 +381,9 @@ __global__ __launch_bounds__(TN == 4 ? 256 : 1024) void gemm_int4_kernel(Int4Par
 
 // Many rows, the activations as planes: a wave takes 4 tiles of rows and 64 columns
 // over its share of the pairs, A operands straight from the planes (1 KB in lane
-// order), one run ahead.
+// order), one run ahead. 100 x 2304 x 5760 in groups of 128: planes 4.5 us, this 15, 0.18
+// POP/s (0.7 on the matrix units: four bytes a value). Bound by the A operands, which every
+// 64 columns read again through the caches, at two waves a SIMD.
 constexpr int I4_TM = 4, I4_TN = 4;
 
 template <int GM>

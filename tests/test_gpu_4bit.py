@@ -9,7 +9,7 @@ Tolerances (u = 2^-24, half a step of f32):
    error counts), three products and the rotation's sum 6 u, sine and cosine 4 u of
    their own and 2 pi u of the f32 angle, against the pair's length: 32 u.
  * cache: codes, meta and values are equal bit for bit (the definition is f32).
- * attention: a score is off by ds = (32 + hd/8) u scale sum|q||k| (q in 24 bits below
+ * attention: a score is off by ds = (32 + hd/8) u scale sum|q||k| (q in 31 bits below
    its largest, a sum over hd/32 groups of exact products), a weight by twice that
    and the exponential's few u, and the sums over n positions by (n/128 + 64) u of the
    largest |v|: (4 ds + (n/128 + 64) u) * max|v|."""
