@@ -406,9 +406,8 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
         kv4_codes(k, mk, ck);
         kv4_codes(v, mv, cv);
         if (lane < HD / 4) {
-            *(uint16_t *)(lds + M::NK + c4 / 2) =
-                (uint16_t)(ck[0] | ck[1] << 4 | ck[2] << 8 | ck[3] << 12);
-            *(uint32_t *)(lds + M::NV + c4) = cv[0] | cv[1] << 8 | cv[2] << 16 | cv[3] << 24;
+            *(uint16_t *)(lds + M::NK + c4 / 2) = kv4_nibbles(ck);
+            *(uint32_t *)(lds + M::NV + c4) = kv4_bytes(cv);
             if ((lane & 7) == 0) {
                 nm[lane / 8] = mk;
                 nm[NG + lane / 8] = mv;

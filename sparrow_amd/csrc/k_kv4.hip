@@ -43,9 +43,9 @@ __device__ __forceinline__ bool kv4_rows(const Kv4Params &p, int b, int blk, int
 // channels of a position; V's codes cross LDS to be packed along positions, and a
 // block's bytes that hold other positions keep their nibbles. Bound by the f32 rows;
 // all of a thread's loads are issued before the first is used. 16 prompts of up to 128
-// rows, 36 heads of 64, 31 MB of rows and codes: 11.2 us, 2.8 TB/s; the two dozen operations a
+// rows, 36 heads of 64, 31 MB of rows and codes: 11 us, 2.8 TB/s; the two dozen operations a
 // value and V's way through LDS are what a copy does not have. (K and V in one workgroup: 7.0 us
-// instead of 6.1 for 3 x 333 rows of 8 heads of 128.)
+// instead of 6.1 then for 3 x 333 rows of 8 heads of 128.)
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Params p) {
     constexpr int NG = HD / 32, LD = HD + 4;  // bytes of a position in LDS
@@ -76,10 +76,9 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Params p) {
         uint32_t c[4];
         kv4_codes(x, m, c);
         if (isv)
-            *(uint32_t *)(codes + o * LD + ch) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+            *(uint32_t *)(codes + o * LD + ch) = kv4_bytes(c);
         else
-            *(uint16_t *)(p.c.k + pos * (HD / 2) + ch / 2) =
-                (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
+            *(uint16_t *)(p.c.k + pos * (HD / 2) + ch / 2) = kv4_nibbles(c);
         if (l == 0) meta[pos * NG + g] = m;
     }
     if (!isv) return;
@@ -110,46 +109,65 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Params p) {
     }
 }
 
+// Neighbouring heads of a workgroup that reads: 128 channels, fewer workgroups to start
+// (for 16 prompts of up to 128 rows, 36 heads of 64, 7.8 us instead of 8.3; appending takes
+// 11 us either way).
+constexpr int read_heads(int hd) { return hd < 128 ? 128 / hd : 1; }
+
 // The block's codes and meta through LDS, then four channels of a position a thread:
 // whole 16-byte stores of a row. Bound by the f32 rows that it writes: 16 prompts of up to
-// 128 rows, 36 heads of 64, 31 MB in 8.7 us, 3.6 TB/s.
+// 128 rows, 36 heads of 64, 31 MB in 7.8 us, 4.0 TB/s.
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Params p) {
-    constexpr int NG = HD / 32, LV = 20;  // LDS bytes of a V channel
-    __shared__ __align__(4) uint8_t codes[HD * LV];
-    __shared__ uint32_t meta[KV4_BLOCK * NG];
-    const int b = blockIdx.z, h = blockIdx.y >> 1, isv = blockIdx.y & 1, tid = threadIdx.x;
+    constexpr int NH = read_heads(HD), NG = HD / 32, LV = 20;  // LDS bytes of a V channel
+    constexpr int CODES = HD * 4, METAS = KV4_BLOCK * NG;      // dwords of a head's block
+    __shared__ __align__(4) uint8_t codes[NH * HD * LV];
+    __shared__ uint32_t meta[NH * METAS];
+    const int b = blockIdx.z, h0 = (blockIdx.y >> 1) * NH, isv = blockIdx.y & 1, tid = threadIdx.x;
+    const int nh = min(NH, p.c.Hkv - h0);
     int first, pos0, t0, t1;
     if (!kv4_rows(p, b, blockIdx.x, &first, &pos0, &t0, &t1)) return;
-    const size_t head = (size_t)b * p.c.Hkv + h, pos = head * p.c.cap + first;
-    // a V block is as long as its positions' K rows
+    const size_t pos = ((size_t)b * p.c.Hkv + h0) * p.c.cap + first;
+    // a V block is as long as its positions' K rows; a head's is cap positions on
     const uint32_t *cb = (const uint32_t *)((isv ? p.c.v : p.c.k) + pos * (HD / 2));
     const uint32_t *mb = (isv ? p.c.vm : p.c.km) + pos * NG;
+    uint32_t c[NH * CODES / 256];
 #pragma unroll
-    for (int i = tid; i < HD * 4; i += 256)
-        *(uint32_t *)(codes + (isv ? i / 4 * LV + i % 4 * 4 : i * 4)) = cb[i];
-    if (tid < KV4_BLOCK * NG) meta[tid] = mb[tid];
+    for (int i = 0; i < NH * CODES / 256; ++i) {
+        const int x = tid + i * 256, h = min(x / CODES, nh - 1);
+        c[i] = cb[(size_t)h * p.c.cap * (HD / 8) + x % CODES];
+    }
+    const int mh = min(tid / METAS, nh - 1);
+    const uint32_t m0 = mb[(size_t)mh * p.c.cap * NG + tid % METAS];
+#pragma unroll
+    for (int i = 0; i < NH * CODES / 256; ++i) {
+        const int x = tid + i * 256;
+        *(uint32_t *)(codes + (isv ? x / 4 * LV + x % 4 * 4 : x * 4)) = c[i];
+    }
+    if (tid < NH * METAS) meta[tid] = m0;
     __syncthreads();
     float *dst = isv ? p.vo : p.ko;
     const size_t ld = isv ? p.ldv : p.ldk;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        const int x = tid + i * 256, o = x / (HD / 4), ch = x % (HD / 4) * 4, t = first + o - pos0;
-        if (t < t0 || t >= t1) continue;
-        const uint32_t m = meta[o * NG + ch / 32];
+    for (int i = 0; i < NH * NG; ++i) {
+        constexpr int RD = NH * HD / 4;  // threads of a position
+        const int x = tid + i * 256, o = x / RD, all = x % RD * 4, t = first + o - pos0;
+        const int h = all / HD, ch = all % HD;
+        if (t < t0 || t >= t1 || h >= nh) continue;
+        const uint32_t m = meta[h * METAS + o * NG + ch / 32];
         uint32_t c;
         if (isv) {
             c = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                c |= ((uint32_t)codes[(ch + e) * LV + o / 2] >> (4 * (o & 1)) & 15u) << (4 * e);
+                c |= ((uint32_t)codes[(all + e) * LV + o / 2] >> (4 * (o & 1)) & 15u) << (4 * e);
         } else {
-            c = ((const uint16_t *)codes)[x];
+            c = ((const uint16_t *)codes)[(h * KV4_BLOCK + o) * (HD / 4) + ch / 4];
         }
         f32x4a y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = kv4_value(c >> (4 * e), kv4_min(m), kv4_scale(m));
-        *(f32x4a *)(dst + ((size_t)b * p.S + t) * ld + (size_t)h * HD + ch) = y;
+        *(f32x4a *)(dst + ((size_t)b * p.S + t) * ld + (size_t)(h0 + h) * HD + ch) = y;
     }
 }
 
@@ -161,14 +179,14 @@ void launch_hd(const Kv4Params &p, dim3 grid, hipStream_t st) {
         kv4_read_kernel<HD><<<grid, 256, 0, st>>>(p);
 }
 
-dim3 kv4_grid(const Kv4View &c, int S) {
+dim3 kv4_grid(const Kv4View &c, int S, int heads) {
     // the blocks that S rows can touch, from any position of the first
     const size_t blocks = std::min((size_t)c.cap / KV4_BLOCK, ((size_t)S + 30) / KV4_BLOCK + 1);
-    return dim3((unsigned)blocks, 2 * (unsigned)c.Hkv, (unsigned)c.B);
+    return dim3((unsigned)blocks, 2 * cdiv((size_t)c.Hkv, heads), (unsigned)c.B);
 }
 
 int launch_kv4(const Kv4Params &p, hipStream_t st) {
-    const dim3 grid = kv4_grid(p.c, p.S);
+    const dim3 grid = kv4_grid(p.c, p.S, p.k ? 1 : read_heads(p.c.hd));
     switch (p.c.hd) {
     case 32: launch_hd<32>(p, grid, st); break;
     case 64: launch_hd<64>(p, grid, st); break;

@@ -34,25 +34,38 @@ __device__ __forceinline__ float kv4_scale(uint32_t meta) { return __uint_as_flo
 __device__ __forceinline__ float kv4_min(uint32_t meta) {
     return __uint_as_float(meta & 0xffff0000u);
 }
-// the nibble of x, by the definition's quotient
+// the code of x, by the definition's quotient
 __device__ __forceinline__ uint32_t kv4_code(float x, float mn, float sc) {
     const float u = sc > 0.0f ? fminf(fmaxf(rintf((x - mn) / sc), 0.0f), 15.0f) : 0.0f;
-    return (uint32_t)u ^ 8u;
+    return (uint32_t)u;
 }
-// The nibbles of four values. A product with 1 / scale is within 2^-22 of the quotient
-// relative to it, 2^-18 in all, so it decides every code whose quotient is not
-// nearer than 2^-16 to a half; the wave takes the quotients themselves where one is,
-// or where the scale is so small or large that its reciprocal is not normal.
+// Four codes as 16 bits of nibbles, and as a byte each with the nibble in its low half.
+__device__ __forceinline__ uint16_t kv4_nibbles(const uint32_t (&c)[4]) {
+    return (uint16_t)((c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12) ^ 0x8888u);
+}
+__device__ __forceinline__ uint32_t kv4_bytes(const uint32_t (&c)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u);
+    const uint32_t b = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+    return (a | b) ^ 0x08080808u;
+}
+// The codes u = nibble ^ 8 of four values, each in the low 16 bits of its dword. A
+// product with 1 / scale is within 2^-22 of the quotient relative to it, 2^-18 in all, so
+// it decides every code whose quotient is not nearer than 2^-16 to a half; the wave takes
+// the quotients themselves where one is, or where the scale is so small or large that its
+// reciprocal is not normal. (Clamped first: 0 and 15 are no halves. 1.5 * 2^23 added
+// rounds to an integer and leaves it in the low bits.)
 __device__ __forceinline__ void kv4_codes(const float (&x)[4], uint32_t meta, uint32_t (&c)[4]) {
     const float mn = kv4_min(meta), sc = kv4_scale(meta), r = __builtin_amdgcn_rcpf(sc);
-    bool near = !(sc > 1e-36f && sc < 1e36f);
+    float off[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float q = (x[e] - mn) * r, n = rintf(q);
-        near |= !(fabsf(q - n) < 0.5f - 0x1p-16f);
-        c[e] = (uint32_t)(int)fminf(fmaxf(n, 0.0f), 15.0f) ^ 8u;
+        const float q = __builtin_amdgcn_fmed3f((x[e] - mn) * r, 0.0f, 15.0f);
+        const float t = q + 0x1.8p23f;
+        off[e] = fabsf(q - (t - 0x1.8p23f));
+        c[e] = __float_as_uint(t);
     }
-    if (__builtin_expect(__any(near), 0)) {
+    const float most = fmaxf(fmaxf(off[0], off[1]), fmaxf(off[2], off[3]));
+    if (__builtin_expect(__any(!(sc > 1e-36f && sc < 1e36f && most < 0.5f - 0x1p-16f)), 0)) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) c[e] = kv4_code(x[e], mn, sc);
     }
@@ -64,18 +77,22 @@ __device__ __forceinline__ float kv4_value(uint32_t nib, float mn, float sc) {
 
 // The meta of 32 values held by 8 neighbouring lanes, four each; the same in all
 // eight. (Minimum and maximum that keep a NaN; lanes swapped within a quad, then the
-// half row mirrored.)
+// half row mirrored. All eight take part: no lane's own value is kept for an absent one.)
+template <int CTRL>
+__device__ __forceinline__ float kv4_swap(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
+}
 __device__ __forceinline__ uint32_t kv4_meta8(const float (&x)[4]) {
     float lo = __builtin_elementwise_minimum(__builtin_elementwise_minimum(x[0], x[1]),
                                              __builtin_elementwise_minimum(x[2], x[3]));
     float hi = __builtin_elementwise_maximum(__builtin_elementwise_maximum(x[0], x[1]),
                                              __builtin_elementwise_maximum(x[2], x[3]));
-    lo = __builtin_elementwise_minimum(lo, dpp_mov<0xB1>(lo));
-    hi = __builtin_elementwise_maximum(hi, dpp_mov<0xB1>(hi));
-    lo = __builtin_elementwise_minimum(lo, dpp_mov<0x4E>(lo));
-    hi = __builtin_elementwise_maximum(hi, dpp_mov<0x4E>(hi));
-    lo = __builtin_elementwise_minimum(lo, dpp_mov<0x141>(lo));
-    hi = __builtin_elementwise_maximum(hi, dpp_mov<0x141>(hi));
+    lo = __builtin_elementwise_minimum(lo, kv4_swap<0xB1>(lo));
+    hi = __builtin_elementwise_maximum(hi, kv4_swap<0xB1>(hi));
+    lo = __builtin_elementwise_minimum(lo, kv4_swap<0x4E>(lo));
+    hi = __builtin_elementwise_maximum(hi, kv4_swap<0x4E>(hi));
+    lo = __builtin_elementwise_minimum(lo, kv4_swap<0x141>(lo));
+    hi = __builtin_elementwise_maximum(hi, kv4_swap<0x141>(hi));
     return kv4_meta(lo, hi);
 }
 
