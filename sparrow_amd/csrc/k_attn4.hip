@@ -333,7 +333,8 @@ __device__ __forceinline__ Shares shares_of(const Attn4Params &p, int at, int wa
 }
 
 // LDS of a workgroup: the query terms [head][term][group][32], zeros, their factors and group
-// sums, the new token's codes and meta, the V offsets of each wave, and one region
+// sums, the new token's codes and meta, a number for each wave, head and group (the weight
+// terms' power of two, then the V offset), and one region
 // that holds the waves' weight terms, then their results.
 template <int HD, int HEADS>
 struct Lds {
@@ -492,6 +493,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) O[ct] = 0.0f;
     uint8_t *pb = lds + M::R + w * (GH * NG * 4 * TB);
+    int *ex = (int *)(lds + M::OFF) + w * GH * NG;  // the terms' powers of two; in the end V offsets
 
     for (int ch = c0 + w; ch < c1; ch += W) {
         const int p0 = ch * CH;
@@ -584,23 +586,16 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
         uint32_t vm[NS][GL];
         vmeta.spread(vm);
         if (put) new_meta(vm, NG);
-        // 5. V's scales and middles (none past the last position) in their group's fixed point
+        // 5. V's scales and middles (none past the last position)
         float vs[NS][GL], vo[NS][GL];
-        int ev[GL];
 #pragma unroll
-        for (int e = 0; e < GL; ++e) {
-            float mx = 0.0f;
+        for (int e = 0; e < GL; ++e)
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 const bool in = p0 + place(i) <= pos;
                 vs[i][e] = in ? kv4_scale(vm[i][e]) : 0.0f;
                 vo[i][e] = in ? __builtin_fmaf(8.0f, vs[i][e], kv4_min(vm[i][e])) : 0.0f;
-                mx = fmaxf(mx, vs[i][e]);
             }
-            ev[e] = fixed_exp(rows_red<GR>(row16_max(mx), max_f));
-#pragma unroll
-            for (int i = 0; i < NS; ++i) vs[i][e] = ldexpf(vs[i][e], ev[e]);
-        }
 
         float corr[GH];
 #pragma unroll
@@ -626,13 +621,30 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
 #pragma unroll
             for (int e = 0; e < GL; ++e) {
                 off[h][e] *= corr[h];
-                uint32_t d[NS];
+                // The fixed point lies below the largest weight times scale, not below the
+                // largest scale: a value row that stands out and is not attended would take
+                // the others' bits.
+                float wt[NS], mw = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
                     off[h][e] = __builtin_fmaf(P[i], vo[i][e], off[h][e]);
+                    wt[i] = P[i] * vs[i][e];
+                    mw = fmaxf(mw, wt[i]);
+                }
+                const int ev = fixed_exp(rows_red<GR>(row16_max(mw), max_f));
+                if (n == 0 && kb < GR) ex[h * NG + kb + 4 * e] = ev;
+                // (the power of two of a product below 2^-98 is no f32)
+                if (__any(ev > 127)) {
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) wt[i] = ldexpf(wt[i], max(ev - 127, 0));
+                }
+                const float up = ldexpf(1.0f, min(ev, 127));
+                uint32_t d[NS];
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
                     // signed_bytes of the product (below 2^30), the sum rounded to an integer
                     // (or to f32's 24 bits)
-                    d[i] = (uint32_t)__builtin_fmaf(P[i], vs[i][e], (float)0x808080) ^ 0x808080u;
+                    d[i] = (uint32_t)__builtin_fmaf(wt[i], up, (float)0x808080) ^ 0x808080u;
                 }
                 store_terms<HD>(pb + (h * NG + g0 + 4 * e) * 4 * TB, n, kb, d);
             }
@@ -642,26 +654,24 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
         float cq = corr[0];
 #pragma unroll
         for (int h = 1; h < GH; ++h) cq = kb == h ? corr[h] : cq;
-        const int hq = min(n >> 2, GH - 1);
+        const int hq = min(n >> 2, GH - 1), hd4 = min(kb, GH - 1);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             const int g = ct / 2;
             const i32x4 d = vc[ct].product(pb + ((hq * NG + g) * 4 + term) * TB + kb * 16);
-            const int eg = __builtin_amdgcn_readlane(ev[g / 4], (g % GR) * 16);
-            O[ct] = __builtin_fmaf(O[ct], cq, ldexpf(undigits(d), -eg - 4));
+            O[ct] = __builtin_fmaf(O[ct], cq, ldexpf(undigits(d), -4 - ex[hd4 * NG + g]));
         }
         __builtin_amdgcn_wave_barrier();
     }
 
     // 8. the waves' results
-    float *offl = (float *)(lds + M::OFF) + w * GH * NG;
 #pragma unroll
     for (int h = 0; h < GH; ++h) {
         l[h] = rows_red<1>(row16_sum(l[h]), add_f);
 #pragma unroll
         for (int e = 0; e < GL; ++e) {
             const float o = rows_red<GR>(row16_sum(off[h][e]), add_f);
-            if (n == 0 && kb < GR) offl[h * NG + kb + 4 * e] = o;
+            if (n == 0 && kb < GR) ex[h * NG + kb + 4 * e] = __float_as_int(o);
         }
     }
     __syncthreads();  // the weights' bytes are read; the region is the results' now
@@ -669,7 +679,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
     if (kb < G) {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
-            mo[(w * GH + kb) * HD + ct * 16 + n] = O[ct] + offl[kb * NG + ct / 2];
+            mo[(w * GH + kb) * HD + ct * 16 + n] = O[ct] + __int_as_float(ex[kb * NG + ct / 2]);
     }
 #pragma unroll
     for (int h = 0; h < GH; ++h)

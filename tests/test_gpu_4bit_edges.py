@@ -1,0 +1,127 @@
+"""The 4-bit operators on the GPU where their arithmetic, their masks and their sizes
+are at an edge, against their definitions in 64 bits.
+
+Tolerances (u = 2^-24, half a step of f32), where no other is derived beside a test:
+ * attention, per output channel: with p the weights, R the largest value that a
+   position's 32 channels can hold and t a score's distance from the largest one,
+   sum_p p R (e + mean e) where e = ds + (64 + n / 16 + 4 t) u. The score is off by
+   ds = 33 u scale sum_g |q_g|_1 K_g over the groups g of 32 channels (K the largest
+   value its key's group can hold): q to 2^-30 of its group's largest value, its sum, the
+   products' conversions and the sums over groups, all below 33 roundings of that sum; 0
+   where every step is exact. 4 t u is the exponent's product with log2(e) and its
+   rounding; 64 u the exponential, the weights' fixed point (24 bits, and 2^-30 of the
+   largest weight times scale of 128 positions, which is 3 u of sum_p p R), the
+   conversions and the joins; n / 16 u the sums over the positions that a lane adds one
+   after another."""
+import ctypes as C
+
+import numpy as np
+import pytest
+from test_gpu_4bit import (U, Buf, Dev, cache_codes, dev, device_cache, held, int4_case,  # noqa: F401
+                           int4_check, int4_ref, new_model, nibbles, norm_ref, ops, put, same_cache)
+
+pytestmark = pytest.mark.gpu
+
+
+def spread(meta):
+    """(min, scale) of each 32 channels, f64."""
+    lo = (meta & np.uint32(0xFFFF0000)).view(np.float32).astype(np.float64)
+    return lo, (meta << np.uint32(16)).view(np.float32).astype(np.float64)
+
+
+def attn_exact(m, q, pos, Hkv, hd, scale, ds=True):
+    """(out in 64 bits, its bound) for live rows; ds False: scores are exact in f32."""
+    B, H = q.shape[0], q.shape[1] // hd
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(B):
+        n = pos[b] + 1
+        for h in range(H if n > 0 else 0):
+            kv, at = h // (H // Hkv), slice(h * hd, (h + 1) * hd)
+            x = q[b, at].astype(np.float64)
+            s = m["k"][b, kv, :n].astype(np.float64) @ x * scale
+            t = s.max() - s
+            p = np.exp(-t)
+            p /= p.sum()
+            most = []
+            for name in ("km", "vm"):
+                lo, sc = spread(m[name][b, kv, :n])
+                most.append(np.maximum(np.abs(lo), np.abs(lo + 15 * sc)))
+            e = (64 + n / 16 + 4 * t) * U
+            if ds:
+                e += 33 * U * scale * (most[0] @ np.abs(x).reshape(-1, 32).sum(1))
+            out[b, at] = p @ m["v"][b, kv, :n].astype(np.float64)
+            # (a weight below 2^-126 may be none)
+            w = (p * (e + p @ e))[:, None] * most[1] + 2.0 ** -126 * most[1]
+            tol[b, at] = np.repeat(w.sum(0), 32) + 2.0 ** -138
+    return out, tol
+
+
+def stored(ops, k, v, Hkv, cap):
+    """Rows [B, n, Hkv * hd] in a cache and in its model."""
+    B, n, hd = k.shape[0], k.shape[1], k.shape[2] // Hkv
+    c, m = ops.Kv4Cache(B, Hkv, cap, hd), new_model(B, Hkv, cap, hd)
+    c.append(k, v, np.zeros(B))
+    for b in range(B):
+        put(m, k[b], v[b], b, 0, n, Hkv)
+    return c, m
+
+
+def close(out, ref, tol):
+    assert (np.abs(out - ref) <= tol).all(), (np.abs(out - ref) / tol).max()
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("times", [1e3, 1e6, 1e10, 1e20])
+@pytest.mark.parametrize("H,Hkv,hd,n,at", [(1, 1, 64, 200, 77), (4, 1, 128, 130, 129), (2, 2, 32, 100, 0),
+                                           (2, 1, 256, 90, 64), (7, 1, 64, 60, 59), (2, 2, 128, 2500, 1300)])
+@pytest.mark.parametrize("append", [False, True])
+def test_attention_value_that_no_query_attends(ops, H, Hkv, hd, n, at, times, append):
+    """A value row that stands out at a position whose weight is nothing (e^-100):
+    the others keep all their bits."""
+    rng = np.random.default_rng(n + hd)
+    base = rng.standard_normal((1, Hkv, 1, hd))
+    q = (base + 0.1 * rng.standard_normal((1, Hkv, H // Hkv, hd))).astype(np.float32).reshape(1, -1)
+    k, v = rng.standard_normal((2, 1, n, Hkv * hd), dtype=np.float32)
+    scale = float(np.float32(hd ** -0.5))
+    k[0, at] = (-100 / scale * base / (base * base).sum(-1, keepdims=True)).reshape(-1)
+    v[0, at] *= np.float32(times)
+    cap = -(-n // 32) * 32
+    c, m = stored(ops, k, v, Hkv, cap)
+    new = (k[:, -1], v[:, -1]) if append else ()
+    if append:  # the last row again, by the attention itself
+        c.k[:, :, n - 1] = 0
+        c.k_meta[:, :, n - 1] = c.v_meta[:, :, n - 1] = 0x7FC07FC0
+    out = c.attention_decode(q, [n - 1], *new)
+    close(out, *attn_exact(m, q, [n - 1], Hkv, hd, scale))
+
+
+@pytest.mark.parametrize("H,Hkv,hd", [(1, 1, 32), (1, 1, 64), (4, 1, 128), (3, 1, 256), (2, 1, 64)])
+def test_attention_every_bit_of_the_weights(ops, H, Hkv, hd):
+    """One position has nearly all the weight, and half of its channels hold an exact
+    zero (u = 8, min = -8 scale): there the output is the sum of weights near 2^-15 of the
+    largest, in fixed point below it. Off by half a step (2^-30 of the largest) each
+    times a code up to 8, besides the roundings of the weights themselves; without their
+    lowest byte it would be off by 3.5e-6 in the mean."""
+    rng = np.random.default_rng(hd)
+    n = 60
+    q = np.zeros((1, H, hd), np.float32)
+    q[0, :, 0] = 8
+    k = np.zeros((1, n, hd), np.float32)
+    scale = 0.125
+    k[0, 1:, 0] = -rng.uniform(9, 12, n - 1)
+    v = rng.integers(-8, 8, (1, n, hd)).astype(np.float32)
+    v[0, :, 0::32], v[0, :, 1::32] = -8, 7
+    zero = np.arange(hd) % 2 == 0
+    v[0, 0, zero & (np.arange(hd) % 32 > 1)] = 0
+    c, m = stored(ops, k, v, Hkv, 64)
+    assert np.array_equal(m["v"][0, 0, :n], v[0])
+    out = c.attention_decode(q.reshape(1, -1), [n - 1], scale=scale).reshape(H, hd)
+    ref, tol = attn_exact(m, q.reshape(1, -1), [n - 1], Hkv, hd, scale)
+    close(out, ref.reshape(H, hd), tol.reshape(H, hd))
+    see = v[0, 0] == 0
+    s = m["k"][0, 0, :n, 0].astype(np.float64) * 8 * scale
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    e = (64 + n / 16 + 4 * 13 + 33 * 13) * U  # (a score is above -13)
+    bound = (2 * e * p[1:].sum() + (n - 1) * 2.0 ** -30) * 8
+    assert see.any() and np.abs(out - ref.reshape(H, hd))[:, see].max() <= bound
