@@ -368,7 +368,11 @@ int vmlm_hip_kv4_read(const vmlm_kv4_cache *cache, float *k, size_t ldk, float *
  * n_kv_heads)): out [batch][ldo]. q and k_new come rotated (vmlm_hip_qk_norm_rope).
  * Sequences with pos < 0 are idle: their cache and output row stay as they are; pos >=
  * cap trips the device guard and is treated so. A query head with a NaN or an
- * infinity gives NaN. n_heads is a multiple of n_kv_heads, up to 16 times it.
+ * infinity gives NaN. Queries are held in 31 bits below the largest of their 32 channels,
+ * a position's weight times its values' scale in 31 below the largest such product of
+ * 128 positions: results are off by f32 roundings of the queries times the largest value
+ * that a key's 32 channels can hold, and of the weights times the values' likewise.
+ * n_heads is a multiple of n_kv_heads, up to 16 times it.
  * `work`: vmlm_hip_attention_decode_kv4_work() bytes, 16-byte aligned, used by one
  * call at a time; null: the stream's own workspace, which a call under stream capture may
  * not use (9), since graphs that run at once would share it. */

@@ -9,11 +9,12 @@
 // matrix instructions over the nibbles as they lie:
 //  * A nibble in the high half of a byte is 16 (u - 8) as a signed byte, so a
 //    16-byte load becomes two int8 operands (low and high nibbles) with 12
-//    operations. q, and for the output the weights, are 31-bit fixed-point numbers
-//    below their largest value, as four signed bytes: with 16 (u - 8) every product
-//    and sum is exact in int32, and two conversions and an FMA put the terms
-//    together. 32-bit sums, then, at 8-bit rates. (Three bytes left the many small
-//    weights 2^-22 of the largest: 1.4e-6 off where f32 sums are 4e-7.)
+//    operations. q, and for the output the weights times V's scale, are 31-bit fixed-point
+//    numbers below the largest of their group (32 channels of q, a chunk's positions
+//    for the weights), as four signed bytes: with 16 (u - 8) every product and sum is
+//    exact in int32, and two conversions and an FMA put the terms together. 32-bit
+//    sums, then, at 8-bit rates. (Three bytes left the many small weights 2^-22 of the
+//    largest: 1.4e-6 off where f32 sums are 4e-7.)
 //  * Scores: a wave takes 128 positions. Lane (row kb, column n) loads the 32
 //    channels of group kb mod NG at one position. The A operand has a row (j, t) for
 //    each kb = j and term t that is zero outside kb = j, so D's rows 4 kb + t at column n
@@ -332,8 +333,8 @@ __device__ __forceinline__ Shares shares_of(const Attn4Params &p, int at, int wa
     return r;
 }
 
-// LDS of a workgroup: the query terms [head][term][group][32], zeros, their factors and group
-// sums, the new token's codes and meta, a number for each wave, head and group (the weight
+// LDS of a workgroup: the query terms [head][term][group][32], zeros, the heads' powers of two,
+// a factor and a sum for each head and group, the new token's codes and meta, a number for each wave, head and group (the weight
 // terms' power of two, then the V offset), and one region
 // that holds the waves' weight terms, then their results.
 template <int HD, int HEADS>
@@ -343,7 +344,7 @@ struct Lds {
     static constexpr int Z = Q + HEADS * 4 * HD;  // as many zeros
     static constexpr int F = Z + HEADS * 4 * HD;
     static constexpr int S = F + HEADS * 4;
-    static constexpr int NK = (S + HEADS * NG * 4 + 15) / 16 * 16;
+    static constexpr int NK = (S + HEADS * NG * 8 + 15) / 16 * 16;
     static constexpr int NV = NK + HD / 2;
     static constexpr int NM = NV + HD;
     static constexpr int OFF = NM + 2 * NG * 4;
@@ -416,38 +417,44 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
         }
     }
     for (int i = tid; i < GH * HD / 4; i += W * 64) ((u32x4 *)(lds + M::Z))[i] = u32x4{0, 0, 0, 0};
-    float *qf = (float *)(lds + M::F), *qs = (float *)(lds + M::S);
+    int *qe = (int *)(lds + M::F);
+    float *qs = (float *)(lds + M::S);
     for (int h = w; h < GH; h += W) {
         const float *q = p.q + b * p.ldq + ((size_t)kvh * p.G + h0 + min(h, G - 1)) * HD;
         constexpr int CL = (HD + 63) / 64;
-        float x[CL], mx = 0.0f;
+        float x[CL], mx[CL], most = 0.0f;
         int bad = 0;
 #pragma unroll
         for (int i = 0; i < CL; ++i) {
             const int c = i * 64 + lane;
             x[i] = c < HD ? q[c] : 0.0f;
-            mx = fmaxf(mx, fabsf(x[i]));
+            mx[i] = swap16(row16_max(fabsf(x[i])), max_f);  // of its 32 channels
+            most = fmaxf(most, mx[i]);
             bad |= !(fabsf(x[i]) <= 3.40282347e38f);
         }
-        mx = wave_max(mx);
+        most = swap32(most, max_f);
         bad = __any(bad);
-        const int e = fixed_exp(mx);
+        // Each group's fixed point lies below its own largest value: keys may be small just
+        // where queries are large. The sums come in units that keep them below 2^-5 of the
+        // largest key value (2^eh takes them back): no step between leaves f32.
+        const int eh = bad || most == 0.0f ? 0 : ilogbf(most) + 14;
 #pragma unroll
         for (int i = 0; i < CL; ++i) {
-            const int c = i * 64 + lane;
+            const int c = i * 64 + lane, e = fixed_exp(mx[i]);
             const int f = bad ? 0 : (int)rintf(ldexpf(x[i], e));
-            float s = (float)f;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) s += __shfl_xor(s, o, 64);
+            const float s = swap16(row16_sum((float)f), add_f);
             if (c >= HD) continue;
             const uint32_t d = signed_bytes(f);
             uint8_t *t = lds + M::Q + ((h * 4) * NG + c / 32) * 32 + (c & 1) * 16 + c % 32 / 2;
 #pragma unroll
             for (int k = 0; k < 4; ++k) t[k * NG * 32] = (uint8_t)(d >> (24 - 8 * k));
-            if ((c & 31) == 0) qs[h * NG + c / 32] = 16.0f * s;
+            if ((c & 31) == 0) {
+                float *o = qs + (h * NG + c / 32) * 2;
+                o[0] = mx[i] > 0.0f && !bad ? ldexpf(1.0f, -4 - e - eh) : 0.0f;
+                o[1] = bad ? __builtin_nanf("") : ldexpf(s, -e - eh);
+            }
         }
-        if (lane == 0)
-            qf[h] = bad ? __builtin_nanf("") : ldexpf(p.scale2, 30 - e);  // 2^34 of it is in K's scales
+        if (lane == 0) qe[h] = eh;
     }
     __syncthreads();
 
@@ -561,12 +568,18 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             for (int i = 0; i < NS; ++i)
 #pragma unroll
                 for (int e = 0; e < GL; ++e) {
-                    ks[i][e] = kv4_scale(km[i][e]) * 0x1p-34f;
-                    ko[i][e] = __builtin_fmaf(8.0f, ks[i][e], kv4_min(km[i][e]) * 0x1p-34f);
+                    ks[i][e] = kv4_scale(km[i][e]);
+                    ko[i][e] = __builtin_fmaf(8.0f, ks[i][e], kv4_min(km[i][e]));
                 }
 #pragma unroll
             for (int h = 0; h < GH; ++h) {
-                float part_s[NS];
+                float part_s[NS], unit[GL], sum[GL];
+#pragma unroll
+                for (int e = 0; e < GL; ++e) {
+                    const float *o = qs + (h * NG + g0 + 4 * e) * 2;
+                    unit[e] = o[0];
+                    sum[e] = o[1];
+                }
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
                     part_s[i] = 0.0f;
@@ -575,8 +588,8 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
                         i32x4 d = {0, 0, 0, 0};
                         d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 0), nib_lo(kc[i][e]), d, 0, 0, 0);
                         d = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa(h, e, 1), nib_hi(kc[i][e]), d, 0, 0, 0);
-                        part_s[i] = __builtin_fmaf(ko[i][e], qs[h * NG + g0 + 4 * e], part_s[i]);
-                        part_s[i] = __builtin_fmaf(undigits(d), ks[i][e], part_s[i]);
+                        part_s[i] = __builtin_fmaf(ko[i][e], sum[e], part_s[i]);
+                        part_s[i] = __builtin_fmaf(undigits(d) * unit[e], ks[i][e], part_s[i]);
                     }
                 }
                 sum_groups<GR>(part_s, s[h]);
@@ -604,7 +617,8 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             float mx = m[h];
 #pragma unroll
             for (int j = 0; j < NS / GR; ++j) {
-                s[h][j] = p0 + own_place(j) <= pos ? s[h][j] * qf[h] : -__builtin_inff();
+                s[h][j] = p0 + own_place(j) <= pos ? ldexpf(s[h][j] * p.scale2, qe[h])
+                                                   : -__builtin_inff();
                 mx = fmaxf(mx, s[h][j]);
             }
             mx = swap32(swap16(row16_max(mx), max_f), max_f);

@@ -125,3 +125,59 @@ def test_attention_every_bit_of_the_weights(ops, H, Hkv, hd):
     e = (64 + n / 16 + 4 * 13 + 33 * 13) * U  # (a score is above -13)
     bound = (2 * e * p[1:].sum() + (n - 1) * 2.0 ** -30) * 8
     assert see.any() and np.abs(out - ref.reshape(H, hd))[:, see].max() <= bound
+
+
+@pytest.mark.parametrize("H,Hkv,hd", [(1, 1, 64), (4, 1, 128), (2, 2, 256)])
+@pytest.mark.parametrize("times", [1e4, 1e6, 1e12])
+def test_attention_query_groups_of_other_magnitudes(ops, H, Hkv, hd, times):
+    """Queries whose first 32 channels are large against keys that are small there (and
+    the other way round in the last 32): each group's products keep their bits."""
+    rng = np.random.default_rng(hd + H)
+    n = 150
+    q = rng.standard_normal((1, H, hd), dtype=np.float32)
+    k, v = rng.standard_normal((2, 1, n, Hkv, hd), dtype=np.float32)
+    q[..., :32] *= np.float32(times)
+    k[..., :32] /= np.float32(times)
+    q[..., -32:] /= np.float32(times)
+    k[..., -32:] *= np.float32(times)
+    c, m = stored(ops, k.reshape(1, n, -1), v.reshape(1, n, -1), Hkv, 160)
+    q = q.reshape(1, -1)
+    scale = float(np.float32(hd ** -0.5))
+    close(c.attention_decode(q, [n - 1]), *attn_exact(m, q, [n - 1], Hkv, hd, scale))
+
+
+@pytest.mark.parametrize("times", [1e-37, 1e-20, 1e20, 1e36])
+def test_attention_tiny_and_huge_queries(ops, times):
+    """Queries and keys at opposite ends of f32, with a group of zeros and a zero head."""
+    rng = np.random.default_rng(21)
+    n, hd = 70, 128
+    q = rng.standard_normal((1, 3, hd), dtype=np.float32) * np.float32(times)
+    q[:, :, 32:64] = 0
+    q[:, 2] = 0
+    k, v = rng.standard_normal((2, 1, n, hd), dtype=np.float32)
+    k /= np.float32(times)
+    c, m = stored(ops, k, v, 1, 96)
+    q = q.reshape(1, -1)
+    close(c.attention_decode(q, [n - 1], scale=0.125), *attn_exact(m, q, [n - 1], 1, hd, 0.125))
+
+
+@pytest.mark.parametrize("H,hd", [(1, 32), (1, 64), (4, 128), (3, 256)])
+def test_attention_every_bit_of_the_queries(ops, H, hd):
+    """Two channels of a group, 24 bits each, that nearly cancel against equal keys: the
+    score is their difference, exact in every step."""
+    rng = np.random.default_rng(hd)
+    q = np.zeros((1, H, hd), np.float32)
+    big = rng.integers(2 ** 23, 2 ** 24 - 2 ** 18, (H, hd // 32))
+    q[0, :, 5::32] = big
+    q[0, :, 20::32] = -(big - rng.integers(1, 4, big.shape))
+    k = np.zeros((1, 3, hd), np.float32)
+    k[0, 0, 5::32] = k[0, 0, 20::32] = 15
+    k[0, 1, 5::32] = k[0, 1, 20::32] = 15
+    k[0, 1, 3::32] = 1
+    k[0, 2, 7::32] = 15
+    v = rng.standard_normal((1, 3, hd), dtype=np.float32)
+    c, m = stored(ops, k, v, 1, 32)
+    assert np.array_equal(m["k"][0, 0, :3], k[0])
+    q = q.reshape(1, -1)
+    close(c.attention_decode(q, [2], scale=2.0 ** -7),
+          *attn_exact(m, q, [2], 1, hd, 2.0 ** -7, ds=False))
