@@ -50,6 +50,9 @@ typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
 // Positions of a wave at a time: what the registers hold. (64 for heads of 128 too, more
 // waves at once: 36.0 us instead of 34.3 for 8 sequences of 16000 with 4 queries a kv head.)
 constexpr int attn4_ch(int hd) { return hd <= 128 ? 128 : 64; }
+// The maximum of no score yet, or of scores that all left f32 downwards: finite, so that
+// its distance from itself is none (not -inf - -inf).
+constexpr float A4_NONE = -3.40282347e38f;
 constexpr int A4_MAX_GH = 4;   // query heads of a workgroup (rows of the A operand / 4)
 constexpr int A4_MAX_W = 8;    // waves of a workgroup
 constexpr int A4_MAX_SPLIT = 64;  // shares of a sequence
@@ -492,7 +495,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
     float m[GH], l[GH], off[GH][GL], O[CT];
 #pragma unroll
     for (int h = 0; h < GH; ++h) {
-        m[h] = -__builtin_inff();
+        m[h] = A4_NONE;
         l[h] = 0.0f;
 #pragma unroll
         for (int e = 0; e < GL; ++e) off[h][e] = 0.0f;
@@ -704,12 +707,10 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
     __syncthreads();
     for (int i = tid; i < G * HD; i += blockDim.x) {
         const int h = i / HD, c = i % HD;
-        float mx = -__builtin_inff(), L = 0.0f, o = 0.0f;
+        float mx = A4_NONE, L = 0.0f, o = 0.0f;
         for (int x = 0; x < W; ++x) mx = fmaxf(mx, ml[(x * GH + h) * 2]);
         for (int x = 0; x < W; ++x) {
-            const float mw = ml[(x * GH + h) * 2];
-            // a wave without a chunk has no maximum
-            const float f = mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - mx);
+            const float f = __builtin_amdgcn_exp2f(ml[(x * GH + h) * 2] - mx);
             L = __builtin_fmaf(f, ml[(x * GH + h) * 2 + 1], L);
             o = __builtin_fmaf(f, mo[(x * GH + h) * HD + c], o);
         }

@@ -181,3 +181,39 @@ def test_attention_every_bit_of_the_queries(ops, H, hd):
     q = q.reshape(1, -1)
     close(c.attention_decode(q, [2], scale=2.0 ** -7),
           *attn_exact(m, q, [2], 1, hd, 2.0 ** -7, ds=False))
+
+
+@pytest.mark.parametrize("n", [129, 257, 300, 1025, 1200])
+@pytest.mark.parametrize("H,Hkv,hd", [(1, 1, 64), (4, 1, 128), (2, 2, 32), (1, 1, 256)])
+def test_attention_nan_keys_fill_a_chunk(ops, H, Hkv, hd, n):
+    """Poisoned keys at every position of the last chunk, or of the first 128: the head
+    is NaN, also where a wave has nothing else."""
+    rng = np.random.default_rng(n)
+    q = rng.standard_normal((1, H * hd), dtype=np.float32)
+    for bad in (slice((n - 1) // 128 * 128, n), slice((n - 1) // 64 * 64, n), slice(0, 128)):
+        k, v = rng.standard_normal((2, 1, n, Hkv * hd), dtype=np.float32)
+        k[0, bad, 3::hd] = np.nan
+        c = ops.Kv4Cache(1, Hkv, -(-n // 32) * 32, hd)
+        c.append(k, v, [0])
+        assert np.isnan(c.attention_decode(q, [n - 1])).all()
+
+
+@pytest.mark.parametrize("B,Hkv,n", [(1, 1, 200), (16, 32, 1150), (1, 1, 5000)])
+def test_attention_scores_of_minus_infinity(ops, B, Hkv, n):
+    """Finite queries and keys whose product leaves f32 downwards at the first 128
+    positions: those have no weight, as in f32."""
+    rng = np.random.default_rng(n)
+    hd, cap = 64, -(-n // 32) * 32
+    q = rng.standard_normal((B, Hkv, hd), dtype=np.float32)
+    q[..., 0] = 1e30
+    k, v = rng.standard_normal((2, B, n, Hkv, hd), dtype=np.float32)
+    k[..., :32] = 0
+    k[:, :128, :, 0] = -1e30
+    c, m = stored(ops, k.reshape(B, n, -1), v.reshape(B, n, -1), Hkv, cap)
+    out = c.attention_decode(q.reshape(B, -1), [n - 1] * B)
+    # the definition without those positions
+    keep = slice(128, n)
+    part = {x: y[:, :, keep] for x, y in m.items()}
+    q[..., 0] = 0
+    ref, tol = attn_exact(part, q.reshape(B, -1), [n - 129] * B, Hkv, hd, 0.125)
+    close(out, ref, tol)
