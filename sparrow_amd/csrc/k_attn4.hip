@@ -66,7 +66,7 @@ struct Attn4Params {
     int H, G, ch, W;
     int shares;  // of a split launch (0: one workgroup a pair of head and sequence)
     int parts;  // workgroups that share a kv head's queries
-    float scale2;  // score scale * log2(e)
+    float scale;
     int *guard;
 };
 
@@ -79,6 +79,11 @@ __device__ __forceinline__ float swap32(float v, float (*f)(float, float)) {
     const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
                                                     false);
     return f(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+// log2(e) multiplies scores' distances from the maximum: in the score scale it would
+// round at a score's own magnitude, 2^-10 of a weight at scores of 16000.
+__device__ __forceinline__ float a4_exp(float x) {
+    return __builtin_amdgcn_exp2f(x * 1.44269504f);
 }
 __device__ __forceinline__ float add_f(float a, float b) { return a + b; }
 __device__ __forceinline__ float max_f(float a, float b) { return fmaxf(a, b); }
@@ -560,7 +565,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             }
         }
 
-        // 4. scores in powers of two, each position's in one of the lanes that hold it
+        // 4. scores, each position's in one of the lanes that hold it
         float s[GH][NS / GR];
         {
             uint32_t km[NS][GL];
@@ -620,17 +625,17 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
             float mx = m[h];
 #pragma unroll
             for (int j = 0; j < NS / GR; ++j) {
-                s[h][j] = p0 + own_place(j) <= pos ? ldexpf(s[h][j] * p.scale2, qe[h])
+                s[h][j] = p0 + own_place(j) <= pos ? ldexpf(s[h][j] * p.scale, qe[h])
                                                    : -__builtin_inff();
                 mx = fmaxf(mx, s[h][j]);
             }
             mx = swap32(swap16(row16_max(mx), max_f), max_f);
-            corr[h] = __builtin_amdgcn_exp2f(m[h] - mx);
+            corr[h] = a4_exp(m[h] - mx);
             m[h] = mx;
             l[h] *= corr[h];
 #pragma unroll
             for (int j = 0; j < NS / GR; ++j) {
-                s[h][j] = __builtin_amdgcn_exp2f(s[h][j] - mx);
+                s[h][j] = a4_exp(s[h][j] - mx);
                 l[h] += s[h][j];
             }
             float P[NS];
@@ -710,7 +715,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
         float mx = A4_NONE, L = 0.0f, o = 0.0f;
         for (int x = 0; x < W; ++x) mx = fmaxf(mx, ml[(x * GH + h) * 2]);
         for (int x = 0; x < W; ++x) {
-            const float f = __builtin_amdgcn_exp2f(ml[(x * GH + h) * 2] - mx);
+            const float f = a4_exp(ml[(x * GH + h) * 2] - mx);
             L = __builtin_fmaf(f, ml[(x * GH + h) * 2 + 1], L);
             o = __builtin_fmaf(f, mo[(x * GH + h) * HD + c], o);
         }
@@ -745,7 +750,7 @@ __global__ __launch_bounds__(KV4_MAX_HD) void attn4_merge_kernel(Attn4Params p) 
         const int s = min(c, live - 1);
         const float m = pw[s * ld + hd], l = pw[s * ld + hd + 1];
         const float mx = swap32(swap16(row16_max(m), max_f), max_f);
-        const float e = __builtin_amdgcn_exp2f(m - mx), f = c < live ? e : 0.0f;
+        const float e = a4_exp(m - mx), f = c < live ? e : 0.0f;
         weight[c] = f;
         const float t = wave_sum_dpp(c < live ? f * l : 0.0f);
         if (c == 0) sum = t;
@@ -840,7 +845,7 @@ int launch_attn4(const Attn4Args &a, hipStream_t st) {
     p.W = pl.W;
     p.parts = pl.parts;
     p.ch = attn4_ch(a.c.hd);
-    p.scale2 = a.scale * 1.44269504088896340736f;
+    p.scale = a.scale;
     p.guard = guard_flag_ptr();
     VMLM_GUARD(!p.shares || p.work, "kv4 attention: split positions need a workspace");
     const int rows = p.shares ? attn4_rows(pl, a.c.B) : a.c.B;

@@ -217,3 +217,22 @@ def test_attention_scores_of_minus_infinity(ops, B, Hkv, n):
     q[..., 0] = 0
     ref, tol = attn_exact(part, q.reshape(B, -1), [n - 129] * B, Hkv, hd, 0.125)
     close(out, ref, tol)
+
+
+@pytest.mark.parametrize("H,Hkv,hd,n", [(1, 1, 64, 100), (4, 1, 128, 300), (2, 2, 32, 60), (2, 1, 256, 200),
+                                        (1, 1, 64, 3000)])
+def test_attention_scores_far_from_zero(ops, H, Hkv, hd, n):
+    """Scores of 15360 and a few more, exact in f32: the weights depend on their
+    differences, so that log2(e) must not round the scores themselves."""
+    rng = np.random.default_rng(n)
+    q = np.zeros((1, H, hd), np.float32)
+    q[..., 0], q[..., 1] = 8192, 8
+    k = np.zeros((1, n, Hkv, hd), np.float32)
+    k[..., 0] = 15
+    k[..., 1] = rng.integers(0, 6, (1, n, Hkv))
+    v = rng.standard_normal((1, n, Hkv * hd), dtype=np.float32)
+    c, m = stored(ops, k.reshape(1, n, -1), v, Hkv, -(-n // 32) * 32)
+    assert np.array_equal(m["k"][0, :, :n], k[0].transpose(1, 0, 2))
+    q = q.reshape(1, -1)
+    close(c.attention_decode(q, [n - 1], scale=0.125),
+          *attn_exact(m, q, [n - 1], Hkv, hd, 0.125, ds=False))
