@@ -21,13 +21,15 @@ namespace vmlm {
 constexpr int KV4_BLOCK = 32;
 
 // The meta of 32 values with lowest lo and highest hi (NaN among them gives both
-// NaN); NaN twice where one of them is not finite or their range leaves f32.
+// NaN); NaN twice where one of them is not finite or their range leaves f32. (Judged
+// before the bits are rounded outward, where a NaN's may wrap to zero.)
 __device__ __forceinline__ uint32_t kv4_meta(float lo, float hi) {
     const uint32_t b = __float_as_uint(lo);
     const uint32_t mn = ((b >> 31) ? b + 0xffffu : b) & 0xffff0000u;
     const float q = (hi - __uint_as_float(mn)) / 15.0f;
     const uint32_t sc = (__float_as_uint(q) + 0xffffu) & 0xffff0000u;
-    const bool ok = (mn & 0x7f800000u) != 0x7f800000u && (sc & 0x7f800000u) != 0x7f800000u;
+    const bool ok = fabsf(lo) <= 3.40282347e38f && fabsf(q) <= 3.40282347e38f &&
+                    (mn & 0x7f800000u) != 0x7f800000u && (sc & 0x7f800000u) != 0x7f800000u;
     return ok ? mn | (sc >> 16) : 0x7fc07fc0u;
 }
 __device__ __forceinline__ float kv4_scale(uint32_t meta) { return __uint_as_float(meta << 16); }

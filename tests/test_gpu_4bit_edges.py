@@ -236,3 +236,34 @@ def test_attention_scores_far_from_zero(ops, H, Hkv, hd, n):
     q = q.reshape(1, -1)
     close(c.attention_decode(q, [n - 1], scale=0.125),
           *attn_exact(m, q, [n - 1], Hkv, hd, 0.125, ds=False))
+
+
+# ------------------------------------------------------------------ the cache
+def nan_of(bits):
+    return np.array([bits], np.uint32).view(np.float32)[0]
+
+
+@pytest.mark.parametrize("bits", [0x7FC00000, 0xFFC00000, 0x7F800001, 0x7FFFFFFF, 0xFF800001, 0xFFFF0000,
+                                  0xFFFF0001, 0xFFFFFFFF])
+def test_cache_any_nan_poisons(ops, bits):
+    """Every NaN, whatever its bits, and also 32 of them, gives NaN in its 32 channels
+    alone; the same for a row that the attention appends."""
+    rng = np.random.default_rng(6)
+    x = rng.standard_normal((1, 4, 128), dtype=np.float32)
+    x.view(np.uint32)[0, 0, 5] = bits
+    x.view(np.uint32)[0, 1, 32:64] = bits
+    x.view(np.uint32)[0, 2, 64] = bits
+    poisoned = np.zeros((1, 4, 128), bool)
+    poisoned[0, 0, :32] = poisoned[0, 1, 32:64] = poisoned[0, 2, 64:96] = True
+    c = ops.Kv4Cache(1, 1, 32, 128)
+    c.append(x, x, [0])
+    for y in c.read([0], 4):
+        assert np.isnan(y[poisoned]).all() and np.isfinite(y[~poisoned]).all()
+    q = rng.standard_normal((1, 128), dtype=np.float32)
+    for at in range(3):
+        good = rng.standard_normal((1, 128), dtype=np.float32)
+        c = ops.Kv4Cache(1, 1, 32, 128)
+        out = c.attention_decode(q, [0], good, x[:, at])
+        assert np.isnan(out[poisoned[:, at]]).all() and np.isfinite(out[~poisoned[:, at]]).all()
+        c = ops.Kv4Cache(1, 1, 32, 128)
+        assert np.isnan(c.attention_decode(q, [0], x[:, at], good)).all()
