@@ -267,3 +267,61 @@ def test_cache_any_nan_poisons(ops, bits):
         assert np.isnan(out[poisoned[:, at]]).all() and np.isfinite(out[~poisoned[:, at]]).all()
         c = ops.Kv4Cache(1, 1, 32, 128)
         assert np.isnan(c.attention_decode(q, [0], x[:, at], good)).all()
+
+
+# ------------------------------------------------------------------ a prompt, then its decode
+def test_prompt_then_decode(dev, ops):
+    """A prompt as the documentation has it, for as many kv heads as heads: the head
+    norms alone for the prefill attention, which rotates; norm and rotation for the cache's
+    rows; then decode steps over the cache. The prefill's outputs are checked against the
+    rotated rows' attention, the cache's rows against the rotated rows, and the
+    decode steps against 64 bits over what the cache holds."""
+    rng = np.random.default_rng(17)
+    H, hd, S, steps, cap, theta = 3, 64, 70, 4, 96, 10000.0
+    w, scale = H * hd, 0.125
+    x = rng.standard_normal((S + steps, 3 * w), dtype=np.float32)  # fused q, k, v
+    g = (1 + rng.standard_normal((2, hd)) / 8).astype(np.float32)
+    pos = np.arange(S + steps, dtype=np.int32)
+    q, k, v = np.split(x, 3, 1)
+    rot = [norm_ref(t, gg, pos, hd, 1e-5, theta)[0] for t, gg in ((q, g[0]), (k, g[1]))]
+    dx, dg, dp = dev.up(x), dev.up(g), dev.up(pos)
+    nq, nk, rk, out, vv = (dev.zeros(S, w) for _ in range(5))
+    vv.put(v[:S])
+    c = ops.Kv4Cache(1, H, cap, hd)
+    keep, d = device_cache(dev, c)
+    zero = dev.up(np.zeros(1, np.int32))
+    dev.sync()
+
+    def norm(qo, ko, first, rows, at):
+        src = dx.ptr + first * 12 * w
+        dev.check(dev.L.vmlm_hip_qk_norm_rope(qo.ptr, w, ko.ptr, w, src, 3 * w, src + 4 * w, 3 * w,
+                                              dg.ptr, dg.ptr + 4 * hd, at, rows, H, H, hd, 1e-5, theta,
+                                              None))
+    norm(nq, nk, 0, S, None)
+    dev.check(dev.L.vmlm_hip_attention_prefill(nq.ptr, nk.ptr, vv.ptr, out.ptr, S, H, hd, theta, 0,
+                                               scale, True, None))
+    norm(nq, rk, 0, S, dp.ptr)
+    dev.check(dev.L.vmlm_hip_kv4_append(d, rk.ptr, w, dx.ptr + 8 * w, 3 * w, zero.ptr, None, S, None))
+    dev.sync()
+    got = out.get().astype(np.float64)
+    for h in range(H):
+        at = slice(h * hd, (h + 1) * hd)
+        s = rot[0][:S, at] @ rot[1][:S, at].T * scale
+        s = np.where(np.tril(np.ones((S, S), bool)), s, -np.inf)
+        p = np.exp(s - s.max(1, keepdims=True))
+        ref = p / p.sum(1, keepdims=True) @ v[:S, at].astype(np.float64)
+        # the prefill's own bound: bf16 terms, 1e-4 of the RMS
+        assert np.abs(got[:, at] - ref).max() <= 1e-4 * np.sqrt((ref ** 2).mean())
+    m = new_model(1, H, cap, hd)
+    hk = rk.get()
+    close(hk, rot[1][:S], norm_ref(k[:S], g[1], pos[:S], hd, 1e-5, theta)[1])
+    put(m, hk, v[:S], 0, 0, S, H)
+    sq, sk, so = (dev.zeros(1, w) for _ in range(3))
+    for i in range(S, S + steps):
+        norm(sq, sk, i, 1, dp.ptr + 4 * i)
+        dev.check(dev.L.vmlm_hip_attention_decode_kv4(
+            d, sq.ptr, w, sk.ptr, dx.ptr + i * 12 * w + 8 * w, w, dp.ptr + 4 * i, so.ptr, w, H, scale,
+            None, 0, None))
+        dev.sync()
+        put(m, sk.get(), v[i:i + 1], 0, i, 1, H)
+        close(so.get(), *attn_exact(m, sq.get(), [i], H, hd, scale))
