@@ -1062,12 +1062,22 @@ static int check_kv4(const vmlm_kv4_cache *c, Kv4View *v, bool device = true) {
     VMLM_GUARD(!device || ((((uintptr_t)v->k | (uintptr_t)v->v) & 15) == 0 &&
                            (((uintptr_t)v->km | (uintptr_t)v->vm) & 3) == 0),
                "kv4: k and v must be 16-byte aligned, k_meta and v_meta 4-byte");
+    const size_t vals = c->batch * c->n_kv_heads * c->cap * c->head_dim;
+    VMLM_GUARD(!overlap(v->k, vals / 2, v->v, vals / 2) && !overlap(v->km, vals / 8, v->vm, vals / 8) &&
+                   !overlap(v->k, vals / 2, v->km, vals / 8) &&
+                   !overlap(v->k, vals / 2, v->vm, vals / 8) &&
+                   !overlap(v->v, vals / 2, v->km, vals / 8) &&
+                   !overlap(v->v, vals / 2, v->vm, vals / 8),
+               "kv4: the cache's arrays lie over each other");
     return VMLM_OK;
 }
 
-// Whether `rows` rows of w floats at stride ld lie over one of the cache's arrays.
-static bool over_cache(const Kv4View &c, const float *p, size_t ld, size_t w, size_t rows) {
-    const size_t vals = (size_t)c.B * c.Hkv * c.cap * c.hd, bytes = ((rows - 1) * ld + w) * 4;
+// The bytes from the first of `rows` rows of w floats at stride ld to the end of the last.
+static size_t span(size_t ld, size_t w, size_t rows) { return ((rows - 1) * ld + w) * 4; }
+
+// Whether `rows` rows of w floats (or int32) at stride ld lie over one of the cache's arrays.
+static bool over_cache(const Kv4View &c, const void *p, size_t ld, size_t w, size_t rows) {
+    const size_t vals = (size_t)c.B * c.Hkv * c.cap * c.hd, bytes = span(ld, w, rows);
     return overlap(p, bytes, c.k, vals / 2) || overlap(p, bytes, c.v, vals / 2) ||
            overlap(p, bytes, c.km, vals / 8) || overlap(p, bytes, c.vm, vals / 8);
 }
@@ -1147,6 +1157,9 @@ static int check_headnorm(const HeadNormArgs &a, size_t rows, size_t H, size_t H
                        !rows_overlap(g, hd, hd, a.ko, (rows - 1) * a.ldko + wk,
                                      Hkv ? (rows - 1) * a.ldko + wk : 0, 1),
                    "qk_norm_rope: an output lies over a gain");
+    VMLM_GUARD(!a.pos || ((H == 0 || !overlap(a.pos, rows * 4, a.qo, span(a.ldqo, wq, rows))) &&
+                          (Hkv == 0 || !overlap(a.pos, rows * 4, a.ko, span(a.ldko, wk, rows)))),
+               "qk_norm_rope: an output lies over the positions");
     return VMLM_OK;
 }
 
@@ -1182,7 +1195,7 @@ int vmlm_hip_qk_norm_rope(float *q_out, size_t ldqo, float *k_out, size_t ldko, 
 
 // Rows [B][S] of the cache's width beside it.
 static int check_kv4_rows(const Kv4View &c, const float *k, size_t ldk, const float *v, size_t ldv,
-                          const int32_t *pos0, size_t S) {
+                          const int32_t *pos0, const int32_t *count, size_t S, bool read) {
     VMLM_GUARD(S <= DIM_MAX, "kv4: %zu rows a sequence (limit 2^30)", S);
     if (c.B == 0 || c.Hkv == 0 || S == 0) return VMLM_OK;
     VMLM_GUARD(c.cap > 0, "kv4: capacity 0");
@@ -1194,6 +1207,17 @@ static int check_kv4_rows(const Kv4View &c, const float *k, size_t ldk, const fl
     VMLM_GUARD(rows <= ((size_t)1 << 50) / most, "kv4: %zu rows of %zu values (limit 2^50)", rows, most);
     VMLM_GUARD(!over_cache(c, k, ldk, w, rows) && !over_cache(c, v, ldv, w, rows),
                "kv4: rows lie over the cache");
+    const size_t nb = (size_t)c.B * 4;
+    if (read) {
+        VMLM_GUARD(!rows_overlap(k, ldk, w, v, ldv, w, rows), "kv4_read: k and v lie over each other");
+        for (const int32_t *p : {pos0, count})
+            VMLM_GUARD(!p || (!overlap(p, nb, k, span(ldk, w, rows)) &&
+                              !overlap(p, nb, v, span(ldv, w, rows))),
+                       "kv4_read: rows lie over the positions or counts");
+    } else {
+        VMLM_GUARD(!over_cache(c, pos0, c.B, c.B, 1) && (!count || !over_cache(c, count, c.B, c.B, 1)),
+                   "kv4_append: positions or counts lie over the cache");
+    }
     return VMLM_OK;
 }
 
@@ -1202,7 +1226,7 @@ int vmlm_hip_kv4_append(const vmlm_kv4_cache *cache, const float *k, size_t ldk,
                         void *stream) {
     Kv4View c;
     int rc = check_kv4(cache, &c);
-    if (!rc) rc = check_kv4_rows(c, k, ldk, v, ldv, pos0, S);
+    if (!rc) rc = check_kv4_rows(c, k, ldk, v, ldv, pos0, count, S, false);
     if (rc || c.B == 0 || c.Hkv == 0 || S == 0) return rc;
     INIT_OR_RETURN();
     if ((rc = on_library_device())) return rc;
@@ -1213,11 +1237,8 @@ int vmlm_hip_kv4_read(const vmlm_kv4_cache *cache, float *k, size_t ldk, float *
                       const int32_t *pos0, const int32_t *count, size_t S, void *stream) {
     Kv4View c;
     int rc = check_kv4(cache, &c);
-    if (!rc) rc = check_kv4_rows(c, k, ldk, v, ldv, pos0, S);
+    if (!rc) rc = check_kv4_rows(c, k, ldk, v, ldv, pos0, count, S, true);
     if (rc || c.B == 0 || c.Hkv == 0 || S == 0) return rc;
-    const size_t w = (size_t)c.Hkv * c.hd;
-    VMLM_GUARD(!rows_overlap(k, ldk, w, v, ldv, w, (size_t)c.B * S),
-               "kv4_read: k and v lie over each other");
     INIT_OR_RETURN();
     if ((rc = on_library_device())) return rc;
     return launch_kv4_read(c, k, ldk, v, ldv, pos0, count, (int)S, as_stream(stream));
@@ -1261,14 +1282,21 @@ int vmlm_hip_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, s
                                !rows_overlap(out, ldo, w, v_new, ldkv, wk, B))),
                "kv4 attention: the output lies over its input");
     VMLM_GUARD(!over_cache(a.c, out, ldo, w, B), "kv4 attention: the output lies over the cache");
+    VMLM_GUARD(!overlap(out, span(ldo, w, B), pos, B * 4),
+               "kv4 attention: the output lies over the positions");
+    VMLM_GUARD(!k_new || (!over_cache(a.c, q, ldq, w, B) && !over_cache(a.c, k_new, ldkv, wk, B) &&
+                          !over_cache(a.c, v_new, ldkv, wk, B) && !over_cache(a.c, pos, B, B, 1)),
+               "kv4 attention: an input lies over the cache, which takes the new rows");
     const size_t wf = attn4_work_floats(a.c, (int)n_heads);
     if (wf && work) {
         VMLM_GUARD(work_bytes >= wf * 4 && ((uintptr_t)work & 15) == 0,
                    "kv4 attention: workspace of %zu bytes, %zu needed (16-byte aligned)",
                    work_bytes, wf * 4);
-        VMLM_GUARD(!overlap(work, wf * 4, out, ((B - 1) * ldo + w) * 4) &&
-                       !overlap(work, wf * 4, q, ((B - 1) * ldq + w) * 4) &&
-                       !over_cache(a.c, (float *)work, wf, wf, 1),
+        VMLM_GUARD(!overlap(work, wf * 4, out, span(ldo, w, B)) &&
+                       !overlap(work, wf * 4, q, span(ldq, w, B)) &&
+                       (!k_new || (!overlap(work, wf * 4, k_new, span(ldkv, wk, B)) &&
+                                   !overlap(work, wf * 4, v_new, span(ldkv, wk, B)))) &&
+                       !overlap(work, wf * 4, pos, B * 4) && !over_cache(a.c, work, wf, wf, 1),
                    "kv4 attention: the workspace lies over an operand");
     }
     INIT_OR_RETURN();
@@ -1798,7 +1826,7 @@ int vmlm_kv4_append(const vmlm_kv4_cache *cache, const float *k, const float *v,
     Kv4View c;
     int rc = check_kv4(cache, &c, false);
     const size_t w = rc ? 0 : (size_t)c.Hkv * c.hd, rows = rc ? 0 : c.B * S;
-    if (!rc) rc = check_kv4_rows(c, k, w, v, w, pos0, S);
+    if (!rc) rc = check_kv4_rows(c, k, w, v, w, pos0, count, S, false);
     if (rc || rows == 0 || w == 0) return rc;
     HOST_CALL_BEGIN();
     {
@@ -1819,7 +1847,7 @@ int vmlm_kv4_read(const vmlm_kv4_cache *cache, float *k, float *v, const int32_t
     Kv4View c;
     int rc = check_kv4(cache, &c, false);
     const size_t w = rc ? 0 : (size_t)c.Hkv * c.hd, rows = rc ? 0 : c.B * S;
-    if (!rc) rc = check_kv4_rows(c, k, w, v, w, pos0, S);
+    if (!rc) rc = check_kv4_rows(c, k, w, v, w, pos0, count, S, true);
     if (rc || rows == 0 || w == 0) return rc;
     HOST_CALL_BEGIN();
     {

@@ -194,3 +194,68 @@ def test_quantize_int4_round_trip():
         back = ((u.astype(np.int8) ^ 8) - 8) * np.repeat(s, group, 1)[:, :96]
         # half a step, and the rounding of w / s
         assert (np.abs(back - w) <= np.repeat(s, group, 1)[:, :96] * (0.5 + 1e-5)).all()
+
+
+# ------------------------------------------------------------------ operands over each other
+FAR = 0x60000000  # behind every operand of the calls above
+
+
+def test_norm_output_over_the_positions_refused(L):
+    """Rows that other workgroups have yet to look up would find values there."""
+    for bad in (dict(pos=Y), dict(pos=Y + 4 * (3 * 256 - 1)), dict(pos=Z - 8), dict(pos=Z + 4 * 200)):
+        assert norm(L, **bad) == 9, bad
+        assert "over the positions" in message(L)
+
+
+def test_cache_arrays_over_each_other_refused(L):
+    """2 * 2 * 64 * 64 values: 8192 bytes of codes, 2048 of meta."""
+    for bad in (dict(v=A), dict(v=A + 8176), dict(k_meta=A + 4096), dict(v_meta=A + 8188),
+                dict(k_meta=Q), dict(v_meta=Q + 8188), dict(v_meta=S), dict(v_meta=S + 2044),
+                dict(k_meta=S + 0x1000000 - 2044)):
+        for fn in ("vmlm_hip_kv4_append", "vmlm_hip_kv4_read"):
+            assert rows(L, fn, cache(**bad)) == 9, bad
+            assert "over each other" in message(L)
+        assert attend(L, cache(**bad)) == 9, bad
+        n = C.c_size_t()
+        assert L.vmlm_hip_attention_decode_kv4_work(cache(**bad), 4, C.byref(n)) == 9
+
+
+def test_positions_over_what_is_written_refused(L):
+    at_cache = (A, A + 8188, Q + 8188, S + 2044, S + 0x1000000)
+    for at in at_cache:
+        assert rows(L, "vmlm_hip_kv4_append", cache(), pos0=at) == 9, hex(at)
+        assert rows(L, "vmlm_hip_kv4_append", cache(), count=at) == 9, hex(at)
+        assert "positions or counts" in message(L)
+        assert attend(L, cache(), pos=at) == 9, hex(at)
+    # 2 x 3 rows of 128 floats
+    for at in (Y, Y + 4 * 767, Z, Z + 4 * 767, Z - 4):
+        assert rows(L, "vmlm_hip_kv4_read", cache(), pos0=at) == 9, hex(at)
+        assert rows(L, "vmlm_hip_kv4_read", cache(), count=at) == 9, hex(at)
+        assert "positions or counts" in message(L)
+    assert attend(L, cache(), pos=Y + 0x100000 + 4 * 511) == 9
+    assert "positions" in message(L)
+
+
+def test_inputs_over_the_cache_that_takes_new_rows_refused(L):
+    for at in (A, A + 8188, Q, S + 2044, S + 0x1000000):
+        for bad in (dict(q=at), dict(k=at), dict(v=at)):
+            assert attend(L, cache(), **bad) == 9, bad
+            assert "over the cache" in message(L)
+
+
+def test_workspace_over_any_operand_refused(L):
+    n = C.c_size_t()
+    long = cache(cap=65536, batch=1)
+    assert L.vmlm_hip_attention_decode_kv4_work(long, 4, C.byref(n)) == 0 and n.value
+    args = dict(q=FAR, k=FAR + 0x100000, v=FAR + 0x200000, pos=FAR + 0x300000, out=FAR + 0x400000)
+    width = dict(q=1024, k=512, v=512, pos=4, out=1024)
+    for name, at in args.items():
+        for work in (at, at + width[name] // 16 * 16 - 16 if width[name] > 16 else at,
+                     (at - n.value) // 16 * 16 + 16):
+            assert attend(L, long, **args, work=work, nbytes=n.value) == 9, (name, hex(work))
+            assert "workspace" in message(L)
+
+
+def test_host_read_over_itself_refused(L):
+    assert L.vmlm_kv4_read(cache(), Y, Y + 4, A - 64, None, 3) == 9
+    assert "over each other" in message(L)
