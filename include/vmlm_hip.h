@@ -359,7 +359,8 @@ int vmlm_hip_kv4_append(const vmlm_kv4_cache *cache, const float *k, size_t ldk,
                         size_t ldv, const int32_t *pos0, const int32_t *count, size_t S,
                         void *stream);
 /* The other way: the same rows as the f32 values that the cache holds. Rows of idle
- * sequences, from count[b] on and from cap on are left as they are. */
+ * sequences, from count[b] on and from cap on are left as they are (the last reported
+ * as above). */
 int vmlm_hip_kv4_read(const vmlm_kv4_cache *cache, float *k, size_t ldk, float *v, size_t ldv,
                       const int32_t *pos0, const int32_t *count, size_t S, void *stream);
 /* One token a sequence: k_new, v_new [batch][ldkv] (both null: nothing) are stored

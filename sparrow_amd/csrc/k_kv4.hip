@@ -27,11 +27,9 @@ __device__ __forceinline__ bool kv4_rows(const Kv4Params &p, int b, int blk, int
     if (pos0 < 0) return false;  // idle
     int n = p.count ? min(max(p.count[b], 0), p.S) : p.S;
     const int room = p.c.cap - pos0;
-    if (n > room) {
-        if (blk == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(p.guard, 1);
-        if (room <= 0) return false;
-        n = room;
-    }
+    if (n > max(room, 0) && blk == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(p.guard, 1);
+    n = min(n, room);
+    if (n <= 0) return false;
     *first = (pos0 / KV4_BLOCK + blk) * KV4_BLOCK;
     *pos = pos0;
     *t0 = max(0, *first - pos0);

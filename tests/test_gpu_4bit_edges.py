@@ -269,6 +269,16 @@ def test_cache_any_nan_poisons(ops, bits):
         assert np.isnan(c.attention_decode(q, [0], x[:, at], good)).all()
 
 
+def test_cache_no_rows_to_drop(ops):
+    """A sequence without a row trips no guard, wherever its first position lies."""
+    c = ops.Kv4Cache(2, 1, 64, 64)
+    x = np.ones((2, 3, 64), np.float32)
+    c.append(x, x, [1000, 5], [0, 3])
+    c.append(x, x, [2 ** 31 - 1, 5], [-4, 3])
+    k, _ = c.read([65, 5], 3, [0, 3])
+    assert not k[0].any() and (k[1] == 1).all()
+
+
 # ------------------------------------------------------------------ a prompt, then its decode
 def test_prompt_then_decode(dev, ops):
     """A prompt as the documentation has it, for as many kv heads as heads: the head
