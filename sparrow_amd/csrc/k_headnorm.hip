@@ -16,6 +16,8 @@
 // Angles: pos * theta^(-2i/hd) / 2 pi is formed in 64 bits and its whole turns
 // dropped there; a 32-bit product would be off by 2^-24 of the angle itself (0.006 at
 // position 100000), more than the values' own rounding from a few positions on.
+#include <algorithm>
+
 #include "internal.hpp"
 
 namespace vmlm {
@@ -102,6 +104,23 @@ int launch_lh(const HeadNormParams &p, hipStream_t st) {
 
 int launch_headnorm(const HeadNormArgs &a, hipStream_t st) {
     HeadNormParams p;
+    // (a grid has at most 2^32 - 1 threads along its rows)
+    constexpr int ROWS = 1 << 23;
+    if (a.rows > ROWS) {
+        for (int r = 0; r < a.rows;) {
+            HeadNormArgs part = a;
+            part.rows = std::min(ROWS, a.rows - r);
+            part.q = a.q + r * a.ldq;
+            part.k = a.k + r * a.ldk;
+            part.qo = a.qo + r * a.ldqo;
+            part.ko = a.ko + r * a.ldko;
+            part.pos = a.pos ? a.pos + r : nullptr;
+            const int rc = launch_headnorm(part, st);
+            if (rc) return rc;
+            r += part.rows;
+        }
+        return VMLM_OK;
+    }
     p.q = a.q;
     p.k = a.k;
     p.gq = a.gq ? a.gq : a.gk;

@@ -335,3 +335,26 @@ def test_prompt_then_decode(dev, ops):
         dev.sync()
         put(m, sk.get(), v[i:i + 1], 0, i, 1, H)
         close(so.get(), *attn_exact(m, sq.get(), [i], H, hd, scale))
+
+
+# ------------------------------------------------------------------ sizes past a launch's grid
+def test_norm_rows_past_one_grid(dev):
+    """More rows than a grid of 256 threads a row can have."""
+    rng = np.random.default_rng(7)
+    rows, hd, tile = (1 << 24) + 5, 8, 1 << 18
+    x = rng.standard_normal((tile, hd), dtype=np.float32)
+    p = rng.integers(0, 1000, tile).astype(np.int32)
+    reps = -(-rows // tile)
+    q, pos = (dev.up(np.concatenate([t] * reps)[:rows]) for t in (x, p))
+    g = np.ones(hd, np.float32)
+    dg, out = dev.up(g), dev.zeros(rows + 1, hd)
+    dev.sync()
+    dev.check(dev.L.vmlm_hip_qk_norm_rope(out.ptr, hd, None, 0, q.ptr, hd, None, 0, dg.ptr, None,
+                                          pos.ptr, rows, 1, 0, hd, 1e-5, 1e4, None))
+    dev.sync()
+    got = out.get()
+    assert not got[rows].any()
+    ref, tol = norm_ref(x, g, p, hd, 1e-5, 1e4)
+    for i in range(reps):
+        part = got[i * tile:min(rows, (i + 1) * tile)]
+        assert (np.abs(part - ref[:len(part)]) <= tol[:len(part)]).all(), i
