@@ -82,8 +82,10 @@ __global__ __launch_bounds__(256) void headnorm_kernel(HeadNormParams p) {
         for (int e = 0; e < 4; ++e) {
             const float a = x0[e] * inv * (isq ? gq0[e] : gk0[e]);
             const float b = x1[e] * inv * (isq ? gq1[e] : gk1[e]);
-            y0[e] = a * c[e] - b * s[e];
-            y1[e] = a * s[e] + b * c[e];
+            // (a pair is turned where there are positions only: an infinity or a NaN of one
+            // channel is not its partner's in the norm alone)
+            y0[e] = p.pos ? a * c[e] - b * s[e] : a;
+            y1[e] = p.pos ? a * s[e] + b * c[e] : b;
         }
         if (live) {
             *(f32x4a *)(dst + i0) = y0;

@@ -358,3 +358,19 @@ def test_norm_rows_past_one_grid(dev):
     for i in range(reps):
         part = got[i * tile:min(rows, (i + 1) * tile)]
         assert (np.abs(part - ref[:len(part)]) <= tol[:len(part)]).all(), i
+
+
+# ------------------------------------------------------------------ norms
+def test_norm_alone_keeps_channels_apart(ops):
+    """Without positions nothing is rotated: a channel whose gain or value is not
+    finite leaves its partner in the other half as it is."""
+    rng = np.random.default_rng(9)
+    q = rng.standard_normal((2, 64), dtype=np.float32)
+    g = np.ones(64, np.float32)
+    g[3], g[40] = np.inf, np.nan
+    got, _ = ops.qk_norm_rope(q, q[:, :0], g, g, None, 64)
+    finite = np.ones(64, np.float32)
+    ref, tol = norm_ref(q, finite, None, 64, 1e-5, 1e4)
+    ok = np.isfinite(g)
+    assert (np.abs(got - ref)[:, ok] <= tol[:, ok]).all()
+    assert np.isinf(got[:, 3]).all() and np.isnan(got[:, 40]).all()
