@@ -6,9 +6,8 @@
 //
 // A head is held by LH lanes (the power of two from hd/8), each with four values
 // of the first half and the four that they are turned with: two 16-byte loads,
-// no exchange between lanes but the sum of squares. A wave keeps one row's
-// sines and cosines in registers and carries 64 / LH of the row's heads at a
-// time through them.
+// no exchange between lanes but the sum of squares. A wave takes 64 / LH of a
+// row's heads, each lane its four sines and cosines.
 //
 // Bound by the rows' bytes, read once and written once: 2048 rows of 36 + 36 heads of 64
 // take 14.6 us, 5.2 TB/s (a large copy 5.1). One row takes 2.8 us, a launch and a latency.
@@ -33,71 +32,76 @@ struct HeadNormParams {
     size_t ldq, ldk, ldqo, ldko;
     const int32_t *pos;
     int rows, H, Hkv, hd;
-    int per;  // heads a wave carries
     float eps;
     // theta^(-2i/hd) / 2 pi = coarse[i / 16] * fine[i % 16] (256 bytes of arguments: with the
     // table itself, 2 KB of them, a call of one row took 6.2 us instead of 5.0)
     double coarse[HEADNORM_MAX_HD / 32], fine[16];
 };
 
-template <int LH>
+// TURN: with positions. (A pair is turned there only: an infinity or a NaN of one channel
+// is not its partner's in the norm alone.)
+template <int LH, bool TURN>
 __global__ __launch_bounds__(256) void headnorm_kernel(HeadNormParams p) {
     constexpr int HW = 64 / LH;  // heads of a wave at a time
     const int row = blockIdx.x;
     const int wave = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l = lane % LH, half = p.hd / 2, heads = p.H + p.Hkv;
-    int h = wave * p.per;
-    const int hend = min(heads, h + p.per);
-    if (h >= hend) return;
-    const int pos = p.pos ? p.pos[row] : 0;
-    if (pos < 0) return;  // an idle row
+    if (wave * HW >= heads) return;
     const bool in = 4 * l < half;
     const int i0 = in ? 4 * l : 0;
     float s[4], c[4];
+    if constexpr (TURN) {
+        const int pos = p.pos[row];
+        if (pos < 0) return;  // an idle row
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const double t = (double)pos * (p.coarse[i0 / 16] * p.fine[i0 % 16 + e]);
-        sincospif(2.0f * (float)(t - __builtin_rint(t)), &s[e], &c[e]);
+        for (int e = 0; e < 4; ++e) {
+            const double t = (double)pos * (p.coarse[i0 / 16] * p.fine[i0 % 16 + e]);
+            sincospif(2.0f * (float)(t - __builtin_rint(t)), &s[e], &c[e]);
+        }
     }
     const f32x4a gq0 = *(const f32x4a *)(p.gq + i0), gq1 = *(const f32x4a *)(p.gq + half + i0);
     const f32x4a gk0 = *(const f32x4a *)(p.gk + i0), gk1 = *(const f32x4a *)(p.gk + half + i0);
-    for (; h < hend; h += HW) {
-        const int hh = h + lane / LH;
-        const bool live = in && hh < hend, isq = hh < p.H;
-        const int hc = min(hh, hend - 1);
-        const float *src = hc < p.H ? p.q + row * p.ldq + (size_t)hc * p.hd
-                                    : p.k + row * p.ldk + (size_t)(hc - p.H) * p.hd;
-        float *dst = hc < p.H ? p.qo + row * p.ldqo + (size_t)hc * p.hd
-                              : p.ko + row * p.ldko + (size_t)(hc - p.H) * p.hd;
-        f32x4a x0 = *(const f32x4a *)(src + i0), x1 = *(const f32x4a *)(src + half + i0);
-        float ss = 0.0f;
+    const int hh = wave * HW + lane / LH, hc = min(hh, heads - 1);
+    const bool live = in && hh < heads, isq = hc < p.H;
+    const float *src = isq ? p.q + row * p.ldq + (size_t)hc * p.hd
+                           : p.k + row * p.ldk + (size_t)(hc - p.H) * p.hd;
+    float *dst = isq ? p.qo + row * p.ldqo + (size_t)hc * p.hd
+                     : p.ko + row * p.ldko + (size_t)(hc - p.H) * p.hd;
+    f32x4a x0 = *(const f32x4a *)(src + i0), x1 = *(const f32x4a *)(src + half + i0);
+    float ss = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ss = __builtin_fmaf(x0[e], x0[e], __builtin_fmaf(x1[e], x1[e], ss));
-        if (!in) ss = 0.0f;
+    for (int e = 0; e < 4; ++e) ss = __builtin_fmaf(x0[e], x0[e], __builtin_fmaf(x1[e], x1[e], ss));
+    if (!in) ss = 0.0f;
 #pragma unroll
-        for (int o = LH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        const float inv = 1.0f / sqrtf(ss / (float)p.hd + p.eps);
-        f32x4a y0, y1;
+    for (int o = LH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    const float inv = 1.0f / sqrtf(ss / (float)p.hd + p.eps);
+    f32x4a y0, y1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float a = x0[e] * inv * (isq ? gq0[e] : gk0[e]);
-            const float b = x1[e] * inv * (isq ? gq1[e] : gk1[e]);
-            // (a pair is turned where there are positions only: an infinity or a NaN of one
-            // channel is not its partner's in the norm alone)
-            y0[e] = p.pos ? a * c[e] - b * s[e] : a;
-            y1[e] = p.pos ? a * s[e] + b * c[e] : b;
+    for (int e = 0; e < 4; ++e) {
+        const float a = x0[e] * inv * (isq ? gq0[e] : gk0[e]);
+        const float b = x1[e] * inv * (isq ? gq1[e] : gk1[e]);
+        if constexpr (TURN) {
+            y0[e] = a * c[e] - b * s[e];
+            y1[e] = a * s[e] + b * c[e];
+        } else {
+            y0[e] = a;
+            y1[e] = b;
         }
-        if (live) {
-            *(f32x4a *)(dst + i0) = y0;
-            *(f32x4a *)(dst + half + i0) = y1;
-        }
+    }
+    if (live) {
+        *(f32x4a *)(dst + i0) = y0;
+        *(f32x4a *)(dst + half + i0) = y1;
     }
 }
 
 template <int LH>
 int launch_lh(const HeadNormParams &p, hipStream_t st) {
-    const unsigned waves = cdiv((size_t)(p.H + p.Hkv), (size_t)p.per);
-    headnorm_kernel<LH><<<dim3((unsigned)p.rows, cdiv(waves, 4)), 256, 0, st>>>(p);
+    const unsigned waves = cdiv((size_t)(p.H + p.Hkv), 64 / LH);
+    const dim3 grid((unsigned)p.rows, cdiv(waves, 4));
+    if (p.pos)
+        headnorm_kernel<LH, true><<<grid, 256, 0, st>>>(p);
+    else
+        headnorm_kernel<LH, false><<<grid, 256, 0, st>>>(p);
     VMLM_HIP_CHECK(hipGetLastError());
     return VMLM_OK;
 }
@@ -147,7 +151,6 @@ int launch_headnorm(const HeadNormArgs &a, hipStream_t st) {
         p.coarse[i] = p.coarse[i - 1] * (p.fine[15] * ratio);
     int lh = 1;
     while (lh * 8 < a.hd) lh *= 2;
-    p.per = 64 / lh;
     switch (lh) {
     case 1: return launch_lh<1>(p, st);
     case 2: return launch_lh<2>(p, st);
