@@ -50,6 +50,7 @@ struct Int4Params {
     const uint8_t *Q;
     float *C;
     int M, N, K, G, ng, runs;
+    size_t ldc;
     int rg;  // runs of a group (G a multiple of 128)
     // the activations as planes (int4_planes_kernel), or null
     const uint8_t *planes;
@@ -271,7 +272,7 @@ __device__ __forceinline__ void int4_finish(const Int4Params &p, const float (&a
             for (int g = 0; g < 128 / GM; ++g) v += s[(q0 + g * RM) * 16];
         }
         if (v != v) v = int4_f32(p, m, j);
-        p.C[(size_t)m * p.N + j] = v;
+        p.C[m * p.ldc + j] = v;
     }
 }
 
@@ -481,7 +482,6 @@ int launch_t(Int4Params p, hipStream_t st) {
     int rc = allow_lds((const void *)gemm_int4_kernel<GM, MT, TN>, W * wave, most * wave);
     if (rc) return rc;
     const size_t all = (size_t)cdiv((size_t)p.N, 16 * TN) * cdiv((size_t)p.M, GM / 32 * MT);
-    VMLM_GUARD(all < (size_t)1 << 30, "int4 gemm: M=%d N=%d is too large", p.M, p.N);
     gemm_int4_kernel<GM, MT, TN><<<cdiv(all, 8) * 8, 64 * W, W * wave, st>>>(p);
     VMLM_HIP_CHECK(hipGetLastError());
     return VMLM_OK;
@@ -494,7 +494,6 @@ int launch_rows(const Int4Params &p, hipStream_t st) {
     int rc = allow_lds((const void *)gemm_int4_rows_kernel<GM>, W * wave, 8 * wave);
     if (rc) return rc;
     const size_t all = (size_t)cdiv((size_t)p.N, 16 * I4_TN) * cdiv((size_t)p.M, GM / 32 * I4_TM);
-    VMLM_GUARD(all < (size_t)1 << 30, "int4 gemm: M=%d N=%d is too large", p.M, p.N);
     gemm_int4_rows_kernel<GM><<<cdiv(all, 8) * 8, 64 * W, W * wave, st>>>(p);
     VMLM_HIP_CHECK(hipGetLastError());
     return VMLM_OK;
@@ -526,6 +525,17 @@ int launch_gm(const Int4Params &p, hipStream_t st) {
 // The planes' rows: whole slabs of 16, so that every lane's row exists.
 size_t plane_rows(int M) { return ((size_t)M + I4_SLAB - 1) / I4_SLAB * I4_SLAB; }
 
+// Columns and rows of a launch, so that its threads stay below 2^32 (a grid's limit): there are at
+// most 64 for each 4 rows x 64 columns (256 where there are no more than 4 rows), and in the
+// planes' launch 256 for each 16 runs of a row.
+constexpr int I4_COLS = 1 << 26;
+int piece_rows(int M, int N, int runs) {
+    const int n = std::min(N, I4_COLS), by_tiles = (1 << 30) / n / I4_SLAB * I4_SLAB;
+    const int by_runs = (1 << 23) / (int)cdiv((size_t)runs, 16) / I4_SLAB * I4_SLAB;
+    return std::min(M, std::max((int)I4_SLAB, std::min(by_tiles, by_runs)));
+}
+int pair_runs(int K) { return (K + 2 * I4_RUN - 1) / (2 * I4_RUN) * 2; }  // whole pairs
+
 }  // namespace
 
 // Planes cost a launch and their bytes, splitting in place the split again for every
@@ -536,41 +546,48 @@ size_t plane_rows(int M) { return ((size_t)M + I4_SLAB - 1) / I4_SLAB * I4_SLAB;
 // four rows either way: 64 rows of 2304 21.9 and 21.7, of 20000 122 and 113.
 size_t gemm_int4_work_bytes(int M, int N, int K, int G) {
     if (G == 32 || M <= 4 || (size_t)M * N <= (G == 64 ? 60000 : 100000)) return 0;
-    const size_t runs = cdiv((size_t)K, 2 * I4_RUN) * 2;
-    return plane_rows(M) * runs * (512 + 4);
+    const int runs = pair_runs(K);
+    return plane_rows(piece_rows(M, N, runs)) * runs * (512 + 4);
 }
 
 int launch_gemm_int4(const Int4Args &a, hipStream_t st) {
     Int4Params p;
-    p.A = a.A;
-    p.Q = a.Q;
-    p.scale = a.scale;
-    p.C = a.C;
-    p.M = a.M;
-    p.N = a.N;
     p.K = a.K;
     p.G = a.G;
     p.ng = (a.K + a.G - 1) / a.G;
-    p.runs = (a.K + 2 * I4_RUN - 1) / (2 * I4_RUN) * 2;  // whole pairs
+    p.runs = pair_runs(a.K);
     p.rg = std::max(1, a.G / I4_RUN);
+    p.ldc = a.N;
     p.planes = nullptr;
     p.fac = nullptr;
     p.rows = 0;
-    if (a.work) {
-        const int rows = (int)plane_rows(a.M);
-        uint8_t *planes = (uint8_t *)a.work;
-        float *fac = (float *)(planes + (size_t)rows * p.runs * 512);
-        const size_t wgs = (size_t)a.M * cdiv((size_t)p.runs, 16);
-        VMLM_GUARD(wgs < (size_t)1 << 31, "int4 gemm: M=%d K=%d is too large", a.M, a.K);
-        int4_planes_kernel<<<(unsigned)wgs, 256, 0, st>>>(a.A, a.M, a.K, p.runs, rows, planes, fac);
-        VMLM_HIP_CHECK(hipGetLastError());
-        p.planes = planes;
-        p.fac = fac;
-        p.rows = rows;
+    const int each = piece_rows(a.M, a.N, p.runs);
+    for (int m = 0; m < a.M; m += each) {  // (one piece of nearly any call)
+        p.A = a.A + (size_t)m * a.K;
+        p.M = std::min(each, a.M - m);
+        if (a.work) {
+            const int rows = (int)plane_rows(p.M);
+            uint8_t *planes = (uint8_t *)a.work;
+            float *fac = (float *)(planes + (size_t)rows * p.runs * 512);
+            const unsigned wgs = (unsigned)p.M * cdiv((size_t)p.runs, 16);
+            int4_planes_kernel<<<wgs, 256, 0, st>>>(p.A, p.M, a.K, p.runs, rows, planes, fac);
+            VMLM_HIP_CHECK(hipGetLastError());
+            p.planes = planes;
+            p.fac = fac;
+            p.rows = rows;
+        }
+        for (int n = 0; n < a.N; n += p.N) {
+            p.N = std::min(I4_COLS, a.N - n);
+            p.Q = a.Q + (size_t)n * (a.K / 2);
+            p.scale = a.scale + (size_t)n * p.ng;
+            p.C = a.C + (size_t)m * a.N + n;
+            const int rc = a.G == 32   ? launch_gm<32>(p, st)
+                           : a.G == 64 ? launch_gm<64>(p, st)
+                                       : launch_gm<128>(p, st);
+            if (rc) return rc;
+        }
     }
-    if (a.G == 32) return launch_gm<32>(p, st);
-    if (a.G == 64) return launch_gm<64>(p, st);
-    return launch_gm<128>(p, st);
+    return VMLM_OK;
 }
 
 }  // namespace vmlm

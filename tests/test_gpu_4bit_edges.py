@@ -360,6 +360,34 @@ def test_norm_rows_past_one_grid(dev):
         assert (np.abs(part - ref[:len(part)]) <= tol[:len(part)]).all(), i
 
 
+def test_int4_rows_past_one_grid(dev):
+    """More rows than the grid of the launch that splits them can have."""
+    rng = np.random.default_rng(8)
+    m, n, k, group, tile = (1 << 24) + 16, 16, 32, 64, 1 << 18
+    a, w, s = int4_case(rng, tile, n, k, group)
+    p = C.c_void_p()
+    for count in (m * k, m * n + n):
+        dev.check(dev.L.vmlm_hip_malloc(C.byref(p), count * 4))
+        dev.bufs.append(p.value)
+    pa, pc = dev.bufs[-2:]
+    for r in range(0, m, tile):
+        part = a[:min(tile, m - r)]
+        dev.check(dev.L.vmlm_hip_memcpy_h2d(pa + r * k * 4, part.ctypes.data, part.nbytes))
+    mark = np.full(n, 5, np.float32)
+    dev.check(dev.L.vmlm_hip_memcpy_h2d(pc + m * n * 4, mark.ctypes.data, mark.nbytes))
+    dw, ds = dev.up(w), dev.up(s)
+    dev.sync()
+    dev.check(dev.L.vmlm_hip_gemm_nt_int4(pa, dw.ptr, ds.ptr, pc, m, n, k, group, None))
+    dev.sync()
+    got = np.empty((m + 1, n), np.float32)
+    dev.check(dev.L.vmlm_hip_memcpy_d2h(got.ctypes.data, pc, got.nbytes))
+    assert (got[m] == 5).all()
+    int4_check(got[:tile], a, w, s, group)
+    for r in range(tile, m, tile):
+        part = got[r:min(m, r + tile)]
+        assert np.array_equal(part, got[:len(part)]), r
+
+
 # ------------------------------------------------------------------ norms
 def test_norm_alone_keeps_channels_apart(ops):
     """Without positions nothing is rotated: a channel whose gain or value is not
