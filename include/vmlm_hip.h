@@ -354,7 +354,7 @@ int vmlm_hip_qk_norm_rope(float *q_out, size_t ldqo, float *k_out, size_t ldko, 
 /* Stores rows k [batch][S][ldk] and v [batch][S][ldv] (n_kv_heads * head_dim values
  * each): row (b, t) at position pos0[b] + t, for t < count[b] (count null: all S). Sequences
  * with pos0 < 0 are idle. Rows from cap on are dropped and reported by the
- * next vmlm_hip_check_guards() as status 9. */
+ * next vmlm_hip_check_guards() as status 9. S or cap is below 2^29 - 64. */
 int vmlm_hip_kv4_append(const vmlm_kv4_cache *cache, const float *k, size_t ldk, const float *v,
                         size_t ldv, const int32_t *pos0, const int32_t *count, size_t S,
                         void *stream);

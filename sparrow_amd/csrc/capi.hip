@@ -1196,7 +1196,9 @@ int vmlm_hip_qk_norm_rope(float *q_out, size_t ldqo, float *k_out, size_t ldko, 
 // Rows [B][S] of the cache's width beside it.
 static int check_kv4_rows(const Kv4View &c, const float *k, size_t ldk, const float *v, size_t ldv,
                           const int32_t *pos0, const int32_t *count, size_t S, bool read) {
-    VMLM_GUARD(S <= DIM_MAX, "kv4: %zu rows a sequence (limit 2^30)", S);
+    // (a workgroup of 256 threads for each block of 32 positions that they can touch)
+    VMLM_GUARD(S <= DIM_MAX && std::min((size_t)c.cap / 32, (S + 30) / 32 + 1) < (size_t)1 << 24,
+               "kv4: %zu rows a sequence of capacity %d (limit 2^29 - 64)", S, c.cap);
     if (c.B == 0 || c.Hkv == 0 || S == 0) return VMLM_OK;
     VMLM_GUARD(c.cap > 0, "kv4: capacity 0");
     VMLM_GUARD(k && v && pos0, "kv4: null rows or positions");

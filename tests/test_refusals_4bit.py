@@ -259,3 +259,17 @@ def test_workspace_over_any_operand_refused(L):
 def test_host_read_over_itself_refused(L):
     assert L.vmlm_kv4_read(cache(), Y, Y + 4, A - 64, None, 3) == 9
     assert "over each other" in message(L)
+
+
+@pytest.mark.parametrize("fn", ["vmlm_hip_kv4_append", "vmlm_hip_kv4_read"])
+def test_rows_past_a_grid_refused(L, fn):
+    """A grid of 256 threads for each block of 32 positions ends at 2^24 blocks; one
+    block of a long cache, or many rows of a short one, are no such call (a batch of 0
+    has no work)."""
+    wide = dict(k=1 << 40, v=1 << 41, k_meta=1 << 42, v_meta=1 << 43, n_kv_heads=1, head_dim=32)
+    at = dict(k=1 << 44, v=1 << 45, ldk=32, ldv=32)
+    big = cache(batch=1, cap=2 ** 30, **wide)
+    assert rows(L, fn, big, **at, S=2 ** 29) == 9
+    assert "capacity" in message(L)
+    assert rows(L, fn, cache(batch=0, cap=2 ** 30, **wide), **at, S=2 ** 29 - 64) == 0
+    assert rows(L, fn, cache(batch=0, cap=64, **wide), **at, S=2 ** 30) == 0
