@@ -101,7 +101,7 @@ def test_attention_every_bit_of_the_weights(ops, H, Hkv, hd):
     zero (u = 8, min = -8 scale): there the output is the sum of weights near 2^-15 of the
     largest, in fixed point below it. Off by half a step (2^-30 of the largest) each
     times a code up to 8, besides the roundings of the weights themselves; without their
-    lowest byte it would be off by 3.5e-6 in the mean."""
+    lowest byte it would be off by 1e-5, six times the bound."""
     rng = np.random.default_rng(hd)
     n = 60
     q = np.zeros((1, H, hd), np.float32)
@@ -277,6 +277,39 @@ def test_cache_no_rows_to_drop(ops):
     c.append(x, x, [2 ** 31 - 1, 5], [-4, 3])
     k, _ = c.read([65, 5], 3, [0, 3])
     assert not k[0].any() and (k[1] == 1).all()
+
+
+# ------------------------------------------------------------------ the cache's end
+@pytest.mark.parametrize("at", [60, 63, 64, 1000, 2 ** 31 - 1])
+@pytest.mark.parametrize("append", [True, False])
+def test_cache_rows_up_to_the_capacity(ops, at, append):
+    """Of rows that run past cap the ones before it are stored, and read; the others
+    are dropped and reported, and no other sequence sees it."""
+    from sparrow_amd import VmlmError
+    rng = np.random.default_rng(at % 1000)
+    c, m = ops.Kv4Cache(2, 1, 64, 64), new_model(2, 1, 64, 64)
+    k, v = rng.standard_normal((2, 2, 10, 64), dtype=np.float32)
+    fit = max(0, min(10, 64 - at))
+    where = np.zeros((2, 64), bool)
+    for b, (p, n) in enumerate(((at, fit), (20, 10))):
+        put(m, k[b], v[b], b, p, n, 1)
+        where[b, p:p + n] = True
+    if append:
+        with pytest.raises(VmlmError) as e:
+            c.append(k, v, [at, 20])
+        assert e.value.code == 9
+        same_cache(c, m, where)
+        return
+    c.append(k, v, [at, 20], [fit, 10])
+    rk = np.full((2, 10, 64), 3, np.float32)
+    rv, pos = rk.copy(), np.array([at, 20], np.int32)
+    p = [x.ctypes.data_as(C.c_void_p) for x in (rk, rv, pos)]
+    from sparrow_amd import lib
+    assert lib().vmlm_kv4_read(c.descriptor(), *p, None, 10) == 9
+    for got, name in ((rk, "k"), (rv, "v")):
+        assert np.array_equal(got[0, :fit], m[name][0, 0, at:at + fit] if fit else got[0, :0])
+        assert (got[0, fit:] == 3).all()
+        assert np.array_equal(got[1], m[name][1, 0, 20:30])
 
 
 # ------------------------------------------------------------------ a prompt, then its decode
