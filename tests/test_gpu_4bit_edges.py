@@ -435,3 +435,91 @@ def test_norm_alone_keeps_channels_apart(ops):
     ok = np.isfinite(g)
     assert (np.abs(got - ref)[:, ok] <= tol[:, ok]).all()
     assert np.isinf(got[:, 3]).all() and np.isnan(got[:, 40]).all()
+
+
+# ------------------------------------------------------------------ gemm_nt_int4
+# In place with one, two and four tiles of columns, and over byte planes, with groups
+# that end inside a wave's share of K.
+PATHS = [(1, 50, 384, 128), (3, 70, 640, 32), (7, 5000, 256, 64), (1, 33000, 256, 64), (20, 40, 352, 32),
+         (20, 5100, 384, 128), (21, 5100, 1280, 384), (18, 3500, 320, 64), (40, 2600, 3328, 640)]
+
+
+@pytest.mark.parametrize("m,n,k,group", PATHS)
+def test_int4_every_bit(ops, m, n, k, group):
+    """One power of two in each weight row: the product is one activation times it, so
+    all 24 bits come back. (Activations within 2^-6 of a power of two are left
+    out: with the term that makes their bytes signed they need 25.)"""
+    rng = np.random.default_rng(m * n + k)
+    a = rng.integers(2 ** 23, 2 ** 24 - 2 ** 18, (m, k)) * rng.choice([-1, 1], (m, k))
+    runs = -(-k // 128)
+    a = a * np.repeat(2.0 ** rng.integers(-60, 20, (m, runs)), 128, 1)[:, :k]
+    a = a.astype(np.float32)
+    at, v = rng.integers(0, k, n), rng.choice([-8, -4, -1, 1, 2, 4], n)
+    w = np.zeros((n, k), np.int8)
+    w[np.arange(n), at] = v
+    s = 2.0 ** rng.integers(-6, 7, (n, -(-k // group)))
+    u = (w & 15).astype(np.uint8)
+    got = ops.gemm_nt_int4(a, u[:, 0::2] | (u[:, 1::2] << 4), s, group)
+    want = a[:, at].astype(np.float64) * (v * s[np.arange(n), at // group])
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("m,n,k,group", PATHS)
+def test_int4_norm_of_the_error(ops, m, n, k, group):
+    """Roundings of both signs: the split rounds each activation once (half a step, 0.3
+    u in the mean of a uniform one), each run's sum is rounded at most five times and its
+    addition once more, at the partial sums' magnitude, so the error is below
+    sqrt(0.3 + 5 + k / 256) u of the result's norm, 4.5 u at k = 3328. Without the lowest two
+    of the four bytes it would be 2^-16."""
+    rng = np.random.default_rng(m + n * k)
+    a, q, s = int4_case(rng, m, n, k, group)
+    ref, _ = int4_ref(a, q, s, group)
+    err = np.linalg.norm(ops.gemm_nt_int4(a, q, s, group) - ref)
+    assert err <= (0.3 + 5 + k / 256) ** 0.5 * U * np.linalg.norm(ref)
+
+
+@pytest.mark.parametrize("m,n,k,group", PATHS)
+def test_int4_wide_rows(ops, m, n, k, group):
+    """Rows from 1e-30 to 1e30, values that stand out by 1e4, a zero row and zero runs."""
+    rng = np.random.default_rng(m + k)
+    a, q, s = int4_case(rng, m, n, k, group)
+    a[:, 5::97] *= np.float32(1e4)
+    a *= np.float32(10.0) ** rng.integers(-30, 31, (m, 1)).astype(np.float32)
+    a[0, 128:300] = 0
+    a[m // 2] = 0
+    got = ops.gemm_nt_int4(a, q, s, group)
+    int4_check(got, a, q, s, group)
+    assert not got[m // 2].any()
+
+
+@pytest.mark.parametrize("m,n,k,group", [p for p in PATHS if p[0] > 2])
+def test_int4_rows_that_are_not_finite(ops, m, n, k, group):
+    """An infinity gives +-inf by its weight's sign (NaN against a zero weight), a
+    NaN gives NaN; the other rows do not see them."""
+    rng = np.random.default_rng(m * k)
+    a, q, s = int4_case(rng, m, n, k, group)
+    clean = ops.gemm_nt_int4(a, q, s, group)
+    a[0, 130], a[1, 7], a[m - 1, k - 1] = np.inf, np.nan, -np.inf
+    got = ops.gemm_nt_int4(a, q, s, group)
+    w = nibbles(q).astype(np.float32)
+    with np.errstate(invalid="ignore"):
+        assert np.array_equal(got[0], np.float32(np.inf) * w[:, 130], equal_nan=True)
+        assert np.array_equal(got[m - 1], -np.float32(np.inf) * w[:, k - 1], equal_nan=True)
+    assert np.isnan(got[1]).all() and np.array_equal(got[2:m - 1], clean[2:m - 1])
+
+
+@pytest.mark.parametrize("m,n,k,group", PATHS)
+def test_int4_odd_addresses(dev, m, n, k, group):
+    """Operands at odd addresses (the codes at any byte); what lies beside C stays."""
+    rng = np.random.default_rng(m + n)
+    a, q, s = int4_case(rng, m, n, k, group)
+    buf = lambda x, pad: dev.up(np.concatenate([np.full(pad, 77, x.dtype), x.ravel()]))  # noqa: E731
+    da, dq, ds = buf(a, 1), buf(q, 5), buf(s, 3)
+    dc = dev.up(np.full(m * n + 10, 5.0, np.float32))
+    dev.sync()
+    dev.check(dev.L.vmlm_hip_gemm_nt_int4(da.ptr + 4, dq.ptr + 5, ds.ptr + 12, dc.ptr + 20, m, n, k,
+                                          group, None))
+    dev.sync()
+    got = dc.get()
+    assert (got[:5] == 5).all() and (got[5 + m * n:] == 5).all()
+    int4_check(got[5:5 + m * n].reshape(m, n), a, q, s, group)
