@@ -66,7 +66,8 @@ struct Attn4Params {
     int H, G, ch, W;
     int shares;  // of a split launch (0: one workgroup a pair of head and sequence)
     int parts;  // workgroups that share a kv head's queries
-    float scale;
+    float scale;  // of the scores: scale * 2^scale_e, |scale| in [1/2, 1)
+    int scale_e;
     int *guard;
 };
 
@@ -462,7 +463,7 @@ __global__ __launch_bounds__(64 * A4_MAX_W) void attn4_kernel(Attn4Params p) {
                 o[1] = bad ? __builtin_nanf("") : ldexpf(s, -e - eh);
             }
         }
-        if (lane == 0) qe[h] = eh;
+        if (lane == 0) qe[h] = eh + p.scale_e;
     }
     __syncthreads();
 
@@ -845,7 +846,7 @@ int launch_attn4(const Attn4Args &a, hipStream_t st) {
     p.W = pl.W;
     p.parts = pl.parts;
     p.ch = attn4_ch(a.c.hd);
-    p.scale = a.scale;
+    p.scale = frexpf(a.scale, &p.scale_e);
     p.guard = guard_flag_ptr();
     VMLM_GUARD(!p.shares || p.work, "kv4 attention: split positions need a workspace");
     const int rows = p.shares ? attn4_rows(pl, a.c.B) : a.c.B;

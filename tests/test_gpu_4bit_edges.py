@@ -48,7 +48,7 @@ def attn_exact(m, q, pos, Hkv, hd, scale, ds=True):
                 most.append(np.maximum(np.abs(lo), np.abs(lo + 15 * sc)))
             e = (64 + n / 16 + 4 * t) * U
             if ds:
-                e += 33 * U * scale * (most[0] @ np.abs(x).reshape(-1, 32).sum(1))
+                e += 33 * U * abs(scale) * (most[0] @ np.abs(x).reshape(-1, 32).sum(1))
             out[b, at] = p @ m["v"][b, kv, :n].astype(np.float64)
             # (a weight below 2^-126 may be none)
             w = (p * (e + p @ e))[:, None] * most[1] + 2.0 ** -126 * most[1]
@@ -159,6 +159,20 @@ def test_attention_tiny_and_huge_queries(ops, times):
     c, m = stored(ops, k, v, 1, 96)
     q = q.reshape(1, -1)
     close(c.attention_decode(q, [n - 1], scale=0.125), *attn_exact(m, q, [n - 1], 1, hd, 0.125))
+
+
+@pytest.mark.parametrize("q,k,scale", [(2.0 ** -138, 2.0 ** 127, 2.0 ** 20), (2.0 ** -122, 2.0 ** 122, -200.0),
+                                       (2.0 ** 100, 2.0 ** -60, 2.0 ** -45), (1.0, 1.0, 0.0)])
+def test_attention_any_scale_of_the_scores(ops, q, k, scale):
+    """Scales that bring scores of a few out of queries and keys near f32's ends: no
+    step between leaves f32."""
+    rng = np.random.default_rng(22)
+    n, hd = 70, 64
+    x = (rng.standard_normal((1, 2 * hd)) * q / 8).astype(np.float32)
+    y, v = rng.standard_normal((2, 1, n, hd), dtype=np.float32)
+    y = (y.astype(np.float64) * k / 64).astype(np.float32)
+    c, m = stored(ops, y, v, 1, 96)
+    close(c.attention_decode(x, [n - 1], scale=scale), *attn_exact(m, x, [n - 1], 1, hd, scale))
 
 
 @pytest.mark.parametrize("H,hd", [(1, 32), (1, 64), (4, 128), (3, 256)])
