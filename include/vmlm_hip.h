@@ -334,9 +334,12 @@ int vmlm_hip_attention_decode_split(const float *q, const float *k_new, const fl
  * multiple of 32, group 32, 64 or a multiple of 128 (the last group may be short).
  * The rows of A become fixed-point numbers of 31 bits below the largest of 128
  * neighbours, as four int8 terms, and the products are summed in integers within a
- * group: results are as near as f32 sums are (values below 2^-7 of that largest one
- * keep fewer bits than f32's 24). Rows with a NaN or an infinity are summed in f32.
- * Many rows go through the stream's workspace, in a captured call through none. */
+ * group. Rows whose values are of like size come out nearer than f32 sums; a value below
+ * 2^-7 of that largest one keeps fewer bits than f32's 24, also where the largest meets a
+ * weight of zero (one channel of each 128 at 1e4 times the others: 6e-6 of the result's
+ * norm then, and in proportion; f32 sums leave 1e-7 to 4e-7). Rows with a NaN or an
+ * infinity are summed in f32. Many rows go through the stream's workspace, in a captured call through none: its
+ * results may differ from an eager call's in their last bits (sums in another order). */
 int vmlm_hip_gemm_nt_int4(const float *a, const uint8_t *q, const float *scale, float *c,
                           size_t m, size_t n, size_t k, size_t group, void *stream);
 /* RMSNorm of each head of q [rows][ldq] (n_heads heads) and k [rows][ldk]

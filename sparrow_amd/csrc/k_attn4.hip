@@ -33,9 +33,9 @@
 //
 // Measured (kernel times; a large copy moves 5.1 TB/s): 65500 positions of 36 heads of 64,
 // one sequence, 39 us, 4.8 TB/s, and 4.7 us of merging; 8 sequences of up to 16000 with 8 kv
-// heads of 128 and 4 queries each 34 us, 3.4 TB/s: there the softmax and the bytes of
+// heads of 128 and 4 queries each 36 us, 3.3 TB/s: there the softmax and the bytes of
 // 4 queries' weights keep the vector units as busy as the memory, at two waves a SIMD.
-// 1024 positions: 6.9 us, a launch and a few latencies.
+// 1024 positions: 7.0 us, a launch and a few latencies.
 #include <algorithm>
 
 #include "kv4.hpp"
@@ -48,7 +48,7 @@ typedef uint32_t u32x4m __attribute__((ext_vector_type(4), aligned(4)));
 typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
 
 // Positions of a wave at a time: what the registers hold. (64 for heads of 128 too, more
-// waves at once: 36.0 us instead of 34.3 for 8 sequences of 16000 with 4 queries a kv head.)
+// waves at once: 36.0 us instead of 34.3, then, for 8 sequences of 16000 with 4 queries a kv head.)
 constexpr int attn4_ch(int hd) { return hd <= 128 ? 128 : 64; }
 // The maximum of no score yet, or of scores that all left f32 downwards: finite, so that
 // its distance from itself is none (not -inf - -inf).
@@ -772,7 +772,9 @@ __global__ __launch_bounds__(KV4_MAX_HD) void attn4_merge_kernel(Attn4Params p) 
 
 // Where the sequences can be long and the pairs of head and sequence are fewer than
 // the workgroups that the chip holds, the pairs are split into about as many shares: 512
-// of eight waves where a wave keeps to 128 registers, else of four. (768 for heads of
+// of eight waves where a wave keeps to 128 registers, else of four. As many sequences as
+// shares or more stay whole, whatever their lengths: of 16 with 36 heads one of 60000 positions
+// runs on 36 workgroups, 114 us where it takes 35 alone. (768 for heads of
 // 128: one sequence of 16000, 8 kv heads of 4 queries 21.0 us instead of 18.8, four of 30000, 8
 // heads 36.8 instead of 38.2.) Short ones: a wave a chunk, up to eight, and no second launch.
 struct Attn4Plan {

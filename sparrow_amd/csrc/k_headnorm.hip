@@ -10,7 +10,7 @@
 // row's heads, each lane its four sines and cosines.
 //
 // Bound by the rows' bytes, read once and written once: 2048 rows of 36 + 36 heads of 64
-// take 14.6 us, 5.2 TB/s (a large copy 5.1). One row takes 2.8 us, a launch and a latency.
+// take 14.7 us, 5.1 TB/s (as a large copy). One row takes 2.8 us, a launch and a latency.
 //
 // Angles: pos * theta^(-2i/hd) / 2 pi is formed in 64 bits and its whole turns
 // dropped there; a 32-bit product would be off by 2^-24 of the angle itself (0.006 at

@@ -9,7 +9,8 @@
 // conversion. The activations of a run of 128 k are 31-bit fixed-point numbers
 // below the row's largest value there, as four signed bytes, so every product and
 // sum over a group is exact in int32 and two conversions, an FMA and two products make
-// an f32 of it: errors are those of K/128 f32 additions.
+// an f32 of it: errors are the split's (2^-29 of that largest value) and those of K/128 f32
+// additions.
 //
 // D = A . B^T per v_mfma_i32_16x16x64_i8, B the nibbles of 16 weight rows, the 16
 // rows of A the four bytes of
@@ -168,7 +169,8 @@ __device__ __forceinline__ float split8(const float *row, int k, int K, uint32_t
     const int es = in && ok ? e2 : -1000;  // none behind K, nor of a row without a factor
     uint32_t d[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)  // signed_bytes, the sum rounded to an integer or f32's 24 bits
+    for (int e = 0; e < 8; ++e)  // signed_bytes of an integer at most one step off: the sum has
+                                 // f32's 24 bits, and the conversion cuts a fraction off
         d[e] = (uint32_t)(int)(ldexpf(x[e], es) + (float)0x808080) ^ 0x808080u;
     transpose_bytes({d[0], d[2], d[4], d[6]}, ev);
     transpose_bytes({d[1], d[3], d[5], d[7]}, od);
@@ -539,11 +541,12 @@ int pair_runs(int K) { return (K + 2 * I4_RUN - 1) / (2 * I4_RUN) * 2; }  // who
 }  // namespace
 
 // Planes cost a launch and their bytes, splitting in place the split again for every
-// 16 to 64 columns (K = 2304, planes and in place, us; group 128: 16 rows of 5760 columns 10.2 and
+// 16 to 64 columns. (K = 2304, planes and in place, us; group 128: 16 rows of 5760 columns 10.2 and
 // 8.7, 20 rows 10.7 and 15.6, 32 rows of 2304 10.4 and 8.7, 64 rows 10.9 and 15.8, 6 rows of
 // 20000 16.8 and 16.9, 12 rows 17.4 and 21.6; group 64: 8 rows of 5760 9.3 and 7.0, 12 rows 9.7
 // and 12.2, 20 rows of 2304 9.5 and 7.0, 32 rows 9.6 and 12.0). With groups of 32 a slab is
-// four rows either way: 64 rows of 2304 21.9 and 21.7, of 20000 122 and 113.
+// four rows either way: 64 rows of 2304 21.9 and 21.7, of 20000 122 and 113. Other K were not
+// measured.)
 size_t gemm_int4_work_bytes(int M, int N, int K, int G) {
     if (G == 32 || M <= 4 || (size_t)M * N <= (G == 64 ? 60000 : 100000)) return 0;
     const int runs = pair_runs(K);
