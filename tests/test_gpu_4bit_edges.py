@@ -17,8 +17,8 @@ import ctypes as C
 
 import numpy as np
 import pytest
-from test_gpu_4bit import (U, Buf, Dev, cache_codes, dev, device_cache, held, int4_case,  # noqa: F401
-                           int4_check, int4_ref, new_model, nibbles, norm_ref, ops, put, same_cache)
+from test_gpu_4bit import (U, dev, device_cache, int4_case, int4_check, int4_ref,  # noqa: F401
+                           new_model, nibbles, norm_ref, ops, put, same_cache)
 
 pytestmark = pytest.mark.gpu
 
