@@ -249,6 +249,40 @@ int vmlm_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, const
                               const float *v_new, const int32_t *pos, float *out, size_t n_heads,
                               float scale);
 
+/* A step that verifies drafted tokens, over host arrays (contracts at the device forms
+ * below). Rows are contiguous; what a call leaves as it is keeps the caller's values. */
+int vmlm_rope_qk(float *q_out, float *k_out, const float *q, const float *k, const int32_t *pos,
+                 const double *freq, size_t rows, size_t n_heads, size_t n_kv_heads,
+                 size_t head_dim, size_t rot_dim, bool interleaved, float factor);
+int vmlm_attention_tree_kv4(const vmlm_kv4_cache *cache, const float *q, const int32_t *pos0,
+                            const int32_t *count, const int32_t *parent, size_t S, float *out,
+                            size_t n_heads, float scale);
+int vmlm_sample(const float *logits, const float *u, const float *temperature,
+                const int32_t *top_k, const float *top_p, const float *min_p, size_t rows,
+                size_t vocab, int32_t *token, float *prob);
+int vmlm_tree_accept_kv4(const vmlm_kv4_cache *caches, size_t n_caches, const int32_t *pos0,
+                         const int32_t *count, const int32_t *parent, const int32_t *drafted,
+                         const int32_t *chosen, size_t S, int32_t *path, int32_t *kept,
+                         int32_t *next);
+/* Frequencies for the rotation, on the host: freq[i] = theta^(-2i / rot_dim) radians a
+ * position, i < rot_dim / 2, and *factor = 1, changed as `scaling` (null: not) says, whose
+ * positions are `factor` times as many as the `trained` ones:
+ *   VMLM_ROPE_LINEAR  all frequencies divided by `factor`
+ *   VMLM_ROPE_BANDS   with n = trained * freq / 2 pi turns within the trained length: kept for n >=
+ *                     high, divided by `factor` for n <= low, between them the mean of both by
+ *                     (n - low) / (high - low)
+ *   VMLM_ROPE_RAMP    the same by the pair's index, between floor and ceil of the (real) indices whose pairs
+ *                     make high and low turns (within 0 .. rot_dim - 1); *factor = 0.1 ln(factor) + 1 */
+#define VMLM_ROPE_LINEAR 1
+#define VMLM_ROPE_BANDS 2
+#define VMLM_ROPE_RAMP 3
+typedef struct vmlm_rope_scaling {
+    int kind;
+    double factor, low, high, trained;
+} vmlm_rope_scaling;
+int vmlm_rope_freqs(double *freq, float *factor, size_t rot_dim, double theta,
+                    const vmlm_rope_scaling *scaling);
+
 /* ================================================================ layer 2
  * Device pointers, asynchronous on `stream`. Same semantics as layer 1.
  * The result of the f32, int8 and bf16 weight GEMMs may lie over their operands (C
@@ -386,6 +420,69 @@ int vmlm_hip_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, s
                                   float scale, void *work, size_t work_bytes, void *stream);
 int vmlm_hip_attention_decode_kv4_work(const vmlm_kv4_cache *cache, size_t n_heads,
                                        size_t *bytes);
+
+/* ---- a step that verifies drafted tokens (no reference counterparts): rotation of the new
+ * rows, attention of a tree of tokens over the 4-bit cache, a token drawn for each of them, and
+ * the accepted ones' rows moved up. Kernels only, overlapping operands refused (9) and the
+ * GPU the current device's, as above.
+ *
+ * The tree: sequence b has count[b] <= S tokens (count null: S), token t's row stored at
+ * position pos0[b] + t (kv4_append). parent[b][t] < t is the token it follows, -1 the text before
+ * pos0[b]; parent null: each follows the one before it. Sequences with pos0 < 0 or no token
+ * are idle. Parents that are no earlier token and tokens past the capacity trip the device guard, and
+ * their sequence is taken as idle. */
+
+/* The pairs of the first rot_dim channels of each head of q [rows][ldq] and k [rows][ldk]:
+ * (a, b) -> factor * (a cos - b sin, a sin + b cos) of the angle pos[row] * freq[i] (formed in 64
+ * bits), where pair i is channels (i, i + rot_dim / 2) or, interleaved, (2i, 2i + 1); the other channels as they
+ * are. freq: rot_dim / 2 doubles on the device (vmlm_rope_freqs). Rows with pos < 0 are left
+ * as they are. Outputs have strides of their own and may be the inputs (same address and
+ * stride). Either side may be absent (0 heads). head_dim and rot_dim are even, up to 512. */
+int vmlm_hip_rope_qk(float *q_out, size_t ldqo, float *k_out, size_t ldko, const float *q,
+                     size_t ldq, const float *k, size_t ldk, const int32_t *pos,
+                     const double *freq, size_t rows, size_t n_heads, size_t n_kv_heads,
+                     size_t head_dim, size_t rot_dim, bool interleaved, float factor,
+                     void *stream);
+/* Each head of q [batch][S][ldq] attends, at token t, the positions before pos0[b], its own and
+ * those of the tokens that it follows, directly or through others (head h reads kv head h / (n_heads /
+ * n_kv_heads)): out [batch][S][ldo]; rows from count[b] on and of idle sequences are left as they are. q and
+ * the cache's keys come rotated. S is at most 64 with parents, 65535 without. A
+ * query head with a NaN or an infinity gives NaN, a position with one in its key or value to the queries
+ * that see it. `work`: vmlm_hip_attention_tree_kv4_work() bytes, 16-byte aligned, used by one
+ * call at a time; null: the stream's own workspace, which a call under stream capture may
+ * not use (9), since graphs that run at once would share it. */
+int vmlm_hip_attention_tree_kv4(const vmlm_kv4_cache *cache, const float *q, size_t ldq,
+                                const int32_t *pos0, const int32_t *count, const int32_t *parent,
+                                size_t S, float *out, size_t ldo, size_t n_heads, float scale,
+                                void *work, size_t work_bytes, void *stream);
+int vmlm_hip_attention_tree_kv4_work(const vmlm_kv4_cache *cache, size_t n_heads, size_t S,
+                                     size_t *bytes);
+/* A token of each row of logits [rows][ld]. The tokens in order of their logits, the largest first,
+ * of equal ones the lowest index, have weights exp((l - l_max) / temperature[row]). Kept are
+ * the first top_k[row] (<= 0: all), of those the ones before which the weights sum to less than
+ * top_p[row] of theirs (>= 1: all; the first one always), of those the ones of at least
+ * min_p[row] times the first one's. token[row] is the first whose weight and those before it sum to
+ * more than u[row] times the kept ones', prob[row] its share of them. Borders are decided in more
+ * than 32 bits (sums to 2^-30 of a weight). temperature 0: the first token, prob 1. u < 0: the row is
+ * idle, token and prob stay as they are. A row of which all is -infinity has no token: -1, prob 0;
+ * one with a NaN or +infinity: -1, prob NaN. Settings out of range (u >= 1, temperature < 0 or not
+ * finite, min_p outside 0 .. 1, NaN) trip the device guard and leave the row as it is. top_k, top_p, min_p and prob may be null.
+ * vocab is below 2^20, rows at most 2^20. `work` as above. */
+int vmlm_hip_sample(const float *logits, size_t ld, const float *u, const float *temperature,
+                    const int32_t *top_k, const float *top_p, const float *min_p, size_t rows,
+                    size_t vocab, int32_t *token, float *prob, void *work, size_t work_bytes,
+                    void *stream);
+int vmlm_hip_sample_work(size_t rows, size_t vocab, size_t *bytes);
+/* From token 0 of each tree on, the first child whose drafted[b][t] is chosen[b][its parent] (and not
+ * negative) is accepted next: path[b][i] is the i-th accepted token (-1 from the last one on, S entries),
+ * kept[b] their number, next[b] the token chosen at the last of them. In each of the caches (a layer's each,
+ * of one shape, none over another) row path[b][i] moves to position pos0[b] + i, its codes as they are.
+ * The rows behind are the rejected tokens' and may be overwritten. Idle sequences' outputs stay
+ * as they are. S is at most 64, n_caches at most 256; `caches` is read during the call. */
+int vmlm_hip_tree_accept_kv4(const vmlm_kv4_cache *caches, size_t n_caches, const int32_t *pos0,
+                             const int32_t *count, const int32_t *parent, const int32_t *drafted,
+                             const int32_t *chosen, size_t S, int32_t *path, int32_t *kept,
+                             int32_t *next, void *stream);
 
 /* ================================================================ layer 3 */
 

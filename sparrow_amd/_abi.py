@@ -37,6 +37,12 @@ class Kv4Cache(C.Structure):
                 ("n_kv_heads", SZ), ("cap", SZ), ("head_dim", SZ)]
 
 
+class RopeScaling(C.Structure):
+    """How frequencies change for long contexts, vmlm_rope_scaling."""
+    _fields_ = [("kind", I), ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("trained", C.c_double)]
+
+
 class DecoderCfg(C.Structure):
     _fields_ = [("n_layers", U32), ("hidden", U32), ("n_heads", U32), ("head_dim", U32),
                 ("inter", U32), ("vocab", U32), ("batch", U32), ("cap", U32),
@@ -105,6 +111,11 @@ SIGNATURES = {
     "vmlm_kv4_append": (I, [C.POINTER(Kv4Cache), P, P, P, P, SZ]),
     "vmlm_kv4_read": (I, [C.POINTER(Kv4Cache), P, P, P, P, SZ]),
     "vmlm_attention_decode_kv4": (I, [C.POINTER(Kv4Cache), P, P, P, P, P, SZ, F]),
+    "vmlm_rope_qk": (I, [P, P, P, P, P, P, SZ, SZ, SZ, SZ, SZ, B, F]),
+    "vmlm_attention_tree_kv4": (I, [C.POINTER(Kv4Cache), P, P, P, P, SZ, P, SZ, F]),
+    "vmlm_sample": (I, [P, P, P, P, P, P, SZ, SZ, P, P]),
+    "vmlm_tree_accept_kv4": (I, [C.POINTER(Kv4Cache), SZ, P, P, P, P, P, SZ, P, P, P]),
+    "vmlm_rope_freqs": (I, [P, C.POINTER(F), SZ, C.c_double, C.POINTER(RopeScaling)]),
     # layer 2
     "vmlm_hip_gemm_nt_int8": (I, [P, P, P, P, SZ, SZ, SZ, P]),
     "vmlm_hip_gemm_nt_int8_noalloc": (I, [P, P, P, P, SZ, SZ, SZ, P]),
@@ -140,6 +151,13 @@ SIGNATURES = {
     "vmlm_hip_attention_decode_kv4": (I, [C.POINTER(Kv4Cache), P, SZ, P, P, SZ, P, P, SZ, SZ, F,
                                           P, SZ, P]),
     "vmlm_hip_attention_decode_kv4_work": (I, [C.POINTER(Kv4Cache), SZ, C.POINTER(SZ)]),
+    "vmlm_hip_rope_qk": (I, [P, SZ, P, SZ, P, SZ, P, SZ, P, P, SZ, SZ, SZ, SZ, SZ, B, F, P]),
+    "vmlm_hip_attention_tree_kv4": (I, [C.POINTER(Kv4Cache), P, SZ, P, P, P, SZ, P, SZ, SZ, F, P,
+                                        SZ, P]),
+    "vmlm_hip_attention_tree_kv4_work": (I, [C.POINTER(Kv4Cache), SZ, SZ, C.POINTER(SZ)]),
+    "vmlm_hip_sample": (I, [P, SZ, P, P, P, P, P, SZ, SZ, P, P, P, SZ, P]),
+    "vmlm_hip_sample_work": (I, [SZ, SZ, C.POINTER(SZ)]),
+    "vmlm_hip_tree_accept_kv4": (I, [C.POINTER(Kv4Cache), SZ, P, P, P, P, P, SZ, P, P, P, P]),
     # layer 3
     "vmlm_decoder_create": (I, [C.POINTER(DecoderCfg), C.POINTER(P)]),
     "vmlm_decoder_destroy": (I, [P]),

@@ -1328,6 +1328,370 @@ int vmlm_hip_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, s
     return launch_attn4(a, st);
 }
 
+// ---------------------------------------------------------------- drafted tokens
+// Rows of w values at stride ld whose addresses stay in 64 bits.
+static bool rows_fit(size_t rows, size_t ld, size_t w) {
+    const size_t most = std::max(w, rows > 1 ? ld : 0);
+    return most == 0 || rows <= ((size_t)1 << 50) / most;
+}
+
+static int check_rope(const RopeArgs &a, size_t rows, size_t H, size_t Hkv, size_t hd, size_t rot) {
+    VMLM_GUARD(hd >= 2 && hd % 2 == 0 && hd <= ROPE_MAX_HD && rot >= 2 && rot % 2 == 0 && rot <= hd,
+               "rope_qk: head_dim %zu, rot_dim %zu (even, rot_dim <= head_dim <= %d)", hd, rot,
+               ROPE_MAX_HD);
+    VMLM_GUARD(a.m - a.m == 0.0f, "rope_qk: the factor is not finite");
+    VMLM_GUARD(rows <= DIM_MAX && H <= 65535 && Hkv <= 65535,
+               "rope_qk: rows %zu over 2^30, or n_heads %zu, n_kv_heads %zu over 65535", rows, H, Hkv);
+    if (rows == 0 || H + Hkv == 0) return VMLM_OK;
+    const size_t wq = H * hd, wk = Hkv * hd;
+    VMLM_GUARD(H == 0 || (a.q && a.qo), "rope_qk: null query rows");
+    VMLM_GUARD(Hkv == 0 || (a.k && a.ko), "rope_qk: null key rows");
+    VMLM_GUARD(a.pos && a.freq, "rope_qk: null positions or frequencies");
+    VMLM_GUARD(((uintptr_t)a.freq & 7) == 0, "rope_qk: the frequencies must be 8-byte aligned");
+    VMLM_GUARD(rows == 1 || ((H == 0 || (a.ldq >= wq && a.ldqo >= wq)) &&
+                             (Hkv == 0 || (a.ldk >= wk && a.ldko >= wk))),
+               "rope_qk: a row stride is below the row's width");
+    VMLM_GUARD((H == 0 || (rows_fit(rows, a.ldq, wq) && rows_fit(rows, a.ldqo, wq))) &&
+                   (Hkv == 0 || (rows_fit(rows, a.ldk, wk) && rows_fit(rows, a.ldko, wk))),
+               "rope_qk: rows of over 2^50 values");
+    const bool same_q = a.qo == a.q && a.ldqo == a.ldq, same_k = a.ko == a.k && a.ldko == a.ldk;
+    VMLM_GUARD((same_q || !rows_overlap(a.qo, a.ldqo, wq, a.q, a.ldq, wq, rows)) &&
+                   (same_k || !rows_overlap(a.ko, a.ldko, wk, a.k, a.ldk, wk, rows)) &&
+                   !rows_overlap(a.qo, a.ldqo, wq, a.k, a.ldk, wk, rows) &&
+                   !rows_overlap(a.ko, a.ldko, wk, a.q, a.ldq, wq, rows) &&
+                   !rows_overlap(a.qo, a.ldqo, wq, a.ko, a.ldko, wk, rows),
+               "rope_qk: an output lies over another operand (only its own input may be it)");
+    for (const auto &[p, nb] : {std::pair<const void *, size_t>{a.pos, rows * 4}, {a.freq, rot * 4}})
+        VMLM_GUARD((H == 0 || !overlap(p, nb, a.qo, span(a.ldqo, wq, rows))) &&
+                       (Hkv == 0 || !overlap(p, nb, a.ko, span(a.ldko, wk, rows))),
+                   "rope_qk: an output lies over the positions or frequencies");
+    return VMLM_OK;
+}
+
+int vmlm_hip_rope_qk(float *q_out, size_t ldqo, float *k_out, size_t ldko, const float *q,
+                     size_t ldq, const float *k, size_t ldk, const int32_t *pos,
+                     const double *freq, size_t rows, size_t n_heads, size_t n_kv_heads,
+                     size_t head_dim, size_t rot_dim, bool interleaved, float factor,
+                     void *stream) {
+    RopeArgs a;
+    a.q = q;
+    a.k = k;
+    a.qo = q_out;
+    a.ko = k_out;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldqo = ldqo;
+    a.ldko = ldko;
+    a.pos = pos;
+    a.freq = freq;
+    a.inter = interleaved;
+    a.m = factor;
+    int rc = check_rope(a, rows, n_heads, n_kv_heads, head_dim, rot_dim);
+    if (rc || rows == 0 || n_heads + n_kv_heads == 0) return rc;
+    INIT_OR_RETURN();
+    if ((rc = on_library_device())) return rc;
+    a.rows = (int)rows;
+    a.H = (int)n_heads;
+    a.Hkv = (int)n_kv_heads;
+    a.hd = (int)head_dim;
+    a.rot = (int)rot_dim;
+    return launch_rope_qk(a, as_stream(stream));
+}
+
+int vmlm_rope_freqs(double *freq, float *factor, size_t rot_dim, double theta,
+                    const vmlm_rope_scaling *scaling) {
+    VMLM_GUARD(rot_dim >= 2 && rot_dim % 2 == 0 && rot_dim <= ROPE_MAX_HD,
+               "rope_freqs: rot_dim %zu is not even, or over %d", rot_dim, ROPE_MAX_HD);
+    VMLM_GUARD(freq && factor, "rope_freqs: null result");
+    VMLM_GUARD(theta > 0.0 && theta < HUGE_VAL, "rope_freqs: theta must be > 0");
+    const int kind = scaling ? scaling->kind : 0;
+    const double f = scaling ? scaling->factor : 1.0, pi2 = 6.28318530717958647693;
+    if (scaling) {
+        VMLM_GUARD(kind >= VMLM_ROPE_LINEAR && kind <= VMLM_ROPE_RAMP,
+                   "rope_freqs: unknown kind of scaling %d", kind);
+        VMLM_GUARD(f >= 1.0 && f < HUGE_VAL, "rope_freqs: the scaling's factor must be >= 1");
+        VMLM_GUARD(kind == VMLM_ROPE_LINEAR ||
+                       (scaling->low > 0.0 && scaling->high > scaling->low && scaling->high < HUGE_VAL &&
+                        scaling->trained > 0.0 && scaling->trained < HUGE_VAL),
+                   "rope_freqs: 0 < low < high turns of a trained length > 0 are needed");
+        VMLM_GUARD(kind != VMLM_ROPE_RAMP || theta > 1.0, "rope_freqs: a ramp needs theta > 1");
+    }
+    double lo = 0.0, hi = 0.0;
+    if (kind == VMLM_ROPE_RAMP) {
+        auto index = [&](double turns) {
+            return (double)rot_dim * log(scaling->trained / (pi2 * turns)) / (2.0 * log(theta));
+        };
+        lo = std::max(floor(index(scaling->high)), 0.0);
+        hi = std::min(ceil(index(scaling->low)), (double)rot_dim - 1.0);
+    }
+    for (size_t i = 0; i < rot_dim / 2; ++i) {
+        const double w = pow(theta, -2.0 * (double)i / (double)rot_dim);
+        double keep = 1.0;  // of the frequency; the rest of it divided
+        if (kind == VMLM_ROPE_LINEAR) keep = 0.0;
+        if (kind == VMLM_ROPE_BANDS)
+            keep = (scaling->trained * w / pi2 - scaling->low) / (scaling->high - scaling->low);
+        if (kind == VMLM_ROPE_RAMP) keep = 1.0 - ((double)i - lo) / std::max(hi - lo, 1e-3);
+        keep = std::min(std::max(keep, 0.0), 1.0);
+        freq[i] = w * keep + w / f * (1.0 - keep);
+    }
+    *factor = kind == VMLM_ROPE_RAMP ? (float)(0.1 * log(f) + 1.0) : 1.0f;
+    return VMLM_OK;
+}
+
+// The trees' arrays, [B] and [B][S].
+static int check_tree(const char *who, const Kv4View &c, const int32_t *pos0, size_t S, size_t most) {
+    VMLM_GUARD(S <= most, "%s: %zu tokens a sequence (limit %zu)", who, S, most);
+    if (c.B == 0 || S == 0) return VMLM_OK;
+    VMLM_GUARD(pos0, "%s: null positions", who);
+    return VMLM_OK;
+}
+
+static int check_tree_attn(const Kv4View &c, const float *q, size_t ldq, const int32_t *pos0,
+                           const int32_t *count, const int32_t *parent, size_t S, const float *out,
+                           size_t ldo, size_t H, float scale) {
+    VMLM_GUARD(c.Hkv > 0 && H % c.Hkv == 0 && H <= 65535, "kv4 tree attention: %zu heads over %d kv heads", H, c.Hkv);
+    int rc = check_tree("kv4 tree attention", c, pos0, S, parent ? TREE_MAX : 65535);
+    if (rc || c.B == 0 || S == 0 || H == 0) return rc;
+    const size_t rows = (size_t)c.B * S, w = H * c.hd, nb = (size_t)c.B * 4;
+    VMLM_GUARD(c.cap > 0, "kv4 tree attention: capacity 0");
+    VMLM_GUARD(q && out, "kv4 tree attention: null queries or output");
+    VMLM_GUARD(rows == 1 || (ldq >= w && ldo >= w),
+               "kv4 tree attention: a row stride is below the row's width");
+    VMLM_GUARD(rows_fit(rows, ldq, w) && rows_fit(rows, ldo, w),
+               "kv4 tree attention: rows of over 2^50 values");
+    VMLM_GUARD(scale - scale == 0.0f, "kv4 tree attention: the score scale is not finite");
+    VMLM_GUARD(!rows_overlap(out, ldo, w, q, ldq, w, rows),
+               "kv4 tree attention: the output lies over its input");
+    VMLM_GUARD(!over_cache(c, out, ldo, w, rows), "kv4 tree attention: the output lies over the cache");
+    const size_t ob = span(ldo, w, rows);
+    VMLM_GUARD(!overlap(out, ob, pos0, nb) && (!count || !overlap(out, ob, count, nb)) &&
+                   (!parent || !overlap(out, ob, parent, rows * 4)),
+               "kv4 tree attention: the output lies over the positions, counts or parents");
+    return VMLM_OK;
+}
+
+int vmlm_hip_attention_tree_kv4_work(const vmlm_kv4_cache *cache, size_t n_heads, size_t S,
+                                     size_t *bytes) {
+    VMLM_GUARD(bytes, "kv4 tree attention: null size");
+    Kv4View c;
+    int rc = check_kv4(cache, &c);
+    if (rc) return rc;
+    VMLM_GUARD(c.Hkv > 0 && n_heads % c.Hkv == 0 && n_heads <= 65535 && S <= 65535,
+               "kv4 tree attention: %zu heads over %d kv heads, %zu tokens (limits 65535)", n_heads, c.Hkv, S);
+    *bytes = tree_attn_work_floats(c, (int)n_heads, (int)S) * 4;
+    return VMLM_OK;
+}
+
+int vmlm_hip_attention_tree_kv4(const vmlm_kv4_cache *cache, const float *q, size_t ldq,
+                                const int32_t *pos0, const int32_t *count, const int32_t *parent,
+                                size_t S, float *out, size_t ldo, size_t n_heads, float scale,
+                                void *work, size_t work_bytes, void *stream) {
+    TreeAttnArgs a;
+    int rc = check_kv4(cache, &a.c);
+    if (!rc) rc = check_tree_attn(a.c, q, ldq, pos0, count, parent, S, out, ldo, n_heads, scale);
+    if (rc || a.c.B == 0 || S == 0 || n_heads == 0) return rc;
+    const size_t wf = tree_attn_work_floats(a.c, (int)n_heads, (int)S);
+    if (wf && work) {
+        const size_t rows = (size_t)a.c.B * S, w = n_heads * a.c.hd, nb = (size_t)a.c.B * 4;
+        VMLM_GUARD(work_bytes >= wf * 4 && ((uintptr_t)work & 15) == 0,
+                   "kv4 tree attention: workspace of %zu bytes, %zu needed (16-byte aligned)",
+                   work_bytes, wf * 4);
+        VMLM_GUARD(!overlap(work, wf * 4, out, span(ldo, w, rows)) &&
+                       !overlap(work, wf * 4, q, span(ldq, w, rows)) &&
+                       !overlap(work, wf * 4, pos0, nb) &&
+                       (!count || !overlap(work, wf * 4, count, nb)) &&
+                       (!parent || !overlap(work, wf * 4, parent, rows * 4)) &&
+                       !over_cache(a.c, work, wf, wf, 1),
+                   "kv4 tree attention: the workspace lies over an operand");
+    }
+    INIT_OR_RETURN();
+    if ((rc = on_library_device())) return rc;
+    hipStream_t st = as_stream(stream);
+    a.q = q;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.pos0 = pos0;
+    a.count = count;
+    a.parent = parent;
+    a.S = (int)S;
+    a.H = (int)n_heads;
+    a.out = out;
+    a.scale = scale;
+    if (wf == 0 || work) {
+        a.work = (float *)work;
+        return launch_tree_attn(a, st);
+    }
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    VMLM_HIP_CHECK(hipStreamIsCapturing(st, &cs));
+    VMLM_GUARD(cs == hipStreamCaptureStatusNone,
+               "kv4 tree attention: a captured call needs a workspace of its own (%zu bytes)", wf * 4);
+    Stage stg(st);
+    a.work = stg.alloc<float>(wf);
+    STAGE_OK(stg);
+    return launch_tree_attn(a, st);
+}
+
+static int check_sample(const SampleArgs &a, size_t ld, size_t rows, size_t vocab) {
+    VMLM_GUARD(rows <= (size_t)1 << 20, "sample: %zu rows (limit 2^20)", rows);
+    VMLM_GUARD(vocab >= 1 && vocab <= SAMPLE_MAX_VOCAB, "sample: vocab %zu (1 .. %zu)", vocab,
+               SAMPLE_MAX_VOCAB);
+    if (rows == 0) return VMLM_OK;
+    VMLM_GUARD(a.logits && a.u && a.t && a.token, "sample: null logits, random numbers, temperatures or tokens");
+    VMLM_GUARD(rows == 1 || ld >= vocab, "sample: row stride %zu is below the vocabulary %zu", ld, vocab);
+    VMLM_GUARD(rows_fit(rows, ld, vocab), "sample: rows of over 2^50 values");
+    const size_t nb = rows * 4;
+    VMLM_GUARD(!a.prob || !overlap(a.token, nb, a.prob, nb), "sample: token and prob lie over each other");
+    for (const void *o : {(const void *)a.token, (const void *)a.prob}) {
+        if (!o) continue;
+        VMLM_GUARD(!overlap(o, nb, a.logits, span(ld, vocab, rows)), "sample: a result lies over the logits");
+        for (const void *i : {(const void *)a.u, (const void *)a.t, (const void *)a.top_k,
+                              (const void *)a.top_p, (const void *)a.min_p})
+            VMLM_GUARD(!i || !overlap(o, nb, i, nb), "sample: a result lies over a setting");
+    }
+    return VMLM_OK;
+}
+
+int vmlm_hip_sample_work(size_t rows, size_t vocab, size_t *bytes) {
+    VMLM_GUARD(bytes, "sample: null size");
+    VMLM_GUARD(rows <= (size_t)1 << 20 && vocab >= 1 && vocab <= SAMPLE_MAX_VOCAB,
+               "sample: %zu rows (limit 2^20), vocab %zu (1 .. %zu)", rows, vocab, SAMPLE_MAX_VOCAB);
+    *bytes = sample_work_bytes((int)rows, (int)vocab);
+    return VMLM_OK;
+}
+
+int vmlm_hip_sample(const float *logits, size_t ld, const float *u, const float *temperature,
+                    const int32_t *top_k, const float *top_p, const float *min_p, size_t rows,
+                    size_t vocab, int32_t *token, float *prob, void *work, size_t work_bytes,
+                    void *stream) {
+    SampleArgs a;
+    a.logits = logits;
+    a.ld = ld;
+    a.u = u;
+    a.t = temperature;
+    a.top_k = top_k;
+    a.top_p = top_p;
+    a.min_p = min_p;
+    a.token = token;
+    a.prob = prob;
+    int rc = check_sample(a, ld, rows, vocab);
+    if (rc || rows == 0) return rc;
+    a.rows = (int)rows;
+    a.vocab = (int)vocab;
+    const size_t wb = sample_work_bytes(a.rows, a.vocab), nb = rows * 4;
+    if (wb && work) {
+        VMLM_GUARD(work_bytes >= wb && ((uintptr_t)work & 15) == 0,
+                   "sample: workspace of %zu bytes, %zu needed (16-byte aligned)", work_bytes, wb);
+        VMLM_GUARD(!overlap(work, wb, logits, span(ld, vocab, rows)), "sample: the workspace lies over the logits");
+        for (const void *p : {(const void *)u, (const void *)temperature, (const void *)top_k,
+                              (const void *)top_p, (const void *)min_p, (const void *)token,
+                              (const void *)prob})
+            VMLM_GUARD(!p || !overlap(work, wb, p, nb), "sample: the workspace lies over an operand");
+    }
+    INIT_OR_RETURN();
+    if ((rc = on_library_device())) return rc;
+    hipStream_t st = as_stream(stream);
+    if (wb == 0 || work) {
+        a.work = (char *)work;
+        return launch_sample(a, st);
+    }
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    VMLM_HIP_CHECK(hipStreamIsCapturing(st, &cs));
+    VMLM_GUARD(cs == hipStreamCaptureStatusNone,
+               "sample: a captured call needs a workspace of its own (%zu bytes)", wb);
+    Stage stg(st);
+    a.work = stg.alloc<char>(wb);
+    STAGE_OK(stg);
+    return launch_sample(a, st);
+}
+
+constexpr size_t ACCEPT_CACHES = 256;
+
+// The caches, of one shape; view: the first one's (or an empty one).
+static int check_accept(const vmlm_kv4_cache *caches, size_t n, const int32_t *pos0,
+                        const int32_t *count, const int32_t *parent, const int32_t *drafted,
+                        const int32_t *chosen, size_t S, const int32_t *path, const int32_t *kept,
+                        const int32_t *next, Kv4View *view, bool device) {
+    VMLM_GUARD(n >= 1 && n <= ACCEPT_CACHES, "tree accept: %zu caches (1 .. %zu)", n, ACCEPT_CACHES);
+    VMLM_GUARD(caches, "tree accept: null caches");
+    struct Range {
+        uintptr_t at, end;
+    } r[4 * ACCEPT_CACHES];
+    size_t nr = 0;
+    for (size_t i = 0; i < n; ++i) {
+        Kv4View c;
+        int rc = check_kv4(caches + i, &c, device);
+        if (rc) return rc;
+        if (i == 0) *view = c;
+        VMLM_GUARD(c.B == view->B && c.Hkv == view->Hkv && c.cap == view->cap && c.hd == view->hd,
+                   "tree accept: cache %zu has another shape than the first", i);
+        const size_t vals = (size_t)c.B * c.Hkv * c.cap * c.hd;
+        for (const void *p : {(const void *)c.k, (const void *)c.v})
+            r[nr++] = Range{(uintptr_t)p, (uintptr_t)p + vals / 2};
+        for (const void *p : {(const void *)c.km, (const void *)c.vm})
+            r[nr++] = Range{(uintptr_t)p, (uintptr_t)p + vals / 8};
+    }
+    const Kv4View &c = *view;
+    int rc = check_tree("tree accept", c, pos0, S, TREE_MAX);
+    if (rc || c.B == 0 || S == 0) return rc;
+    VMLM_GUARD(c.cap > 0 && c.Hkv > 0, "tree accept: capacity 0 or no heads");
+    VMLM_GUARD(drafted && chosen && path && kept && next, "tree accept: null tokens or results");
+    std::sort(r, r + nr, [](const Range &a, const Range &b) { return a.at < b.at; });
+    for (size_t i = 1; i < nr; ++i)
+        VMLM_GUARD(r[i].at >= r[i - 1].end, "tree accept: two caches lie over each other");
+    const size_t nb = (size_t)c.B * 4, ns = nb * S;
+    const std::pair<const void *, size_t> in[] = {{pos0, nb}, {count, nb}, {parent, ns}, {drafted, ns}, {chosen, ns}},
+                                          out[] = {{path, ns}, {kept, nb}, {next, nb}};
+    for (size_t o = 0; o < 3; ++o) {
+        for (const auto &i : in)
+            VMLM_GUARD(!i.first || !overlap(out[o].first, out[o].second, i.first, i.second),
+                       "tree accept: a result lies over an input");
+        for (size_t x = 0; x < o; ++x)
+            VMLM_GUARD(!overlap(out[o].first, out[o].second, out[x].first, out[x].second),
+                       "tree accept: two results lie over each other");
+    }
+    auto in_caches = [&](const void *p, size_t bytes) {  // the ranges are in order and apart
+        size_t i = 0;
+        while (i < nr && r[i].end <= (uintptr_t)p) ++i;
+        return p && i < nr && r[i].at < (uintptr_t)p + bytes;
+    };
+    for (const auto &i : in)
+        VMLM_GUARD(!in_caches(i.first, i.second), "tree accept: an input lies over a cache");
+    for (const auto &o : out)
+        VMLM_GUARD(!in_caches(o.first, o.second), "tree accept: a result lies over a cache");
+    return VMLM_OK;
+}
+
+int vmlm_hip_tree_accept_kv4(const vmlm_kv4_cache *caches, size_t n_caches, const int32_t *pos0,
+                             const int32_t *count, const int32_t *parent, const int32_t *drafted,
+                             const int32_t *chosen, size_t S, int32_t *path, int32_t *kept,
+                             int32_t *next, void *stream) {
+    Kv4View c;
+    int rc = check_accept(caches, n_caches, pos0, count, parent, drafted, chosen, S, path, kept, next, &c, true);
+    if (rc || c.B == 0 || S == 0) return rc;
+    INIT_OR_RETURN();
+    if ((rc = on_library_device())) return rc;
+    Kv4Arrays arrays[ACCEPT_CACHES];
+    for (size_t i = 0; i < n_caches; ++i)
+        arrays[i] = Kv4Arrays{caches[i].k, caches[i].v, caches[i].k_meta, caches[i].v_meta};
+    AcceptArgs a;
+    a.c = arrays;
+    a.caches = n_caches;
+    a.B = c.B;
+    a.Hkv = c.Hkv;
+    a.cap = c.cap;
+    a.hd = c.hd;
+    a.pos0 = pos0;
+    a.count = count;
+    a.parent = parent;
+    a.drafted = drafted;
+    a.chosen = chosen;
+    a.S = (int)S;
+    a.path = path;
+    a.kept = kept;
+    a.next = next;
+    return launch_tree_accept(a, as_stream(stream));
+}
+
 // ================================================================ layer 1
 int vmlm_gemm_nt_int8(const float *a, const int8_t *q, const float *scale, float *c, size_t m,
                       size_t n, size_t k) {
@@ -1890,6 +2254,133 @@ int vmlm_attention_decode_kv4(const vmlm_kv4_cache *cache, const float *q, const
                                            nullptr, 0, st);
         if (!rc) rc = download(out, dout, B * w * sizeof(float), st);
         if (!rc && k_new) rc = dc.back(*cache, st);
+        if (rc) return rc;
+    }
+    FINISH(st);
+}
+
+// ---------------------------------------------------------------- drafted tokens
+int vmlm_rope_qk(float *q_out, float *k_out, const float *q, const float *k, const int32_t *pos,
+                 const double *freq, size_t rows, size_t n_heads, size_t n_kv_heads,
+                 size_t head_dim, size_t rot_dim, bool interleaved, float factor) {
+    RopeArgs a;
+    const size_t wq = n_heads * head_dim, wk = n_kv_heads * head_dim;
+    a.q = q;
+    a.k = k;
+    a.qo = q_out;
+    a.ko = k_out;
+    a.ldq = a.ldqo = wq;
+    a.ldk = a.ldko = wk;
+    a.pos = pos;
+    a.freq = freq;
+    a.m = factor;
+    int rc = check_rope(a, rows, n_heads, n_kv_heads, head_dim, rot_dim);
+    if (rc || rows == 0 || n_heads + n_kv_heads == 0) return rc;
+    HOST_CALL_BEGIN();
+    {
+        Stage stg(st);
+        float *dq = stg.upload(q, rows * wq), *dk = stg.upload(k, rows * wk);
+        int32_t *dp = stg.upload(pos, rows);
+        double *df = stg.upload(freq, rot_dim / 2);
+        // idle rows come back as they are
+        float *dqo = q_out == q ? dq : stg.upload((const float *)q_out, rows * wq);
+        float *dko = k_out == k ? dk : stg.upload((const float *)k_out, rows * wk);
+        STAGE_OK(stg);
+        rc = vmlm_hip_rope_qk(dqo, wq, dko, wk, dq, wq, dk, wk, dp, df, rows, n_heads, n_kv_heads,
+                              head_dim, rot_dim, interleaved, factor, st);
+        if (!rc) rc = download(q_out, dqo, rows * wq * sizeof(float), st);
+        if (!rc) rc = download(k_out, dko, rows * wk * sizeof(float), st);
+        if (rc) return rc;
+    }
+    FINISH(st);
+}
+
+int vmlm_attention_tree_kv4(const vmlm_kv4_cache *cache, const float *q, const int32_t *pos0,
+                            const int32_t *count, const int32_t *parent, size_t S, float *out,
+                            size_t n_heads, float scale) {
+    Kv4View c;
+    int rc = check_kv4(cache, &c, false);
+    const size_t w = rc ? 0 : n_heads * c.hd;
+    if (!rc) rc = check_tree_attn(c, q, w, pos0, count, parent, S, out, w, n_heads, scale);
+    if (rc || c.B == 0 || S == 0 || n_heads == 0) return rc;
+    HOST_CALL_BEGIN();
+    {
+        const size_t rows = (size_t)c.B * S;
+        Stage stg(st);
+        Kv4Staged dc(stg, *cache);
+        float *dq = stg.upload(q, rows * w), *dout = stg.upload((const float *)out, rows * w);
+        int32_t *dp = stg.upload(pos0, c.B), *dn = count ? stg.upload(count, c.B) : nullptr;
+        int32_t *dt = parent ? stg.upload(parent, rows) : nullptr;
+        STAGE_OK(stg);
+        rc = vmlm_hip_attention_tree_kv4(&dc.d, dq, w, dp, dn, dt, S, dout, w, n_heads, scale,
+                                         nullptr, 0, st);
+        if (!rc) rc = download(out, dout, rows * w * sizeof(float), st);
+        if (rc) return rc;
+    }
+    FINISH(st);
+}
+
+int vmlm_sample(const float *logits, const float *u, const float *temperature,
+                const int32_t *top_k, const float *top_p, const float *min_p, size_t rows,
+                size_t vocab, int32_t *token, float *prob) {
+    SampleArgs a;
+    a.logits = logits;
+    a.u = u;
+    a.t = temperature;
+    a.top_k = top_k;
+    a.top_p = top_p;
+    a.min_p = min_p;
+    a.token = token;
+    a.prob = prob;
+    int rc = check_sample(a, vocab, rows, vocab);
+    if (rc || rows == 0) return rc;
+    HOST_CALL_BEGIN();
+    {
+        Stage stg(st);
+        float *dl = stg.upload(logits, rows * vocab), *du = stg.upload(u, rows);
+        float *dt = stg.upload(temperature, rows);
+        int32_t *dk = top_k ? stg.upload(top_k, rows) : nullptr;
+        float *dp = top_p ? stg.upload(top_p, rows) : nullptr;
+        float *dm = min_p ? stg.upload(min_p, rows) : nullptr;
+        int32_t *dtok = stg.upload((const int32_t *)token, rows);
+        float *dprob = prob ? stg.upload((const float *)prob, rows) : nullptr;
+        STAGE_OK(stg);
+        rc = vmlm_hip_sample(dl, vocab, du, dt, dk, dp, dm, rows, vocab, dtok, dprob, nullptr, 0, st);
+        if (!rc) rc = download(token, dtok, rows * sizeof(int32_t), st);
+        if (!rc && prob) rc = download(prob, dprob, rows * sizeof(float), st);
+        if (rc) return rc;
+    }
+    FINISH(st);
+}
+
+int vmlm_tree_accept_kv4(const vmlm_kv4_cache *caches, size_t n_caches, const int32_t *pos0,
+                         const int32_t *count, const int32_t *parent, const int32_t *drafted,
+                         const int32_t *chosen, size_t S, int32_t *path, int32_t *kept,
+                         int32_t *next) {
+    Kv4View c;
+    int rc = check_accept(caches, n_caches, pos0, count, parent, drafted, chosen, S, path, kept, next, &c, false);
+    if (rc || c.B == 0 || S == 0) return rc;
+    HOST_CALL_BEGIN();
+    {
+        const size_t rows = (size_t)c.B * S;
+        Stage stg(st);
+        int32_t *dp = stg.upload(pos0, c.B), *dn = count ? stg.upload(count, c.B) : nullptr;
+        int32_t *dt = parent ? stg.upload(parent, rows) : nullptr;
+        int32_t *dd = stg.upload(drafted, rows), *dc = stg.upload(chosen, rows);
+        int32_t *dpath = stg.upload((const int32_t *)path, rows);
+        int32_t *dkept = stg.upload((const int32_t *)kept, c.B);
+        int32_t *dnext = stg.upload((const int32_t *)next, c.B);
+        STAGE_OK(stg);
+        for (size_t i = 0; i < n_caches; ++i) {  // (one at a time: the same walk for each)
+            Kv4Staged one(stg, caches[i]);
+            STAGE_OK(stg);
+            rc = vmlm_hip_tree_accept_kv4(&one.d, 1, dp, dn, dt, dd, dc, S, dpath, dkept, dnext, st);
+            if (!rc) rc = one.back(caches[i], st);
+            if (rc) return rc;
+        }
+        rc = download(path, dpath, rows * sizeof(int32_t), st);
+        if (!rc) rc = download(kept, dkept, c.B * sizeof(int32_t), st);
+        if (!rc) rc = download(next, dnext, c.B * sizeof(int32_t), st);
         if (rc) return rc;
     }
     FINISH(st);

@@ -554,6 +554,69 @@ struct Attn4Args {
 size_t attn4_work_floats(const Kv4View &c, int H);
 int launch_attn4(const Attn4Args &a, hipStream_t st);
 
+// Positions rotated into query and key heads (k_rope.hip): the pairs of the first `rot` channels
+// by pos * freq[i], times m. Rows with pos < 0 are left as they are.
+constexpr int ROPE_MAX_HD = 512;
+struct RopeArgs {
+    const float *q = nullptr, *k = nullptr;
+    float *qo = nullptr, *ko = nullptr;
+    size_t ldq = 0, ldk = 0, ldqo = 0, ldko = 0;
+    const int32_t *pos = nullptr;
+    const double *freq = nullptr;
+    int rows = 0, H = 0, Hkv = 0, hd = 0, rot = 0;
+    bool inter = false;
+    float m = 1.0f;
+};
+int launch_rope_qk(const RopeArgs &a, hipStream_t st);
+
+// Several tokens a sequence (tree.hpp) over the 4-bit cache (k_treeattn.hip). `work`:
+// tree_attn_work_floats() floats.
+constexpr int TREE_MAX = 64;  // tokens of a tree
+struct TreeAttnArgs {
+    Kv4View c;
+    const float *q = nullptr;
+    size_t ldq = 0, ldo = 0;
+    const int32_t *pos0 = nullptr, *count = nullptr, *parent = nullptr;
+    int S = 0, H = 0;
+    float *out = nullptr;
+    float scale = 0.0f;
+    float *work = nullptr;
+};
+size_t tree_attn_work_floats(const Kv4View &c, int H, int S);
+int launch_tree_attn(const TreeAttnArgs &a, hipStream_t st);
+
+// The accepted rows of drafted trees to the front, in caches of one shape (k_tree.hip).
+constexpr int TREE_CACHES = 16;  // of a launch
+struct Kv4Arrays {
+    uint8_t *k, *v;
+    uint32_t *km, *vm;
+};
+struct AcceptArgs {
+    const Kv4Arrays *c = nullptr;
+    size_t caches = 0;
+    int B = 0, Hkv = 0, cap = 0, hd = 0;
+    const int32_t *pos0 = nullptr, *count = nullptr, *parent = nullptr, *drafted = nullptr,
+                  *chosen = nullptr;
+    int S = 0;
+    int32_t *path = nullptr, *kept = nullptr, *next = nullptr;
+};
+int launch_tree_accept(const AcceptArgs &a, hipStream_t st);
+
+// A token of each row of logits (k_sample.hip).
+constexpr size_t SAMPLE_MAX_VOCAB = ((size_t)1 << 20) - 1;
+struct SampleArgs {
+    const float *logits = nullptr;
+    size_t ld = 0;
+    const float *u = nullptr, *t = nullptr, *top_p = nullptr, *min_p = nullptr;
+    const int32_t *top_k = nullptr;
+    int rows = 0, vocab = 0;
+    int32_t *token = nullptr;
+    float *prob = nullptr;
+    char *work = nullptr;  // sample_work_bytes() bytes
+};
+size_t sample_work_bytes(int rows, int vocab);
+int launch_sample(const SampleArgs &a, hipStream_t st);
+
 // B1 gather forward over source-major activations.
 int launch_b1_forward(const float *w, const uint32_t *src, int n, int k0, const float *xt,
                       size_t t8, int n_tokens, float *yt, int mode, int act, hipStream_t st);

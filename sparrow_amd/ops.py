@@ -360,3 +360,87 @@ class Kv4Cache:
                                               *(None if x is None else _p(x) for x in new),
                                               _p(pos), _p(out), n_heads, float(scale)))
         return out
+
+    def attention_tree(self, q, pos0, count=None, parent=None, scale=None, out=None):
+        """q [batch, S, n_heads * head_dim]: token t of a sequence, its row stored at pos0 + t,
+        attends the positions before pos0, itself and the tokens it follows (parent
+        [batch, S], -1: none; None: each the one before it). Rows from count on and of sequences
+        with pos0 < 0 keep `out`'s values (None: zeros)."""
+        q = _c(q, np.float32)
+        S, n_heads = q.shape[1], q.shape[2] // self.head_dim
+        assert q.shape == (self.batch, S, n_heads * self.head_dim)
+        pos0, count = self._rows(pos0, count)
+        parent = None if parent is None else _c(parent, np.int32)
+        assert parent is None or parent.shape == (self.batch, S)
+        if scale is None:
+            scale = float(np.float32(1.0 / np.sqrt(self.head_dim)))
+        out = np.zeros_like(q) if out is None else _c(out, np.float32).copy()
+        assert out.shape == q.shape
+        check(lib().vmlm_attention_tree_kv4(self.descriptor(), _p(q), _p(pos0), _opt(count),
+                                            _opt(parent), S, _p(out), n_heads, float(scale)))
+        return out
+
+
+# ---------------------------------------------------------------- drafted tokens
+def _opt(a):
+    return None if a is None else _p(a)
+
+
+def rope_freqs(rot_dim, theta=10000.0, scaling=None):
+    """(radians a position for each pair, the factor of the rotated values). scaling:
+    None, ("linear", factor), or ("bands" or "ramp", factor, low, high, trained)."""
+    freq, factor = np.empty(rot_dim // 2), C.c_float()
+    if scaling is not None:
+        kind = {"linear": 1, "bands": 2, "ramp": 3}[scaling[0]]
+        scaling = _abi.RopeScaling(kind, *map(float, scaling[1:]))
+    check(lib().vmlm_rope_freqs(_p(freq), C.byref(factor), rot_dim, float(theta),
+                                None if scaling is None else C.byref(scaling)))
+    return freq, factor.value
+
+
+def rope_qk(q, k, pos, freq, head_dim, interleaved=False, factor=1.0):
+    """Rotates the first 2 * len(freq) channels of every head of q [rows, H * head_dim] and k
+    [rows, Hkv * head_dim] to `pos` [rows]. Rows with pos < 0 give zeros."""
+    q, k, pos = _c(q, np.float32), _c(k, np.float32), _c(pos, np.int32)
+    freq = _c(freq, np.float64)
+    rows = q.shape[0]
+    assert k.shape[0] == rows and pos.size == rows
+    assert q.shape[1] % head_dim == 0 and k.shape[1] % head_dim == 0
+    qo, ko = np.zeros_like(q), np.zeros_like(k)
+    check(lib().vmlm_rope_qk(_p(qo), _p(ko), _p(q), _p(k), _p(pos), _p(freq), rows,
+                             q.shape[1] // head_dim, k.shape[1] // head_dim, head_dim,
+                             2 * freq.size, bool(interleaved), float(factor)))
+    return qo, ko
+
+
+def sample(logits, u, temperature, top_k=None, top_p=None, min_p=None):
+    """(token, prob) of each row of logits [rows, vocab], drawn with u [rows] in [0, 1);
+    settings [rows] or one for all. Rows with u < 0 give -1 and 0."""
+    logits = _c(logits, np.float32)
+    rows, vocab = logits.shape
+
+    def each(x, dt):
+        return None if x is None else _c(np.broadcast_to(np.asarray(x, dt), (rows,)), dt)
+    u, t = each(u, np.float32), each(temperature, np.float32)
+    k, p, m = each(top_k, np.int32), each(top_p, np.float32), each(min_p, np.float32)
+    token, prob = np.full(rows, -1, np.int32), np.zeros(rows, np.float32)
+    check(lib().vmlm_sample(_p(logits), _p(u), _p(t), _opt(k), _opt(p), _opt(m), rows, vocab,
+                            _p(token), _p(prob)))
+    return token, prob
+
+
+def tree_accept(caches, pos0, drafted, chosen, count=None, parent=None):
+    """(path [batch, S], kept [batch], next [batch]): the accepted tokens of each tree, whose rows
+    move up to pos0 in every one of `caches` (Kv4Cache). -1, 0 and -1 for idle sequences."""
+    drafted, chosen = _c(drafted, np.int32), _c(chosen, np.int32)
+    batch, S = drafted.shape
+    assert chosen.shape == (batch, S) and all(c.batch == batch for c in caches)
+    pos0, count = caches[0]._rows(pos0, count)
+    parent = None if parent is None else _c(parent, np.int32)
+    assert parent is None or parent.shape == (batch, S)
+    path = np.full((batch, S), -1, np.int32)
+    kept, nxt = np.zeros(batch, np.int32), np.full(batch, -1, np.int32)
+    desc = (_abi.Kv4Cache * len(caches))(*(c.descriptor() for c in caches))
+    check(lib().vmlm_tree_accept_kv4(desc, len(caches), _p(pos0), _opt(count), _opt(parent),
+                                     _p(drafted), _p(chosen), S, _p(path), _p(kept), _p(nxt)))
+    return path, kept, nxt
