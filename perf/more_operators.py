@@ -8,7 +8,6 @@ tokens or the angle of a far position needs it); with `own` true it makes the
 library's calls, on the library's own stream (a null stream), as a program without
 streams of its own makes them.
 """
-import ctypes
 import functools
 import math
 
@@ -511,8 +510,7 @@ def _own_accept(st):
         desc, len(desc), _p(st["pos0"]), _p(st["count"]), _p(st["parent"]), _p(st["drafted"]),
         _p(st["chosen"]), s, _p(st["path"]), _p(st["kept"]), _p(st["next"]), None))
     for n in range(len(desc)):
-        one = ctypes.byref(desc, n * ctypes.sizeof(desc._type_))
-        check(L.vmlm_hip_kv4_read(one, _p(st["rows"][2 * n]), w, _p(st["rows"][2 * n + 1]), w,
+        check(L.vmlm_hip_kv4_read(desc[n], _p(st["rows"][2 * n]), w, _p(st["rows"][2 * n + 1]), w,
                                   _p(st["pos0"]), None, s, None))
     return [st["path"], st["kept"], st["next"], *st["rows"]]
 
