@@ -43,6 +43,9 @@ typedef int i32x4l __attribute__((ext_vector_type(4)));
 constexpr int TA_W = 4;  // waves of a workgroup
 constexpr float TA_NONE = -3.40282347e38f;  // the maximum of no score yet
 constexpr int TA_NO_GROUP = -1000;          // the weight of channels where all queries are 0
+constexpr int TA_UNSET = -100000;
+constexpr int TA_SPAN = 7;                  // positions of like size: within 2^7
+constexpr float TA_FAR = 4194304.0f;        // scores whose f32 steps are no longer small
 
 struct TreeAttnParams {
     Kv4View c;
@@ -52,7 +55,7 @@ struct TreeAttnParams {
     int S, H, G;
     int tiles, shares;  // of queries; of the positions
     float *out, *work;
-    float scale;  // of the scores: scale * 2^scale_e, |scale| in [1/2, 1), times log2(e)
+    float scale, sign;  // of the scores: sign * scale * 2^scale_e, scale in [1/2, 1) (or 0), times log2(e)
     int scale_e;
     int *guard;
 };
@@ -78,14 +81,28 @@ __device__ __forceinline__ uint32_t f16_pair(float a, float b) {
     const hw_f32x2 v = {a, b};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
 }
-__device__ __forceinline__ float f16_low(uint32_t v) { return (float)__builtin_bit_cast(f16x2, v)[0]; }
-__device__ __forceinline__ float f16_high(uint32_t v) { return (float)__builtin_bit_cast(f16x2, v)[1]; }
+// x less the f16 in the low or high half of v, in one operation (which the compiler
+// makes two of)
+template <int HIGH>
+__device__ __forceinline__ float f16_rest(uint32_t v, float x) {
+    float r;
+    if (HIGH)
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(v), "v"(x));
+    else
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(v), "v"(x));
+    return r;
+}
 
 // x as two f16 terms
 __device__ __forceinline__ uint32_t two_terms(float x) {
     const _Float16 hi = (_Float16)x;
     const f16x2 v = {hi, (_Float16)(x - (float)hi)};
     return __builtin_bit_cast(uint32_t, v);
+}
+
+// A number that is the same in all lanes, in a scalar register.
+__device__ __forceinline__ float uniform(float v) {
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
 }
 
 // The exponent e of a magnitude below 2^e (of numbers that are not normal -126).
@@ -96,12 +113,11 @@ __device__ __forceinline__ int exp_of(float mag) { return (int)(__float_as_uint(
 struct Codes8 {
     f16x8 v;
     __device__ __forceinline__ Codes8(uint32_t w, const uint32_t (&s)[4], const uint32_t (&c)[4]) {
-        w ^= 0x88888888u;
         const uint32_t t[4] = {w << 6, w << 2, w >> 2, w >> 6};
         uint32_t r[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const uint32_t x = (t[k] & 0x03C003C0u) | 0x4C004C00u;
+            const uint32_t x = (t[k] & 0x03C003C0u) ^ 0x4E004E00u;  // (nibble ^ 8)
             r[k] = __builtin_bit_cast(
                 uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, x),
                                                     __builtin_bit_cast(f16x2, s[k]),
@@ -148,11 +164,15 @@ struct RawBlock {
     uint32_t k[2][KD], km[2][GX], own[2][OWN], v[HD / 16], vm[VM];
     __device__ __forceinline__ void load(const Kv4View &c, size_t head, int blk, int lane) {
         const int r = lane & 15, j = lane >> 4;
+        // (addresses: the same for all lanes, and 32 bits of a lane's own)
+        const size_t row0 = head * c.cap + blk * KV4_BLOCK;
+        const uint8_t *kb = c.k + row0 * (HD / 2);
+        const uint32_t *kmb = c.km + row0 * NG;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const size_t row = head * c.cap + blk * KV4_BLOCK + 8 * (r >> 2) + (r & 3) + 4 * x;
-            const uint8_t *kp = c.k + row * (HD / 2) + j * (HD / 8);
-            const uint32_t *mp = c.km + row * NG;
+            const uint32_t row = 8 * (r >> 2) + (r & 3) + 4 * x;
+            const uint8_t *kp = kb + (row * (HD / 2) + j * (HD / 8));
+            const uint32_t *mp = kmb + row * NG;
             if constexpr (HD == 32) {
                 k[x][0] = *(const uint32_t *)kp;
                 km[x][0] = own[x][0] = mp[0];
@@ -177,10 +197,10 @@ struct RawBlock {
                 for (int e = 0; e < OWN; ++e) own[x][e] = mp[j * OWN + e];
             }
         }
-        const uint32_t *vp = (const uint32_t *)(c.v + (head * (c.cap / KV4_BLOCK) + blk) * (size_t)(HD * 16));
+        const uint32_t *vp = (const uint32_t *)(c.v + row0 * (HD / 2));
 #pragma unroll
-        for (int n = 0; n < HD / 16; ++n) v[n] = vp[(n * 16 + r) * 4 + j];
-        const uint32_t *mp = c.vm + (head * c.cap + blk * KV4_BLOCK + (lane & 31)) * NG + (lane >> 5) * (NG / 2);
+        for (int n = 0; n < HD / 16; ++n) v[n] = vp[(uint32_t)((n * 16 + r) * 4 + j)];
+        const uint32_t *mp = c.vm + row0 * NG + (uint32_t)((lane & 31) * NG + (lane >> 5) * (NG / 2));
 #pragma unroll
         for (int i = 0; i < VM; ++i) vm[i] = mp[i];
     }
@@ -193,7 +213,8 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     using Raw = RawBlock<HD>;
     constexpr int NG = HD / 32, KS = HD / 32, NT = HD / 16, CL = HD / 4, ROWS = 16 * MT;
     extern __shared__ __align__(16) uint8_t lds[];
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, col = lane & 15, j = lane >> 4;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int col = lane & 15, j = lane >> 4;
     // the tiles that read the same positions lie 8 workgroups apart: on one XCD
     const int x8 = blockIdx.x / 8, stream = x8 / p.tiles * 8 + (int)(blockIdx.x % 8), tile = x8 % p.tiles;
     const int share = stream % p.shares, pair = stream / p.shares, kvh = pair % p.c.Hkv, b = pair / p.c.Hkv;
@@ -267,11 +288,17 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
             if (lane >= t_lo && lane <= t_hi)
                 for (int r = max(lane * p.G - row0, 0); r < min((lane + 1) * p.G - row0, rows); ++r) mask[r] = seen;
         }
+    } else if (tid < ROWS) {
+        mask[tid] = (uint32_t)(tr.pos0 + (row0 + min(tid, rows - 1)) / p.G);  // the last position
     }
     __syncthreads();
     int group_e[NG];
+    float weight[NG];  // (only to choose powers of two: 0 where it leaves f32)
 #pragma unroll
-    for (int g = 0; g < NG; ++g) group_e[g] = __builtin_amdgcn_readfirstlane(ge[g]);
+    for (int g = 0; g < NG; ++g) {
+        group_e[g] = __builtin_amdgcn_readfirstlane(ge[g]);
+        weight[g] = uniform(ldexpf(1.0f, group_e[g]));
+    }
     for (int r = w; r < ROWS; r += TA_W) {
         float x[CW];
         int bad = 0;
@@ -284,7 +311,7 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
 #pragma unroll
         for (int i = 0; i < CW; ++i) {
             const int c = i * 64 + lane, g = min(c / 32, NG - 1);
-            const float y = bad ? __builtin_nanf("") : ldexpf(x[i], 8 - F - ge[g]);  // below 2^9
+            const float y = bad ? __builtin_nanf("") : ldexpf(x[i] * p.sign, 8 - F - ge[g]);  // below 2^9
             const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
             const float sum = ta_swap16(ta_row16((float)hi + (float)lo, ta_add), ta_add);
             if (c >= HD) continue;
@@ -301,168 +328,195 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     }
     __syncthreads();
 
-    float m[MT], l[MT];
+    float m[MT], l[MT], cq[MT];
     f32x4 O[MT][NT + 1];
-    int fq[MT], lim[MT];
-    unsigned long long see[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        const int r = t * 16 + col;
         m[t] = TA_NONE;
         l[t] = 0.0f;
 #pragma unroll
         for (int n = 0; n <= NT; ++n) O[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        fq[t] = fe[r];
-        see[t] = p.parent ? mask[r] : 0;
-        lim[t] = tr.pos0 + (row0 + min(r, rows - 1)) / p.G;
     }
     uint8_t *wl = lds + M::WAVE + w * M::WB;
     int *ek = (int *)(wl + M::N);
     float *ev = (float *)(wl + M::N + 128), *iev = ev + 32;
     const uint8_t *qf = lds + M::Q + lane * 16;
     const float cs = p.scale;
-    // group g's number, g the same in all lanes or not
-    auto pick = [&](int g) {
-        int e = group_e[0];
-#pragma unroll
-        for (int i = 1; i < NG; ++i) e = g == i ? group_e[i] : e;
-        return e;
+    // the powers of two that keys and values of a block stand below where all its positions
+    // are within 2^TA_SPAN of them (ek_run, ev_run), and the factors that they mean
+    int ek_run = TA_UNSET, ev_run = TA_UNSET;
+    float kmul[NG], vmul = 0.0f, vsum = 0.0f;
+    bool plain = false, far_any = false;
+
+    // (nothing is moved over it, nor kept in registers for what comes after: fewer of them)
+    auto apart = [] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
     };
 
-    Raw next;
-    if (b0 + w < b1) next.load(p.c, head, b0 + w, lane);
-    for (int blk = b0 + w; blk < b1; blk += TA_W) {
-        const Raw raw = next;
-        if (blk + TA_W < b1) next.load(p.c, head, blk + TA_W, lane);
+    float mid[2][Raw::GX], sc[2][Raw::GX], vmid[Raw::VM], vsc[Raw::VM], vmag;
+    unsigned long long nan_p[Raw::VM];  // lanes whose value's meta is a NaN
+    // f of the group of the lane's o-th own codes
+    auto own_group = [&](int o, auto f) {
+        const int g = NG == 1 ? 0 : NG == 2 ? j >> 1 : j * Raw::OWN + o;
+        auto e = f(0);
+#pragma unroll
+        for (int i = 1; i < NG; ++i) e = g == i ? f(i) : e;
+        return e;
+    };
+    // of the group g of key_meta's
+    auto meta_group = [&](const auto (&v)[NG], int g) { return NG == 8 && (j & 1) ? v[NG > 4 ? 4 + g : g] : v[g]; };
+    // a position's codes and middles as the product's operand
+    auto key_codes = [&](const Raw &raw, int x, const float (&own)[Raw::OWN], const uint32_t (&middles)[Raw::GX],
+                         f16x8 (&kf)[KS + 1]) {
+        uint32_t ex[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int g = 0; g < Raw::GX; ++g) ex[g] = NG <= 4 && (j & 1) ? 0u : middles[g];  // (no group 4 ..)
+        kf[KS] = __builtin_bit_cast(f16x8, u32x4{ex[0], ex[1], ex[2], ex[3]});
+#pragma unroll
+        for (int o = 0; o < Raw::OWN; ++o) {
+            const uint32_t sp = f16_pair(own[o], own[o]), cp = minus24(sp);
+            const uint32_t s4[4] = {sp, sp, sp, sp}, c4[4] = {cp, cp, cp, cp};
+            constexpr int D = KS / Raw::OWN;
+#pragma unroll
+            for (int i = 0; i < D; ++i) kf[o * D + i] = Codes8(raw.k[x][o * D + i], s4, c4).v;
+        }
+    };
+    auto scores = [&](int t, const f16x8 (&kf)[KS + 1]) {
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 2 * KS + 1; ++i) {
+            const f16x8 qv = *(const f16x8 *)(qf + (t * M::FR + i) * 1024);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i == 2 * KS ? KS : i / 2], qv, acc, 0, 0, 0);
+        }
+        return acc;
+    };
+    // values' meta as f16 (scaled by f), where the lanes that hold their codes find it
+    auto stage_values = [&](auto f) {
+        if (NG == 1 && lane >= 32) return;
+        _Float16 *o = (_Float16 *)wl + (lane & 24) + slot8(lane & 7);
+#pragma unroll
+        for (int i = 0; i < Raw::VM; ++i) {
+            const int g = (lane >> 5) * (NG / 2) + i;
+            const f16x2 t = __builtin_bit_cast(f16x2, two_terms(f(vmid[i], 3)));
+            o[g * 64] = t[0];
+            o[g * 64 + 32] = t[1];
+            o[M::SC / 2 + g * 32] = (_Float16)f(vsc[i], 0);
+        }
+    };
+    auto value_codes = [&](const Raw &raw, int n) {
+        if (n == NT) return *(const f16x8 *)(wl + col * 64 + j * 16);
+        const u32x4 s = *(const u32x4 *)(wl + M::SC + n / 2 * 64 + j * 16);
+        const uint32_t s4[4] = {s[0], s[1], s[2], s[3]};
+        const uint32_t c4[4] = {minus24(s[0]), minus24(s[1]), minus24(s[2]), minus24(s[3])};
+        return Codes8(raw.v[n], s4, c4).v;
+    };
+    // What follows a block's meta. `like`: all queries see all of it, and its positions are of
+    // like size; else every position has a power of two of its own. (One copy of the
+    // products for both: with two, the accumulators took their registers twice.)
+    auto block = [&](const Raw &raw, int blk, bool edge, bool like) {
         const int p0 = blk * KV4_BLOCK;
-        const bool edge = p0 + KV4_BLOCK > zone || p0 + KV4_BLOCK > last + 1;
-
-        // 2. keys: rows of S^T, 4 j' + i of tile x is position 8 j' + 4 x + i
-        f16x8 kf[2][KS + 1];
+        // (kept from splitting the code after it in two)
+        auto is_like = [&] {
+            int v = __builtin_amdgcn_readfirstlane(like);
+            asm volatile("" : "+s"(v));
+            return v != 0;
+        };
+        // 4. values' meta, keys' powers of two and factors
+        uint32_t middles[2][Raw::GX];
+        float own[2][Raw::OWN];
+        if (is_like()) {
+            stage_values([&](float v, int e) { return v * (vmul * (float)(1 << e)); });
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int g = 0; g < Raw::GX; ++g)
+                    middles[x][g] = two_terms(mid[x][g] * (8.0f * meta_group(kmul, g)));
+#pragma unroll
+                for (int o = 0; o < Raw::OWN; ++o)
+                    own[x][o] = kv4_scale(raw.own[x][o]) * own_group(o, [&](int g) { return kmul[g]; });
+            }
+        } else {
+            const int ve = max(exp_of(vmag) - 11, -105);
+            stage_values([&](float v, int e) { return ldexpf(v, e - ve); });
+            if (lane < 32) {
+                ev[lane] = (float)ve;
+                iev[lane] = ldexpf(1.0f, -ve - 14);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                int e = -0x1000;
+#pragma unroll
+                for (int g = 0; g < Raw::GX; ++g)
+                    e = max(e, exp_of(fmaxf(fabsf(mid[x][g]), sc[x][g])) + meta_group(group_e, g));
+                if (NG == 8) e = max(e, __shfl_xor(e, 16, 64));
+                e -= 11;
+                const int at = 8 * (col >> 2) + (col & 3) + 4 * x;
+                if (j == 0) ek[at] = e;
+                const bool in = !edge || p0 + at <= last;
+#pragma unroll
+                for (int g = 0; g < Raw::GX; ++g)
+                    middles[x][g] = two_terms(ldexpf(mid[x][g], meta_group(group_e, g) - e + 3));
+#pragma unroll
+                for (int o = 0; o < Raw::OWN; ++o) {
+                    const int ge = own_group(o, [&](int g) { return group_e[g]; });
+                    own[x][o] = in ? ldexpf(kv4_scale(raw.own[x][o]), ge - e) : 0.0f;
+                }
+            }
+        }
+        // 5. scores: rows of S^T, 4 j' + i of tile x is position 8 j' + 4 x + i
+        f32x4 S[MT][2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const int at = 8 * (col >> 2) + (col & 3) + 4 * x;
-            const bool in = !edge || p0 + at <= last;
-            float mid[Raw::GX];
-            int e = -0x1000;
-            const int gb = NG == 8 ? 4 * (j & 1) : 0;
-            int eg[Raw::GX];
+            f16x8 kf[KS + 1];
+            key_codes(raw, x, own[x], middles[x], kf);
 #pragma unroll
-            for (int g = 0; g < Raw::GX; ++g) {
-                const uint32_t meta = in ? raw.km[x][g] : 0u;
-                mid[g] = __builtin_fmaf(8.0f, kv4_scale(meta), kv4_min(meta));
-                eg[g] = NG == 8 ? (j & 1 ? group_e[NG > 4 ? 4 + g : g] : group_e[g]) : group_e[g];
-                e = max(e, exp_of(fmaxf(fabsf(mid[g]) * 0.125f, kv4_scale(meta))) + eg[g]);
-            }
-            if (NG == 8) e = max(e, __shfl_xor(e, 16, 64));
-            e -= 11;
-            if (j == 0) ek[at] = e;
-            uint32_t ex[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int g = 0; g < Raw::GX; ++g)
-                ex[g] = two_terms(ldexpf(mid[g], eg[g] - e));
-            if (NG <= 4 && (j & 1)) ex[0] = ex[1] = ex[2] = ex[3] = 0;  // (no group 4 ..)
-            kf[x][KS] = __builtin_bit_cast(f16x8, u32x4{ex[0], ex[1], ex[2], ex[3]});
-#pragma unroll
-            for (int o = 0; o < Raw::OWN; ++o) {
-                const int g = NG == 1 ? 0 : NG == 2 ? j >> 1 : j * Raw::OWN + o;
-                const float s = in ? ldexpf(kv4_scale(raw.own[x][o]), pick(g) - e) : 0.0f;
-                const uint32_t sp = f16_pair(s, s), cp = minus24(sp);
-                const uint32_t s4[4] = {sp, sp, sp, sp}, c4[4] = {cp, cp, cp, cp};
-                constexpr int D = KS / Raw::OWN;
-#pragma unroll
-                for (int i = 0; i < D; ++i) kf[x][o * D + i] = Codes8(raw.k[x][o * D + i], s4, c4).v;
-            }
-        }
-        // 3. values' meta: lane (position, half of the groups)
-        unsigned long long nan_p[Raw::VM];  // lanes whose meta is a NaN
-        {
-            const int at = lane & 31;
-            float mid[Raw::VM], sc[Raw::VM], mag = 0.0f;
-#pragma unroll
-            for (int i = 0; i < Raw::VM; ++i) {
-                const uint32_t meta = !edge || p0 + at <= last ? raw.vm[i] : 0u;
-                sc[i] = kv4_scale(meta);
-                mid[i] = __builtin_fmaf(8.0f, sc[i], kv4_min(meta));
-                nan_p[i] = 0;
-                if (edge) {  // what some queries see and others do not: told below
-                    const bool bad = !(mid[i] == mid[i]);
-                    nan_p[i] = __ballot(bad);
-                    if (bad) mid[i] = sc[i] = 0.0f;
-                }
-                mag = fmaxf(mag, fmaxf(fabsf(mid[i]) * 0.125f, sc[i]));
-            }
-            if (NG > 1) mag = ta_swap32(mag, ta_max);
-            const int e = max(exp_of(mag) - 11, -105);
-            _Float16 *o = (_Float16 *)wl + (at & ~7) + slot8(at & 7);
-            if (NG > 1 || lane < 32) {
-#pragma unroll
-                for (int i = 0; i < Raw::VM; ++i) {
-                    const int g = (lane >> 5) * (NG / 2) + i;
-                    const f16x2 t = __builtin_bit_cast(f16x2, two_terms(ldexpf(mid[i], -e)));
-                    o[g * 64] = t[0];
-                    o[g * 64 + 32] = t[1];
-                    o[M::SC / 2 + g * 32] = (_Float16)ldexpf(sc[i], -e);
-                }
-            }
-            if (lane < 32) {
-                ev[at] = (float)e;
-                iev[at] = ldexpf(1.0f, -e - 14);
+            for (int t = 0; t < MT; ++t) {
+                S[t][x] = scores(t, kf);
+                apart();
             }
         }
         __builtin_amdgcn_wave_barrier();
-        // 4. values: rows of O^T
-        f16x8 vf[NT + 1];
+        // 6. the running maximum of weight times value
+        // whether query t of the lane sees position at
+        auto sees = [&](int t, int at) {
+            const unsigned long long v = mask[t * 16 + col];
+            const int at0 = at - tr.pos0;
+            return p.parent ? at0 < 0 || (at0 < 64 && (v >> (at0 & 63) & 1)) : at <= (int)(uint32_t)v;
+        };
+        float top[MT];
+        uint32_t seen = 0;  // a byte a tile
+        if (is_like()) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const u32x4 s = *(const u32x4 *)(wl + M::SC + g * 64 + j * 16);
-            const uint32_t s4[4] = {s[0], s[1], s[2], s[3]};
-            const uint32_t c4[4] = {minus24(s[0]), minus24(s[1]), minus24(s[2]), minus24(s[3])};
-            vf[2 * g] = Codes8(raw.v[2 * g], s4, c4).v;
-            vf[2 * g + 1] = Codes8(raw.v[2 * g + 1], s4, c4).v;
-        }
-        vf[NT] = *(const f16x8 *)(wl + col * 64 + j * 16);
-        const i32x4l ka = *(const i32x4l *)(ek + 8 * j), kb = *(const i32x4l *)(ek + 8 * j + 4);
-        const f32x4l va = *(const f32x4l *)(ev + 8 * j), vb = *(const f32x4l *)(ev + 8 * j + 4);
-        const f32x4l ia = *(const f32x4l *)(iev + 8 * j), ib = *(const f32x4l *)(iev + 8 * j + 4);
-        __builtin_amdgcn_wave_barrier();
-
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            // 5. scores of 16 queries at 32 positions
-            f32x4 sa = {0.0f, 0.0f, 0.0f, 0.0f}, sb = sa;
-#pragma unroll
-            for (int i = 0; i < 2 * KS + 1; ++i) {
-                const f16x8 qv = *(const f16x8 *)(qf + (t * M::FR + i) * 1024);
-                const int k = i == 2 * KS ? KS : i / 2;
-                sa = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][k], qv, sa, 0, 0, 0);
-                sb = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][k], qv, sb, 0, 0, 0);
+            for (int t = 0; t < MT; ++t) {
+                float a = fmaxf(fmaxf(S[t][0][0], S[t][0][1]), S[t][0][2]);
+                a = fmaxf(fmaxf(a, S[t][0][3]), S[t][1][0]);
+                a = fmaxf(fmaxf(a, S[t][1][1]), S[t][1][2]);
+                top[t] = __builtin_fmaf(fmaxf(a, S[t][1][3]), cq[t], (float)ev_run);
             }
-            // 6. their powers of two, what is seen, the maximum of weight times value
-            float y[8], mx = TA_NONE;
+        } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                y[i] = ldexpf(i < 4 ? sa[i] : sb[i - 4], (i < 4 ? ka[i] : kb[i - 4]) + fq[t]);
-            }
-            bool seen[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) seen[i] = true;
-            if (edge) {
+            for (int t = 0; t < MT; ++t) {
+                const int f = fe[t * 16 + col];
+                top[t] = TA_NONE;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int at = p0 + 8 * j + i, own = at - tr.pos0;
-                    seen[i] = p.parent ? own < 0 || (own < 64 && (see[t] >> (own & 63) & 1)) : at <= lim[t];
+                    const float y = ldexpf(S[t][i / 4][i % 4], ek[8 * j + i] + f);
+                    S[t][i / 4][i % 4] = y;
+                    const bool in = !edge || sees(t, p0 + 8 * j + i);
+                    seen |= (in ? 1u : 0u) << (8 * t + i);
+                    top[t] = in ? fmaxf(top[t], __builtin_fmaf(y, cs, ev[8 * j + i])) : top[t];
                 }
+                apart();
             }
-            float x[8];
+        }
+        bool more = false;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = __builtin_fmaf(y[i], cs, i < 4 ? va[i] : vb[i - 4]);
-                if (!seen[i]) x[i] = -__builtin_inff();
-                mx = fmaxf(mx, x[i]);
-            }
-            mx = __builtin_ceilf(ta_swap32(ta_swap16(mx, ta_max), ta_max));
-            if (__any(mx > m[t])) {
+        for (int t = 0; t < MT; ++t) more |= top[t] > m[t];
+        if (__any(more)) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float mx = __builtin_ceilf(ta_swap32(ta_swap16(top[t], ta_max), ta_max));
                 const float to = fmaxf(m[t], mx), corr = __builtin_amdgcn_exp2f(m[t] - to);
                 m[t] = to;
                 l[t] *= corr;
@@ -470,59 +524,171 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
                 for (int n = 0; n <= NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) O[t][n][i] *= corr;
+                far_any |= __any(fabsf(to) >= TA_FAR && to > TA_NONE);
             }
-            // 7. weights (2^14 of them at the maximum), two f16 terms
-            const float top = m[t] - 14.0f;
-            float P[8];
+        }
+        // 7. weights (2^14 of them at the maximum), in S's place
+        if (is_like()) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = __builtin_fmaf(y[i], cs, (i < 4 ? va[i] : vb[i - 4]) - top);
-                P[i] = __builtin_amdgcn_exp2f(d);
-                if (!seen[i]) P[i] = 0.0f;
-            }
-            // scores of millions: their rounding is larger than a weight's
-            const bool far = fabsf(m[t]) >= 4194304.0f && m[t] > TA_NONE;
-            if (__builtin_expect(__any(far), 0)) {
+            for (int t = 0; t < MT; ++t) {
+                const float b14 = (float)ev_run - (m[t] - 14.0f);
+                float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float e = __builtin_amdgcn_exp2f((x[i] - m[t]) + 14.0f);
-                    P[i] = far ? e : P[i];
+                    const float w8 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i / 4][i % 4], cq[t], b14));
+                    S[t][i / 4][i % 4] = w8;
+                    sum += w8;
                 }
+                l[t] = __builtin_fmaf(sum, vsum, l[t]);
             }
+        } else {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float b14 = m[t] - 14.0f;
+                // scores of millions: their rounding is larger than a weight's
+                const bool far = fabsf(m[t]) >= TA_FAR && m[t] > TA_NONE;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float y = S[t][i / 4][i % 4], v = ev[8 * j + i];
+                    float d = __builtin_fmaf(y, cs, v - b14);
+                    if (far) d = (__builtin_fmaf(y, cs, v) - m[t]) + 14.0f;
+                    const float w8 = seen >> (8 * t + i) & 1 ? __builtin_amdgcn_exp2f(d) : 0.0f;
+                    S[t][i / 4][i % 4] = w8;
+                    l[t] = __builtin_fmaf(w8, iev[8 * j + i], l[t]);
+                }
+                apart();
+            }
+        }
+        f16x8 ph[MT], pl[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {  // two f16 terms
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                l[t] = __builtin_fmaf(P[i], ia[i], l[t]);
-                l[t] = __builtin_fmaf(P[i + 4], ib[i], l[t]);
-                hi[i] = f16_pair(P[i], P[i + 4]);
-                lo[i] = f16_pair(__builtin_fmaf(f16_low(hi[i]), -1.0f, P[i]),
-                                 __builtin_fmaf(f16_high(hi[i]), -1.0f, P[i + 4]));
+                const float a = S[t][0][i], c = S[t][1][i];
+                hi[i] = f16_pair(a, c);
+                lo[i] = f16_pair(f16_rest<0>(hi[i], a), f16_rest<1>(hi[i], c));
             }
-            const f16x8 ph = __builtin_bit_cast(f16x8, u32x4{hi[0], hi[1], hi[2], hi[3]});
-            const f16x8 pl = __builtin_bit_cast(f16x8, u32x4{lo[0], lo[1], lo[2], lo[3]});
-            // 8. the outputs
+            ph[t] = __builtin_bit_cast(f16x8, u32x4{hi[0], hi[1], hi[2], hi[3]});
+            pl[t] = __builtin_bit_cast(f16x8, u32x4{lo[0], lo[1], lo[2], lo[3]});
+        }
+        // 8. outputs: rows of O^T
 #pragma unroll
-            for (int n = 0; n <= NT; ++n) {
-                O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[n], ph, O[t][n], 0, 0, 0);
-                O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[n], pl, O[t][n], 0, 0, 0);
+        for (int n = 0; n <= NT; ++n) {
+            const f16x8 vf = value_codes(raw, n);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t], O[t][n], 0, 0, 0);
+                O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t], O[t][n], 0, 0, 0);
             }
-            if (edge) {  // values that are NaN, to the queries that see them: through the middles' sums
+        }
+        // 9. values that are NaN, to the queries that see them: through the middles' sums
+        unsigned long long any_nan = 0;
 #pragma unroll
-                for (int i = 0; i < Raw::VM; ++i) {
-                    for (unsigned long long left = nan_p[i]; left; left &= left - 1) {
-                        const int at = __builtin_ctzll(left), pos = p0 + (at & 31), own = pos - tr.pos0;
-                        const int g = NG == 1 ? 0 : (at >> 5) * (NG / 2) + i;
-                        const bool hit = p.parent ? own < 0 || (own < 64 && (see[t] >> (own & 63) & 1))
-                                                  : pos <= lim[t];
-                        if (hit && j == g / 2) O[t][NT][0] = g % 2 ? O[t][NT][0] : __builtin_nanf("");
-                        if (hit && j == g / 2) O[t][NT][2] = g % 2 ? __builtin_nanf("") : O[t][NT][2];
-                    }
+        for (int i = 0; i < Raw::VM; ++i) any_nan |= nan_p[i];
+        if (any_nan) {
+#pragma unroll
+            for (int i = 0; i < Raw::VM; ++i) {
+                for (unsigned long long left = nan_p[i]; left; left &= left - 1) {
+                    const int at = __builtin_ctzll(left);
+                    const int g = NG == 1 ? 0 : (at >> 5) * (NG / 2) + i;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+                        if (sees(t, p0 + (at & 31)) && j == g / 2) {
+                            O[t][NT][0] = g % 2 ? O[t][NT][0] : __builtin_nanf("");
+                            O[t][NT][2] = g % 2 ? __builtin_nanf("") : O[t][NT][2];
+                        }
                 }
             }
         }
+        __builtin_amdgcn_wave_barrier();
+    };
+
+    // 2. an eighth of each group's middle, and its scale; nothing past the last position
+    auto key_meta = [&](const Raw &raw, int p0, bool edge) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const bool in = !edge || p0 + 8 * (col >> 2) + (col & 3) + 4 * x <= last;
+#pragma unroll
+            for (int g = 0; g < Raw::GX; ++g) {
+                const uint32_t meta = in ? raw.km[x][g] : 0u;
+                sc[x][g] = kv4_scale(meta);
+                mid[x][g] = __builtin_fmaf(0.125f, kv4_min(meta), sc[x][g]);
+            }
+        }
+    };
+    auto value_meta = [&](const Raw &raw, int p0, bool edge) {
+        vmag = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Raw::VM; ++i) {
+            const uint32_t meta = !edge || p0 + (lane & 31) <= last ? raw.vm[i] : 0u;
+            vsc[i] = kv4_scale(meta);
+            vmid[i] = __builtin_fmaf(0.125f, kv4_min(meta), vsc[i]);
+            nan_p[i] = 0;
+            if (edge) {  // what some queries see and others do not: told at the end
+                const bool bad = !(vmid[i] == vmid[i]);
+                nan_p[i] = __ballot(bad);
+                if (bad) vmid[i] = vsc[i] = 0.0f;
+            }
+            vmag = fmaxf(vmag, fmaxf(fabsf(vmid[i]), vsc[i]));
+        }
+        if (NG > 1) vmag = ta_swap32(vmag, ta_max);
+    };
+    // 3. whether all positions stand within 2^TA_SPAN below the powers of two, or below the
+    // block's own, which are taken then, with room above
+    auto alike = [&] {
+        float kmag[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            kmag[x] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < Raw::GX; ++g) {
+                kmag[x] = fmaxf(kmag[x], fmaxf(fabsf(mid[x][g]), sc[x][g]) * meta_group(weight, g));
+            }
+            if (NG == 8) kmag[x] = ta_swap16(kmag[x], ta_max);
+        }
+        auto near = [&](float v, int e) { return (unsigned)(e - exp_of(v)) <= (unsigned)TA_SPAN; };
+        auto all_near = [&] {
+            return __all(near(kmag[0], ek_run) && near(kmag[1], ek_run) && near(vmag, ev_run + 11));
+        };
+        if (plain && all_near()) return true;
+        float k = fmaxf(kmag[0], kmag[1]);
+        k = ta_swap32(ta_swap16(ta_row16(k, ta_max), ta_max), ta_max);
+        const float v = ta_swap16(ta_row16(vmag, ta_max), ta_max);
+        ek_run = __builtin_amdgcn_readfirstlane(exp_of(k)) + 2;
+        ev_run = __builtin_amdgcn_readfirstlane(exp_of(v)) - 9;
+        vmul = uniform(ldexpf(1.0f, -ev_run));
+        vsum = uniform(ldexpf(1.0f, -ev_run - 14));
+        bool fits = ev_run >= -100 && ev_run <= 100 && ek_run >= -100 && ek_run <= 100;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const int e = group_e[g] - (ek_run - 11);
+            kmul[g] = uniform(ldexpf(1.0f, e));
+            fits &= e <= 100 && (e >= -100 || group_e[g] == TA_NO_GROUP);
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int f = fe[t * 16 + col] + ek_run;
+            cq[t] = ldexpf(cs, f - 11);
+            fits &= f <= 100;
+        }
+        plain = __all(fits);
+        return plain && all_near();
+    };
+
+    const int whole = min(b1, min(zone, last + 1) / KV4_BLOCK);  // blocks that all queries see
+    Raw next;
+    if (b0 + w < b1) next.load(p.c, head, b0 + w, lane);
+    for (int blk = b0 + w; blk < b1; blk += TA_W) {
+        const Raw raw = next;
+        if (blk + TA_W < b1) next.load(p.c, head, blk + TA_W, lane);
+        const bool edge = blk >= whole;
+        key_meta(raw, blk * KV4_BLOCK, edge);
+        value_meta(raw, blk * KV4_BLOCK, edge);
+        block(raw, blk, edge, !edge && !far_any && alike());
     }
 
-    // 9. the waves' results
+    // 10. the waves' results
     float *off = (float *)(lds + M::OFF) + w * ROWS * 8;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
@@ -657,7 +823,8 @@ int launch_tree_attn(const TreeAttnArgs &a, hipStream_t st) {
     p.shares = pl.shares;
     p.out = a.out;
     p.work = a.work;
-    p.scale = frexpf(a.scale, &p.scale_e) * 1.44269504f;
+    p.scale = frexpf(fabsf(a.scale), &p.scale_e) * 1.44269504f;
+    p.sign = a.scale < 0.0f ? -1.0f : 1.0f;
     p.guard = guard_flag_ptr();
     VMLM_GUARD(p.shares == 1 || p.work, "kv4 tree attention: split positions need a workspace");
     switch (a.c.hd) {
