@@ -45,6 +45,11 @@ constexpr float TA_NONE = -3.40282347e38f;  // the maximum of no score yet
 constexpr int TA_NO_GROUP = -1000;          // the weight of channels where all queries are 0
 constexpr int TA_UNSET = -100000;
 constexpr int TA_SPAN = 7;                  // positions of like size: within 2^7
+// A weight is 2^TA_BASE at the maximum that its wave knew when it last raised it, which it
+// does where one is 2^TA_SLACK larger: with 64 queries some maximum grows in nearly every block
+// (tree_long: 192 us when each was followed).
+constexpr int TA_BASE = 9, TA_SLACK = 6;
+constexpr float TA_UNBASE = 1.0f / (1 << TA_BASE);
 constexpr float TA_FAR = 4194304.0f;        // scores whose f32 steps are no longer small
 
 struct TreeAttnParams {
@@ -219,9 +224,20 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     const int x8 = blockIdx.x / 8, stream = x8 / p.tiles * 8 + (int)(blockIdx.x % 8), tile = x8 % p.tiles;
     const int share = stream % p.shares, pair = stream / p.shares, kvh = pair % p.c.Hkv, b = pair / p.c.Hkv;
     if (b >= p.c.B) return;
+    // the wave's query rows, loaded before anything is known of the sequence
+    constexpr int CW = (HD + 63) / 64, RW = ROWS / TA_W;
+    const int row0 = tile * ROWS;
+    float x[RW][CW];
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        const int R = min(row0 + w + i * TA_W, p.S * p.G - 1), t = R / p.G;
+        const float *q = p.q + ((size_t)b * p.S + t) * p.ldq + ((size_t)kvh * p.G + R % p.G) * HD;
+#pragma unroll
+        for (int c = 0; c < CW; ++c) x[i][c] = q[min(c * 64 + lane, HD - 1)];
+    }
     const TreeRows tr = tree_rows(p.pos0, p.count, p.parent, p.S, p.c.cap, b, p.guard,
                                   kvh == 0 && tile == 0 && share == 0);
-    const int row0 = tile * ROWS, rows = min(ROWS, tr.n * p.G - row0);
+    const int rows = min(ROWS, tr.n * p.G - row0);
     if (rows <= 0) return;
     const int t_lo = row0 / p.G, t_hi = (row0 + rows - 1) / p.G;
     const int last = tr.pos0 + t_hi;                               // the last position seen
@@ -239,34 +255,27 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         *(u32x4 *)(lds + M::WAVE + (i >> 6) * M::WB + (i & 63) * 16) = u32x4{0, 0, 0, 0};
     if (tid < 16) ge[tid] = TA_NO_GROUP;
     __syncthreads();
-    constexpr int CW = (HD + 63) / 64;
-    auto query = [&](int r, float (&x)[CW]) {
-        const int R = row0 + min(r, rows - 1), t = R / p.G;
-        const float *q = p.q + ((size_t)b * p.S + t) * p.ldq + ((size_t)kvh * p.G + R % p.G) * HD;
+    int own_e[RW], bad[RW];  // a row's power of two
 #pragma unroll
-        for (int i = 0; i < CW; ++i) {
-            const int c = i * 64 + lane;
-            x[i] = c < HD && r < rows ? q[c] : 0.0f;
-        }
-    };
-    for (int r = w; r < ROWS; r += TA_W) {
-        float x[CW], mx[CW], most = 0.0f;
-        int bad = 0;
-        query(r, x);
+    for (int i = 0; i < RW; ++i) {
+        const int r = w + i * TA_W;
+        float mx[CW], most = 0.0f;
+        bad[i] = 0;
 #pragma unroll
-        for (int i = 0; i < CW; ++i) {
-            mx[i] = ta_swap16(ta_row16(fabsf(x[i]), ta_max), ta_max);  // of its 32 channels
-            most = fmaxf(most, mx[i]);
-            bad |= !(fabsf(x[i]) <= 3.40282347e38f);
+        for (int c = 0; c < CW; ++c) {
+            if (r >= rows || c * 64 + lane >= HD) x[i][c] = 0.0f;
+            mx[c] = ta_swap16(ta_row16(fabsf(x[i][c]), ta_max), ta_max);  // of its 32 channels
+            most = fmaxf(most, mx[c]);
+            bad[i] |= !(fabsf(x[i][c]) <= 3.40282347e38f);
         }
         most = ta_swap32(most, ta_max);
-        bad = __any(bad);
-        const int F = most > 0.0f && !bad ? ilogbf(most) : 0;
-        if (lane == 0) fe[r] = F - 8 + p.scale_e;
+        bad[i] = __any(bad[i]);
+        own_e[i] = most > 0.0f && !bad[i] ? ilogbf(most) : 0;
+        if (lane == 0) fe[r] = own_e[i] - 8 + p.scale_e;
 #pragma unroll
-        for (int i = 0; i < CW; ++i)
-            if ((lane & 31) == 0 && i * 64 + lane < HD && mx[i] > 0.0f && !bad)
-                atomicMax(&ge[i * 2 + lane / 32], ilogbf(mx[i]) - F);
+        for (int c = 0; c < CW; ++c)
+            if ((lane & 31) == 0 && c * 64 + lane < HD && mx[c] > 0.0f && !bad[i])
+                atomicMax(&ge[c * 2 + lane / 32], ilogbf(mx[c]) - own_e[i]);
     }
     if (p.parent) {
         if (w == 0) {  // ancestors by doubling: of 2, 4, 8 .. tokens at once
@@ -299,19 +308,14 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         group_e[g] = __builtin_amdgcn_readfirstlane(ge[g]);
         weight[g] = uniform(ldexpf(1.0f, group_e[g]));
     }
-    for (int r = w; r < ROWS; r += TA_W) {
-        float x[CW];
-        int bad = 0;
-        query(r, x);
-        const int F = fe[r] + 8 - p.scale_e;
 #pragma unroll
-        for (int i = 0; i < CW; ++i) bad |= !(fabsf(x[i]) <= 3.40282347e38f);
-        bad = __any(bad);
+    for (int i = 0; i < RW; ++i) {
+        const int r = w + i * TA_W;
         uint8_t *at = lds + M::Q + (r / 16) * M::FR * 1024 + (r % 16) * 16;
 #pragma unroll
-        for (int i = 0; i < CW; ++i) {
-            const int c = i * 64 + lane, g = min(c / 32, NG - 1);
-            const float y = bad ? __builtin_nanf("") : ldexpf(x[i] * p.sign, 8 - F - ge[g]);  // below 2^9
+        for (int cc = 0; cc < CW; ++cc) {
+            const int c = cc * 64 + lane, g = min(c / 32, NG - 1);
+            const float y = bad[i] ? __builtin_nanf("") : ldexpf(x[i][cc] * p.sign, 8 - own_e[i] - ge[g]);  // below 2^9
             const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
             const float sum = ta_swap16(ta_row16((float)hi + (float)lo, ta_add), ta_add);
             if (c >= HD) continue;
@@ -382,14 +386,15 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
             for (int i = 0; i < D; ++i) kf[o * D + i] = Codes8(raw.k[x][o * D + i], s4, c4).v;
         }
     };
-    auto scores = [&](int t, const f16x8 (&kf)[KS + 1]) {
-        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto scores = [&](int t, const f16x8 (&kf)[2][KS + 1], f32x4 (&acc)[2]) {
+        acc[0] = acc[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 2 * KS + 1; ++i) {
             const f16x8 qv = *(const f16x8 *)(qf + (t * M::FR + i) * 1024);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i == 2 * KS ? KS : i / 2], qv, acc, 0, 0, 0);
+            const int k = i == 2 * KS ? KS : i / 2;
+            acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][k], qv, acc[0], 0, 0, 0);
+            acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][k], qv, acc[1], 0, 0, 0);
         }
-        return acc;
     };
     // values' meta as f16 (scaled by f), where the lanes that hold their codes find it
     auto stage_values = [&](auto f) {
@@ -441,7 +446,7 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
             stage_values([&](float v, int e) { return ldexpf(v, e - ve); });
             if (lane < 32) {
                 ev[lane] = (float)ve;
-                iev[lane] = ldexpf(1.0f, -ve - 14);
+                iev[lane] = ldexpf(1.0f, -ve - TA_BASE);
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
@@ -466,15 +471,13 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         }
         // 5. scores: rows of S^T, 4 j' + i of tile x is position 8 j' + 4 x + i
         f32x4 S[MT][2];
+        f16x8 kf[2][KS + 1];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            f16x8 kf[KS + 1];
-            key_codes(raw, x, own[x], middles[x], kf);
+        for (int x = 0; x < 2; ++x) key_codes(raw, x, own[x], middles[x], kf[x]);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                S[t][x] = scores(t, kf);
-                apart();
-            }
+        for (int t = 0; t < MT; ++t) {
+            apart();
+            scores(t, kf, S[t]);
         }
         __builtin_amdgcn_wave_barrier();
         // 6. the running maximum of weight times value
@@ -512,7 +515,7 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         }
         bool more = false;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) more |= top[t] > m[t];
+        for (int t = 0; t < MT; ++t) more |= top[t] > m[t] + TA_SLACK;
         if (__any(more)) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
@@ -527,15 +530,15 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
                 far_any |= __any(fabsf(to) >= TA_FAR && to > TA_NONE);
             }
         }
-        // 7. weights (2^14 of them at the maximum), in S's place
+        // 7. weights, in S's place
         if (is_like()) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float b14 = (float)ev_run - (m[t] - 14.0f);
+                const float base = (float)ev_run - (m[t] - TA_BASE);
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float w8 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i / 4][i % 4], cq[t], b14));
+                    const float w8 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i / 4][i % 4], cq[t], base));
                     S[t][i / 4][i % 4] = w8;
                     sum += w8;
                 }
@@ -544,14 +547,14 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         } else {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float b14 = m[t] - 14.0f;
+                const float base = m[t] - TA_BASE;
                 // scores of millions: their rounding is larger than a weight's
                 const bool far = fabsf(m[t]) >= TA_FAR && m[t] > TA_NONE;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float y = S[t][i / 4][i % 4], v = ev[8 * j + i];
-                    float d = __builtin_fmaf(y, cs, v - b14);
-                    if (far) d = (__builtin_fmaf(y, cs, v) - m[t]) + 14.0f;
+                    float d = __builtin_fmaf(y, cs, v - base);
+                    if (far) d = (__builtin_fmaf(y, cs, v) - m[t]) + TA_BASE;
                     const float w8 = seen >> (8 * t + i) & 1 ? __builtin_amdgcn_exp2f(d) : 0.0f;
                     S[t][i / 4][i % 4] = w8;
                     l[t] = __builtin_fmaf(w8, iev[8 * j + i], l[t]);
@@ -579,6 +582,9 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t], O[t][n], 0, 0, 0);
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
                 O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t], O[t][n], 0, 0, 0);
             }
         }
@@ -658,7 +664,7 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         ek_run = __builtin_amdgcn_readfirstlane(exp_of(k)) + 2;
         ev_run = __builtin_amdgcn_readfirstlane(exp_of(v)) - 9;
         vmul = uniform(ldexpf(1.0f, -ev_run));
-        vsum = uniform(ldexpf(1.0f, -ev_run - 14));
+        vsum = uniform(ldexpf(1.0f, -ev_run - TA_BASE));
         bool fits = ev_run >= -100 && ev_run <= 100 && ek_run >= -100 && ek_run <= 100;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -725,7 +731,7 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         }
         if (p.shares == 1) {
             const int R = row0 + r;
-            p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * 0x1p-14f / L;
+            p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * TA_UNBASE / L;
         } else {
             float *pw = p.work + (((size_t)pair * p.tiles + tile) * p.shares + share) * (ROWS * (HD + 2));
             pw[r * HD + c] = o;
@@ -753,7 +759,7 @@ __global__ __launch_bounds__(HD < 64 ? 64 : HD) void tree_merge_kernel(TreeAttnP
         L = __builtin_fmaf(f, pw[s * ld + ROWS * HD + 2 * r + 1], L);
         o = __builtin_fmaf(f, pw[s * ld + r * HD + c], o);
     }
-    p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * 0x1p-14f / L;
+    p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * TA_UNBASE / L;
 }
 
 struct TreePlan {
