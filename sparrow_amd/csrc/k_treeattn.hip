@@ -43,8 +43,10 @@ typedef int i32x4l __attribute__((ext_vector_type(4)));
 constexpr int TA_W = 4;  // waves of a workgroup
 constexpr float TA_NONE = -3.40282347e38f;  // the maximum of no score yet
 constexpr int TA_NO_GROUP = -1000;          // the weight of channels where all queries are 0
-constexpr int TA_UNSET = -100000;
-constexpr int TA_SPAN = 7;                  // positions of like size: within 2^7
+// Keys' and values' f16 stand below 2^TA_TOP_E (8 scale and the middle of a group do); positions of
+// like size are within 2^TA_SPAN of that: their smallest middles keep 22 bits.
+constexpr int TA_TOP_E = 11, TA_SPAN = 14;
+constexpr float TA_TOP = 1 << TA_TOP_E;
 // A weight is 2^TA_BASE at the maximum that its wave knew when it last raised it, which it
 // does where one is 2^TA_SLACK larger: with 64 queries some maximum grows in nearly every block
 // (tree_long: 192 us when each was followed).
@@ -86,22 +88,19 @@ __device__ __forceinline__ uint32_t f16_pair(float a, float b) {
     const hw_f32x2 v = {a, b};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
 }
-// x less the f16 in the low or high half of v, in one operation (which the compiler
-// makes two of)
-template <int HIGH>
-__device__ __forceinline__ float f16_rest(uint32_t v, float x) {
-    float r;
-    if (HIGH)
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(v), "v"(x));
-    else
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(v), "v"(x));
-    return r;
-}
-
+// x less an f16, rounded to f16: one operation where the factor -1 is not known to the
+// compiler, which else converts, subtracts and converts.
+struct Rest {
+    float minus_one = -1.0f;
+    __device__ __forceinline__ Rest() { asm("" : "+s"(minus_one)); }
+    __device__ __forceinline__ _Float16 operator()(float x, _Float16 h) const {
+        return (_Float16)__builtin_fmaf((float)h, minus_one, x);
+    }
+};
 // x as two f16 terms
-__device__ __forceinline__ uint32_t two_terms(float x) {
+__device__ __forceinline__ uint32_t two_terms(float x, const Rest &rest) {
     const _Float16 hi = (_Float16)x;
-    const f16x2 v = {hi, (_Float16)(x - (float)hi)};
+    const f16x2 v = {hi, rest(x, hi)};
     return __builtin_bit_cast(uint32_t, v);
 }
 
@@ -146,6 +145,7 @@ template <int HD, int MT>
 struct TreeLds {
     static constexpr int KS = HD / 32, NG = HD / 32;
     static constexpr int FR = 2 * KS + 1;
+    static constexpr bool ONES = NG < 8;  // the middles' rows leave one for the weights' sum
     static constexpr int Q = 0;
     static constexpr int WAVE = Q + MT * FR * 1024;
     static constexpr int SC = 1024, N = SC + 512;  // scales [8][32], numbers
@@ -252,7 +252,8 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     for (int i = tid; i < MT * 64; i += 64 * TA_W)  // the sums' step: zeros where there is no group
         *(u32x4 *)(lds + M::Q + ((i >> 6) * M::FR + 2 * KS) * 1024 + (i & 63) * 16) = u32x4{0, 0, 0, 0};
     for (int i = tid; i < TA_W * 64; i += 64 * TA_W)
-        *(u32x4 *)(lds + M::WAVE + (i >> 6) * M::WB + (i & 63) * 16) = u32x4{0, 0, 0, 0};
+        *(u32x4 *)(lds + M::WAVE + (i >> 6) * M::WB + (i & 63) * 16) =
+            M::ONES && (i & 63) >= 60 ? u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u} : u32x4{0, 0, 0, 0};
     if (tid < 16) ge[tid] = TA_NO_GROUP;
     __syncthreads();
     int own_e[RW], bad[RW];  // a row's power of two
@@ -301,13 +302,6 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         mask[tid] = (uint32_t)(tr.pos0 + (row0 + min(tid, rows - 1)) / p.G);  // the last position
     }
     __syncthreads();
-    int group_e[NG];
-    float weight[NG];  // (only to choose powers of two: 0 where it leaves f32)
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        group_e[g] = __builtin_amdgcn_readfirstlane(ge[g]);
-        weight[g] = uniform(ldexpf(1.0f, group_e[g]));
-    }
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
         const int r = w + i * TA_W;
@@ -346,138 +340,213 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     float *ev = (float *)(wl + M::N + 128), *iev = ev + 32;
     const uint8_t *qf = lds + M::Q + lane * 16;
     const float cs = p.scale;
-    // the powers of two that keys and values of a block stand below where all its positions
-    // are within 2^TA_SPAN of them (ek_run, ev_run), and the factors that they mean
-    int ek_run = TA_UNSET, ev_run = TA_UNSET;
-    float kmul[NG], vmul = 0.0f, vsum = 0.0f;
-    bool plain = false, far_any = false;
+    const Rest rest;
+    // Blocks that all queries see and whose positions are of like size share their powers of
+    // two: keys stand below 2^ek, values below 2^ev, those of the block that they were taken from with
+    // room above. kg and vg bring scales to them, cq scores back.
+    int ek_run = 0, ev_run = 0;
+    float kg[Raw::GX], kown[Raw::OWN], vg = 0.0f;
+#pragma unroll
+    for (int g = 0; g < Raw::GX; ++g) kg[g] = 0.0f;
+#pragma unroll
+    for (int o = 0; o < Raw::OWN; ++o) kown[o] = 0.0f;
+    bool far_any = false;
 
     // (nothing is moved over it, nor kept in registers for what comes after: fewer of them)
     auto apart = [] {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
+    // the group of the lane's g-th meta, and of its o-th codes
+    auto meta_group = [&](int g) { return NG == 8 ? 4 * (j & 1) + g : g; };
+    auto own_group = [&](int o) { return NG == 1 ? 0 : NG == 2 ? j >> 1 : j * Raw::OWN + o; };
 
-    float mid[2][Raw::GX], sc[2][Raw::GX], vmid[Raw::VM], vsc[Raw::VM], vmag;
+    // What the products take of a block's meta: middles as two f16 terms, scales.
+    uint32_t middles[2][Raw::GX], vmiddles[Raw::VM];
+    float own[2][Raw::OWN], vscales[Raw::VM];
     unsigned long long nan_p[Raw::VM];  // lanes whose value's meta is a NaN
-    // f of the group of the lane's o-th own codes
-    auto own_group = [&](int o, auto f) {
-        const int g = NG == 1 ? 0 : NG == 2 ? j >> 1 : j * Raw::OWN + o;
-        auto e = f(0);
+
+    // 2. by the shared powers of two; false where a position is too large for them, or smaller
+    // than 2^-TA_SPAN of them
+    auto shared_meta = [&](const Raw &raw) {
+        float hi = 0.0f, lo = __builtin_inff();
 #pragma unroll
-        for (int i = 1; i < NG; ++i) e = g == i ? f(i) : e;
-        return e;
-    };
-    // of the group g of key_meta's
-    auto meta_group = [&](const auto (&v)[NG], int g) { return NG == 8 && (j & 1) ? v[NG > 4 ? 4 + g : g] : v[g]; };
-    // a position's codes and middles as the product's operand
-    auto key_codes = [&](const Raw &raw, int x, const float (&own)[Raw::OWN], const uint32_t (&middles)[Raw::GX],
-                         f16x8 (&kf)[KS + 1]) {
-        uint32_t ex[4] = {0, 0, 0, 0};
+        for (int x = 0; x < 2; ++x) {
+            float most = 0.0f;
 #pragma unroll
-        for (int g = 0; g < Raw::GX; ++g) ex[g] = NG <= 4 && (j & 1) ? 0u : middles[g];  // (no group 4 ..)
-        kf[KS] = __builtin_bit_cast(f16x8, u32x4{ex[0], ex[1], ex[2], ex[3]});
+            for (int g = 0; g < Raw::GX; ++g) {
+                const float s = 8.0f * (kv4_scale(raw.km[x][g]) * kg[g]);
+                const float mid = __builtin_fmaf(kv4_min(raw.km[x][g]), kg[g], s);
+                most = fmaxf(most, fmaxf(fabsf(mid), s));
+                middles[x][g] = two_terms(mid, rest);
+            }
+            hi = fmaxf(hi, most);
+            lo = fminf(lo, most);
 #pragma unroll
-        for (int o = 0; o < Raw::OWN; ++o) {
-            const uint32_t sp = f16_pair(own[o], own[o]), cp = minus24(sp);
-            const uint32_t s4[4] = {sp, sp, sp, sp}, c4[4] = {cp, cp, cp, cp};
-            constexpr int D = KS / Raw::OWN;
-#pragma unroll
-            for (int i = 0; i < D; ++i) kf[o * D + i] = Codes8(raw.k[x][o * D + i], s4, c4).v;
+            for (int o = 0; o < Raw::OWN; ++o) own[x][o] = kv4_scale(raw.own[x][o]) * kown[o];
         }
-    };
-    auto scores = [&](int t, const f16x8 (&kf)[2][KS + 1], f32x4 (&acc)[2]) {
-        acc[0] = acc[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < 2 * KS + 1; ++i) {
-            const f16x8 qv = *(const f16x8 *)(qf + (t * M::FR + i) * 1024);
-            const int k = i == 2 * KS ? KS : i / 2;
-            acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][k], qv, acc[0], 0, 0, 0);
-            acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][k], qv, acc[1], 0, 0, 0);
-        }
-    };
-    // values' meta as f16 (scaled by f), where the lanes that hold their codes find it
-    auto stage_values = [&](auto f) {
-        if (NG == 1 && lane >= 32) return;
-        _Float16 *o = (_Float16 *)wl + (lane & 24) + slot8(lane & 7);
+        float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < Raw::VM; ++i) {
-            const int g = (lane >> 5) * (NG / 2) + i;
-            const f16x2 t = __builtin_bit_cast(f16x2, two_terms(f(vmid[i], 3)));
-            o[g * 64] = t[0];
-            o[g * 64 + 32] = t[1];
-            o[M::SC / 2 + g * 32] = (_Float16)f(vsc[i], 0);
+            vscales[i] = kv4_scale(raw.vm[i]) * vg;
+            const float mid = __builtin_fmaf(kv4_min(raw.vm[i]), vg, 8.0f * vscales[i]);
+            most = fmaxf(most, fmaxf(fabsf(mid), 8.0f * vscales[i]));
+            vmiddles[i] = two_terms(mid, rest);
+            nan_p[i] = 0;
+        }
+        return __all(fmaxf(hi, most) < TA_TOP && fminf(lo, most) >= TA_TOP / (1 << TA_SPAN));
+    };
+    // 3. the powers of two of a block whose positions did not suit the ones there were; false
+    // where they leave the range that the shared form keeps to
+    auto choose = [&](const Raw &raw) {
+        int e = -0x1000;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int g = 0; g < Raw::GX; ++g) {
+                const float s = kv4_scale(raw.km[x][g]), mid = __builtin_fmaf(0.125f, kv4_min(raw.km[x][g]), s);
+                e = max(e, exp_of(fmaxf(fabsf(mid), s)) + ge[meta_group(g)]);
+            }
+        const float ke = ta_swap32(ta_swap16(ta_row16((float)e, ta_max), ta_max), ta_max);
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Raw::VM; ++i) {
+            const float s = kv4_scale(raw.vm[i]);
+            v = fmaxf(v, fmaxf(fabsf(__builtin_fmaf(0.125f, kv4_min(raw.vm[i]), s)), s));
+        }
+        v = ta_swap32(ta_swap16(ta_row16(v, ta_max), ta_max), ta_max);
+        // (a group's middle / 8 and its scale are below 2^e; 8 times that, with two bits of room)
+        const int old = ev_run;
+        ek_run = __builtin_amdgcn_readfirstlane((int)ke) + 5;
+        ev_run = __builtin_amdgcn_readfirstlane(exp_of(v)) + 5;
+        bool fits = ev_run >= -90 && ev_run <= 120 && ek_run >= -90 && ek_run <= 120;
+        auto factor = [&](int g) { return ldexpf(1.0f, ge[g] + TA_TOP_E - ek_run); };
+#pragma unroll
+        for (int g = 0; g < Raw::GX; ++g) kg[g] = NG == 8 ? factor(meta_group(g)) : uniform(factor(g));
+#pragma unroll
+        for (int o = 0; o < Raw::OWN; ++o) kown[o] = factor(own_group(o));
+#pragma unroll
+        for (int g = 0; g < NG; ++g) fits &= ge[g] == TA_NO_GROUP || (ge[g] - ek_run <= 100 && ge[g] - ek_run >= -100);
+        vg = uniform(ldexpf(1.0f, TA_TOP_E - ev_run));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int f = fe[t * 16 + col] + ek_run - TA_TOP_E;
+            cq[t] = ldexpf(cs, f);
+            fits &= f <= 100;
+            // the sums of weights that stand in O are in units of 2^ev_run
+            if (M::ONES && j == 3) O[t][NT][3] = ldexpf(O[t][NT][3], ev_run - old);
+        }
+        fits = __all(fits);
+        if (!fits) {  // (nothing is shared until the next choice)
+#pragma unroll
+            for (int g = 0; g < Raw::GX; ++g) kg[g] = 0.0f;
+        }
+        return fits;
+    };
+    // 2'. by a power of two for every position, which the other lanes find in LDS; nothing past
+    // the last position
+    auto own_meta = [&](const Raw &raw, int p0, bool edge) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int at = 8 * (col >> 2) + (col & 3) + 4 * x;
+            const bool in = !edge || p0 + at <= last;
+            float mid[Raw::GX];
+            int e = -0x1000, eg[Raw::GX];
+#pragma unroll
+            for (int g = 0; g < Raw::GX; ++g) {
+                const uint32_t meta = in ? raw.km[x][g] : 0u;
+                const float s = kv4_scale(meta);
+                mid[g] = __builtin_fmaf(0.125f, kv4_min(meta), s);
+                eg[g] = ge[meta_group(g)];
+                e = max(e, exp_of(fmaxf(fabsf(mid[g]), s)) + eg[g]);
+            }
+            if (NG == 8) e = max(e, __shfl_xor(e, 16, 64));
+            e += 3 - TA_TOP_E;
+            if (j == 0) ek[at] = e;
+#pragma unroll
+            for (int g = 0; g < Raw::GX; ++g) middles[x][g] = two_terms(ldexpf(mid[g], eg[g] - e + 3), rest);
+#pragma unroll
+            for (int o = 0; o < Raw::OWN; ++o)
+                own[x][o] = in ? ldexpf(kv4_scale(raw.own[x][o]), ge[own_group(o)] - e) : 0.0f;
+        }
+        float mid[Raw::VM], mag = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Raw::VM; ++i) {
+            const uint32_t meta = !edge || p0 + (lane & 31) <= last ? raw.vm[i] : 0u;
+            vscales[i] = kv4_scale(meta);
+            mid[i] = __builtin_fmaf(0.125f, kv4_min(meta), vscales[i]);
+            nan_p[i] = 0;
+            if (edge) {  // what some queries see and others do not: told at the end
+                const bool bad = !(mid[i] == mid[i]);
+                nan_p[i] = __ballot(bad);
+                if (bad) mid[i] = vscales[i] = 0.0f;
+            }
+            mag = fmaxf(mag, fmaxf(fabsf(mid[i]), vscales[i]));
+        }
+        if (NG > 1) mag = ta_swap32(mag, ta_max);
+        const int e = max(exp_of(mag) + 3 - TA_TOP_E, -105);
+#pragma unroll
+        for (int i = 0; i < Raw::VM; ++i) {
+            vmiddles[i] = two_terms(ldexpf(mid[i], 3 - e), rest);
+            vscales[i] = ldexpf(vscales[i], -e);
+        }
+        if (lane < 32) {
+            ev[lane] = (float)e;
+            iev[lane] = ldexpf(1.0f, -e - TA_BASE);
         }
     };
-    auto value_codes = [&](const Raw &raw, int n) {
-        if (n == NT) return *(const f16x8 *)(wl + col * 64 + j * 16);
-        const u32x4 s = *(const u32x4 *)(wl + M::SC + n / 2 * 64 + j * 16);
-        const uint32_t s4[4] = {s[0], s[1], s[2], s[3]};
-        const uint32_t c4[4] = {minus24(s[0]), minus24(s[1]), minus24(s[2]), minus24(s[3])};
-        return Codes8(raw.v[n], s4, c4).v;
-    };
-    // What follows a block's meta. `like`: all queries see all of it, and its positions are of
-    // like size; else every position has a power of two of its own. (One copy of the
-    // products for both: with two, the accumulators took their registers twice.)
-    auto block = [&](const Raw &raw, int blk, bool edge, bool like) {
+
+    // What follows a block's meta. (One copy of the products for both kinds of blocks: with
+    // two, the accumulators took their registers twice.)
+    auto block = [&](const Raw &raw, int blk, bool edge, bool shared) {
         const int p0 = blk * KV4_BLOCK;
         // (kept from splitting the code after it in two)
-        auto is_like = [&] {
-            int v = __builtin_amdgcn_readfirstlane(like);
+        auto is_shared = [&] {
+            int v = __builtin_amdgcn_readfirstlane(shared);
             asm volatile("" : "+s"(v));
             return v != 0;
         };
-        // 4. values' meta, keys' powers of two and factors
-        uint32_t middles[2][Raw::GX];
-        float own[2][Raw::OWN];
-        if (is_like()) {
-            stage_values([&](float v, int e) { return v * (vmul * (float)(1 << e)); });
+        // 4. values' meta, where the lanes that hold their codes find it
+        if (NG > 1 || lane < 32) {
+            _Float16 *o = (_Float16 *)wl + (lane & 24) + slot8(lane & 7);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                for (int g = 0; g < Raw::GX; ++g)
-                    middles[x][g] = two_terms(mid[x][g] * (8.0f * meta_group(kmul, g)));
-#pragma unroll
-                for (int o = 0; o < Raw::OWN; ++o)
-                    own[x][o] = kv4_scale(raw.own[x][o]) * own_group(o, [&](int g) { return kmul[g]; });
-            }
-        } else {
-            const int ve = max(exp_of(vmag) - 11, -105);
-            stage_values([&](float v, int e) { return ldexpf(v, e - ve); });
-            if (lane < 32) {
-                ev[lane] = (float)ve;
-                iev[lane] = ldexpf(1.0f, -ve - TA_BASE);
-            }
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                int e = -0x1000;
-#pragma unroll
-                for (int g = 0; g < Raw::GX; ++g)
-                    e = max(e, exp_of(fmaxf(fabsf(mid[x][g]), sc[x][g])) + meta_group(group_e, g));
-                if (NG == 8) e = max(e, __shfl_xor(e, 16, 64));
-                e -= 11;
-                const int at = 8 * (col >> 2) + (col & 3) + 4 * x;
-                if (j == 0) ek[at] = e;
-                const bool in = !edge || p0 + at <= last;
-#pragma unroll
-                for (int g = 0; g < Raw::GX; ++g)
-                    middles[x][g] = two_terms(ldexpf(mid[x][g], meta_group(group_e, g) - e + 3));
-#pragma unroll
-                for (int o = 0; o < Raw::OWN; ++o) {
-                    const int ge = own_group(o, [&](int g) { return group_e[g]; });
-                    own[x][o] = in ? ldexpf(kv4_scale(raw.own[x][o]), ge - e) : 0.0f;
-                }
+            for (int i = 0; i < Raw::VM; ++i) {
+                const int g = (lane >> 5) * (NG / 2) + i;
+                const f16x2 t = __builtin_bit_cast(f16x2, vmiddles[i]);
+                o[g * 64] = t[0];
+                o[g * 64 + 32] = t[1];
+                o[M::SC / 2 + g * 32] = (_Float16)vscales[i];
             }
         }
         // 5. scores: rows of S^T, 4 j' + i of tile x is position 8 j' + 4 x + i
         f32x4 S[MT][2];
         f16x8 kf[2][KS + 1];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) key_codes(raw, x, own[x], middles[x], kf[x]);
+        for (int x = 0; x < 2; ++x) {
+            uint32_t ex[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int g = 0; g < Raw::GX; ++g) ex[g] = NG <= 4 && (j & 1) ? 0u : middles[x][g];  // (no group 4 ..)
+            kf[x][KS] = __builtin_bit_cast(f16x8, u32x4{ex[0], ex[1], ex[2], ex[3]});
+#pragma unroll
+            for (int o = 0; o < Raw::OWN; ++o) {
+                const uint32_t sp = f16_pair(own[x][o], own[x][o]), cp = minus24(sp);
+                const uint32_t s4[4] = {sp, sp, sp, sp}, c4[4] = {cp, cp, cp, cp};
+                constexpr int D = KS / Raw::OWN;
+#pragma unroll
+                for (int i = 0; i < D; ++i) kf[x][o * D + i] = Codes8(raw.k[x][o * D + i], s4, c4).v;
+            }
+        }
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             apart();
-            scores(t, kf, S[t]);
+            S[t][0] = S[t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 2 * KS + 1; ++i) {
+                const f16x8 qv = *(const f16x8 *)(qf + (t * M::FR + i) * 1024);
+                const int k = i == 2 * KS ? KS : i / 2;
+                S[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][k], qv, S[t][0], 0, 0, 0);
+                S[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][k], qv, S[t][1], 0, 0, 0);
+            }
         }
         __builtin_amdgcn_wave_barrier();
         // 6. the running maximum of weight times value
@@ -489,13 +558,13 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         };
         float top[MT];
         uint32_t seen = 0;  // a byte a tile
-        if (is_like()) {
+        if (is_shared()) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 float a = fmaxf(fmaxf(S[t][0][0], S[t][0][1]), S[t][0][2]);
                 a = fmaxf(fmaxf(a, S[t][0][3]), S[t][1][0]);
                 a = fmaxf(fmaxf(a, S[t][1][1]), S[t][1][2]);
-                top[t] = __builtin_fmaf(fmaxf(a, S[t][1][3]), cq[t], (float)ev_run);
+                top[t] = __builtin_fmaf(fmaxf(a, S[t][1][3]), cq[t], (float)(ev_run - TA_TOP_E));
             }
         } else {
 #pragma unroll
@@ -531,18 +600,19 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
             }
         }
         // 7. weights, in S's place
-        if (is_like()) {
+        if (is_shared()) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float base = (float)ev_run - (m[t] - TA_BASE);
-                float sum = 0.0f;
+                const float base = (float)(ev_run - TA_TOP_E) - (m[t] - TA_BASE);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float w8 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i / 4][i % 4], cq[t], base));
-                    S[t][i / 4][i % 4] = w8;
-                    sum += w8;
+                for (int i = 0; i < 8; ++i)
+                    S[t][i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i / 4][i % 4], cq[t], base));
+                if (!M::ONES) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum += S[t][i / 4][i % 4];
+                    l[t] = __builtin_fmaf(sum, uniform(ldexpf(1.0f, TA_TOP_E - ev_run - TA_BASE)), l[t]);
                 }
-                l[t] = __builtin_fmaf(sum, vsum, l[t]);
             }
         } else {
 #pragma unroll
@@ -565,28 +635,36 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         f16x8 ph[MT], pl[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {  // two f16 terms
-            uint32_t hi[4], lo[4];
+            f16x2 hi[4], lo[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float a = S[t][0][i], c = S[t][1][i];
-                hi[i] = f16_pair(a, c);
-                lo[i] = f16_pair(f16_rest<0>(hi[i], a), f16_rest<1>(hi[i], c));
+                hi[i] = __builtin_bit_cast(f16x2, f16_pair(a, c));
+                lo[i] = f16x2{rest(a, hi[i][0]), rest(c, hi[i][1])};
             }
-            ph[t] = __builtin_bit_cast(f16x8, u32x4{hi[0], hi[1], hi[2], hi[3]});
-            pl[t] = __builtin_bit_cast(f16x8, u32x4{lo[0], lo[1], lo[2], lo[3]});
+            ph[t] = __builtin_shufflevector(__builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3),
+                                            __builtin_shufflevector(hi[2], hi[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+            pl[t] = __builtin_shufflevector(__builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3),
+                                            __builtin_shufflevector(lo[2], lo[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
         }
         // 8. outputs: rows of O^T
 #pragma unroll
         for (int n = 0; n <= NT; ++n) {
-            const f16x8 vf = value_codes(raw, n);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t], O[t][n], 0, 0, 0);
+            f16x8 vf;
+            if (n == NT) {  // the middles, and ones where the weights' sum is in shared units
+                u32x4 e = *(const u32x4 *)(wl + col * 64 + j * 16);
+                if (M::ONES && !is_shared() && col == 15) e = u32x4{0, 0, 0, 0};
+                vf = __builtin_bit_cast(f16x8, e);
+            } else {
+                const u32x4 s = *(const u32x4 *)(wl + M::SC + n / 2 * 64 + j * 16);
+                const uint32_t s4[4] = {s[0], s[1], s[2], s[3]};
+                const uint32_t c4[4] = {minus24(s[0]), minus24(s[1]), minus24(s[2]), minus24(s[3])};
+                vf = Codes8(raw.v[n], s4, c4).v;
             }
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t], O[t][n], 0, 0, 0);
-            }
+            for (int t = 0; t < MT; ++t) O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t], O[t][n], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t], O[t][n], 0, 0, 0);
         }
         // 9. values that are NaN, to the queries that see them: through the middles' sums
         unsigned long long any_nan = 0;
@@ -610,78 +688,6 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         __builtin_amdgcn_wave_barrier();
     };
 
-    // 2. an eighth of each group's middle, and its scale; nothing past the last position
-    auto key_meta = [&](const Raw &raw, int p0, bool edge) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const bool in = !edge || p0 + 8 * (col >> 2) + (col & 3) + 4 * x <= last;
-#pragma unroll
-            for (int g = 0; g < Raw::GX; ++g) {
-                const uint32_t meta = in ? raw.km[x][g] : 0u;
-                sc[x][g] = kv4_scale(meta);
-                mid[x][g] = __builtin_fmaf(0.125f, kv4_min(meta), sc[x][g]);
-            }
-        }
-    };
-    auto value_meta = [&](const Raw &raw, int p0, bool edge) {
-        vmag = 0.0f;
-#pragma unroll
-        for (int i = 0; i < Raw::VM; ++i) {
-            const uint32_t meta = !edge || p0 + (lane & 31) <= last ? raw.vm[i] : 0u;
-            vsc[i] = kv4_scale(meta);
-            vmid[i] = __builtin_fmaf(0.125f, kv4_min(meta), vsc[i]);
-            nan_p[i] = 0;
-            if (edge) {  // what some queries see and others do not: told at the end
-                const bool bad = !(vmid[i] == vmid[i]);
-                nan_p[i] = __ballot(bad);
-                if (bad) vmid[i] = vsc[i] = 0.0f;
-            }
-            vmag = fmaxf(vmag, fmaxf(fabsf(vmid[i]), vsc[i]));
-        }
-        if (NG > 1) vmag = ta_swap32(vmag, ta_max);
-    };
-    // 3. whether all positions stand within 2^TA_SPAN below the powers of two, or below the
-    // block's own, which are taken then, with room above
-    auto alike = [&] {
-        float kmag[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            kmag[x] = 0.0f;
-#pragma unroll
-            for (int g = 0; g < Raw::GX; ++g) {
-                kmag[x] = fmaxf(kmag[x], fmaxf(fabsf(mid[x][g]), sc[x][g]) * meta_group(weight, g));
-            }
-            if (NG == 8) kmag[x] = ta_swap16(kmag[x], ta_max);
-        }
-        auto near = [&](float v, int e) { return (unsigned)(e - exp_of(v)) <= (unsigned)TA_SPAN; };
-        auto all_near = [&] {
-            return __all(near(kmag[0], ek_run) && near(kmag[1], ek_run) && near(vmag, ev_run + 11));
-        };
-        if (plain && all_near()) return true;
-        float k = fmaxf(kmag[0], kmag[1]);
-        k = ta_swap32(ta_swap16(ta_row16(k, ta_max), ta_max), ta_max);
-        const float v = ta_swap16(ta_row16(vmag, ta_max), ta_max);
-        ek_run = __builtin_amdgcn_readfirstlane(exp_of(k)) + 2;
-        ev_run = __builtin_amdgcn_readfirstlane(exp_of(v)) - 9;
-        vmul = uniform(ldexpf(1.0f, -ev_run));
-        vsum = uniform(ldexpf(1.0f, -ev_run - TA_BASE));
-        bool fits = ev_run >= -100 && ev_run <= 100 && ek_run >= -100 && ek_run <= 100;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const int e = group_e[g] - (ek_run - 11);
-            kmul[g] = uniform(ldexpf(1.0f, e));
-            fits &= e <= 100 && (e >= -100 || group_e[g] == TA_NO_GROUP);
-        }
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const int f = fe[t * 16 + col] + ek_run;
-            cq[t] = ldexpf(cs, f - 11);
-            fits &= f <= 100;
-        }
-        plain = __all(fits);
-        return plain && all_near();
-    };
-
     const int whole = min(b1, min(zone, last + 1) / KV4_BLOCK);  // blocks that all queries see
     Raw next;
     if (b0 + w < b1) next.load(p.c, head, b0 + w, lane);
@@ -689,9 +695,15 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         const Raw raw = next;
         if (blk + TA_W < b1) next.load(p.c, head, blk + TA_W, lane);
         const bool edge = blk >= whole;
-        key_meta(raw, blk * KV4_BLOCK, edge);
-        value_meta(raw, blk * KV4_BLOCK, edge);
-        block(raw, blk, edge, !edge && !far_any && alike());
+        bool shared = !edge && !far_any;
+        if (shared && !shared_meta(raw)) shared = choose(raw) && shared_meta(raw);
+        if (!shared) own_meta(raw, blk * KV4_BLOCK, edge);
+        block(raw, blk, edge, shared);
+    }
+    if (M::ONES) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            if (j == 3) l[t] += ldexpf(O[t][NT][3], TA_TOP_E - ev_run - TA_BASE);
     }
 
     // 10. the waves' results
