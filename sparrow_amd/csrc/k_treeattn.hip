@@ -211,9 +211,15 @@ struct RawBlock {
     }
 };
 
+// Waves a SIMD that the registers are held to: one more where they nearly suffice (16 sequences
+// with 32 tokens, heads of 64: 43 us at two, 34 at three).
+constexpr int ta_waves(int hd, int mt) {
+    return mt == 1 ? (hd == 32 ? 5 : hd == 64 ? 4 : 2) : mt == 2 && hd <= 64 ? 3 : 2;
+}
+
 // A tile of 16 MT (token, head) pairs of one sequence and kv head, and one share of the positions.
 template <int HD, int MT>
-__global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams p) {
+__global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(TreeAttnParams p) {
     using M = TreeLds<HD, MT>;
     using Raw = RawBlock<HD>;
     constexpr int NG = HD / 32, KS = HD / 32, NT = HD / 16, CL = HD / 4, ROWS = 16 * MT;
@@ -755,23 +761,38 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     }
 }
 
-// The shares of a query, in order.
+// The shares of a query, in order: lane s takes the s-th one's maximum and sum, the threads
+// eight of their rows at a time.
 template <int HD>
 __global__ __launch_bounds__(HD < 64 ? 64 : HD) void tree_merge_kernel(TreeAttnParams p, int ROWS) {
-    const int r = blockIdx.x % ROWS, tile = blockIdx.x / ROWS, kvh = blockIdx.y, b = blockIdx.z, c = threadIdx.x;
-    const TreeRows tr = tree_rows(p.pos0, p.count, p.parent, p.S, p.c.cap, b, p.guard, false);
-    const int R = tile * ROWS + r;
-    if (R >= tr.n * p.G || c >= HD) return;
+    const int r = blockIdx.x % ROWS, tile = blockIdx.x / ROWS, kvh = blockIdx.y, b = blockIdx.z;
+    const int lane = threadIdx.x & 63, c = min((int)threadIdx.x, HD - 1);
     const size_t pair = (size_t)b * p.c.Hkv + kvh, ld = (size_t)ROWS * (HD + 2);
     const float *pw = p.work + (pair * p.tiles + tile) * p.shares * ld;
-    float mx = TA_NONE, L = 0.0f, o = 0.0f;
-    for (int s = 0; s < p.shares; ++s) mx = fmaxf(mx, pw[s * ld + ROWS * HD + 2 * r]);
-    for (int s = 0; s < p.shares; ++s) {
-        const float f = __builtin_amdgcn_exp2f(pw[s * ld + ROWS * HD + 2 * r] - mx);
-        L = __builtin_fmaf(f, pw[s * ld + ROWS * HD + 2 * r + 1], L);
-        o = __builtin_fmaf(f, pw[s * ld + r * HD + c], o);
+    const float *px = pw + r * HD + c, *pm = pw + min(lane, p.shares - 1) * ld + ROWS * HD + 2 * r;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = px[min(i, p.shares - 1) * ld];
+    const float m = pm[0], l = pm[1];
+    const TreeRows tr = tree_rows(p.pos0, p.count, p.parent, p.S, p.c.cap, b, p.guard, false);
+    const int R = tile * ROWS + r;
+    if (R >= tr.n * p.G) return;  // (what was read is not this query's)
+    const float mx = ta_swap32(ta_swap16(ta_row16(m, ta_max), ta_max), ta_max);
+    const float f = lane < p.shares ? __builtin_amdgcn_exp2f(m - mx) : 0.0f;
+    const float L = wave_sum_dpp(lane < p.shares ? f * l : 0.0f);
+    float o = 0.0f;
+    for (int s = 0; s < p.shares; s += 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), min(s + i, 63)));
+            o = s + i < p.shares ? __builtin_fmaf(w, x[i], o) : o;
+        }
+        if (s + 8 >= p.shares) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = px[min(s + 8 + i, p.shares - 1) * ld];
     }
-    p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * TA_UNBASE / L;
+    if (threadIdx.x < HD)
+        p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * TA_UNBASE / L;
 }
 
 struct TreePlan {
