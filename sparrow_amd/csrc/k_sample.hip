@@ -24,7 +24,8 @@ namespace {
 
 constexpr int THREADS = 1024;
 constexpr int BINS = 2048;      // the last one's tokens have no weight
-constexpr int LIST = 2048;      // tokens of a bin that are sorted
+constexpr int LIST = 2048;      // tokens that are sorted at once
+constexpr int SLICE_LIST = 256; // tokens of the first bins that a slice lists
 constexpr double PER = 64.0;    // bins of 1
 constexpr int UNIT = 30;        // d in units of 2^-30
 constexpr int COUNT = 44;       // a bin's word: count above, sum of d below
@@ -67,12 +68,21 @@ __device__ __forceinline__ uint32_t loss(double rest) {
     return (uint32_t)(int)__builtin_rint(d * (double)(1 << UNIT));
 }
 
-// Calls f(logit, index) for every token of the row.
-template <typename F>
+// Calls f(logit, index) for the tokens [0, n) at `row`: 16 of a thread at a time, loaded
+// before the first is used. T: threads.
+template <int T, typename F>
 __device__ __forceinline__ void each_token(const float *row, int n, F f) {
-    const int step = THREADS * 4;
     int i = threadIdx.x * 4;
-    for (; i + 3 < n; i += step) {
+    for (; i + 3 + 3 * T * 4 < n; i += 4 * T * 4) {
+        f32x4a v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = *(const f32x4a *)(row + i + k * T * 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f(v[k][e], i + k * T * 4 + e);
+    }
+    for (; i + 3 < n; i += T * 4) {
         const f32x4a v = *(const f32x4a *)(row + i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) f(v[e], i + e);
@@ -116,6 +126,35 @@ __device__ T block_scan(T a, T b, T *out_a, T *out_b, T *scratch) {
     return all;
 }
 
+// The n <= LIST tokens that `each` puts, (order bits, ~index), in s.list: the largest first.
+template <typename F>
+__device__ void gather(Shared &s, int n, F each) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (tid == 0) s.n = 0;
+    int pow2 = 64;
+    while (pow2 < n) pow2 *= 2;
+    for (int i = tid; i < pow2; i += THREADS) s.list[i] = 0;
+    __syncthreads();
+    each([&](unsigned long long v) {
+        const uint32_t k = atomicAdd(&s.n, 1u);
+        if (k < LIST) s.list[k] = v;
+    });
+    __syncthreads();
+    for (int k = 2; k <= pow2; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            for (int i = tid; i < pow2 / 2; i += THREADS) {
+                const int x = i / j * 2 * j + i % j, y = x + j;
+                const unsigned long long a = s.list[x], b = s.list[y];
+                if (((x & k) == 0) == (a < b)) {
+                    s.list[x] = b;
+                    s.list[y] = a;
+                }
+            }
+            __syncthreads();
+        }
+}
+
 // A place in the order: its token's rank in its bin and the bin's weights up to it, in
 // units of 2^-30 of the bin's largest.
 struct Found {
@@ -141,7 +180,7 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         }
         for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
         __syncthreads();
-        each_token(row, vocab, [&](float l, int) {
+        each_token<THREADS>(row, vocab, [&](float l, int) {
             double rest;
             const uint32_t key = order_bits(l);
             if (at.bin(l, &rest) == bin && key >= lo && key <= hi) {
@@ -155,7 +194,7 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         if (lo == hi) break;
         int shift = 0;
         while ((hi - lo) >> shift >= BINS) ++shift;
-        each_token(row, vocab, [&](float l, int) {
+        each_token<THREADS>(row, vocab, [&](float l, int) {
             double rest;
             const uint32_t key = order_bits(l);
             if (at.bin(l, &rest) == bin && key >= lo && key <= hi)
@@ -202,7 +241,7 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         __syncthreads();
         if (tid == 0) s.n = 0;
         __syncthreads();
-        each_token(row, vocab, [&](float l, int) {
+        each_token<THREADS>(row, vocab, [&](float l, int) {
             double rest;
             if (order_bits(l) == lo && at.bin(l, &rest) == bin) s.n = loss(rest);
         });
@@ -233,31 +272,13 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         return f;
     }
     // 3. its tokens, gathered and sorted
-    __syncthreads();
-    if (tid == 0) s.n = 0;
-    int pow2 = 64;
-    while (pow2 < n) pow2 *= 2;
-    for (int i = tid; i < pow2; i += THREADS) s.list[i] = 0;
-    __syncthreads();
-    each_token(row, vocab, [&](float l, int i) {
-        double rest;
-        const uint32_t key = order_bits(l);
-        if (key >= lo && key <= hi && at.bin(l, &rest) == bin)
-            s.list[atomicAdd(&s.n, 1u)] = (unsigned long long)key << 32 | (uint32_t)~i;
+    gather(s, n, [&](auto put) {
+        each_token<THREADS>(row, vocab, [&](float l, int i) {
+            double rest;
+            const uint32_t key = order_bits(l);
+            if (key >= lo && key <= hi && at.bin(l, &rest) == bin) put((unsigned long long)key << 32 | (uint32_t)~i);
+        });
     });
-    __syncthreads();
-    for (int k = 2; k <= pow2; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            for (int i = tid; i < pow2 / 2; i += THREADS) {
-                const int x = i / j * 2 * j + i % j, y = x + j;
-                const unsigned long long a = s.list[x], b = s.list[y];
-                if (((x & k) == 0) == (a < b)) {  // the largest first
-                    s.list[x] = b;
-                    s.list[y] = a;
-                }
-            }
-            __syncthreads();
-        }
     static_assert(LIST == BINS && LIST == 2 * THREADS, "");
     unsigned long long *sum = s.hist, d[2], e[2];
 #pragma unroll
@@ -293,29 +314,33 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
     return f;
 }
 
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
-    __shared__ Shared s;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const float u = p.u[r], t = p.t[r], top_p = p.top_p ? p.top_p[r] : 1.0f,
-                min_p = p.min_p ? p.min_p[r] : 0.0f;
-    const int top_k = p.top_k ? p.top_k[r] : 0, n = p.vocab;
-    if (u < 0.0f) return;  // an idle row
-    if (!(u < 1.0f) || !(t >= 0.0f && t <= 3.40282347e38f) || !(top_p == top_p) ||
-        !(min_p >= 0.0f && min_p <= 1.0f)) {
-        if (tid == 0) atomicOr(p.guard, 1);
-        return;
-    }
-    const float *row = p.logits + r * p.ld;
-    auto answer = [&](int token, float prob) {
-        if (tid == 0) {
-            p.token[r] = token;
-            if (p.prob) p.prob[r] = prob;
-        }
-    };
-    // 1. the largest, the first of equal ones; NaN anywhere
-    uint32_t best = 0, index = 0xffffffffu;
+// A row's settings. live: there is something to draw.
+struct Settings {
+    float u, t, top_p, min_p;
+    int top_k;
+    bool live;
+};
+__device__ __forceinline__ Settings settings_of(const SampleParams &p, int r, bool report) {
+    Settings c;
+    c.u = p.u[r];
+    c.t = p.t[r];
+    c.top_p = p.top_p ? p.top_p[r] : 1.0f;
+    c.min_p = p.min_p ? p.min_p[r] : 0.0f;
+    c.top_k = p.top_k ? p.top_k[r] : 0;
+    const bool ok = c.u < 1.0f && c.t >= 0.0f && c.t <= 3.40282347e38f && c.top_p == c.top_p &&
+                    c.min_p >= 0.0f && c.min_p <= 1.0f;
+    c.live = ok && c.u >= 0.0f;
+    if (!ok && !(c.u < 0.0f) && report && threadIdx.x == 0) atomicOr(p.guard, 1);
+    return c;
+}
+
+// The largest of some tokens, the first of equal ones: (order bits, ~index); a NaN above all.
+constexpr unsigned long long WITH_NAN = ~0ull;
+template <int T>
+__device__ unsigned long long largest(const float *row, int n, int first, unsigned long long *scratch) {
+    uint32_t best = 0, index = 0;
     bool nan = false;
-    each_token(row, n, [&](float l, int i) {
+    each_token<T>(row, n, [&](float l, int i) {
         nan |= l != l;
         const uint32_t key = order_bits(l);
         if (key > best) {
@@ -323,31 +348,54 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             index = i;
         }
     });
-    if (tid == 0) {
-        s.best = 0;
-        s.n = 0;
+    unsigned long long v = nan ? WITH_NAN : (unsigned long long)best << 32 | (uint32_t)~(first + index);
+#pragma unroll
+    for (int o = 32; o; o /= 2) {
+        const unsigned long long w = (unsigned long long)__shfl_xor((uint32_t)(v >> 32), o, 64) << 32 |
+                                     (uint32_t)__shfl_xor((uint32_t)v, o, 64);
+        v = w > v ? w : v;
     }
-    for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
     __syncthreads();
-    if (nan) s.n = 1;
-    atomicMax(&s.best, (unsigned long long)best << 32 | (uint32_t)~index);
+    for (int i = 0; i < T / 64; ++i) v = scratch[i] > v ? scratch[i] : v;
     __syncthreads();
-    index = ~(uint32_t)s.best;
-    const bool any_nan = s.n != 0;
-    __syncthreads();
-    const float max = row[index < (uint32_t)n ? index : 0];
-    if (any_nan || max == __builtin_inff()) return answer(-1, __builtin_nanf(""));
-    if (max == -__builtin_inff()) return answer(-1, 0.0f);  // the mask leaves no token
-    if (t == 0.0f) return answer((int)index, 1.0f);
+    return v;
+}
+// the logit that the order bits came from
+__device__ __forceinline__ float of_bits(uint32_t b) { return __uint_as_float((b >> 31) ? b ^ 0x80000000u : ~b); }
 
-    // 2. the bins
-    const Place at{(double)max, PER / (double)t};
-    each_token(row, n, [&](float l, int) {
+// Counts and losses of some tokens into the bins.
+template <int T>
+__device__ __forceinline__ void count_bins(unsigned long long *hist, const float *row, int n, const Place &at) {
+    each_token<T>(row, n, [&](float l, int) {
         double rest;
         const int b = at.bin(l, &rest);
-        if (b < BINS - 1) atomicAdd(&s.hist[b], (1ull << COUNT) | loss(rest));
+        if (b < BINS - 1) atomicAdd(&hist[b], (1ull << COUNT) | loss(rest));
     });
-    __syncthreads();
+}
+
+// What the slices of a row leave for its last kernel.
+struct SampleSlices {
+    int n, each;                     // their number and tokens
+    unsigned long long *best;        // [rows][n] the largest token
+    unsigned long long *hist;        // [rows][n][BINS]
+    unsigned long long *list;        // [rows][n][SLICE_LIST] the tokens of the first bins
+    int32_t *upto;                   // [rows][n][2]: those below this bin, and their number
+};
+
+// 3. The rest, from a row's bins in s.hist: by one workgroup.
+__device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &c, float first,
+                       const SampleSlices &sl) {
+    const int tid = threadIdx.x, n = p.vocab;
+    const float *row = p.logits + r * p.ld;
+    const float u = c.u, t = c.t;
+    auto answer = [&](int token, float prob) {
+        if (tid == 0) {
+            p.token[r] = token;
+            if (p.prob) p.prob[r] = prob;
+        }
+    };
+    const Place at{(double)first, PER / (double)t};
     uint32_t cnt[2], c0[2];
     double mass[2], m0[2];
     const double unit = 1.0 / (1 << UNIT);
@@ -383,16 +431,97 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         while (b > 0 && tokens(b) == 0) --b;
         return b;
     };
-    // 3. what is kept: the first `kept` of the order, of weight `all`
     uint32_t kept = live;
-    if (top_k > 0 && (uint32_t)top_k < kept) {
-        kept = (uint32_t)top_k;
+    const bool by_k = c.top_k > 0 && (uint32_t)c.top_k < live;
+    const double far = -log((double)c.min_p) * PER;  // min_p's place (+inf: none)
+
+    // The bins up to which tokens can be kept: where they hold few, those are sorted
+    // together and every question is one of their sums.
+    int cut = BINS - 2;
+    if (by_k) cut = bin_of_rank((uint32_t)c.top_k - 1);
+    if (!(by_k && c.top_p < 1.0f)) {  // (p is of the k's weight)
+        if (c.top_p < 1.0f) cut = bin_of_mass((double)c.top_p * all, true);
+        if (far < cut) cut = (int)far + 1;
+    }
+    const int few = (int)s.before[cut + 1];
+    if (few <= LIST) {
+        bool listed = sl.n > 0;
+        for (int i = 0; i < sl.n; ++i) listed &= cut < sl.upto[((size_t)r * sl.n + i) * 2];
+        gather(s, few, [&](auto put) {
+            if (listed) {
+                for (int i = tid / SLICE_LIST; i < sl.n; i += THREADS / SLICE_LIST) {
+                    const size_t x = (size_t)r * sl.n + i;
+                    const int k = tid % SLICE_LIST;
+                    if (k >= sl.upto[x * 2 + 1]) continue;
+                    const unsigned long long v = sl.list[x * SLICE_LIST + k];
+                    double rest;
+                    if (at.bin(of_bits((uint32_t)(v >> 32)), &rest) <= cut) put(v);
+                }
+            } else {
+                each_token<THREADS>(row, n, [&](float l, int i) {
+                    double rest;
+                    if (at.bin(l, &rest) <= cut) put((unsigned long long)order_bits(l) << 32 | (uint32_t)~i);
+                });
+            }
+        });
+        double w[2], up[2];
+        bool over[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int x = tid * 2 + i;
+            w[i] = 0.0;
+            over[i] = false;
+            if (x < few) {
+                double rest;
+                const float l = of_bits((uint32_t)(s.list[x] >> 32));
+                const int b = at.bin(l, &rest);
+                w[i] = scale(b) * (double)((1u << UNIT) - loss(rest));
+                over[i] = c.min_p == 0.0f || exp(((double)l - at.max) / (double)t) >= (double)c.min_p;
+            }
+        }
+        block_scan<double>(w[0], w[1], &up[0], &up[1], s.red);  // weights before a token
+        // counts of a condition that holds up to some token
+        auto upto = [&](bool a, bool b) {
+            uint32_t x, y;
+            return block_scan<uint32_t>(a, b, &x, &y, s.wave);
+        };
+        auto sum_upto = [&](uint32_t k) {  // of the first k > 0
+            if (tid == (int)(k - 1) / 2) s.red[0] = (k - 1) % 2 ? up[1] + w[1] : up[0] + w[0];
+            __syncthreads();
+            const double v = s.red[0];
+            __syncthreads();
+            return v;
+        };
+        kept = (uint32_t)few;
+        if (by_k && c.top_k <= few) {
+            kept = (uint32_t)c.top_k;
+            all = sum_upto(kept);
+        }
+        if (c.top_p < 1.0f) {
+            const double goal = (double)c.top_p * all;
+            kept = min(kept, max(1u, upto(tid * 2 < few && up[0] < goal, tid * 2 + 1 < few && up[1] < goal)));
+        }
+        if (c.min_p > 0.0f) kept = min(kept, max(1u, upto(over[0], over[1])));
+        all = sum_upto(kept);
+        const double goal = (double)u * all;
+        const uint32_t x = min(upto(tid * 2 < few && up[0] + w[0] <= goal, tid * 2 + 1 < few && up[1] + w[1] <= goal),
+                               kept - 1);
+        if (tid == (int)x / 2) {
+            p.token[r] = (int)~(uint32_t)s.list[x];
+            if (p.prob) p.prob[r] = (float)((x % 2 ? w[1] : w[0]) / all);
+        }
+        return;
+    }
+
+    // Else each question by its bin.
+    if (by_k) {
+        kept = (uint32_t)c.top_k;
         const int b = bin_of_rank(kept - 1);
         const Found f = locate(s, row, n, at, b, tokens(b), true, kept - 1 - s.before[b], 0.0, false);
         all = s.above[b] + scale(b) * (double)f.upto;
     }
-    if (top_p < 1.0f) {
-        const double goal = (double)top_p * all;
+    if (c.top_p < 1.0f) {
+        const double goal = (double)c.top_p * all;
         const int b = bin_of_mass(goal, true);
         const Found f = locate(s, row, n, at, b, tokens(b), false, 0, (goal - s.above[b]) / scale(b), true);
         const uint32_t k = s.before[b] + f.rank + 1;
@@ -401,18 +530,17 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             all = s.above[b] + scale(b) * (double)f.upto;
         }
     }
-    if (min_p > 0.0f) {
+    if (c.min_p > 0.0f) {
         // (weights next to the border in 64 bits, the others by their bin)
-        const double x = -log((double)min_p) * PER;
         uint32_t k = 0;
-        each_token(row, n, [&](float l, int) {
+        each_token<THREADS>(row, n, [&](float l, int) {
             double rest;
             const int b = at.bin(l, &rest);
             if (b == BINS - 1) return;
-            if (fabs((double)b - x) > 2.0)
-                k += (double)b < x;
+            if (fabs((double)b - far) > 2.0)
+                k += (double)b < far;
             else
-                k += exp(((double)l - at.max) / (double)t) >= (double)min_p;
+                k += exp(((double)l - at.max) / (double)t) >= (double)c.min_p;
         });
         if (tid == 0) s.n = 0;
         __syncthreads();
@@ -427,7 +555,6 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             all = s.above[b] + scale(b) * (double)f.upto;
         }
     }
-    // 4. the token
     const double goal = (double)u * all;
     int b = bin_of_mass(goal, false);
     Found f = locate(s, row, n, at, b, tokens(b), false, 0, (goal - s.above[b]) / scale(b), false);
@@ -438,14 +565,183 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     answer((int)f.token, (float)(scale(b) * (double)((1u << UNIT) - f.d) / all));
 }
 
+// What there is to say of a row whose largest token is known; true if nothing else is.
+__device__ __forceinline__ bool settled(const SampleParams &p, int r, const Settings &c, unsigned long long best,
+                                        bool write) {
+    const float max = of_bits((uint32_t)(best >> 32));
+    int token = -1;
+    float prob;
+    if (best == WITH_NAN || max == __builtin_inff())
+        prob = __builtin_nanf("");
+    else if (max == -__builtin_inff())
+        prob = 0.0f;  // the mask leaves no token
+    else if (c.t == 0.0f) {
+        token = (int)~(uint32_t)best;
+        prob = 1.0f;
+    } else
+        return false;
+    if (write && threadIdx.x == 0) {
+        p.token[r] = token;
+        if (p.prob) p.prob[r] = prob;
+    }
+    return true;
+}
+
+// A workgroup a row.
+__global__ __launch_bounds__(THREADS) void sample_row_kernel(SampleParams p) {
+    __shared__ Shared s;
+    const int r = blockIdx.x;
+    const Settings c = settings_of(p, r, true);
+    if (!c.live) return;
+    const float *row = p.logits + r * p.ld;
+    for (int i = threadIdx.x; i < BINS; i += THREADS) s.hist[i] = 0;
+    const unsigned long long best = largest<THREADS>(row, p.vocab, 0, s.wave64);
+    if (settled(p, r, c, best, true)) return;
+    const float max = of_bits((uint32_t)(best >> 32));
+    count_bins<THREADS>(s.hist, row, p.vocab, Place{(double)max, PER / (double)c.t});
+    __syncthreads();
+    finish(s, p, r, c, max, SampleSlices{0, 0, nullptr, nullptr, nullptr, nullptr});
+}
+
+// Few rows: a workgroup for each slice of them finds its largest token, then its bins and the
+// tokens of the first ones, then a workgroup a row ends it.
+constexpr int SLICE = 8192, SLICE_THREADS = 512;
+__global__ __launch_bounds__(SLICE_THREADS) void sample_best_kernel(SampleParams p, SampleSlices sl) {
+    __shared__ unsigned long long scratch[SLICE_THREADS / 64];
+    const int r = blockIdx.y, first = blockIdx.x * sl.each;
+    if (!settings_of(p, r, false).live) return;
+    const unsigned long long v = largest<SLICE_THREADS>(p.logits + r * p.ld + first, min(sl.each, p.vocab - first),
+                                                        first, scratch);
+    if (threadIdx.x == 0) sl.best[(size_t)r * sl.n + blockIdx.x] = v;
+}
+
+__device__ __forceinline__ unsigned long long best_of(const SampleSlices &sl, int r) {
+    unsigned long long best = 0;
+    for (int i = 0; i < sl.n; ++i) {
+        const unsigned long long v = sl.best[(size_t)r * sl.n + i];
+        best = v > best ? v : best;
+    }
+    return best;
+}
+
+__global__ __launch_bounds__(SLICE_THREADS) void sample_bins_kernel(SampleParams p, SampleSlices sl) {
+    __shared__ unsigned long long hist[BINS];
+    __shared__ uint32_t wave[SLICE_THREADS / 64], n, last;
+    const int r = blockIdx.y, first = blockIdx.x * sl.each, tid = threadIdx.x, len = min(sl.each, p.vocab - first);
+    const Settings c = settings_of(p, r, false);
+    if (!c.live) return;
+    for (int i = tid; i < BINS; i += SLICE_THREADS) hist[i] = 0;
+    const unsigned long long best = best_of(sl, r);
+    if (settled(p, r, c, best, false)) return;
+    const Place at{(double)of_bits((uint32_t)(best >> 32)), PER / (double)c.t};
+    const float *row = p.logits + r * p.ld + first;
+    if (tid == 0) {
+        n = 0;
+        last = 0;
+    }
+    __syncthreads();
+    count_bins<SLICE_THREADS>(hist, row, len, at);
+    __syncthreads();
+    // the bins that hold at most SLICE_LIST tokens together
+    constexpr int EACH = BINS / SLICE_THREADS;
+    const size_t x = (size_t)r * sl.n + blockIdx.x;
+    uint32_t cnt[EACH], sum = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const unsigned long long h = hist[tid * EACH + i];
+        sl.hist[x * BINS + tid * EACH + i] = h;
+        cnt[i] = (uint32_t)(h >> COUNT);
+        sum += cnt[i];
+    }
+    uint32_t to = sum;
+    const int lane = tid & 63, w = tid >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const uint32_t v = __shfl_up(to, o, 64);
+        if (lane >= o) to += v;
+    }
+    if (lane == 63) wave[w] = to;
+    __syncthreads();
+    to -= sum;
+    for (int i = 0; i < w; ++i) to += wave[i];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {  // bin tid EACH + i is listed where the count up to it fits
+        to += cnt[i];
+        if (to <= SLICE_LIST) atomicMax(&last, (uint32_t)min(tid * EACH + i + 1, BINS - 1));
+    }
+    __syncthreads();
+    const int upto = (int)last;
+    each_token<SLICE_THREADS>(row, len, [&](float l, int i) {
+        double rest;
+        if (at.bin(l, &rest) < upto) {
+            const uint32_t k = atomicAdd(&n, 1u);
+            if (k < SLICE_LIST)
+                sl.list[x * SLICE_LIST + k] = (unsigned long long)order_bits(l) << 32 | (uint32_t)~(first + i);
+        }
+    });
+    __syncthreads();
+    if (tid == 0) {
+        sl.upto[x * 2] = upto;
+        sl.upto[x * 2 + 1] = (int)n;
+    }
+}
+
+__global__ __launch_bounds__(THREADS) void sample_finish_kernel(SampleParams p, SampleSlices sl) {
+    __shared__ Shared s;
+    const int r = blockIdx.x, tid = threadIdx.x;
+    const Settings c = settings_of(p, r, true);
+    if (!c.live) return;
+    const unsigned long long best = best_of(sl, r);
+    if (settled(p, r, c, best, true)) return;
+    unsigned long long a = 0, b = 0;
+    for (int i = 0; i < sl.n; ++i) {
+        const unsigned long long *h = sl.hist + ((size_t)r * sl.n + i) * BINS + tid * 2;
+        a += h[0];
+        b += h[1];
+    }
+    s.hist[tid * 2] = a;
+    s.hist[tid * 2 + 1] = b;
+    __syncthreads();
+    finish(s, p, r, c, of_bits((uint32_t)(best >> 32)), sl);
+}
+
+// SampleSlices where a row is long and they do not fill the chip by themselves: their three launches
+// and the bins' way through memory cost more than a row's own workgroup does from there on.
+int slices_of(int rows, int vocab) {
+    const int n = (vocab + SLICE - 1) / SLICE;
+    return n >= 4 && (long long)rows * n <= 512 ? n : 0;
+}
+
 }  // namespace
 
-size_t sample_work_bytes(int rows, int vocab) { return 0; }
+size_t sample_work_bytes(int rows, int vocab) {
+    const size_t n = slices_of(rows, vocab);
+    return rows * n * ((BINS + SLICE_LIST + 1) * 8 + 8);
+}
 
 int launch_sample(const SampleArgs &a, hipStream_t st) {
     const SampleParams p{a.logits, a.ld,    a.u,    a.t,     a.top_p, a.min_p,
                          a.top_k,  a.rows, a.vocab, a.token, a.prob,  guard_flag_ptr()};
-    sample_kernel<<<(unsigned)a.rows, THREADS, 0, st>>>(p);
+    SampleSlices sl;
+    sl.n = slices_of(a.rows, a.vocab);
+    if (sl.n == 0) {
+        sample_row_kernel<<<(unsigned)a.rows, THREADS, 0, st>>>(p);
+        VMLM_HIP_CHECK(hipGetLastError());
+        return VMLM_OK;
+    }
+    VMLM_GUARD(a.work, "sample: sliced rows need a workspace");
+    const size_t x = (size_t)a.rows * sl.n;
+    sl.each = SLICE;
+    sl.hist = (unsigned long long *)a.work;
+    sl.list = sl.hist + x * BINS;
+    sl.best = sl.list + x * SLICE_LIST;
+    sl.upto = (int32_t *)(sl.best + x);
+    const dim3 grid((unsigned)sl.n, (unsigned)a.rows);
+    sample_best_kernel<<<grid, SLICE_THREADS, 0, st>>>(p, sl);
+    VMLM_HIP_CHECK(hipGetLastError());
+    sample_bins_kernel<<<grid, SLICE_THREADS, 0, st>>>(p, sl);
+    VMLM_HIP_CHECK(hipGetLastError());
+    sample_finish_kernel<<<(unsigned)a.rows, THREADS, 0, st>>>(p, sl);
     VMLM_HIP_CHECK(hipGetLastError());
     return VMLM_OK;
 }
