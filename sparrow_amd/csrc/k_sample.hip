@@ -26,7 +26,7 @@ constexpr int THREADS = 1024;
 constexpr int BINS = 2048;      // the last one's tokens have no weight
 constexpr int LIST = 2048;      // tokens that are sorted at once
 constexpr int SLICE_LIST = 256; // tokens of the first bins that a slice lists
-constexpr double PER = 64.0;    // bins of 1
+constexpr double PER = 64.0;    // bins of a distance of 1
 constexpr int UNIT = 30;        // d in units of 2^-30
 constexpr int COUNT = 44;       // a bin's word: count above, sum of d below
 
@@ -50,22 +50,31 @@ __device__ __forceinline__ uint32_t order_bits(float v) {
     return (b >> 31) ? ~b : b | 0x80000000u;
 }
 
-// A logit's place: its bin, and the rest of its distance in [0, 1) of a bin.
+// A logit's place: its bin, and the rest of its distance as a fraction of a bin in units of
+// 2^-32. 2^20 added to the distance leaves both in the bits of the sum.
 struct Place {
     double max, per;  // PER / T
-    __device__ __forceinline__ int bin(float l, double *rest) const {
-        const double x = (max - (double)l) * per;  // (+inf for a masked one)
-        if (!(x < BINS - 1)) return BINS - 1;
-        const double f = __builtin_floor(x);
-        *rest = x - f;
-        return (int)f;
+    __device__ __forceinline__ int bin(float l, uint32_t *rest) const {
+        const double y = __builtin_fma(max - (double)l, per, 0x1p20);  // (+inf for a masked one)
+        const unsigned long long b = __builtin_bit_cast(unsigned long long, y);
+        *rest = (uint32_t)b;
+        return (int)min((uint32_t)(b >> 32) - 0x41300000u, (uint32_t)(BINS - 1));
+    }
+    // Logits below this one are not in bin b or before it; above it, not in bin b or behind it.
+    // (f32: by a part of a bin, and where a bin is narrower than its steps by a few of those)
+    __device__ __forceinline__ float below(int b) const {
+        return (float)(max - ((double)b + 1.02) / per - fabs(max) * 0x1p-21);
+    }
+    __device__ __forceinline__ float above(int b) const {
+        return (float)(max - ((double)b - 0.02) / per + fabs(max) * 0x1p-21);
     }
 };
-// 1 - exp(-r / 64), in units of 2^-30 (the next term of the series is below 2^-36)
-__device__ __forceinline__ uint32_t loss(double rest) {
-    const double r = rest * (1.0 / PER);
-    const double d = r * (1.0 - r * (0.5 - r * (1.0 / 6 - r * (1.0 / 24))));
-    return (uint32_t)(int)__builtin_rint(d * (double)(1 << UNIT));
+// 1 - exp(-r) of the rest r = f 2^-38 < 2^-6, in units of 2^-30, off by at most one: r itself
+// from the bits, the other terms below 2^-13 in f32 (the next of the series is below 2^-36)
+__device__ __forceinline__ uint32_t loss(uint32_t f) {
+    const float r = (float)f * 0x1p-38f;
+    const float q = r * r * __builtin_fmaf(__builtin_fmaf(r, 1.0f / 24, -1.0f / 6), r, 0.5f);
+    return (uint32_t)((f >> 8) + (f >> 7 & 1)) - (uint32_t)(int)rintf(q * 0x1p30f);
 }
 
 // Calls f(logit, index) for the tokens [0, n) at `row`: 16 of a thread at a time, loaded
@@ -95,6 +104,7 @@ struct Shared {
     double above[BINS];             // the mass before a bin
     uint32_t before[BINS];          // the tokens before a bin
     unsigned long long list[LIST];  // (order bits, ~index), the largest first
+    uint32_t rank[512];
     double red[16];
     unsigned long long wave64[16];
     unsigned long long best;
@@ -126,21 +136,37 @@ __device__ T block_scan(T a, T b, T *out_a, T *out_b, T *scratch) {
     return all;
 }
 
-// The n <= LIST tokens that `each` puts, (order bits, ~index), in s.list: the largest first.
+// The n <= LIST tokens that `each` puts, (order bits, ~index), in s.list: the largest first. Up
+// to 512 by the number of larger ones, which as many threads as there are count together
+// (256 tokens: 64 reads each, where a sort of them has 36 steps); more by a bitonic sort.
 template <typename F>
 __device__ void gather(Shared &s, int n, F each) {
     const int tid = threadIdx.x;
+    const bool count = n <= 512;
+    unsigned long long *raw = count ? s.hist : s.list;
     __syncthreads();
     if (tid == 0) s.n = 0;
     int pow2 = 64;
     while (pow2 < n) pow2 *= 2;
-    for (int i = tid; i < pow2; i += THREADS) s.list[i] = 0;
+    for (int i = tid; i < pow2; i += THREADS) raw[i] = 0;
+    if (count && tid < 512) s.rank[tid] = 0;
     __syncthreads();
     each([&](unsigned long long v) {
         const uint32_t k = atomicAdd(&s.n, 1u);
-        if (k < LIST) s.list[k] = v;
+        if (k < LIST) raw[k] = v;
     });
     __syncthreads();
+    if (count) {
+        const int parts = THREADS / pow2, x = tid % pow2, each_part = pow2 / parts, a = tid / pow2 * each_part;
+        const unsigned long long v = raw[x];
+        uint32_t larger = 0;
+        for (int i = a; i < a + each_part; ++i) larger += raw[i] > v;
+        if (larger) atomicAdd(&s.rank[x], larger);
+        __syncthreads();
+        if (tid < n) s.list[s.rank[tid]] = raw[tid];
+        __syncthreads();
+        return;
+    }
     for (int k = 2; k <= pow2; k *= 2)
         for (int j = k / 2; j > 0; j /= 2) {
             for (int i = tid; i < pow2 / 2; i += THREADS) {
@@ -169,6 +195,7 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
                         bool by_rank, uint32_t rank, double mass, bool with_equal) {
     const int tid = threadIdx.x;
     uint32_t lo = 0, hi = 0xffffffffu;  // of the order bits
+    const float from = at.below(bin), to = at.above(bin);
     uint32_t rank0 = 0;                 // the bin's tokens above them, and their weights
     unsigned long long mass0 = 0;
     // 1. a bin of too many tokens: ranges of their order bits, the narrowest that hold the place
@@ -181,9 +208,9 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
         __syncthreads();
         each_token<THREADS>(row, vocab, [&](float l, int) {
-            double rest;
+            uint32_t rest;
             const uint32_t key = order_bits(l);
-            if (at.bin(l, &rest) == bin && key >= lo && key <= hi) {
+            if (l >= from && l <= to && at.bin(l, &rest) == bin && key >= lo && key <= hi) {
                 atomicMin(&s.lo, key);
                 atomicMax(&s.hi, key);
             }
@@ -195,9 +222,9 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         int shift = 0;
         while ((hi - lo) >> shift >= BINS) ++shift;
         each_token<THREADS>(row, vocab, [&](float l, int) {
-            double rest;
+            uint32_t rest;
             const uint32_t key = order_bits(l);
-            if (at.bin(l, &rest) == bin && key >= lo && key <= hi)
+            if (l >= from && l <= to && at.bin(l, &rest) == bin && key >= lo && key <= hi)
                 atomicAdd(&s.hist[(hi - key) >> shift], (1ull << COUNT) | loss(rest));
         });
         __syncthreads();
@@ -242,8 +269,11 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         if (tid == 0) s.n = 0;
         __syncthreads();
         each_token<THREADS>(row, vocab, [&](float l, int) {
-            double rest;
-            if (order_bits(l) == lo && at.bin(l, &rest) == bin) s.n = loss(rest);
+            uint32_t rest;
+            if (order_bits(l) == lo) {
+                at.bin(l, &rest);
+                s.n = loss(rest);
+            }
         });
         __syncthreads();
         f.d = s.n;
@@ -274,9 +304,9 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
     // 3. its tokens, gathered and sorted
     gather(s, n, [&](auto put) {
         each_token<THREADS>(row, vocab, [&](float l, int i) {
-            double rest;
+            uint32_t rest;
             const uint32_t key = order_bits(l);
-            if (key >= lo && key <= hi && at.bin(l, &rest) == bin) put((unsigned long long)key << 32 | (uint32_t)~i);
+            if (l >= from && l <= to && key >= lo && key <= hi && at.bin(l, &rest) == bin) put((unsigned long long)key << 32 | (uint32_t)~i);
         });
     });
     static_assert(LIST == BINS && LIST == 2 * THREADS, "");
@@ -284,7 +314,7 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int x = tid * 2 + i;
-        double rest;
+        uint32_t rest;
         d[i] = 0;
         if (x < n) {
             at.bin(row[~(uint32_t)s.list[x]], &rest);
@@ -334,6 +364,16 @@ __device__ __forceinline__ Settings settings_of(const SampleParams &p, int r, bo
     return c;
 }
 
+__device__ __forceinline__ unsigned long long wave_most(unsigned long long v) {
+#pragma unroll
+    for (int o = 32; o; o /= 2) {
+        const unsigned long long w = (unsigned long long)__shfl_xor((uint32_t)(v >> 32), o, 64) << 32 |
+                                     (uint32_t)__shfl_xor((uint32_t)v, o, 64);
+        v = w > v ? w : v;
+    }
+    return v;
+}
+
 // The largest of some tokens, the first of equal ones: (order bits, ~index); a NaN above all.
 constexpr unsigned long long WITH_NAN = ~0ull;
 template <int T>
@@ -349,14 +389,10 @@ __device__ unsigned long long largest(const float *row, int n, int first, unsign
         }
     });
     unsigned long long v = nan ? WITH_NAN : (unsigned long long)best << 32 | (uint32_t)~(first + index);
-#pragma unroll
-    for (int o = 32; o; o /= 2) {
-        const unsigned long long w = (unsigned long long)__shfl_xor((uint32_t)(v >> 32), o, 64) << 32 |
-                                     (uint32_t)__shfl_xor((uint32_t)v, o, 64);
-        v = w > v ? w : v;
-    }
+    v = wave_most(v);
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
     __syncthreads();
+#pragma unroll
     for (int i = 0; i < T / 64; ++i) v = scratch[i] > v ? scratch[i] : v;
     __syncthreads();
     return v;
@@ -368,7 +404,7 @@ __device__ __forceinline__ float of_bits(uint32_t b) { return __uint_as_float((b
 template <int T>
 __device__ __forceinline__ void count_bins(unsigned long long *hist, const float *row, int n, const Place &at) {
     each_token<T>(row, n, [&](float l, int) {
-        double rest;
+        uint32_t rest;
         const int b = at.bin(l, &rest);
         if (b < BINS - 1) atomicAdd(&hist[b], (1ull << COUNT) | loss(rest));
     });
@@ -446,7 +482,11 @@ __device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &
     const int few = (int)s.before[cut + 1];
     if (few <= LIST) {
         bool listed = sl.n > 0;
-        for (int i = 0; i < sl.n; ++i) listed &= cut < sl.upto[((size_t)r * sl.n + i) * 2];
+        if (listed) {
+            const int lane = tid & 63;
+            const int32_t *q = sl.upto + (size_t)r * sl.n * 2;
+            listed = __all(cut < q[min(lane, sl.n - 1) * 2] && cut < q[min(lane + 64, sl.n - 1) * 2]);
+        }
         gather(s, few, [&](auto put) {
             if (listed) {
                 for (int i = tid / SLICE_LIST; i < sl.n; i += THREADS / SLICE_LIST) {
@@ -454,13 +494,14 @@ __device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &
                     const int k = tid % SLICE_LIST;
                     if (k >= sl.upto[x * 2 + 1]) continue;
                     const unsigned long long v = sl.list[x * SLICE_LIST + k];
-                    double rest;
+                    uint32_t rest;
                     if (at.bin(of_bits((uint32_t)(v >> 32)), &rest) <= cut) put(v);
                 }
             } else {
+                const float from = at.below(cut);
                 each_token<THREADS>(row, n, [&](float l, int i) {
-                    double rest;
-                    if (at.bin(l, &rest) <= cut) put((unsigned long long)order_bits(l) << 32 | (uint32_t)~i);
+                    uint32_t rest;
+                    if (l >= from && at.bin(l, &rest) <= cut) put((unsigned long long)order_bits(l) << 32 | (uint32_t)~i);
                 });
             }
         });
@@ -472,7 +513,7 @@ __device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &
             w[i] = 0.0;
             over[i] = false;
             if (x < few) {
-                double rest;
+                uint32_t rest;
                 const float l = of_bits((uint32_t)(s.list[x] >> 32));
                 const int b = at.bin(l, &rest);
                 w[i] = scale(b) * (double)((1u << UNIT) - loss(rest));
@@ -534,7 +575,7 @@ __device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &
         // (weights next to the border in 64 bits, the others by their bin)
         uint32_t k = 0;
         each_token<THREADS>(row, n, [&](float l, int) {
-            double rest;
+            uint32_t rest;
             const int b = at.bin(l, &rest);
             if (b == BINS - 1) return;
             if (fabs((double)b - far) > 2.0)
@@ -616,12 +657,11 @@ __global__ __launch_bounds__(SLICE_THREADS) void sample_best_kernel(SampleParams
 }
 
 __device__ __forceinline__ unsigned long long best_of(const SampleSlices &sl, int r) {
-    unsigned long long best = 0;
-    for (int i = 0; i < sl.n; ++i) {
-        const unsigned long long v = sl.best[(size_t)r * sl.n + i];
-        best = v > best ? v : best;
-    }
-    return best;
+    // (a lane two of them at most; by whole waves)
+    const int lane = threadIdx.x & 63;
+    const unsigned long long *p = sl.best + (size_t)r * sl.n;
+    const unsigned long long a = p[min(lane, sl.n - 1)], b = p[min(lane + 64, sl.n - 1)];
+    return wave_most(a > b ? a : b);
 }
 
 __global__ __launch_bounds__(SLICE_THREADS) void sample_bins_kernel(SampleParams p, SampleSlices sl) {
@@ -671,9 +711,10 @@ __global__ __launch_bounds__(SLICE_THREADS) void sample_bins_kernel(SampleParams
     }
     __syncthreads();
     const int upto = (int)last;
+    const float from = at.below(upto - 1);
     each_token<SLICE_THREADS>(row, len, [&](float l, int i) {
-        double rest;
-        if (at.bin(l, &rest) < upto) {
+        uint32_t rest;
+        if (l >= from && at.bin(l, &rest) < upto) {
             const uint32_t k = atomicAdd(&n, 1u);
             if (k < SLICE_LIST)
                 sl.list[x * SLICE_LIST + k] = (unsigned long long)order_bits(l) << 32 | (uint32_t)~(first + i);
@@ -694,10 +735,16 @@ __global__ __launch_bounds__(THREADS) void sample_finish_kernel(SampleParams p, 
     const unsigned long long best = best_of(sl, r);
     if (settled(p, r, c, best, true)) return;
     unsigned long long a = 0, b = 0;
-    for (int i = 0; i < sl.n; ++i) {
-        const unsigned long long *h = sl.hist + ((size_t)r * sl.n + i) * BINS + tid * 2;
-        a += h[0];
-        b += h[1];
+    const unsigned long long *h = sl.hist + (size_t)r * sl.n * BINS + tid * 2;
+    for (int i = 0; i < sl.n; i += 8) {
+        ulonglong2 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = *(const ulonglong2 *)(h + (size_t)min(i + k, sl.n - 1) * BINS);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            a += i + k < sl.n ? v[k].x : 0;
+            b += i + k < sl.n ? v[k].y : 0;
+        }
     }
     s.hist[tid * 2] = a;
     s.hist[tid * 2 + 1] = b;
