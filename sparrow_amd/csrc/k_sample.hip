@@ -7,28 +7,37 @@
 // the ones with w_j >= min_p. The token is the first whose weights up to it sum to more
 // than u times the kept ones'.
 //
-// Nothing is sorted but one bin: the distance x = (l_max - l) / T falls into bins of 1/64,
-// and every question (the k-th token, the mass p, the token drawn) is answered by the
-// bins' counts and masses down to one bin, whose few tokens are gathered and sorted.
-// 2048 bins reach weights of 2^-46; what lies behind has none.
+// Nothing is sorted but what can be kept: -l / T falls into bins of 1/64, and every question
+// (the k-th token, the mass p, the token drawn) is answered by the bins' counts and masses
+// down to one bin. Where the bins up to the last one that can matter hold few tokens, those are
+// gathered and sorted together; else one bin is, for each question. 2048 bins from the largest logit's
+// reach weights of 2^-46; what lies behind has none.
 //
 // Next to a border between two tokens 32 bits are too few: with 122753 tokens of like weight
-// a sum off by 2^-24 takes the neighbour's token once in 50 rows. So x is formed in 64 bits, and a
+// a sum off by 2^-24 takes the neighbour's token once in 50 rows. So l / T is formed in 64 bits, and a
 // token's weight is exp(-bin / 64) (1 - d), d = 1 - exp(-r) < 1/64 of the rest r, held as an
 // integer in units of 2^-30: a bin's sum of d and its count are one 64-bit atomic add in
-// LDS, whose order changes nothing.
+// LDS, whose order changes nothing. A token's bin and rest depend on its logit and T alone.
+//
+// A row is read once for its bins (a larger logit than those before moves them along), and once more,
+// by f32 comparisons, for the tokens to sort. Few rows are cut into slices, which also list the
+// tokens of their first bins, so that the second reading is seldom needed.
+#include <algorithm>
+
 #include "internal.hpp"
 
 namespace vmlm {
 namespace {
 
 constexpr int THREADS = 1024;
-constexpr int BINS = 2048;      // the last one's tokens have no weight
-constexpr int LIST = 2048;      // tokens that are sorted at once
-constexpr int SLICE_LIST = 256; // tokens of the first bins that a slice lists
-constexpr double PER = 64.0;    // bins of a distance of 1
-constexpr int UNIT = 30;        // d in units of 2^-30
-constexpr int COUNT = 44;       // a bin's word: count above, sum of d below
+constexpr int BINS = 2048;       // the last one's tokens have no weight
+constexpr int LIST = 2048;       // tokens that are sorted at once
+constexpr int SLICE_LIST = 256;  // tokens of the first bins that a slice lists
+constexpr double PER = 64.0;     // bins of a distance of 1
+constexpr int UNIT = 30;         // d in units of 2^-30
+constexpr int COUNT = 44;        // a bin's word: count above, sum of d below
+constexpr unsigned long long LOSSES = (1ull << COUNT) - 1;
+constexpr double TOO_FAR = 0x1p49;  // bins from 0: where f64 no longer holds a rest
 
 typedef float f32x4a __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -43,19 +52,39 @@ struct SampleParams {
     int *guard;
 };
 
-// Order-preserving bits of a logit (of numbers; -0 as 0).
+// Order-preserving bits of a logit (of numbers; -0 as 0), and back.
 __device__ __forceinline__ uint32_t order_bits(float v) {
     if (v == 0.0f) v = 0.0f;
     const uint32_t b = __float_as_uint(v);
     return (b >> 31) ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float of_bits(uint32_t b) {
+    return __uint_as_float((b >> 31) ? b ^ 0x80000000u : ~b);
+}
+// a token: (order bits, ~index), larger for the one that stands first
+__device__ __forceinline__ unsigned long long token_word(float l, int index) {
+    return (unsigned long long)order_bits(l) << 32 | (uint32_t)~index;
+}
 
-// A logit's place: its bin, and the rest of its distance as a fraction of a bin in units of
-// 2^-32. 2^20 added to the distance leaves both in the bits of the sum.
+// A logit's place: its bin from the reference on, and the rest as a fraction of a bin in
+// units of 2^-32. 2^20 in the sum leaves both in its bits.
 struct Place {
-    double max, per;  // PER / T
+    double per = 0.0, ref = 0.0;  // PER / T; the bin of -l / T that is bin 0
+    __device__ __forceinline__ Place() {}
+    __device__ __forceinline__ Place(float t, float max) {
+        per = PER / (double)t;
+        refer(max);
+    }
+    __device__ __forceinline__ void refer(float max) { ref = __builtin_floor(-(double)max * per); }
+    __device__ __forceinline__ bool too_far(float max) const { return !(fabs((double)max * per) < TOO_FAR); }
+    // T so small against the logits that only the largest one's equals can have a weight: a
+    // larger T that leaves f64 its rests says the same (the next logit is 2^25 bins away)
+    __device__ __forceinline__ void widen(float max) {
+        per = TOO_FAR / fabs((double)max);
+        refer(max);
+    }
     __device__ __forceinline__ int bin(float l, uint32_t *rest) const {
-        const double y = __builtin_fma(max - (double)l, per, 0x1p20);  // (+inf for a masked one)
+        const double y = (-(double)l * per) + (0x1p20 - ref);  // (+inf for a masked one)
         const unsigned long long b = __builtin_bit_cast(unsigned long long, y);
         *rest = (uint32_t)b;
         return (int)min((uint32_t)(b >> 32) - 0x41300000u, (uint32_t)(BINS - 1));
@@ -63,10 +92,12 @@ struct Place {
     // Logits below this one are not in bin b or before it; above it, not in bin b or behind it.
     // (f32: by a part of a bin, and where a bin is narrower than its steps by a few of those)
     __device__ __forceinline__ float below(int b) const {
-        return (float)(max - ((double)b + 1.02) / per - fabs(max) * 0x1p-21);
+        const double l = -(ref + (double)b + 1.02) / per;
+        return (float)(l - fabs(l) * 0x1p-21);
     }
     __device__ __forceinline__ float above(int b) const {
-        return (float)(max - ((double)b - 0.02) / per + fabs(max) * 0x1p-21);
+        const double l = -(ref + (double)b - 0.02) / per;
+        return (float)(l + fabs(l) * 0x1p-21);
     }
 };
 // 1 - exp(-r) of the rest r = f 2^-38 < 2^-6, in units of 2^-30, off by at most one: r itself
@@ -76,35 +107,57 @@ __device__ __forceinline__ uint32_t loss(uint32_t f) {
     const float q = r * r * __builtin_fmaf(__builtin_fmaf(r, 1.0f / 24, -1.0f / 6), r, 0.5f);
     return (uint32_t)((f >> 8) + (f >> 7 & 1)) - (uint32_t)(int)rintf(q * 0x1p30f);
 }
+__device__ __forceinline__ void count_token(unsigned long long *hist, const Place &at, float l) {
+    uint32_t rest;
+    const int b = at.bin(l, &rest);
+    if (b < BINS - 1) atomicAdd(&hist[b], (1ull << COUNT) | loss(rest));
+}
 
-// Calls f(logit, index) for the tokens [0, n) at `row`: 16 of a thread at a time, loaded
-// before the first is used. T: threads.
-template <int T, typename F>
-__device__ __forceinline__ void each_token(const float *row, int n, F f) {
-    int i = threadIdx.x * 4;
-    for (; i + 3 + 3 * T * 4 < n; i += 4 * T * 4) {
-        f32x4a v[4];
+// 16 of a thread's tokens of the T * 16 from `first` on: 4 times 4 neighbours; those from n on
+// are -inf.
+template <int T>
+struct Tokens {
+    f32x4a v[4];
+    __device__ __forceinline__ static int index(int k) { return (threadIdx.x + k * T) * 4; }
+    __device__ __forceinline__ void load(const float *row, int first, int n) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = *(const f32x4a *)(row + i + k * T * 4);
+        for (int k = 0; k < 4; ++k) {
+            const int i = first + index(k);
+            if (i + 3 < n) {
+                v[k] = *(const f32x4a *)(row + i);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k][e] = i + e < n ? row[i + e] : -__builtin_inff();
+            }
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(int first, F f) const {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f(v[k][e], i + k * T * 4 + e);
+            for (int e = 0; e < 4; ++e) f(v[k][e], first + index(k) + e);
     }
-    for (; i + 3 < n; i += T * 4) {
-        const f32x4a v = *(const f32x4a *)(row + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f(v[e], i + e);
+};
+// Calls f(logit, index) for every token of a row (and, past its end, with -inf).
+template <int T, typename F>
+__device__ __forceinline__ void each_token(const float *row, int n, F f) {
+    Tokens<T> a;
+    a.load(row, 0, n);
+    for (int first = 0; first < n; first += T * 16) {
+        const Tokens<T> now = a;
+        if (first + T * 16 < n) a.load(row, first + T * 16, n);
+        now.each(first, f);
     }
-    for (; i < n; ++i) f(row[i], i);
 }
 
 struct Shared {
-    unsigned long long hist[BINS];  // counts and losses; then, in a bin, of key ranges, and up to a token
+    unsigned long long hist[BINS];  // counts and losses; what is to be sorted; weights
     double above[BINS];             // the mass before a bin
     uint32_t before[BINS];          // the tokens before a bin
-    unsigned long long list[LIST];  // (order bits, ~index), the largest first
+    unsigned long long list[LIST];  // tokens, the largest first
     uint32_t rank[512];
+    double whole[32], part[64];     // exp(-i), exp(-i / 64)
     double red[16];
     unsigned long long wave64[16];
     unsigned long long best;
@@ -112,19 +165,37 @@ struct Shared {
     uint32_t wave[16];
 };
 
-// Block-wide exclusive prefix sums over 2 values a thread.
+__device__ __forceinline__ unsigned long long shfl_xor64(unsigned long long v, int o) {
+    return (unsigned long long)__shfl_xor((uint32_t)(v >> 32), o, 64) << 32 | (uint32_t)__shfl_xor((uint32_t)v, o, 64);
+}
+__device__ __forceinline__ unsigned long long wave_most(unsigned long long v) {
+#pragma unroll
+    for (int o = 32; o; o /= 2) {
+        const unsigned long long w = shfl_xor64(v, o);
+        v = w > v ? w : v;
+    }
+    return v;
+}
 template <typename T>
-__device__ T block_scan(T a, T b, T *out_a, T *out_b, T *scratch) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    T to = a + b;
+__device__ __forceinline__ T wave_scan(T v) {  // inclusive
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
-        const T v = __shfl_up(to, o, 64);
-        if (lane >= o) to = to + v;
+        const T w = __shfl_up(v, o, 64);
+        if (lane >= o) v = v + w;
     }
+    return v;
+}
+
+// Block-wide exclusive prefix sums over 2 values a thread; the sum of all.
+template <typename T>
+__device__ __forceinline__ T block_scan(T a, T b, T *out_a, T *out_b, T *scratch) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const T to = wave_scan<T>(a + b);
     if (lane == 63) scratch[w] = to;
     __syncthreads();
     T base = 0, all = 0;
+#pragma unroll
     for (int i = 0; i < THREADS / 64; ++i) {
         if (i == w) base = all;
         all = all + scratch[i];
@@ -136,11 +207,63 @@ __device__ T block_scan(T a, T b, T *out_a, T *out_b, T *scratch) {
     return all;
 }
 
-// The n <= LIST tokens that `each` puts, (order bits, ~index), in s.list: the largest first. Up
-// to 512 by the number of larger ones, which as many threads as there are count together
-// (256 tokens: 64 reads each, where a sort of them has 36 steps); more by a bitonic sort.
+// A row's settings. live: there is something to draw.
+struct Settings {
+    float u, t, top_p, min_p;
+    int top_k;
+    bool live;
+};
+__device__ __forceinline__ Settings settings_of(const SampleParams &p, int r, bool report) {
+    Settings c;
+    c.u = p.u[r];
+    c.t = p.t[r];
+    c.top_p = p.top_p ? p.top_p[r] : 1.0f;
+    c.min_p = p.min_p ? p.min_p[r] : 0.0f;
+    c.top_k = p.top_k ? p.top_k[r] : 0;
+    const bool ok = c.u < 1.0f && c.t >= 0.0f && c.t <= 3.40282347e38f && c.top_p == c.top_p &&
+                    c.min_p >= 0.0f && c.min_p <= 1.0f;
+    c.live = ok && c.u >= 0.0f;
+    if (!ok && !(c.u < 0.0f) && report && threadIdx.x == 0) atomicOr(p.guard, 1);
+    return c;
+}
+
+// What there is to say of a row whose first token is known (WITH_NAN: it has a NaN); true if
+// nothing else is.
+constexpr unsigned long long WITH_NAN = ~0ull;
+__device__ __forceinline__ bool settled(const SampleParams &p, int r, const Settings &c, unsigned long long best) {
+    const float max = of_bits((uint32_t)(best >> 32));
+    int token = -1;
+    float prob;
+    if (best == WITH_NAN || max == __builtin_inff())
+        prob = __builtin_nanf("");
+    else if (max == -__builtin_inff())
+        prob = 0.0f;  // the mask leaves no token
+    else if (c.t == 0.0f) {
+        token = (int)~(uint32_t)best;
+        prob = 1.0f;
+    } else
+        return false;
+    if (threadIdx.x == 0) {
+        p.token[r] = token;
+        if (p.prob) p.prob[r] = prob;
+    }
+    return true;
+}
+
+// What the slices of a row leave for its last kernel.
+struct SampleSlices {
+    int n;                     // a row's
+    unsigned long long *best;  // [rows][n] the first token
+    unsigned long long *hist;  // [rows][n][BINS], bins from the slice's largest logit's on
+    unsigned long long *list;  // [rows][n][SLICE_LIST] the tokens of the first bins
+    int32_t *upto;             // [rows][n][2]: those below this bin, and their number
+};
+
+// The n <= LIST tokens that `each` puts, in s.list: the largest first. Up to 512 by the number
+// of larger ones, which as many threads as there are count together (256 tokens: 64 reads
+// each, where a sort has 36 steps); more by a bitonic sort.
 template <typename F>
-__device__ void gather(Shared &s, int n, F each) {
+__device__ __forceinline__ void gather(Shared &s, int n, F each) {
     const int tid = threadIdx.x;
     const bool count = n <= 512;
     unsigned long long *raw = count ? s.hist : s.list;
@@ -157,11 +280,11 @@ __device__ void gather(Shared &s, int n, F each) {
     });
     __syncthreads();
     if (count) {
-        const int parts = THREADS / pow2, x = tid % pow2, each_part = pow2 / parts, a = tid / pow2 * each_part;
+        const int parts = THREADS / pow2, x = tid % pow2, some = pow2 / parts, a = tid / pow2 * some;
         const unsigned long long v = raw[x];
         uint32_t larger = 0;
-        for (int i = a; i < a + each_part; ++i) larger += raw[i] > v;
-        if (larger) atomicAdd(&s.rank[x], larger);
+        for (int i = a; i < a + some; ++i) larger += raw[i] > v;
+        if (larger && x < n) atomicAdd(&s.rank[x], larger);
         __syncthreads();
         if (tid < n) s.list[s.rank[tid]] = raw[tid];
         __syncthreads();
@@ -191,13 +314,20 @@ struct Found {
 
 // The token of rank `rank` in bin `bin` (by_rank), else the first one with weights up to it of
 // more than `mass` (or, with_equal, as much). `n`: the bin's tokens.
-__device__ Found locate(Shared &s, const float *row, int vocab, const Place &at, int bin, int n,
-                        bool by_rank, uint32_t rank, double mass, bool with_equal) {
+__device__ __forceinline__ Found locate(Shared &s, const float *row, int vocab, const Place &at, int bin, int n,
+                                        bool by_rank, uint32_t rank, double mass, bool with_equal) {
     const int tid = threadIdx.x;
     uint32_t lo = 0, hi = 0xffffffffu;  // of the order bits
     const float from = at.below(bin), to = at.above(bin);
-    uint32_t rank0 = 0;                 // the bin's tokens above them, and their weights
+    uint32_t rank0 = 0;  // the bin's tokens above them, and their weights
     unsigned long long mass0 = 0;
+    auto each_of_bin = [&](auto f) {
+        each_token<THREADS>(row, vocab, [&](float l, int i) {
+            uint32_t rest;
+            const uint32_t key = order_bits(l);
+            if (l >= from && l <= to && key >= lo && key <= hi && at.bin(l, &rest) == bin) f(key, rest, i);
+        });
+    };
     // 1. a bin of too many tokens: ranges of their order bits, the narrowest that hold the place
     while (n > LIST && lo < hi) {
         __syncthreads();
@@ -207,13 +337,9 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         }
         for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
         __syncthreads();
-        each_token<THREADS>(row, vocab, [&](float l, int) {
-            uint32_t rest;
-            const uint32_t key = order_bits(l);
-            if (l >= from && l <= to && at.bin(l, &rest) == bin && key >= lo && key <= hi) {
-                atomicMin(&s.lo, key);
-                atomicMax(&s.hi, key);
-            }
+        each_of_bin([&](uint32_t key, uint32_t, int) {
+            atomicMin(&s.lo, key);
+            atomicMax(&s.hi, key);
         });
         __syncthreads();
         lo = s.lo;
@@ -221,30 +347,22 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         if (lo == hi) break;
         int shift = 0;
         while ((hi - lo) >> shift >= BINS) ++shift;
-        each_token<THREADS>(row, vocab, [&](float l, int) {
-            uint32_t rest;
-            const uint32_t key = order_bits(l);
-            if (l >= from && l <= to && at.bin(l, &rest) == bin && key >= lo && key <= hi)
-                atomicAdd(&s.hist[(hi - key) >> shift], (1ull << COUNT) | loss(rest));
+        each_of_bin([&](uint32_t key, uint32_t rest, int) {
+            atomicAdd(&s.hist[(hi - key) >> shift], (1ull << COUNT) | loss(rest));
         });
         __syncthreads();
         if (tid == 0) {
-            uint32_t r = rank0;
-            unsigned long long m = mass0;
-            int i = 0, last = 0;
-            uint32_t rl = r;
-            unsigned long long ml = m;
-            for (; i < BINS; ++i) {  // the last range that is not empty where none reaches it
+            uint32_t r = rank0, rl = rank0;
+            unsigned long long m = mass0, ml = mass0;
+            int last = 0;
+            for (int i = 0; i < BINS; ++i) {  // the last range that is not empty where none reaches it
                 const uint32_t c = (uint32_t)(s.hist[i] >> COUNT);
                 if (c == 0) continue;
-                const unsigned long long w =
-                    ((unsigned long long)c << UNIT) - (s.hist[i] & ((1ull << COUNT) - 1));
+                const unsigned long long w = ((unsigned long long)c << UNIT) - (s.hist[i] & LOSSES);
                 last = i;
                 rl = r;
                 ml = m;
-                if (by_rank ? r + c > rank
-                            : with_equal ? (double)(m + w) >= mass : (double)(m + w) > mass)
-                    break;
+                if (by_rank ? r + c > rank : with_equal ? (double)(m + w) >= mass : (double)(m + w) > mass) break;
                 r += c;
                 m += w;
             }
@@ -253,30 +371,20 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
             s.best = ml;
         }
         __syncthreads();
-        const int i = (int)s.n;
+        const uint32_t i = s.n, span = hi - lo;
         rank0 = s.wave[0];
         mass0 = s.best;
         n = (int)(s.hist[i] >> COUNT);
-        const uint32_t top = hi - ((uint32_t)i << shift);
-        const uint32_t bottom = hi - (uint32_t)min((((unsigned long long)i + 1) << shift) - 1, (unsigned long long)(hi - lo));
-        hi = top;
-        lo = bottom;
+        const unsigned long long end = (((unsigned long long)i + 1) << shift) - 1;
+        lo = hi - (uint32_t)min(end, (unsigned long long)span);
+        hi = hi - (i << shift);
         __syncthreads();
     }
     Found f;
     if (n > LIST) {  // 2. so many equal ones: the place is arithmetic, its index a count
-        __syncthreads();
-        if (tid == 0) s.n = 0;
-        __syncthreads();
-        each_token<THREADS>(row, vocab, [&](float l, int) {
-            uint32_t rest;
-            if (order_bits(l) == lo) {
-                at.bin(l, &rest);
-                s.n = loss(rest);
-            }
-        });
-        __syncthreads();
-        f.d = s.n;
+        uint32_t rest;
+        at.bin(of_bits(lo), &rest);
+        f.d = loss(rest);
         const double w = (double)((1ull << UNIT) - f.d);
         uint32_t k;
         if (by_rank) {
@@ -303,11 +411,7 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
     }
     // 3. its tokens, gathered and sorted
     gather(s, n, [&](auto put) {
-        each_token<THREADS>(row, vocab, [&](float l, int i) {
-            uint32_t rest;
-            const uint32_t key = order_bits(l);
-            if (l >= from && l <= to && key >= lo && key <= hi && at.bin(l, &rest) == bin) put((unsigned long long)key << 32 | (uint32_t)~i);
-        });
+        each_of_bin([&](uint32_t key, uint32_t, int i) { put((unsigned long long)key << 32 | (uint32_t)~i); });
     });
     static_assert(LIST == BINS && LIST == 2 * THREADS, "");
     unsigned long long *sum = s.hist, d[2], e[2];
@@ -317,7 +421,7 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         uint32_t rest;
         d[i] = 0;
         if (x < n) {
-            at.bin(row[~(uint32_t)s.list[x]], &rest);
+            at.bin(of_bits((uint32_t)(s.list[x] >> 32)), &rest);
             d[i] = loss(rest);
         }
     }
@@ -330,8 +434,7 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
         if (x >= n) continue;
         sum[x] = e[i] + d[i];
         const unsigned long long w = mass0 + ((unsigned long long)(x + 1) << UNIT) - (e[i] + d[i]);
-        const bool hit = by_rank ? rank0 + x == rank
-                                 : with_equal ? (double)w >= mass : (double)w > mass;
+        const bool hit = by_rank ? rank0 + x == rank : with_equal ? (double)w >= mass : (double)w > mass;
         if (hit) atomicMin(&s.lo, (uint32_t)x);
     }
     __syncthreads();
@@ -344,103 +447,22 @@ __device__ Found locate(Shared &s, const float *row, int vocab, const Place &at,
     return f;
 }
 
-// A row's settings. live: there is something to draw.
-struct Settings {
-    float u, t, top_p, min_p;
-    int top_k;
-    bool live;
-};
-__device__ __forceinline__ Settings settings_of(const SampleParams &p, int r, bool report) {
-    Settings c;
-    c.u = p.u[r];
-    c.t = p.t[r];
-    c.top_p = p.top_p ? p.top_p[r] : 1.0f;
-    c.min_p = p.min_p ? p.min_p[r] : 0.0f;
-    c.top_k = p.top_k ? p.top_k[r] : 0;
-    const bool ok = c.u < 1.0f && c.t >= 0.0f && c.t <= 3.40282347e38f && c.top_p == c.top_p &&
-                    c.min_p >= 0.0f && c.min_p <= 1.0f;
-    c.live = ok && c.u >= 0.0f;
-    if (!ok && !(c.u < 0.0f) && report && threadIdx.x == 0) atomicOr(p.guard, 1);
-    return c;
-}
-
-__device__ __forceinline__ unsigned long long wave_most(unsigned long long v) {
-#pragma unroll
-    for (int o = 32; o; o /= 2) {
-        const unsigned long long w = (unsigned long long)__shfl_xor((uint32_t)(v >> 32), o, 64) << 32 |
-                                     (uint32_t)__shfl_xor((uint32_t)v, o, 64);
-        v = w > v ? w : v;
-    }
-    return v;
-}
-
-// The largest of some tokens, the first of equal ones: (order bits, ~index); a NaN above all.
-constexpr unsigned long long WITH_NAN = ~0ull;
-template <int T>
-__device__ unsigned long long largest(const float *row, int n, int first, unsigned long long *scratch) {
-    uint32_t best = 0, index = 0;
-    bool nan = false;
-    each_token<T>(row, n, [&](float l, int i) {
-        nan |= l != l;
-        const uint32_t key = order_bits(l);
-        if (key > best) {
-            best = key;
-            index = i;
-        }
-    });
-    unsigned long long v = nan ? WITH_NAN : (unsigned long long)best << 32 | (uint32_t)~(first + index);
-    v = wave_most(v);
-    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < T / 64; ++i) v = scratch[i] > v ? scratch[i] : v;
-    __syncthreads();
-    return v;
-}
-// the logit that the order bits came from
-__device__ __forceinline__ float of_bits(uint32_t b) { return __uint_as_float((b >> 31) ? b ^ 0x80000000u : ~b); }
-
-// Counts and losses of some tokens into the bins.
-template <int T>
-__device__ __forceinline__ void count_bins(unsigned long long *hist, const float *row, int n, const Place &at) {
-    each_token<T>(row, n, [&](float l, int) {
-        uint32_t rest;
-        const int b = at.bin(l, &rest);
-        if (b < BINS - 1) atomicAdd(&hist[b], (1ull << COUNT) | loss(rest));
-    });
-}
-
-// What the slices of a row leave for its last kernel.
-struct SampleSlices {
-    int n, each;                     // their number and tokens
-    unsigned long long *best;        // [rows][n] the largest token
-    unsigned long long *hist;        // [rows][n][BINS]
-    unsigned long long *list;        // [rows][n][SLICE_LIST] the tokens of the first bins
-    int32_t *upto;                   // [rows][n][2]: those below this bin, and their number
-};
-
-// 3. The rest, from a row's bins in s.hist: by one workgroup.
-__device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &c, float first,
-                       const SampleSlices &sl) {
-    const int tid = threadIdx.x, n = p.vocab;
+// The rest, from a row's bins in s.hist, by one workgroup. sl.n 0: no slices. `max`: the largest logit.
+__device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, const Settings &c, float max,
+                                       const Place &at, const SampleSlices &sl) {
+    const int tid = threadIdx.x, lane = tid & 63, n = p.vocab;
     const float *row = p.logits + r * p.ld;
-    const float u = c.u, t = c.t;
-    auto answer = [&](int token, float prob) {
-        if (tid == 0) {
-            p.token[r] = token;
-            if (p.prob) p.prob[r] = prob;
-        }
-    };
-    const Place at{(double)first, PER / (double)t};
+    if (tid < 32) s.whole[tid] = exp(-(double)tid);
+    if (tid >= 64 && tid < 128) s.part[tid - 64] = exp(-(tid - 64) / PER) * (1.0 / (1 << UNIT));
+    __syncthreads();
+    auto scale = [&](int b) { return s.whole[b >> 6] * s.part[b & 63]; };  // of a bin's units
     uint32_t cnt[2], c0[2];
     double mass[2], m0[2];
-    const double unit = 1.0 / (1 << UNIT);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const unsigned long long h = s.hist[tid * 2 + i];
         cnt[i] = (uint32_t)(h >> COUNT);
-        mass[i] = exp(-(tid * 2 + i) / PER) * unit *
-                  (double)(((unsigned long long)cnt[i] << UNIT) - (h & ((1ull << COUNT) - 1)));
+        mass[i] = scale(tid * 2 + i) * (double)(((unsigned long long)cnt[i] << UNIT) - (h & LOSSES));
     }
     const uint32_t live = block_scan<uint32_t>(cnt[0], cnt[1], &c0[0], &c0[1], s.wave);
     double all = block_scan<double>(mass[0], mass[1], &m0[0], &m0[1], s.red);
@@ -451,7 +473,6 @@ __device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &
     }
     __syncthreads();
     auto tokens = [&](int b) { return (int)((b + 1 < BINS ? s.before[b + 1] : live) - s.before[b]); };
-    auto scale = [&](int b) { return exp(-b / PER) * unit; };
     // the bin of a rank, and of a mass (the last one that is not empty and starts below it)
     auto bin_of_rank = [&](uint32_t rank) {
         int b = 0;
@@ -469,21 +490,22 @@ __device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &
     };
     uint32_t kept = live;
     const bool by_k = c.top_k > 0 && (uint32_t)c.top_k < live;
-    const double far = -log((double)c.min_p) * PER;  // min_p's place (+inf: none)
+    // min_p's place, from the largest logit's bin on (behind all bins: none)
+    const double far = c.min_p > 0.0f ? -log((double)c.min_p) * PER + 1.0 : 2.0 * BINS;
+    auto over_min = [&](float l) { return exp(((double)l - (double)max) / (double)c.t) >= (double)c.min_p; };
 
     // The bins up to which tokens can be kept: where they hold few, those are sorted
     // together and every question is one of their sums.
     int cut = BINS - 2;
     if (by_k) cut = bin_of_rank((uint32_t)c.top_k - 1);
     if (!(by_k && c.top_p < 1.0f)) {  // (p is of the k's weight)
-        if (c.top_p < 1.0f) cut = bin_of_mass((double)c.top_p * all, true);
+        if (c.top_p < 1.0f) cut = min(cut, bin_of_mass((double)c.top_p * all, true));
         if (far < cut) cut = (int)far + 1;
     }
     const int few = (int)s.before[cut + 1];
     if (few <= LIST) {
         bool listed = sl.n > 0;
         if (listed) {
-            const int lane = tid & 63;
             const int32_t *q = sl.upto + (size_t)r * sl.n * 2;
             listed = __all(cut < q[min(lane, sl.n - 1) * 2] && cut < q[min(lane + 64, sl.n - 1) * 2]);
         }
@@ -492,46 +514,50 @@ __device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &
                 for (int i = tid / SLICE_LIST; i < sl.n; i += THREADS / SLICE_LIST) {
                     const size_t x = (size_t)r * sl.n + i;
                     const int k = tid % SLICE_LIST;
-                    if (k >= sl.upto[x * 2 + 1]) continue;
                     const unsigned long long v = sl.list[x * SLICE_LIST + k];
                     uint32_t rest;
-                    if (at.bin(of_bits((uint32_t)(v >> 32)), &rest) <= cut) put(v);
+                    if (k < sl.upto[x * 2 + 1] && at.bin(of_bits((uint32_t)(v >> 32)), &rest) <= cut) put(v);
                 }
             } else {
                 const float from = at.below(cut);
                 each_token<THREADS>(row, n, [&](float l, int i) {
                     uint32_t rest;
-                    if (l >= from && at.bin(l, &rest) <= cut) put((unsigned long long)order_bits(l) << 32 | (uint32_t)~i);
+                    if (l >= from && at.bin(l, &rest) <= cut) put(token_word(l, i));
                 });
             }
         });
-        double w[2], up[2];
-        bool over[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int x = tid * 2 + i;
-            w[i] = 0.0;
-            over[i] = false;
-            if (x < few) {
-                uint32_t rest;
-                const float l = of_bits((uint32_t)(s.list[x] >> 32));
-                const int b = at.bin(l, &rest);
-                w[i] = scale(b) * (double)((1u << UNIT) - loss(rest));
-                over[i] = c.min_p == 0.0f || exp(((double)l - at.max) / (double)t) >= (double)c.min_p;
-            }
+        double *w = (double *)s.hist;  // weights
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        for (int x = tid; x < few; x += THREADS) {
+            uint32_t rest;
+            const float l = of_bits((uint32_t)(s.list[x] >> 32));
+            const int b = at.bin(l, &rest);
+            w[x] = scale(b) * (double)((1u << UNIT) - loss(rest));
+            if (c.min_p > 0.0f && over_min(l)) atomicAdd(&s.n, 1u);
         }
-        block_scan<double>(w[0], w[1], &up[0], &up[1], s.red);  // weights before a token
-        // counts of a condition that holds up to some token
-        auto upto = [&](bool a, bool b) {
-            uint32_t x, y;
-            return block_scan<uint32_t>(a, b, &x, &y, s.wave);
+        __syncthreads();
+        if (tid >= 64) return;
+        // the first wave: some neighbouring tokens a lane
+        const int some = (few + 63) / 64, x0 = min(lane * some, few), x1 = min(x0 + some, few);
+        double mine = 0.0;
+        for (int x = x0; x < x1; ++x) mine += w[x];
+        double base = __shfl_up(wave_scan<double>(mine), 1, 64);  // the weights before the lane's
+        if (lane == 0) base = 0.0;
+        // the tokens for which f(weights before it, its own) holds, up to some token
+        auto upto = [&](auto f) {
+            uint32_t k = 0;
+            double up = base;
+            for (int x = x0; x < x1; ++x) {
+                k += f(up, w[x]);
+                up += w[x];
+            }
+            return __shfl(wave_scan<uint32_t>(k), 63, 64);
         };
         auto sum_upto = [&](uint32_t k) {  // of the first k > 0
-            if (tid == (int)(k - 1) / 2) s.red[0] = (k - 1) % 2 ? up[1] + w[1] : up[0] + w[0];
-            __syncthreads();
-            const double v = s.red[0];
-            __syncthreads();
-            return v;
+            double up = base;
+            for (int x = x0; x < x1 && x < (int)k; ++x) up += w[x];
+            return __shfl(up, (int)(k - 1) / some, 64);
         };
         kept = (uint32_t)few;
         if (by_k && c.top_k <= few) {
@@ -540,151 +566,210 @@ __device__ void finish(Shared &s, const SampleParams &p, int r, const Settings &
         }
         if (c.top_p < 1.0f) {
             const double goal = (double)c.top_p * all;
-            kept = min(kept, max(1u, upto(tid * 2 < few && up[0] < goal, tid * 2 + 1 < few && up[1] < goal)));
+            kept = min(kept, std::max(1u, upto([&](double up, double) { return up < goal; })));
         }
-        if (c.min_p > 0.0f) kept = min(kept, max(1u, upto(over[0], over[1])));
+        if (c.min_p > 0.0f) kept = min(kept, std::max(1u, s.n));
         all = sum_upto(kept);
-        const double goal = (double)u * all;
-        const uint32_t x = min(upto(tid * 2 < few && up[0] + w[0] <= goal, tid * 2 + 1 < few && up[1] + w[1] <= goal),
-                               kept - 1);
-        if (tid == (int)x / 2) {
+        const double goal = (double)c.u * all;
+        const uint32_t x = min(upto([&](double up, double v) { return up + v <= goal; }), kept - 1);
+        if (lane == 0) {
             p.token[r] = (int)~(uint32_t)s.list[x];
-            if (p.prob) p.prob[r] = (float)((x % 2 ? w[1] : w[0]) / all);
+            if (p.prob) p.prob[r] = (float)(w[x] / all);
         }
         return;
     }
 
-    // Else each question by its bin.
-    if (by_k) {
-        kept = (uint32_t)c.top_k;
-        const int b = bin_of_rank(kept - 1);
-        const Found f = locate(s, row, n, at, b, tokens(b), true, kept - 1 - s.before[b], 0.0, false);
-        all = s.above[b] + scale(b) * (double)f.upto;
-    }
-    if (c.top_p < 1.0f) {
-        const double goal = (double)c.top_p * all;
-        const int b = bin_of_mass(goal, true);
-        const Found f = locate(s, row, n, at, b, tokens(b), false, 0, (goal - s.above[b]) / scale(b), true);
-        const uint32_t k = s.before[b] + f.rank + 1;
-        if (k < kept) {
+    // Else each question by its bin, one after the other.
+    for (int question = 0; question < 5; ++question) {
+        int b;
+        bool by_rank = false, with_equal = false;
+        uint32_t rank = 0;
+        double goal = 0.0;
+        if (question == 0) {  // the k-th
+            if (!by_k) continue;
+            kept = (uint32_t)c.top_k;
+            by_rank = true;
+        } else if (question == 1) {  // p of their weight
+            if (!(c.top_p < 1.0f)) continue;
+            goal = (double)c.top_p * all;
+            with_equal = true;
+        } else if (question == 2) {  // min_p: weights next to the border in 64 bits, others by their bin
+            if (c.min_p == 0.0f) continue;
+            uint32_t k = 0;
+            each_token<THREADS>(row, n, [&](float l, int) {
+                uint32_t rest;
+                const int bin = at.bin(l, &rest);
+                if (bin == BINS - 1) return;
+                k += fabs((double)bin - far) > 3.0 ? (double)bin < far : over_min(l);
+            });
+            __syncthreads();
+            if (tid == 0) s.n = 0;
+            __syncthreads();
+            atomicAdd(&s.n, k);
+            __syncthreads();
+            k = std::max(1u, s.n);
+            __syncthreads();
+            if (k >= kept) continue;
             kept = k;
-            all = s.above[b] + scale(b) * (double)f.upto;
+            by_rank = true;
+        } else if (question == 3) {  // the token
+            goal = (double)c.u * all;
+        } else {  // a rounding put the goal behind the last one
+            by_rank = true;
         }
-    }
-    if (c.min_p > 0.0f) {
-        // (weights next to the border in 64 bits, the others by their bin)
-        uint32_t k = 0;
-        each_token<THREADS>(row, n, [&](float l, int) {
-            uint32_t rest;
-            const int b = at.bin(l, &rest);
-            if (b == BINS - 1) return;
-            if (fabs((double)b - far) > 2.0)
-                k += (double)b < far;
-            else
-                k += exp(((double)l - at.max) / (double)t) >= (double)c.min_p;
-        });
-        if (tid == 0) s.n = 0;
-        __syncthreads();
-        atomicAdd(&s.n, k);
-        __syncthreads();
-        k = s.n;
-        __syncthreads();
-        if (k < kept) {
-            kept = k;
-            const int b = bin_of_rank(kept - 1);
-            const Found f = locate(s, row, n, at, b, tokens(b), true, kept - 1 - s.before[b], 0.0, false);
+        b = by_rank ? bin_of_rank(kept - 1) : bin_of_mass(goal, with_equal);
+        if (by_rank) rank = kept - 1 - s.before[b];
+        const Found f = locate(s, row, n, at, b, tokens(b), by_rank, rank, (goal - s.above[b]) / scale(b), with_equal);
+        const uint32_t upto = s.before[b] + f.rank + 1;
+        if (question < 3) {
+            if (question == 1 && upto >= kept) continue;
+            kept = upto;
             all = s.above[b] + scale(b) * (double)f.upto;
+            continue;
         }
+        if (question == 3 && upto > kept) continue;
+        if (tid == 0) {
+            p.token[r] = (int)f.token;
+            if (p.prob) p.prob[r] = (float)(scale(b) * (double)((1u << UNIT) - f.d) / all);
+        }
+        return;
     }
-    const double goal = (double)u * all;
-    int b = bin_of_mass(goal, false);
-    Found f = locate(s, row, n, at, b, tokens(b), false, 0, (goal - s.above[b]) / scale(b), false);
-    if (s.before[b] + f.rank >= kept) {  // (a rounding put the goal behind the last one)
-        b = bin_of_rank(kept - 1);
-        f = locate(s, row, n, at, b, tokens(b), true, kept - 1 - s.before[b], 0.0, false);
-    }
-    answer((int)f.token, (float)(scale(b) * (double)((1u << UNIT) - f.d) / all));
 }
 
-// What there is to say of a row whose largest token is known; true if nothing else is.
-__device__ __forceinline__ bool settled(const SampleParams &p, int r, const Settings &c, unsigned long long best,
-                                        bool write) {
-    const float max = of_bits((uint32_t)(best >> 32));
-    int token = -1;
-    float prob;
-    if (best == WITH_NAN || max == __builtin_inff())
-        prob = __builtin_nanf("");
-    else if (max == -__builtin_inff())
-        prob = 0.0f;  // the mask leaves no token
-    else if (c.t == 0.0f) {
-        token = (int)~(uint32_t)best;
-        prob = 1.0f;
-    } else
-        return false;
-    if (write && threadIdx.x == 0) {
-        p.token[r] = token;
-        if (p.prob) p.prob[r] = prob;
-    }
-    return true;
+// The first token of a row or a slice, by its workgroup.
+template <int T>
+__device__ __forceinline__ unsigned long long most_of(unsigned long long v, unsigned long long *scratch) {
+    v = wave_most(v);
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < T / 64; ++i) v = scratch[i] > v ? scratch[i] : v;
+    __syncthreads();
+    return v;
 }
 
-// A workgroup a row.
-__global__ __launch_bounds__(THREADS) void sample_row_kernel(SampleParams p) {
+// The bins of a whole row whose largest logit is known.
+__device__ __forceinline__ void count_row(Shared &s, const float *row, int n, const Place &at) {
+    for (int i = threadIdx.x; i < BINS; i += THREADS) s.hist[i] = 0;
+    __syncthreads();
+    each_token<THREADS>(row, n, [&](float l, int) { count_token(s.hist, at, l); });
+    __syncthreads();
+}
+
+// A workgroup a row; two of them on a CU.
+__global__ __launch_bounds__(THREADS, 8) void sample_row_kernel(SampleParams p) {
     __shared__ Shared s;
-    const int r = blockIdx.x;
+    const int r = blockIdx.x, tid = threadIdx.x, n = p.vocab;
     const Settings c = settings_of(p, r, true);
     if (!c.live) return;
     const float *row = p.logits + r * p.ld;
-    for (int i = threadIdx.x; i < BINS; i += THREADS) s.hist[i] = 0;
-    const unsigned long long best = largest<THREADS>(row, p.vocab, 0, s.wave64);
-    if (settled(p, r, c, best, true)) return;
+    for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
+    unsigned long long best = 0;  // (without the index where T > 0)
+    Place at;
+    bool lost = false;
+    Tokens<THREADS> next;
+    next.load(row, 0, n);
+    for (int first = 0; first < n; first += THREADS * 16) {
+        const Tokens<THREADS> now = next;
+        if (first + THREADS * 16 < n) next.load(row, first + THREADS * 16, n);
+        unsigned long long v = 0;
+        if (c.t == 0.0f) {
+            now.each(first, [&](float l, int i) {
+                const unsigned long long t = l == l ? token_word(l, i) : WITH_NAN;
+                v = t > v ? t : v;
+            });
+        } else {
+            float m = -__builtin_inff();
+            bool nan = false;
+            now.each(first, [&](float l, int) {
+                nan |= l != l;
+                m = fmaxf(m, l);
+            });
+            v = nan ? WITH_NAN : (unsigned long long)order_bits(m) << 32;
+        }
+        v = most_of<THREADS>(v, s.wave64);
+        if (v == WITH_NAN) {
+            best = v;
+            break;
+        }
+        if (v > best) {
+            best = v;
+            const float max = of_bits((uint32_t)(v >> 32));
+            if (c.t > 0.0f && fabsf(max) <= 3.40282347e38f) {
+                const Place old = at;
+                at = Place(c.t, max);
+                lost |= at.too_far(max);
+                // the bins so far move behind by as many as the largest logit came before
+                const double d = fmin(old.ref - at.ref, (double)BINS);
+                const int by = old.per == 0.0 ? 0 : (int)d;
+                if (by > 0) {
+                    unsigned long long h[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int x = tid + i * THREADS - by;
+                        h[i] = x >= 0 && tid + i * THREADS < BINS - 1 ? s.hist[x] : 0;
+                    }
+                    __syncthreads();
+                    s.hist[tid] = h[0];
+                    s.hist[tid + THREADS] = h[1];
+                    __syncthreads();
+                }
+            }
+        }
+        if (c.t > 0.0f && at.per != 0.0) now.each(first, [&](float l, int) { count_token(s.hist, at, l); });
+    }
+    if (settled(p, r, c, best)) return;
     const float max = of_bits((uint32_t)(best >> 32));
-    count_bins<THREADS>(s.hist, row, p.vocab, Place{(double)max, PER / (double)c.t});
     __syncthreads();
-    finish(s, p, r, c, max, SampleSlices{0, 0, nullptr, nullptr, nullptr, nullptr});
+    if (lost) {
+        at.widen(max);
+        count_row(s, row, n, at);
+    }
+    finish(s, p, r, c, max, at, SampleSlices{0, nullptr, nullptr, nullptr, nullptr});
 }
 
-// Few rows: a workgroup for each slice of them finds its largest token, then its bins and the
-// tokens of the first ones, then a workgroup a row ends it.
-constexpr int SLICE = 8192, SLICE_THREADS = 512;
-__global__ __launch_bounds__(SLICE_THREADS) void sample_best_kernel(SampleParams p, SampleSlices sl) {
-    __shared__ unsigned long long scratch[SLICE_THREADS / 64];
-    const int r = blockIdx.y, first = blockIdx.x * sl.each;
-    if (!settings_of(p, r, false).live) return;
-    const unsigned long long v = largest<SLICE_THREADS>(p.logits + r * p.ld + first, min(sl.each, p.vocab - first),
-                                                        first, scratch);
-    if (threadIdx.x == 0) sl.best[(size_t)r * sl.n + blockIdx.x] = v;
-}
-
-__device__ __forceinline__ unsigned long long best_of(const SampleSlices &sl, int r) {
-    // (a lane two of them at most; by whole waves)
-    const int lane = threadIdx.x & 63;
-    const unsigned long long *p = sl.best + (size_t)r * sl.n;
-    const unsigned long long a = p[min(lane, sl.n - 1)], b = p[min(lane + 64, sl.n - 1)];
-    return wave_most(a > b ? a : b);
-}
-
-__global__ __launch_bounds__(SLICE_THREADS) void sample_bins_kernel(SampleParams p, SampleSlices sl) {
-    __shared__ unsigned long long hist[BINS];
-    __shared__ uint32_t wave[SLICE_THREADS / 64], n, last;
-    const int r = blockIdx.y, first = blockIdx.x * sl.each, tid = threadIdx.x, len = min(sl.each, p.vocab - first);
+// Few rows: a workgroup for each slice of them leaves its first token, its bins and the tokens of
+// the first ones, then a workgroup a row ends it.
+constexpr int SLICE_THREADS = 512, SLICE = SLICE_THREADS * 16;
+__global__ __launch_bounds__(SLICE_THREADS) void sample_slice_kernel(SampleParams p, SampleSlices sl) {
+    __shared__ unsigned long long hist[BINS], scratch[SLICE_THREADS / 64];
+    __shared__ uint32_t wave[SLICE_THREADS / 64], count, last;
+    const int r = blockIdx.y, first = blockIdx.x * SLICE, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const float *row = p.logits + r * p.ld;
+    Tokens<SLICE_THREADS> now;
+    now.load(row, first, p.vocab);
     const Settings c = settings_of(p, r, false);
     if (!c.live) return;
     for (int i = tid; i < BINS; i += SLICE_THREADS) hist[i] = 0;
-    const unsigned long long best = best_of(sl, r);
-    if (settled(p, r, c, best, false)) return;
-    const Place at{(double)of_bits((uint32_t)(best >> 32)), PER / (double)c.t};
-    const float *row = p.logits + r * p.ld + first;
     if (tid == 0) {
-        n = 0;
+        count = 0;
         last = 0;
     }
-    __syncthreads();
-    count_bins<SLICE_THREADS>(hist, row, len, at);
+    unsigned long long v = 0;
+    now.each(first, [&](float l, int i) {
+        const unsigned long long t = l == l ? token_word(l, i) : WITH_NAN;
+        v = t > v ? t : v;
+    });
+    v = most_of<SLICE_THREADS>(v, scratch);
+    const size_t x = (size_t)r * sl.n + blockIdx.x;
+    const float max = of_bits((uint32_t)(v >> 32));
+    if (tid == 0) sl.best[x] = v;
+    if (v == WITH_NAN || !(fabsf(max) <= 3.40282347e38f) || c.t == 0.0f) {
+        // (nothing but its first token is asked of it; a slice without a token has empty bins)
+        if (max == -__builtin_inff() && c.t > 0.0f) {
+            for (int i = tid; i < BINS; i += SLICE_THREADS) sl.hist[x * BINS + i] = 0;
+            if (tid == 0) {
+                sl.upto[x * 2] = BINS - 1;
+                sl.upto[x * 2 + 1] = 0;
+            }
+        }
+        return;
+    }
+    const Place at(c.t, max);
+    now.each(first, [&](float l, int) { count_token(hist, at, l); });
     __syncthreads();
     // the bins that hold at most SLICE_LIST tokens together
     constexpr int EACH = BINS / SLICE_THREADS;
-    const size_t x = (size_t)r * sl.n + blockIdx.x;
     uint32_t cnt[EACH], sum = 0;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
@@ -693,67 +778,97 @@ __global__ __launch_bounds__(SLICE_THREADS) void sample_bins_kernel(SampleParams
         cnt[i] = (uint32_t)(h >> COUNT);
         sum += cnt[i];
     }
-    uint32_t to = sum;
-    const int lane = tid & 63, w = tid >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const uint32_t v = __shfl_up(to, o, 64);
-        if (lane >= o) to += v;
-    }
+    uint32_t to = wave_scan<uint32_t>(sum);
     if (lane == 63) wave[w] = to;
     __syncthreads();
     to -= sum;
     for (int i = 0; i < w; ++i) to += wave[i];
+    int upto = 0;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {  // bin tid EACH + i is listed where the count up to it fits
+    for (int i = 0; i < EACH; ++i) {
         to += cnt[i];
-        if (to <= SLICE_LIST) atomicMax(&last, (uint32_t)min(tid * EACH + i + 1, BINS - 1));
+        if (to <= SLICE_LIST) upto = min(tid * EACH + i + 1, BINS - 1);
     }
+    const unsigned long long some = __ballot(upto > 0);
+    if (some && lane == 63 - __builtin_clzll(some)) atomicMax(&last, (uint32_t)upto);
     __syncthreads();
-    const int upto = (int)last;
-    const float from = at.below(upto - 1);
-    each_token<SLICE_THREADS>(row, len, [&](float l, int i) {
+    upto = (int)last;
+    now.each(first, [&](float l, int i) {
         uint32_t rest;
-        if (l >= from && at.bin(l, &rest) < upto) {
-            const uint32_t k = atomicAdd(&n, 1u);
-            if (k < SLICE_LIST)
-                sl.list[x * SLICE_LIST + k] = (unsigned long long)order_bits(l) << 32 | (uint32_t)~(first + i);
+        if (at.bin(l, &rest) < upto) {
+            const uint32_t k = atomicAdd(&count, 1u);
+            if (k < SLICE_LIST) sl.list[x * SLICE_LIST + k] = token_word(l, i);
         }
     });
     __syncthreads();
     if (tid == 0) {
-        sl.upto[x * 2] = upto;
-        sl.upto[x * 2 + 1] = (int)n;
+        sl.upto[x * 2] = at.too_far(max) ? -1 : upto;
+        sl.upto[x * 2 + 1] = (int)count;
     }
 }
 
 __global__ __launch_bounds__(THREADS) void sample_finish_kernel(SampleParams p, SampleSlices sl) {
     __shared__ Shared s;
-    const int r = blockIdx.x, tid = threadIdx.x;
+    __shared__ int shift[128];
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const Settings c = settings_of(p, r, true);
     if (!c.live) return;
-    const unsigned long long best = best_of(sl, r);
-    if (settled(p, r, c, best, true)) return;
-    unsigned long long a = 0, b = 0;
-    const unsigned long long *h = sl.hist + (size_t)r * sl.n * BINS + tid * 2;
-    for (int i = 0; i < sl.n; i += 8) {
-        ulonglong2 v[8];
+    // (a lane two slices at most; by every wave)
+    const unsigned long long *bp = sl.best + (size_t)r * sl.n;
+    int32_t *up = sl.upto + (size_t)r * sl.n * 2;
+    unsigned long long b[2];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = *(const ulonglong2 *)(h + (size_t)min(i + k, sl.n - 1) * BINS);
+    for (int i = 0; i < 2; ++i) b[i] = bp[min(lane + 64 * i, sl.n - 1)];
+    const unsigned long long best = wave_most(b[0] > b[1] ? b[0] : b[1]);
+    if (settled(p, r, c, best)) return;
+    const float max = of_bits((uint32_t)(best >> 32));
+    Place at(c.t, max);
+    if (at.too_far(max)) {
+        at.widen(max);
+        count_row(s, p.logits + r * p.ld, p.vocab, at);
+        finish(s, p, r, c, max, at, SampleSlices{0, nullptr, nullptr, nullptr, nullptr});
+        return;
+    }
+    if (tid < 64) {  // the bins of a slice stand behind the row's by as many as its largest logit's
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            a += i + k < sl.n ? v[k].x : 0;
-            b += i + k < sl.n ? v[k].y : 0;
+        for (int i = 0; i < 2; ++i) {
+            const float m = of_bits((uint32_t)(b[i] >> 32));
+            const int x = lane + 64 * i;
+            int by = 0;
+            if (m > -__builtin_inff()) by = (int)fmin(Place(c.t, m).ref - at.ref, (double)BINS);
+            if (x < sl.n) {
+                shift[x] = by;
+                up[x * 2] += by;
+            }
         }
     }
-    s.hist[tid * 2] = a;
-    s.hist[tid * 2 + 1] = b;
     __syncthreads();
-    finish(s, p, r, c, of_bits((uint32_t)(best >> 32)), sl);
+    unsigned long long h0 = 0, h1 = 0;
+    const unsigned long long *h = sl.hist + (size_t)r * sl.n * BINS;
+    for (int i = 0; i < sl.n; i += 8) {
+        unsigned long long v[8][2];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int x = min(i + k, sl.n - 1), at0 = tid * 2 - shift[x];
+            v[k][0] = h[(size_t)x * BINS + std::max(at0, 0)];
+            v[k][1] = h[(size_t)x * BINS + std::max(at0 + 1, 0)];
+            if (at0 < 0 || i + k >= sl.n) v[k][0] = 0;
+            if (at0 + 1 < 0 || i + k >= sl.n) v[k][1] = 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            h0 += v[k][0];
+            h1 += v[k][1];
+        }
+    }
+    s.hist[tid * 2] = h0;
+    s.hist[tid * 2 + 1] = tid == THREADS - 1 ? 0 : h1;  // (what has no weight)
+    __syncthreads();
+    finish(s, p, r, c, max, at, sl);
 }
 
-// SampleSlices where a row is long and they do not fill the chip by themselves: their three launches
-// and the bins' way through memory cost more than a row's own workgroup does from there on.
+// Slices where a row is long and rows do not fill the chip by themselves: two launches and
+// the bins' way through memory cost more than a row's own workgroup does from there on.
 int slices_of(int rows, int vocab) {
     const int n = (vocab + SLICE - 1) / SLICE;
     return n >= 4 && (long long)rows * n <= 512 ? n : 0;
@@ -778,15 +893,11 @@ int launch_sample(const SampleArgs &a, hipStream_t st) {
     }
     VMLM_GUARD(a.work, "sample: sliced rows need a workspace");
     const size_t x = (size_t)a.rows * sl.n;
-    sl.each = SLICE;
     sl.hist = (unsigned long long *)a.work;
     sl.list = sl.hist + x * BINS;
     sl.best = sl.list + x * SLICE_LIST;
     sl.upto = (int32_t *)(sl.best + x);
-    const dim3 grid((unsigned)sl.n, (unsigned)a.rows);
-    sample_best_kernel<<<grid, SLICE_THREADS, 0, st>>>(p, sl);
-    VMLM_HIP_CHECK(hipGetLastError());
-    sample_bins_kernel<<<grid, SLICE_THREADS, 0, st>>>(p, sl);
+    sample_slice_kernel<<<dim3((unsigned)sl.n, (unsigned)a.rows), SLICE_THREADS, 0, st>>>(p, sl);
     VMLM_HIP_CHECK(hipGetLastError());
     sample_finish_kernel<<<(unsigned)a.rows, THREADS, 0, st>>>(p, sl);
     VMLM_HIP_CHECK(hipGetLastError());
