@@ -142,11 +142,9 @@ struct Tokens {
 // Calls f(logit, index) for every token of a row (and, past its end, with -inf).
 template <int T, typename F>
 __device__ __forceinline__ void each_token(const float *row, int n, F f) {
-    Tokens<T> a;
-    a.load(row, 0, n);
     for (int first = 0; first < n; first += T * 16) {
-        const Tokens<T> now = a;
-        if (first + T * 16 < n) a.load(row, first + T * 16, n);
+        Tokens<T> now;
+        now.load(row, first, n);
         now.each(first, f);
     }
 }
@@ -447,6 +445,19 @@ __device__ __forceinline__ Found locate(Shared &s, const float *row, int vocab, 
     return f;
 }
 
+// The smallest logit with exp((l - max) / t) >= min_p in 64 bits: next to where its logarithm puts
+// it, the lanes try the f32 around it.
+__device__ __forceinline__ float least_of(float max, float t, float min_p) {
+    const float near = (float)fmax((double)max + (double)t * log((double)min_p), -3.40282347e38);
+    const uint32_t key = order_bits(near) + (threadIdx.x & 63) - 32u;
+    const float l = of_bits(key);
+    const bool in = l <= max && l >= -3.40282347e38f && exp(((double)l - (double)max) / (double)t) >= (double)min_p;
+    const unsigned long long keeps = __ballot(in);
+    // (next to 0 f32's steps are below what 64 bits tell apart: any of them then)
+    if (!keeps) return fminf(max, of_bits(__builtin_amdgcn_readlane(key, 63)));
+    return of_bits(__builtin_amdgcn_readlane(key, __builtin_ctzll(keeps)));
+}
+
 // The rest, from a row's bins in s.hist, by one workgroup. sl.n 0: no slices. `max`: the largest logit.
 __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, const Settings &c, float max,
                                        const Place &at, const SampleSlices &sl) {
@@ -492,7 +503,8 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
     const bool by_k = c.top_k > 0 && (uint32_t)c.top_k < live;
     // min_p's place, from the largest logit's bin on (behind all bins: none)
     const double far = c.min_p > 0.0f ? -log((double)c.min_p) * PER + 1.0 : 2.0 * BINS;
-    auto over_min = [&](float l) { return exp(((double)l - (double)max) / (double)c.t) >= (double)c.min_p; };
+    float least = -__builtin_inff();  // the smallest logit that min_p keeps
+    if (c.min_p > 0.0f) least = least_of(max, c.t, c.min_p);
 
     // The bins up to which tokens can be kept: where they hold few, those are sorted
     // together and every question is one of their sums.
@@ -534,7 +546,7 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
             const float l = of_bits((uint32_t)(s.list[x] >> 32));
             const int b = at.bin(l, &rest);
             w[x] = scale(b) * (double)((1u << UNIT) - loss(rest));
-            if (c.min_p > 0.0f && over_min(l)) atomicAdd(&s.n, 1u);
+            if (c.min_p > 0.0f && l >= least) atomicAdd(&s.n, 1u);
         }
         __syncthreads();
         if (tid >= 64) return;
@@ -593,15 +605,10 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
             if (!(c.top_p < 1.0f)) continue;
             goal = (double)c.top_p * all;
             with_equal = true;
-        } else if (question == 2) {  // min_p: weights next to the border in 64 bits, others by their bin
+        } else if (question == 2) {  // what min_p keeps
             if (c.min_p == 0.0f) continue;
             uint32_t k = 0;
-            each_token<THREADS>(row, n, [&](float l, int) {
-                uint32_t rest;
-                const int bin = at.bin(l, &rest);
-                if (bin == BINS - 1) return;
-                k += fabs((double)bin - far) > 3.0 ? (double)bin < far : over_min(l);
-            });
+            each_token<THREADS>(row, n, [&](float l, int) { k += l >= least; });
             __syncthreads();
             if (tid == 0) s.n = 0;
             __syncthreads();
@@ -667,11 +674,9 @@ __global__ __launch_bounds__(THREADS, 8) void sample_row_kernel(SampleParams p) 
     unsigned long long best = 0;  // (without the index where T > 0)
     Place at;
     bool lost = false;
-    Tokens<THREADS> next;
-    next.load(row, 0, n);
     for (int first = 0; first < n; first += THREADS * 16) {
-        const Tokens<THREADS> now = next;
-        if (first + THREADS * 16 < n) next.load(row, first + THREADS * 16, n);
+        Tokens<THREADS> now;
+        now.load(row, first, n);
         unsigned long long v = 0;
         if (c.t == 0.0f) {
             now.each(first, [&](float l, int i) {
