@@ -59,9 +59,13 @@ struct TreeAttnParams {
     const float *q;
     size_t ldq, ldo;
     const int32_t *pos0, *count, *parent;
-    int S, H, G;
-    int tiles, shares;  // of queries; of the positions
-    float *out, *work;
+    int S, G;
+    // tiles of queries; whether positions are dealt out in shares: `per` is the number of workgroups that a
+    // tile of all sequences may have, 0 if each takes all of a sequence's
+    int tiles, per;
+    float *out;
+    int *dealt;   // [B][2]: a sequence's first stream, its shares
+    float *work;  // [stream][tile]: the shares' results
     float scale, sign;  // of the scores: sign * scale * 2^scale_e, scale in [1/2, 1) (or 0), times log2(e)
     int scale_e;
     int *guard;
@@ -217,6 +221,71 @@ constexpr int ta_waves(int hd, int mt) {
     return mt == 1 ? (hd == 32 ? 5 : hd == 64 ? 4 : 2) : mt == 2 && hd <= 64 ? 3 : 2;
 }
 
+// How the positions are dealt out where there are fewer tiles than the card takes workgroups, or a long
+// sequence among short ones: in proportion to a sequence's blocks, which only the card knows. (One of
+// 32700 positions beside 15 of 600, 8 tokens each: 36 heads of 64 53 us, 311 with shares that the capacity
+// set alike for all; 8 of 128 65 and 141; 16 of 2600, where nothing is gained, 58 and 54, 45 and 45.)
+constexpr int TA_SHARES = 64, TA_LEAST = 2 * TA_W;  // at most; blocks of a share
+__device__ __forceinline__ float share_blocks(float blocks, int per) {
+    return fmaxf(blocks / (float)per, (float)TA_LEAST);
+}
+__device__ __forceinline__ int shares_of(int blocks, float each) {
+    return min(max((int)((float)blocks / each), 1), TA_SHARES);
+}
+struct Dealt {
+    int b, shares, rest;  // rest: share * Hkv + kv head
+};
+// The sequence and share of a stream, b < 0 if it has none; every wave finds them by itself.
+__device__ __forceinline__ Dealt deal(const TreeAttnParams &p, int stream, bool first_tile) {
+    const int lane = threadIdx.x & 63;
+    auto blocks_of = [&](int b, bool *bad) {
+        *bad = false;
+        if (b >= p.c.B) return 0;
+        const int at = p.pos0[b], n = p.count ? min(max(p.count[b], 0), p.S) : p.S;
+        if (at < 0 || n == 0) return 0;
+        *bad = at > p.c.cap - n;
+        return *bad ? 0 : (at + n - 1) / KV4_BLOCK + 1;
+    };
+    bool bad = false;
+    int blocks = blocks_of(lane, &bad);
+    float sum = (float)blocks;
+    for (int at = 64; at < p.c.B; at += 64) {
+        bool more;
+        sum += (float)blocks_of(at + lane, &more);
+        bad |= more;
+    }
+    const bool tell = stream == 0 && first_tile && __builtin_amdgcn_readfirstlane(threadIdx.x) == 0;
+    if (tell && __any(bad) && lane == 0) atomicOr(p.guard, 1);
+    const float each = share_blocks(wave_sum_dpp(sum) * (float)p.c.Hkv, p.per);
+    Dealt d{-1, 1, 0};
+    int before = 0;
+    for (int at = 0; at < p.c.B; at += 64) {
+        if (at) blocks = blocks_of(at + lane, &bad);
+        const int s = blocks ? shares_of(blocks, each) : 0, n = s * p.c.Hkv;
+        int upto = n;  // streams of the sequences up to the lane's
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) {
+            const int v = __shfl_up(upto, i, 64);
+            if (lane >= i) upto += v;
+        }
+        const int from = before + upto - n;
+        if (tell && at + lane < p.c.B) {
+            p.dealt[2 * (at + lane)] = from;
+            p.dealt[2 * (at + lane) + 1] = s;
+        }
+        const unsigned long long here = __ballot(stream >= from && stream < from + n);
+        if (here) {
+            const int i = __builtin_ctzll(here);
+            d.b = at + i;
+            d.shares = __builtin_amdgcn_readlane(s, i);
+            d.rest = stream - __builtin_amdgcn_readlane(from, i);
+            if (!tell) break;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return d;
+}
+
 // A tile of 16 MT (token, head) pairs of one sequence and kv head, and one share of the positions.
 template <int HD, int MT>
 __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(TreeAttnParams p) {
@@ -228,8 +297,21 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     const int col = lane & 15, j = lane >> 4;
     // the tiles that read the same positions lie 8 workgroups apart: on one XCD
     const int x8 = blockIdx.x / 8, stream = x8 / p.tiles * 8 + (int)(blockIdx.x % 8), tile = x8 % p.tiles;
-    const int share = stream % p.shares, pair = stream / p.shares, kvh = pair % p.c.Hkv, b = pair / p.c.Hkv;
-    if (b >= p.c.B) return;
+    int b, kvh = stream % p.c.Hkv, share = 0, shares = 1;
+    if (p.per == 0) {
+        b = stream / p.c.Hkv;
+        if (b >= p.c.B) return;
+    } else if (p.c.B == 1) {
+        b = 0;
+        share = stream / p.c.Hkv;
+    } else {
+        const Dealt d = deal(p, stream, tile == 0);
+        if (d.b < 0) return;
+        b = d.b;
+        shares = d.shares;
+        kvh = d.rest % p.c.Hkv;
+        share = d.rest / p.c.Hkv;
+    }
     // the wave's query rows, loaded before anything is known of the sequence
     constexpr int CW = (HD + 63) / 64, RW = ROWS / TA_W;
     const int row0 = tile * ROWS;
@@ -243,13 +325,19 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     }
     const TreeRows tr = tree_rows(p.pos0, p.count, p.parent, p.S, p.c.cap, b, p.guard,
                                   kvh == 0 && tile == 0 && share == 0);
+    if (p.per && p.c.B == 1) {
+        const int all = tr.n ? (tr.pos0 + tr.n - 1) / KV4_BLOCK + 1 : 0;
+        shares = __builtin_amdgcn_readfirstlane(shares_of(all, share_blocks((float)all * (float)p.c.Hkv, p.per)));
+        if (stream == 0 && tile == 0 && tid < 2) p.dealt[tid] = tid * shares;
+    }
     const int rows = min(ROWS, tr.n * p.G - row0);
     if (rows <= 0) return;
     const int t_lo = row0 / p.G, t_hi = (row0 + rows - 1) / p.G;
     const int last = tr.pos0 + t_hi;                               // the last position seen
     const int zone = tr.pos0 + (p.parent ? 0 : t_lo + 1);  // from here on not by all
     const int blocks = last / KV4_BLOCK + 1;
-    const int b0 = (int)((long long)share * blocks / p.shares), b1 = (int)((long long)(share + 1) * blocks / p.shares);
+    if (share >= shares) return;
+    const int b0 = (int)((long long)share * blocks / shares), b1 = (int)((long long)(share + 1) * blocks / shares);
     const size_t head = (size_t)b * p.c.Hkv + kvh;
 
     // 1. the queries' operands
@@ -595,7 +683,8 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const float mx = __builtin_ceilf(ta_swap32(ta_swap16(top[t], ta_max), ta_max));
-                const float to = fmaxf(m[t], mx), corr = __builtin_amdgcn_exp2f(m[t] - to);
+                // (each query by its own scores: nothing that only others see shows in it)
+                const float to = mx > m[t] + TA_SLACK ? mx : m[t], corr = __builtin_amdgcn_exp2f(m[t] - to);
                 m[t] = to;
                 l[t] *= corr;
 #pragma unroll
@@ -747,11 +836,11 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
             L = __builtin_fmaf(f, rm[(x * ROWS + r) * 2 + 1], L);
             o = __builtin_fmaf(f, ((const float *)(lds + M::RO))[(x * ROWS + r) * HD + c], o);
         }
-        if (p.shares == 1) {
+        if (shares == 1) {
             const int R = row0 + r;
             p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * TA_UNBASE / L;
         } else {
-            float *pw = p.work + (((size_t)pair * p.tiles + tile) * p.shares + share) * (ROWS * (HD + 2));
+            float *pw = p.work + ((size_t)stream * p.tiles + tile) * (ROWS * (HD + 2));
             pw[r * HD + c] = o;
             if (c == 0) {
                 pw[ROWS * HD + 2 * r] = mx;
@@ -767,72 +856,80 @@ template <int HD>
 __global__ __launch_bounds__(HD < 64 ? 64 : HD) void tree_merge_kernel(TreeAttnParams p, int ROWS) {
     const int r = blockIdx.x % ROWS, tile = blockIdx.x / ROWS, kvh = blockIdx.y, b = blockIdx.z;
     const int lane = threadIdx.x & 63, c = min((int)threadIdx.x, HD - 1);
-    const size_t pair = (size_t)b * p.c.Hkv + kvh, ld = (size_t)ROWS * (HD + 2);
-    const float *pw = p.work + (pair * p.tiles + tile) * p.shares * ld;
-    const float *px = pw + r * HD + c, *pm = pw + min(lane, p.shares - 1) * ld + ROWS * HD + 2 * r;
+    const int shares = p.dealt[2 * b + 1];
+    if (shares <= 1) return;
+    const size_t one = (size_t)ROWS * (HD + 2), ld = (size_t)p.c.Hkv * p.tiles * one;
+    const float *pw = p.work + ((size_t)(p.dealt[2 * b] + kvh) * p.tiles + tile) * one;
+    const float *px = pw + r * HD + c, *pm = pw + min(lane, shares - 1) * ld + ROWS * HD + 2 * r;
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = px[min(i, p.shares - 1) * ld];
+    for (int i = 0; i < 8; ++i) x[i] = px[min(i, shares - 1) * ld];
     const float m = pm[0], l = pm[1];
     const TreeRows tr = tree_rows(p.pos0, p.count, p.parent, p.S, p.c.cap, b, p.guard, false);
     const int R = tile * ROWS + r;
     if (R >= tr.n * p.G) return;  // (what was read is not this query's)
     const float mx = ta_swap32(ta_swap16(ta_row16(m, ta_max), ta_max), ta_max);
-    const float f = lane < p.shares ? __builtin_amdgcn_exp2f(m - mx) : 0.0f;
-    const float L = wave_sum_dpp(lane < p.shares ? f * l : 0.0f);
+    const float f = lane < shares ? __builtin_amdgcn_exp2f(m - mx) : 0.0f;
+    const float L = wave_sum_dpp(lane < shares ? f * l : 0.0f);
     float o = 0.0f;
-    for (int s = 0; s < p.shares; s += 8) {
+    for (int s = 0; s < shares; s += 8) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), min(s + i, 63)));
-            o = s + i < p.shares ? __builtin_fmaf(w, x[i], o) : o;
+            o = s + i < shares ? __builtin_fmaf(w, x[i], o) : o;
         }
-        if (s + 8 >= p.shares) break;
+        if (s + 8 >= shares) break;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = px[min(s + 8 + i, p.shares - 1) * ld];
+        for (int i = 0; i < 8; ++i) x[i] = px[min(s + 8 + i, shares - 1) * ld];
     }
     if (threadIdx.x < HD)
         p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * TA_UNBASE / L;
 }
 
 struct TreePlan {
-    int mt, tiles, shares;
+    int mt, rows, tiles, per;
+    size_t streams, work;  // work: floats
 };
 TreePlan tree_plan(const Kv4View &c, int H, int S) {
     const long long rows = (long long)S * (H / c.Hkv);
     const int most = c.hd <= 64 ? 4 : c.hd == 128 ? 2 : 1;
     TreePlan pl;
     pl.mt = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : most;
-    pl.tiles = (int)((rows + 16 * pl.mt - 1) / (16 * pl.mt));
-    // workgroups for two a CU, where the capacity gives each wave of a share two blocks
-    const long long streams = (long long)c.B * c.Hkv * pl.tiles;
-    const long long by_length = c.cap / KV4_BLOCK / (2 * TA_W);
-    pl.shares = (int)std::max(1ll, std::min(std::min(512 / streams, by_length), 64ll));
+    pl.rows = 16 * pl.mt;
+    pl.tiles = (int)((rows + pl.rows - 1) / pl.rows);
+    // Workgroups for two a CU, where a sequence's length gives each wave of a share two blocks. Where there are as
+    // many without shares, only a cache of 8192 positions and more, 120 us of one workgroup.
+    const size_t pairs = (size_t)c.B * c.Hkv, slots = 512;
+    pl.per = pairs * pl.tiles < slots || c.cap >= 8192 ? (int)(slots / pl.tiles) : 0;
+    const size_t longest = (size_t)c.cap / KV4_BLOCK / TA_LEAST;  // shares of the longest sequence
+    if (longest <= 1 || (c.B == 1 && pl.per < 2 * c.Hkv)) pl.per = 0;
+    // (one sequence gets no more than `per` in all; of several each may round up to one)
+    pl.streams = pl.per == 0 ? pairs : std::min(c.B == 1 ? (size_t)pl.per : pairs + pl.per, pairs * longest);
+    pl.work = pl.per == 0 ? 0 : ((size_t)c.B * 2 + 63) / 64 * 64 + pl.streams * pl.tiles * pl.rows * (c.hd + 2);
     return pl;
 }
 
 template <int HD, int MT>
-int launch_t(const TreeAttnParams &p, hipStream_t st) {
+int launch_t(const TreeAttnParams &p, const TreePlan &pl, hipStream_t st) {
     using M = TreeLds<HD, MT>;
     int rc = allow_lds((const void *)tree_attn_kernel<HD, MT>, M::SIZE, M::SIZE);
     if (rc) return rc;
-    const size_t streams = (size_t)p.c.B * p.c.Hkv * p.shares;
-    tree_attn_kernel<HD, MT><<<(unsigned)((streams + 7) / 8 * 8 * p.tiles), 64 * TA_W, M::SIZE, st>>>(p);
+    tree_attn_kernel<HD, MT><<<(unsigned)((pl.streams + 7) / 8 * 8 * p.tiles), 64 * TA_W, M::SIZE, st>>>(p);
     VMLM_HIP_CHECK(hipGetLastError());
-    if (p.shares == 1) return VMLM_OK;
-    tree_merge_kernel<HD><<<dim3((unsigned)p.tiles * 16 * MT, (unsigned)p.c.Hkv, (unsigned)p.c.B),
-                            HD < 64 ? 64 : HD, 0, st>>>(p, 16 * MT);
+    if (p.per == 0) return VMLM_OK;
+    tree_merge_kernel<HD><<<dim3((unsigned)(p.tiles * pl.rows), (unsigned)p.c.Hkv, (unsigned)p.c.B),
+                            HD < 64 ? 64 : HD, 0, st>>>(p, pl.rows);
     VMLM_HIP_CHECK(hipGetLastError());
     return VMLM_OK;
 }
 
 template <int HD>
-int launch_hd(const TreeAttnParams &p, int mt, hipStream_t st) {
-    if (mt == 1) return launch_t<HD, 1>(p, st);
+int launch_hd(const TreeAttnParams &p, const TreePlan &pl, hipStream_t st) {
+    if (pl.mt == 1) return launch_t<HD, 1>(p, pl, st);
     if constexpr (HD <= 128) {
-        if (mt == 2) return launch_t<HD, 2>(p, st);
+        if (pl.mt == 2) return launch_t<HD, 2>(p, pl, st);
     }
-    if constexpr (HD <= 64) return launch_t<HD, 4>(p, st);
+    if constexpr (HD <= 64) return launch_t<HD, 4>(p, pl, st);
     return VMLM_OK;
 }
 
@@ -840,9 +937,7 @@ int launch_hd(const TreeAttnParams &p, int mt, hipStream_t st) {
 
 size_t tree_attn_work_floats(const Kv4View &c, int H, int S) {
     if (c.B == 0 || c.Hkv == 0 || c.cap == 0 || H == 0 || S == 0) return 0;
-    const TreePlan pl = tree_plan(c, H, S);
-    if (pl.shares == 1) return 0;
-    return (size_t)c.B * c.Hkv * pl.tiles * pl.shares * (16 * pl.mt) * (c.hd + 2);
+    return tree_plan(c, H, S).work;
 }
 
 int launch_tree_attn(const TreeAttnArgs &a, hipStream_t st) {
@@ -856,21 +951,21 @@ int launch_tree_attn(const TreeAttnArgs &a, hipStream_t st) {
     p.count = a.count;
     p.parent = a.parent;
     p.S = a.S;
-    p.H = a.H;
     p.G = a.H / a.c.Hkv;
     p.tiles = pl.tiles;
-    p.shares = pl.shares;
+    p.per = pl.per;
     p.out = a.out;
-    p.work = a.work;
+    p.dealt = (int *)a.work;
+    p.work = a.work + ((size_t)a.c.B * 2 + 63) / 64 * 64;
     p.scale = frexpf(fabsf(a.scale), &p.scale_e) * 1.44269504f;
     p.sign = a.scale < 0.0f ? -1.0f : 1.0f;
     p.guard = guard_flag_ptr();
-    VMLM_GUARD(p.shares == 1 || p.work, "kv4 tree attention: split positions need a workspace");
+    VMLM_GUARD(p.per == 0 || a.work, "kv4 tree attention: split positions need a workspace");
     switch (a.c.hd) {
-    case 32: return launch_hd<32>(p, pl.mt, st);
-    case 64: return launch_hd<64>(p, pl.mt, st);
-    case 128: return launch_hd<128>(p, pl.mt, st);
-    default: return launch_hd<256>(p, pl.mt, st);
+    case 32: return launch_hd<32>(p, pl, st);
+    case 64: return launch_hd<64>(p, pl, st);
+    case 128: return launch_hd<128>(p, pl, st);
+    default: return launch_hd<256>(p, pl, st);
     }
 }
 
