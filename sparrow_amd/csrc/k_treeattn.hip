@@ -460,8 +460,8 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     float own[2][Raw::OWN], vscales[Raw::VM];
     unsigned long long nan_p[Raw::VM];  // lanes whose value's meta is a NaN
 
-    // 2. by the shared powers of two; false where a position is too large for them, or smaller
-    // than 2^-TA_SPAN of them
+    // 2. by the shared powers of two; false where a position is too large for them, or its keys or a
+    // group of its values smaller than 2^-TA_SPAN of them
     auto shared_meta = [&](const Raw &raw) {
         float hi = 0.0f, lo = __builtin_inff();
 #pragma unroll
@@ -484,11 +484,13 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         for (int i = 0; i < Raw::VM; ++i) {
             vscales[i] = kv4_scale(raw.vm[i]) * vg;
             const float mid = __builtin_fmaf(kv4_min(raw.vm[i]), vg, 8.0f * vscales[i]);
-            most = fmaxf(most, fmaxf(fabsf(mid), 8.0f * vscales[i]));
+            const float v = fmaxf(fabsf(mid), 8.0f * vscales[i]);
+            most = fmaxf(most, v);
+            lo = fminf(lo, v == 0.0f ? TA_TOP : v);  // (zeros lose nothing)
             vmiddles[i] = two_terms(mid, rest);
             nan_p[i] = 0;
         }
-        return __all(fmaxf(hi, most) < TA_TOP && fminf(lo, most) >= TA_TOP / (1 << TA_SPAN));
+        return __all(fmaxf(hi, most) < TA_TOP && lo >= TA_TOP / (1 << TA_SPAN));
     };
     // 3. the powers of two of a block whose positions did not suit the ones there were; false
     // where they leave the range that the shared form keeps to
@@ -527,8 +529,11 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
             const int f = fe[t * 16 + col] + ek_run - TA_TOP_E;
             cq[t] = ldexpf(cs, f);
             fits &= f <= 100;
-            // the sums of weights that stand in O are in units of 2^ev_run
-            if (M::ONES && j == 3) O[t][NT][3] = ldexpf(O[t][NT][3], ev_run - old);
+            // the sums of weights that stand in O are in units of 2^ev: to the others
+            if (M::ONES && j == 3) {
+                l[t] += ldexpf(O[t][NT][3], TA_TOP_E - old - TA_BASE);
+                O[t][NT][3] = 0.0f;
+            }
         }
         fits = __all(fits);
         if (!fits) {  // (nothing is shared until the next choice)
