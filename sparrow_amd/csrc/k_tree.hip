@@ -33,16 +33,29 @@ template <int HD>
 __global__ __launch_bounds__(ACC_THREADS) void accept_kernel(AcceptParams p) {
     constexpr int NG = HD / 32, T = ACC_THREADS;
     constexpr int KW = TREE_MAX * (HD / 8) / T;   // a thread's dwords of K rows,
-    constexpr int MW = (TREE_MAX * NG + T - 1) / T;  // of either meta
+    constexpr int MW = (TREE_MAX * NG + T - 1) / T;  // of either meta,
+    constexpr int VW = (ACC_BLOCKS * HD + T - 1) / T;  // four of V's blocks
     __shared__ int path[TREE_MAX];
     __shared__ __align__(16) uint32_t vc[ACC_BLOCKS * HD * 4];  // V codes from the first block on
     const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     // 1. the walk, by every wave
-    TreeRows t = tree_rows(p.pos0, p.count, p.parent, p.S, p.cap, b, p.guard, h == 0);
+    const size_t at = (size_t)b * p.S + min(lane, p.S - 1);
+    const int drafted = p.drafted[at], chosen = p.chosen[at];
+    const TreeRows t = tree_rows(p.pos0, p.count, p.parent, p.S, p.cap, b, p.guard, h == 0);
     const int n = t.n, pos0 = t.pos0;
     if (n == 0) return;  // an idle sequence
-    const size_t at = (size_t)b * p.S + min(lane, n - 1);
-    const int drafted = p.drafted[at], chosen = p.chosen[at];
+    // (V's blocks are on their way while the tree is walked, whether anything moves or not)
+    const Kv4Arrays c = p.c[blockIdx.z];
+    const size_t head = (size_t)b * p.Hkv + h, row0 = head * p.cap + pos0;
+    const int blk0 = pos0 / KV4_BLOCK, blocks = (pos0 + n - 1) / KV4_BLOCK - blk0 + 1;
+    const size_t vat = (head * (p.cap / KV4_BLOCK) + blk0) * (size_t)(HD * 4);
+    uint32_t *kd = (uint32_t *)c.k, *vd = (uint32_t *)c.v + vat;
+    u32x4 vr[VW];
+#pragma unroll
+    for (int i = 0; i < VW; ++i) {
+        const int x = tid + i * T;
+        if ((int)blockIdx.z < p.caches && x < blocks * HD) vr[i] = ((const u32x4 *)vd)[x];
+    }
     const int parent = p.parent ? t.parent : lane - 1;
     int cur = 0, kept = 1, mine = lane == 0 ? 0 : -1, token;
     int first = 1;  // the first row that moves
@@ -66,12 +79,9 @@ __global__ __launch_bounds__(ACC_THREADS) void accept_kernel(AcceptParams p) {
     if (first >= kept || (int)blockIdx.z >= p.caches) return;
     if (tid < 64) path[lane] = mine;
     // 2. the sources
-    const Kv4Arrays c = p.c[blockIdx.z];
-    const size_t head = (size_t)b * p.Hkv + h, row0 = head * p.cap + pos0;
-    const int blk0 = pos0 / KV4_BLOCK, blocks = (pos0 + n - 1) / KV4_BLOCK - blk0 + 1;
-    const size_t vat = (head * (p.cap / KV4_BLOCK) + blk0) * (size_t)(HD * 4);
-    uint32_t *kd = (uint32_t *)c.k, *vd = (uint32_t *)c.v + vat;
-    for (int i = tid; i < blocks * HD; i += T) ((u32x4 *)vc)[i] = ((const u32x4 *)vd)[i];
+#pragma unroll
+    for (int i = 0; i < VW; ++i)
+        if (tid + i * T < blocks * HD) ((u32x4 *)vc)[tid + i * T] = vr[i];
     __syncthreads();
     uint32_t kr[KW], kmr[MW], vmr[MW];
 #pragma unroll

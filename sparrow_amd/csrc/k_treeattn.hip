@@ -49,7 +49,7 @@ constexpr int TA_TOP_E = 11, TA_SPAN = 14;
 constexpr float TA_TOP = 1 << TA_TOP_E;
 // A weight is 2^TA_BASE at the maximum that its wave knew when it last raised it, which it
 // does where one is 2^TA_SLACK larger: with 64 queries some maximum grows in nearly every block
-// (tree_long: 192 us when each was followed).
+// (63 tokens, 65463 positions, 36 heads of 64: 192 us when each was followed, 158 then).
 constexpr int TA_BASE = 9, TA_SLACK = 6;
 constexpr float TA_UNBASE = 1.0f / (1 << TA_BASE);
 constexpr float TA_FAR = 4194304.0f;        // scores whose f32 steps are no longer small

@@ -19,13 +19,15 @@ __device__ __forceinline__ TreeRows tree_rows(const int32_t *pos0, const int32_t
                                               const int32_t *parent, int S, int cap, int b,
                                               int *guard, bool report) {
     const int lane = threadIdx.x & 63;
+    // (all loads at once: they are the start of every kernel that takes drafted tokens)
+    const int listed = count ? count[b] : S, up = parent && lane < S ? parent[(size_t)b * S + lane] : -1;
     TreeRows r{0, pos0[b], -1};
     if (r.pos0 < 0) return r;
-    const int n = count ? min(max(count[b], 0), S) : S;
+    const int n = min(max(listed, 0), S);
     bool bad = n > 0 && r.pos0 > cap - n;
     if (parent && lane < n) {
-        r.parent = parent[(size_t)b * S + lane];
-        bad |= r.parent < -1 || r.parent >= lane;
+        r.parent = up;
+        bad |= up < -1 || up >= lane;
     }
     if (__any(bad)) {
         if (report && threadIdx.x == 0) atomicOr(guard, 1);
@@ -33,14 +35,6 @@ __device__ __forceinline__ TreeRows tree_rows(const int32_t *pos0, const int32_t
     }
     r.n = n;
     return r;
-}
-
-// Token t and those above it, a bit each; `parent` as tree_rows gives it. Called by whole
-// waves, t the same in all lanes.
-__device__ __forceinline__ unsigned long long tree_ancestors(int parent, int t) {
-    unsigned long long seen = 0;
-    for (int at = t; at >= 0; at = __builtin_amdgcn_readlane(parent, at)) seen |= 1ull << at;
-    return seen;
 }
 
 }  // namespace vmlm
