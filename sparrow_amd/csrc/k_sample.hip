@@ -139,12 +139,19 @@ struct Tokens {
             for (int e = 0; e < 4; ++e) f(v[k][e], first + index(k) + e);
     }
 };
-// Calls f(logit, index) for every token of a row (and, past its end, with -inf).
-template <int T, typename F>
+// Calls f(logit, index) for every token of a row (and, past its end, with -inf). AHEAD: the next
+// part is on its way meanwhile, where registers are not short.
+template <int T, bool AHEAD, typename F>
 __device__ __forceinline__ void each_token(const float *row, int n, F f) {
+    Tokens<T> now, next;
+    if (AHEAD) next.load(row, 0, n);
     for (int first = 0; first < n; first += T * 16) {
-        Tokens<T> now;
-        now.load(row, first, n);
+        if (AHEAD) {
+            now = next;
+            if (first + T * 16 < n) next.load(row, first + T * 16, n);
+        } else {
+            now.load(row, first, n);
+        }
         now.each(first, f);
     }
 }
@@ -153,6 +160,7 @@ struct Shared {
     unsigned long long hist[BINS];  // counts and losses; what is to be sorted; weights
     double above[BINS];             // the mass before a bin
     uint32_t before[BINS];          // the tokens before a bin
+    uint32_t start[BINS];           // where a bin's tokens stand in the list, if they do
     unsigned long long list[LIST];  // tokens, the largest first
     uint32_t rank[512];
     double whole[32], part[64];     // exp(-i), exp(-i / 64)
@@ -310,8 +318,54 @@ struct Found {
     uint32_t token, d;
 };
 
+// The sums of the losses of the n tokens in s.list up to each, in s.hist.
+__device__ __forceinline__ void sum_losses(Shared &s, int n, const Place &at) {
+    static_assert(LIST == BINS && LIST == 2 * THREADS, "");
+    const int tid = threadIdx.x;
+    unsigned long long d[2], e[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int x = tid * 2 + i;
+        uint32_t rest;
+        d[i] = 0;
+        if (x < n) {
+            at.bin(of_bits((uint32_t)(s.list[x] >> 32)), &rest);
+            d[i] = loss(rest);
+        }
+    }
+    block_scan<unsigned long long>(d[0], d[1], &e[0], &e[1], s.wave64);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) s.hist[tid * 2 + i] = e[i] + d[i];
+    __syncthreads();
+}
+// The place in the bin of m tokens that stand in s.list from x0 on, as locate finds it.
+__device__ __forceinline__ Found place_in(const Shared &s, int x0, int m, bool by_rank, uint32_t rank, double mass,
+                                          bool with_equal) {
+    const unsigned long long d0 = x0 ? s.hist[x0 - 1] : 0;
+    auto upto = [&](int i) { return ((unsigned long long)(i + 1) << UNIT) - (s.hist[x0 + i] - d0); };
+    int i = min((int)rank, m - 1);
+    if (!by_rank) {
+        int z = m - 1;
+        for (i = 0; i < z;) {
+            const int mid = (i + z) / 2;
+            const double w = (double)upto(mid);
+            if (with_equal ? w >= mass : w > mass)
+                z = mid;
+            else
+                i = mid + 1;
+        }
+    }
+    Found f;
+    f.rank = i;
+    f.upto = upto(i);
+    f.d = (uint32_t)(s.hist[x0 + i] - (x0 + i ? s.hist[x0 + i - 1] : 0));
+    f.token = ~(uint32_t)s.list[x0 + i];
+    return f;
+}
+
 // The token of rank `rank` in bin `bin` (by_rank), else the first one with weights up to it of
 // more than `mass` (or, with_equal, as much). `n`: the bin's tokens.
+template <bool AHEAD>
 __device__ __forceinline__ Found locate(Shared &s, const float *row, int vocab, const Place &at, int bin, int n,
                                         bool by_rank, uint32_t rank, double mass, bool with_equal) {
     const int tid = threadIdx.x;
@@ -320,7 +374,7 @@ __device__ __forceinline__ Found locate(Shared &s, const float *row, int vocab, 
     uint32_t rank0 = 0;  // the bin's tokens above them, and their weights
     unsigned long long mass0 = 0;
     auto each_of_bin = [&](auto f) {
-        each_token<THREADS>(row, vocab, [&](float l, int i) {
+        each_token<THREADS, AHEAD>(row, vocab, [&](float l, int i) {
             uint32_t rest;
             const uint32_t key = order_bits(l);
             if (l >= from && l <= to && key >= lo && key <= hi && at.bin(l, &rest) == bin) f(key, rest, i);
@@ -411,36 +465,10 @@ __device__ __forceinline__ Found locate(Shared &s, const float *row, int vocab, 
     gather(s, n, [&](auto put) {
         each_of_bin([&](uint32_t key, uint32_t, int i) { put((unsigned long long)key << 32 | (uint32_t)~i); });
     });
-    static_assert(LIST == BINS && LIST == 2 * THREADS, "");
-    unsigned long long *sum = s.hist, d[2], e[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int x = tid * 2 + i;
-        uint32_t rest;
-        d[i] = 0;
-        if (x < n) {
-            at.bin(of_bits((uint32_t)(s.list[x] >> 32)), &rest);
-            d[i] = loss(rest);
-        }
-    }
-    block_scan<unsigned long long>(d[0], d[1], &e[0], &e[1], s.wave64);
-    if (tid == 0) s.lo = n - 1;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int x = tid * 2 + i;
-        if (x >= n) continue;
-        sum[x] = e[i] + d[i];
-        const unsigned long long w = mass0 + ((unsigned long long)(x + 1) << UNIT) - (e[i] + d[i]);
-        const bool hit = by_rank ? rank0 + x == rank : with_equal ? (double)w >= mass : (double)w > mass;
-        if (hit) atomicMin(&s.lo, (uint32_t)x);
-    }
-    __syncthreads();
-    const uint32_t x = s.lo;
-    f.rank = rank0 + x;
-    f.upto = mass0 + ((unsigned long long)(x + 1) << UNIT) - sum[x];
-    f.d = (uint32_t)(sum[x] - (x ? sum[x - 1] : 0));
-    f.token = ~(uint32_t)s.list[x];
+    sum_losses(s, n, at);
+    f = place_in(s, 0, n, by_rank, rank - rank0, mass - (double)mass0, with_equal);
+    f.rank += rank0;
+    f.upto += mass0;
     __syncthreads();
     return f;
 }
@@ -459,6 +487,7 @@ __device__ __forceinline__ float least_of(float max, float t, float min_p) {
 }
 
 // The rest, from a row's bins in s.hist, by one workgroup. sl.n 0: no slices. `max`: the largest logit.
+template <bool AHEAD>
 __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, const Settings &c, float max,
                                        const Place &at, const SampleSlices &sl) {
     const int tid = threadIdx.x, lane = tid & 63, n = p.vocab;
@@ -532,7 +561,7 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
                 }
             } else {
                 const float from = at.below(cut);
-                each_token<THREADS>(row, n, [&](float l, int i) {
+                each_token<THREADS, AHEAD>(row, n, [&](float l, int i) {
                     uint32_t rest;
                     if (l >= from && at.bin(l, &rest) <= cut) put(token_word(l, i));
                 });
@@ -591,7 +620,63 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
         return;
     }
 
-    // Else each question by its bin, one after the other.
+    // Else each question ends in one bin, whose tokens decide it. The bins that they can end in are
+    // known but for what those tokens change: they are gathered and sorted together, in one
+    // reading, and a question that ends in another bin reads the row for itself.
+    int from[4], to[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        from[q] = BINS;
+        to[q] = -1;
+    }
+    auto upto_bin = [&](int b) { return b + 1 < BINS ? s.above[b + 1] : all; };
+    uint32_t rest;
+    const int least_bin = c.min_p > 0.0f ? at.bin(least, &rest) : BINS - 1;
+    double a0 = all, a1 = all;  // the kept ones' weights, between
+    if (by_k) {
+        from[0] = to[0] = bin_of_rank((uint32_t)c.top_k - 1);
+        a0 = s.above[from[0]];
+        a1 = upto_bin(to[0]);
+    }
+    if (c.top_p < 1.0f) {
+        from[1] = bin_of_mass((double)c.top_p * a0, true);
+        to[1] = bin_of_mass((double)c.top_p * a1, true);
+        a0 = s.above[from[1]];
+        a1 = upto_bin(to[1]);
+    }
+    if (least_bin < BINS - 1 && s.above[least_bin] < a1) {
+        from[2] = to[2] = least_bin;
+        a0 = fmin(a0, s.above[least_bin]);
+        a1 = fmin(a1, upto_bin(least_bin));
+    }
+    from[3] = bin_of_mass((double)c.u * a0, false);
+    to[3] = bin_of_mass((double)c.u * a1, false);
+    constexpr uint32_t NONE = ~0u;
+    uint32_t some[2], start[2];
+    bool in[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        in[i] = false;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) in[i] |= from[q] <= tid * 2 + i && tid * 2 + i <= to[q];
+        some[i] = in[i] ? cnt[i] : 0;
+    }
+    const uint32_t together = block_scan<uint32_t>(some[0], some[1], &start[0], &start[1], s.wave);
+    bool listed = together <= LIST;
+    if (listed) {
+        const int first = std::min(std::min(from[0], from[1]), std::min(from[2], from[3]));
+        const int last = std::max(std::max(to[0], to[1]), std::max(to[2], to[3]));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s.start[tid * 2 + i] = in[i] ? start[i] : NONE;
+        const float least_l = at.below(last), most_l = at.above(first);
+        gather(s, (int)together, [&](auto put) {
+            each_token<THREADS, AHEAD>(row, n, [&](float l, int i) {
+                uint32_t rest;
+                if (l >= least_l && l <= most_l && s.start[at.bin(l, &rest)] != NONE) put(token_word(l, i));
+            });
+        });
+        sum_losses(s, (int)together, at);
+    }
     for (int question = 0; question < 5; ++question) {
         int b;
         bool by_rank = false, with_equal = false;
@@ -607,15 +692,30 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
             with_equal = true;
         } else if (question == 2) {  // what min_p keeps
             if (c.min_p == 0.0f) continue;
+            if (least_bin == BINS - 1 || s.before[least_bin] >= kept) continue;
             uint32_t k = 0;
-            each_token<THREADS>(row, n, [&](float l, int) { k += l >= least; });
-            __syncthreads();
-            if (tid == 0) s.n = 0;
-            __syncthreads();
-            atomicAdd(&s.n, k);
-            __syncthreads();
-            k = std::max(1u, s.n);
-            __syncthreads();
+            if (listed && s.start[least_bin] != NONE) {
+                int i = 0, z = tokens(least_bin);
+                const uint32_t key = order_bits(least), x0 = s.start[least_bin];
+                while (i < z) {
+                    const int mid = (i + z) / 2;
+                    if ((uint32_t)(s.list[x0 + mid] >> 32) >= key)
+                        i = mid + 1;
+                    else
+                        z = mid;
+                }
+                k = s.before[least_bin] + i;
+            } else {
+                each_token<THREADS, AHEAD>(row, n, [&](float l, int) { k += l >= least; });
+                __syncthreads();
+                if (tid == 0) s.n = 0;
+                __syncthreads();
+                atomicAdd(&s.n, k);
+                __syncthreads();
+                k = s.n;
+                __syncthreads();
+            }
+            k = std::max(1u, k);
             if (k >= kept) continue;
             kept = k;
             by_rank = true;
@@ -626,7 +726,15 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
         }
         b = by_rank ? bin_of_rank(kept - 1) : bin_of_mass(goal, with_equal);
         if (by_rank) rank = kept - 1 - s.before[b];
-        const Found f = locate(s, row, n, at, b, tokens(b), by_rank, rank, (goal - s.above[b]) / scale(b), with_equal);
+        const double mass = (goal - s.above[b]) / scale(b);
+        Found f;
+        if (listed && s.start[b] != NONE) {
+            f = place_in(s, (int)s.start[b], tokens(b), by_rank, rank, mass, with_equal);
+        } else {
+            __syncthreads();
+            listed = false;  // (the list is written over)
+            f = locate<AHEAD>(s, row, n, at, b, tokens(b), by_rank, rank, mass, with_equal);
+        }
         const uint32_t upto = s.before[b] + f.rank + 1;
         if (question < 3) {
             if (question == 1 && upto >= kept) continue;
@@ -659,7 +767,7 @@ __device__ __forceinline__ unsigned long long most_of(unsigned long long v, unsi
 __device__ __forceinline__ void count_row(Shared &s, const float *row, int n, const Place &at) {
     for (int i = threadIdx.x; i < BINS; i += THREADS) s.hist[i] = 0;
     __syncthreads();
-    each_token<THREADS>(row, n, [&](float l, int) { count_token(s.hist, at, l); });
+    each_token<THREADS, false>(row, n, [&](float l, int) { count_token(s.hist, at, l); });
     __syncthreads();
 }
 
@@ -730,7 +838,7 @@ __global__ __launch_bounds__(THREADS, 8) void sample_row_kernel(SampleParams p) 
         at.widen(max);
         count_row(s, row, n, at);
     }
-    finish(s, p, r, c, max, at, SampleSlices{0, nullptr, nullptr, nullptr, nullptr});
+    finish<false>(s, p, r, c, max, at, SampleSlices{0, nullptr, nullptr, nullptr, nullptr});
 }
 
 // Few rows: a workgroup for each slice of them leaves its first token, its bins and the tokens of
@@ -831,7 +939,7 @@ __global__ __launch_bounds__(THREADS) void sample_finish_kernel(SampleParams p, 
     if (at.too_far(max)) {
         at.widen(max);
         count_row(s, p.logits + r * p.ld, p.vocab, at);
-        finish(s, p, r, c, max, at, SampleSlices{0, nullptr, nullptr, nullptr, nullptr});
+        finish<true>(s, p, r, c, max, at, SampleSlices{0, nullptr, nullptr, nullptr, nullptr});
         return;
     }
     if (tid < 64) {  // the bins of a slice stand behind the row's by as many as its largest logit's
@@ -869,7 +977,7 @@ __global__ __launch_bounds__(THREADS) void sample_finish_kernel(SampleParams p, 
     s.hist[tid * 2] = h0;
     s.hist[tid * 2 + 1] = tid == THREADS - 1 ? 0 : h1;  // (what has no weight)
     __syncthreads();
-    finish(s, p, r, c, max, at, sl);
+    finish<true>(s, p, r, c, max, at, sl);
 }
 
 // Slices where a row is long and rows do not fill the chip by themselves: two launches and
