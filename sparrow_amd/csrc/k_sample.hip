@@ -162,7 +162,7 @@ struct Shared {
     uint32_t before[BINS];          // the tokens before a bin
     uint32_t start[BINS];           // where a bin's tokens stand in the list, if they do
     unsigned long long list[LIST];  // tokens, the largest first
-    uint32_t rank[512];
+    uint32_t slots[LIST];           // of the bins' tokens
     double whole[32], part[64];     // exp(-i), exp(-i / 64)
     double red[16];
     unsigned long long wave64[16];
@@ -265,40 +265,14 @@ struct SampleSlices {
     int32_t *upto;             // [rows][n][2]: those below this bin, and their number
 };
 
-// The n <= LIST tokens that `each` puts, in s.list: the largest first. Up to 512 by the number
-// of larger ones, which as many threads as there are count together (256 tokens: 64 reads
-// each, where a sort has 36 steps); more by a bitonic sort.
-template <typename F>
-__device__ __forceinline__ void gather(Shared &s, int n, F each) {
-    const int tid = threadIdx.x;
-    const bool count = n <= 512;
-    unsigned long long *raw = count ? s.hist : s.list;
-    __syncthreads();
-    if (tid == 0) s.n = 0;
+// The n <= LIST tokens in s.list, zeros behind them, the largest first.
+__device__ __forceinline__ void sort_list(Shared &s, int n) {
     int pow2 = 64;
     while (pow2 < n) pow2 *= 2;
-    for (int i = tid; i < pow2; i += THREADS) raw[i] = 0;
-    if (count && tid < 512) s.rank[tid] = 0;
     __syncthreads();
-    each([&](unsigned long long v) {
-        const uint32_t k = atomicAdd(&s.n, 1u);
-        if (k < LIST) raw[k] = v;
-    });
-    __syncthreads();
-    if (count) {
-        const int parts = THREADS / pow2, x = tid % pow2, some = pow2 / parts, a = tid / pow2 * some;
-        const unsigned long long v = raw[x];
-        uint32_t larger = 0;
-        for (int i = a; i < a + some; ++i) larger += raw[i] > v;
-        if (larger && x < n) atomicAdd(&s.rank[x], larger);
-        __syncthreads();
-        if (tid < n) s.list[s.rank[tid]] = raw[tid];
-        __syncthreads();
-        return;
-    }
     for (int k = 2; k <= pow2; k *= 2)
         for (int j = k / 2; j > 0; j /= 2) {
-            for (int i = tid; i < pow2 / 2; i += THREADS) {
+            for (int i = threadIdx.x; i < pow2 / 2; i += THREADS) {
                 const int x = i / j * 2 * j + i % j, y = x + j;
                 const unsigned long long a = s.list[x], b = s.list[y];
                 if (((x & k) == 0) == (a < b)) {
@@ -462,9 +436,14 @@ __device__ __forceinline__ Found locate(Shared &s, const float *row, int vocab, 
         return f;
     }
     // 3. its tokens, gathered and sorted
-    gather(s, n, [&](auto put) {
-        each_of_bin([&](uint32_t key, uint32_t, int i) { put((unsigned long long)key << 32 | (uint32_t)~i); });
+    __syncthreads();
+    if (tid == 0) s.n = 0;
+    for (int i = tid; i < LIST; i += THREADS) s.list[i] = 0;
+    __syncthreads();
+    each_of_bin([&](uint32_t key, uint32_t, int i) {
+        s.list[min(atomicAdd(&s.n, 1u), (uint32_t)(LIST - 1))] = (unsigned long long)key << 32 | (uint32_t)~i;
     });
+    sort_list(s, n);
     sum_losses(s, n, at);
     f = place_in(s, 0, n, by_rank, rank - rank0, mass - (double)mass0, with_equal);
     f.rank += rank0;
@@ -513,6 +492,74 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
     }
     __syncthreads();
     auto tokens = [&](int b) { return (int)((b + 1 < BINS ? s.before[b + 1] : live) - s.before[b]); };
+    // The n <= LIST tokens of the bins with a place in s.start, in s.list, the largest first; `each` puts
+    // them. Up to 128 go where the number of larger ones says, which as many threads as there are count
+    // together (16 reads each at most; 512 would be 256 reads, 8 us more than the following). Of more, a bin of m tokens is cut into m slots, which hold one or two each: a token goes to its slot, and
+    // counts the larger ones there. (Of 1000 to 2000 tokens a sort's 55 to 66 steps take 10 to 16 us more; it
+    // is left for slots of more than 64, of equal tokens.)
+    constexpr uint32_t NONE = ~0u;
+    auto sort_bins = [&](int n, auto each) {
+        __syncthreads();
+        if (tid == 0) s.n = s.hi = 0;
+        for (int i = tid; i < LIST; i += THREADS) s.slots[i] = 0;
+        __syncthreads();
+        each([&](unsigned long long v) { s.hist[min(atomicAdd(&s.n, 1u), (uint32_t)(LIST - 1))] = v; });
+        __syncthreads();
+        if (n <= 128) {
+            int pow2 = 64;
+            while (pow2 < n) pow2 *= 2;
+            const int x = tid % pow2, part = pow2 * pow2 / THREADS, a = tid / pow2 * part, z = min(a + part, n);
+            const unsigned long long v = s.hist[x];
+            uint32_t larger = 0;
+            for (int i = a; i < z; ++i) larger += s.hist[i] > v;
+            if (larger && x < n) atomicAdd(&s.slots[x], larger);
+            __syncthreads();
+            if (tid < n) s.list[s.slots[tid]] = s.hist[tid];
+            __syncthreads();
+            return;
+        }
+        unsigned long long v[2];
+        uint32_t slot[2], k[2], c[2], o[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int x = tid + i * THREADS;
+            uint32_t rest;
+            v[i] = x < n ? s.hist[x] : 0;
+            s.list[x] = v[i];
+            if (x >= n) continue;
+            const int b = at.bin(of_bits((uint32_t)(v[i] >> 32)), &rest);
+            slot[i] = s.start[b] + __umulhi(rest, (uint32_t)tokens(b));
+            k[i] = atomicAdd(&s.slots[slot[i]], 1u);
+            if (k[i] >= 64) s.hi = 1;
+        }
+        __syncthreads();
+        if (s.hi) {
+            sort_list(s, n);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) c[i] = s.slots[tid * 2 + i];
+        block_scan<uint32_t>(c[0], c[1], &o[0], &o[1], s.wave);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s.slots[tid * 2 + i] = o[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (tid + i * THREADS < n) s.list[s.slots[slot[i]] + k[i]] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (tid + i * THREADS >= n) continue;
+            k[i] = s.slots[slot[i]];
+            const int to = slot[i] + 1 < LIST ? (int)s.slots[slot[i] + 1] : n;
+            for (int y = (int)k[i]; y < to; ++y) k[i] += s.list[y] > v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (tid + i * THREADS < n) s.list[k[i]] = v[i];
+        __syncthreads();
+    };
     // the bin of a rank, and of a mass (the last one that is not empty and starts below it)
     auto bin_of_rank = [&](uint32_t rank) {
         int b = 0;
@@ -550,7 +597,9 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
             const int32_t *q = sl.upto + (size_t)r * sl.n * 2;
             listed = __all(cut < q[min(lane, sl.n - 1) * 2] && cut < q[min(lane + 64, sl.n - 1) * 2]);
         }
-        gather(s, few, [&](auto put) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s.start[tid * 2 + i] = tid * 2 + i <= cut ? c0[i] : NONE;
+        sort_bins(few, [&](auto put) {
             if (listed) {
                 for (int i = tid / SLICE_LIST; i < sl.n; i += THREADS / SLICE_LIST) {
                     const size_t x = (size_t)r * sl.n + i;
@@ -651,7 +700,6 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
     }
     from[3] = bin_of_mass((double)c.u * a0, false);
     to[3] = bin_of_mass((double)c.u * a1, false);
-    constexpr uint32_t NONE = ~0u;
     uint32_t some[2], start[2];
     bool in[2];
 #pragma unroll
@@ -669,7 +717,7 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
 #pragma unroll
         for (int i = 0; i < 2; ++i) s.start[tid * 2 + i] = in[i] ? start[i] : NONE;
         const float least_l = at.below(last), most_l = at.above(first);
-        gather(s, (int)together, [&](auto put) {
+        sort_bins((int)together, [&](auto put) {
             each_token<THREADS, AHEAD>(row, n, [&](float l, int i) {
                 uint32_t rest;
                 if (l >= least_l && l <= most_l && s.start[at.bin(l, &rest)] != NONE) put(token_word(l, i));
