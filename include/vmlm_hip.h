@@ -448,7 +448,11 @@ int vmlm_hip_rope_qk(float *q_out, size_t ldqo, float *k_out, size_t ldko, const
  * n_kv_heads)): out [batch][S][ldo]; rows from count[b] on and of idle sequences are left as they are. q and
  * the cache's keys come rotated. S is at most 64 with parents, 65535 without. A
  * query head with a NaN or an infinity gives NaN, a position with one in its key or value to the queries
- * that see it. `work`: vmlm_hip_attention_tree_kv4_work() bytes, 16-byte aligned, used by one
+ * that see it. Queries and weights are held in 22 bits, and so are a position's keys and values as far as
+ * they reach 2^-14 of the largest of its head (of the keys weighed by the queries' groups of 32 channels),
+ * smaller ones to 2^-36 of that one: results are off by f32 roundings of the queries times the largest value
+ * that a key's 32 channels can hold, and of the weights times the values' likewise. The keys and values
+ * of tokens that a token does not see change no bit of its result. `work`: vmlm_hip_attention_tree_kv4_work() bytes, 16-byte aligned, used by one
  * call at a time; null: the stream's own workspace, which a call under stream capture may
  * not use (9), since graphs that run at once would share it. */
 int vmlm_hip_attention_tree_kv4(const vmlm_kv4_cache *cache, const float *q, size_t ldq,

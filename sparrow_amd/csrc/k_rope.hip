@@ -11,7 +11,8 @@
 // launch.
 //
 // Angles: pos * freq / 2 pi is formed in 64 bits and its whole turns dropped there; a
-// 32-bit product would be off by 2^-24 of the angle itself (0.006 at position 100000).
+// 32-bit product would be off by 2^-24 of the angle itself (0.006 at position 100000). What
+// the fraction of a turn loses in f32 (up to 2^-25 of it) is turned by afterwards.
 #include <algorithm>
 
 #include "internal.hpp"
@@ -56,10 +57,11 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const double t = (double)pos * (p.freq[u * V + e] * 0.15915494309189533577);  // 1 / 2 pi
-            float s, c;
-            sincospif(2.0f * (float)(t - __builtin_rint(t)), &s, &c);
-            s *= p.m;
-            c *= p.m;
+            const double turn = t - __builtin_rint(t);
+            const float hi = (float)turn, rest = (float)(turn - (double)hi) * 6.28318531f;
+            float s0, c0;
+            sincospif(2.0f * hi, &s0, &c0);
+            const float s = p.m * __builtin_fmaf(c0, rest, s0), c = p.m * __builtin_fmaf(-s0, rest, c0);
             const int ia = INTER ? 2 * e : e, ib = INTER ? 2 * e + 1 : V + e;
             w[ia] = v[ia] * c - v[ib] * s;
             w[ib] = v[ia] * s + v[ib] * c;
