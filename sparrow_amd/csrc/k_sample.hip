@@ -22,6 +22,10 @@
 // A row is read once for its bins (a larger logit than those before moves them along), and once more,
 // by f32 comparisons, for the tokens to sort. Few rows are cut into slices, which also list the
 // tokens of their first bins, so that the second reading is seldom needed.
+//
+// 512 rows of 122753 (251 MB): 52 us greedy, HBM's rate; 103 with top_k 50 and 124 without a filter, the first
+// reading bound by 25 vector instructions a token and its LDS addition. One row 25 us (35 without a
+// filter): a slice's 9 and its end's 16, latencies.
 #include <algorithm>
 
 #include "internal.hpp"

@@ -24,7 +24,12 @@
 // small); a value's power of two goes to its weight, and the running maximum is that of
 // weight times value. It is kept an integer: the rescalings are exact, and the exponent
 // score * log2(e) - maximum is one fused operation that rounds at its own small size.
-// 16-bit terms hold 11 bits down to 2^-28 of the largest and round at 2^-39 of it below.
+// 16-bit terms stand below 2^11 and hold 11 bits down to 2^-14 and steps of 2^-24 below it.
+//
+// Bound by its instructions: with 63 tokens over 65463 positions, 36 heads of 64, 146 us, vector
+// instructions 63 % of the cycles and matrix instructions 28 %, which hardly overlap; 190 MB of cache
+// at 1.3 TB/s. 333 tokens of 3 sequences after 4000 positions, 32 heads over 8 of 128: 189 us, 68 % and 28 %. A
+// wave makes a block's operands for 64 queries (heads up to 64) or 32 (the registers there are).
 #include <algorithm>
 
 #include "kv4.hpp"
