@@ -446,7 +446,8 @@ int vmlm_hip_rope_qk(float *q_out, size_t ldqo, float *k_out, size_t ldko, const
 /* Each head of q [batch][S][ldq] attends, at token t, the positions before pos0[b], its own and
  * those of the tokens that it follows, directly or through others (head h reads kv head h / (n_heads /
  * n_kv_heads)): out [batch][S][ldo]; rows from count[b] on and of idle sequences are left as they are. q and
- * the cache's keys come rotated. S is at most 64 with parents, 65535 without. A
+ * the cache's keys come rotated. S is at most 64 with parents, 65535 without;
+ * batch * S * n_heads at most 2^27, batch * n_kv_heads 2^21. A
  * query head with a NaN or an infinity gives NaN, a position with one in its key or value to the queries
  * that see it. Queries and weights are held in 22 bits, and so are a position's keys and values as far as
  * they reach 2^-14 of the largest of its head (of the keys weighed by the queries' groups of 32 channels),

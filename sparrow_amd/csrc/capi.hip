@@ -1454,6 +1454,10 @@ static int check_tree_attn(const Kv4View &c, const float *q, size_t ldq, const i
     if (rc || c.B == 0 || S == 0 || H == 0) return rc;
     const size_t rows = (size_t)c.B * S, w = H * c.hd, nb = (size_t)c.B * 4;
     VMLM_GUARD(c.cap > 0, "kv4 tree attention: capacity 0");
+    // (a workgroup of 256 threads for 16 rows and more)
+    VMLM_GUARD(rows * H <= (size_t)1 << 27 && (size_t)c.B * c.Hkv <= (size_t)1 << 21,
+               "kv4 tree attention: %zu tokens of %zu heads (limit 2^27 together), %d sequences of %d kv heads (2^21)",
+               rows, H, c.B, c.Hkv);
     VMLM_GUARD(q && out, "kv4 tree attention: null queries or output");
     VMLM_GUARD(rows == 1 || (ldq >= w && ldo >= w),
                "kv4 tree attention: a row stride is below the row's width");
@@ -1478,6 +1482,9 @@ int vmlm_hip_attention_tree_kv4_work(const vmlm_kv4_cache *cache, size_t n_heads
     if (rc) return rc;
     VMLM_GUARD(c.Hkv > 0 && n_heads % c.Hkv == 0 && n_heads <= 65535 && S <= 65535,
                "kv4 tree attention: %zu heads over %d kv heads, %zu tokens (limits 65535)", n_heads, c.Hkv, S);
+    VMLM_GUARD(c.B * S * n_heads <= (size_t)1 << 27 && (size_t)c.B * c.Hkv <= (size_t)1 << 21,
+               "kv4 tree attention: %d x %zu tokens of %zu heads (limit 2^27 together), %d kv heads (2^21 of all)",
+               c.B, S, n_heads, c.Hkv);
     *bytes = tree_attn_work_floats(c, (int)n_heads, (int)S) * 4;
     return VMLM_OK;
 }

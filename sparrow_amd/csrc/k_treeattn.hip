@@ -69,8 +69,8 @@ struct TreeAttnParams {
     // tile of all sequences may have, 0 if each takes all of a sequence's
     int tiles, per;
     float *out;
-    int *dealt;   // [B][2]: a sequence's first stream, its shares
-    float *work;  // [stream][tile]: the shares' results
+    int *dealt;   // [B][2]: where a sequence's shares' results begin, how many shares it has
+    float *work;  // [..][tile]: the results, of sequences of more than one share
     float scale, sign;  // of the scores: sign * scale * 2^scale_e, scale in [1/2, 1) (or 0), times log2(e)
     int scale_e;
     int *guard;
@@ -238,7 +238,7 @@ __device__ __forceinline__ int shares_of(int blocks, float each) {
     return min(max((int)((float)blocks / each), 1), TA_SHARES);
 }
 struct Dealt {
-    int b, shares, rest;  // rest: share * Hkv + kv head
+    int b, shares, rest, at;  // rest: share * Hkv + kv head; at: where its shares' results begin
 };
 // The sequence and share of a stream, b < 0 if it has none; every wave finds them by itself.
 __device__ __forceinline__ Dealt deal(const TreeAttnParams &p, int stream, bool first_tile) {
@@ -262,20 +262,24 @@ __device__ __forceinline__ Dealt deal(const TreeAttnParams &p, int stream, bool 
     const bool tell = stream == 0 && first_tile && __builtin_amdgcn_readfirstlane(threadIdx.x) == 0;
     if (tell && __any(bad) && lane == 0) atomicOr(p.guard, 1);
     const float each = share_blocks(wave_sum_dpp(sum) * (float)p.c.Hkv, p.per);
-    Dealt d{-1, 1, 0};
-    int before = 0;
+    Dealt d{-1, 1, 0, 0};
+    uint32_t before = 0;
+    // (streams, 2^21 at most, below those whose results are kept, `per` at most: shares of two and more)
+    constexpr int KEPT = 22;
     for (int at = 0; at < p.c.B; at += 64) {
         if (at) blocks = blocks_of(at + lane, &bad);
         const int s = blocks ? shares_of(blocks, each) : 0, n = s * p.c.Hkv;
-        int upto = n;  // streams of the sequences up to the lane's
+        const uint32_t both = (uint32_t)n + (s > 1 ? (uint32_t)n << KEPT : 0u);
+        uint32_t upto = both;  // of the sequences up to the lane's
 #pragma unroll
         for (int i = 1; i < 64; i *= 2) {
-            const int v = __shfl_up(upto, i, 64);
+            const uint32_t v = __shfl_up(upto, i, 64);
             if (lane >= i) upto += v;
         }
-        const int from = before + upto - n;
+        const uint32_t first = before + upto - both;
+        const int from = (int)(first & ((1u << KEPT) - 1)), kept = (int)(first >> KEPT);
         if (tell && at + lane < p.c.B) {
-            p.dealt[2 * (at + lane)] = from;
+            p.dealt[2 * (at + lane)] = kept;
             p.dealt[2 * (at + lane) + 1] = s;
         }
         const unsigned long long here = __ballot(stream >= from && stream < from + n);
@@ -284,6 +288,7 @@ __device__ __forceinline__ Dealt deal(const TreeAttnParams &p, int stream, bool 
             d.b = at + i;
             d.shares = __builtin_amdgcn_readlane(s, i);
             d.rest = stream - __builtin_amdgcn_readlane(from, i);
+            d.at = __builtin_amdgcn_readlane(kept, i);
             if (!tell) break;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
@@ -302,7 +307,7 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     const int col = lane & 15, j = lane >> 4;
     // the tiles that read the same positions lie 8 workgroups apart: on one XCD
     const int x8 = blockIdx.x / 8, stream = x8 / p.tiles * 8 + (int)(blockIdx.x % 8), tile = x8 % p.tiles;
-    int b, kvh = stream % p.c.Hkv, share = 0, shares = 1;
+    int b, kvh = stream % p.c.Hkv, share = 0, shares = 1, kept = stream;
     if (p.per == 0) {
         b = stream / p.c.Hkv;
         if (b >= p.c.B) return;
@@ -316,6 +321,7 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         shares = d.shares;
         kvh = d.rest % p.c.Hkv;
         share = d.rest / p.c.Hkv;
+        kept = d.at + d.rest;
     }
     // the wave's query rows, loaded before anything is known of the sequence
     constexpr int CW = (HD + 63) / 64, RW = ROWS / TA_W;
@@ -850,7 +856,7 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
             const int R = row0 + r;
             p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * TA_UNBASE / L;
         } else {
-            float *pw = p.work + ((size_t)stream * p.tiles + tile) * (ROWS * (HD + 2));
+            float *pw = p.work + ((size_t)kept * p.tiles + tile) * (ROWS * (HD + 2));
             pw[r * HD + c] = o;
             if (c == 0) {
                 pw[ROWS * HD + 2 * r] = mx;
@@ -913,9 +919,9 @@ TreePlan tree_plan(const Kv4View &c, int H, int S) {
     pl.per = pairs * pl.tiles < slots || c.cap >= 8192 ? (int)(slots / pl.tiles) : 0;
     const size_t longest = (size_t)c.cap / KV4_BLOCK / TA_LEAST;  // shares of the longest sequence
     if (longest <= 1 || (c.B == 1 && pl.per < 2 * c.Hkv)) pl.per = 0;
-    // (one sequence gets no more than `per` in all; of several each may round up to one)
+    // (all shares of sequences of more than one are `per` at most; of several sequences each may round up to one)
     pl.streams = pl.per == 0 ? pairs : std::min(c.B == 1 ? (size_t)pl.per : pairs + pl.per, pairs * longest);
-    pl.work = pl.per == 0 ? 0 : ((size_t)c.B * 2 + 63) / 64 * 64 + pl.streams * pl.tiles * pl.rows * (c.hd + 2);
+    pl.work = pl.per == 0 ? 0 : ((size_t)c.B * 2 + 63) / 64 * 64 + (size_t)pl.per * pl.tiles * pl.rows * (c.hd + 2);
     return pl;
 }
 

@@ -11,6 +11,8 @@ import pytest
 from test_gpu_4bit import U, dev, device_cache, filled, new_model, ops, put  # noqa: F401
 from test_gpu_draft import check_sample, check_tree, random_tree, sample_ref, sees, spread, tree_ref
 
+from sparrow_amd import VmlmError
+
 pytestmark = pytest.mark.gpu
 
 
@@ -278,6 +280,50 @@ def test_attention_long_among_many(ops):
     check_tree(out[3:4], tree_ref(one, q[3:4], [n - S], [S], None, H, hd, scale))
     pos0[3], out[3] = -1, 0
     check_tree(out, tree_ref(few, q, pos0, [S] * B, None, H, hd, scale))
+
+
+@pytest.mark.parametrize("B", [1, 3])
+def test_attention_shares_refused_on_the_device(ops, B):
+    """Sequences whose positions are dealt out: tokens past the capacity and parents that are no earlier
+    token trip the guard, the others are right."""
+    rng = np.random.default_rng(78)
+    cap, hd, S = 4096, 64, 4
+    c, m = filled(ops, rng, B, 1, cap, hd, [cap] * B)
+    q = rng.standard_normal((B, S, hd), dtype=np.float32)
+    good = np.array([[-1, 0, 1, 0]] * B, np.int32)
+    bad = good.copy()
+    bad[0, 2] = 2
+    at = [4000] * B
+    for pos0, parent in (([cap - S + 1] + at[1:], good), ([2 ** 31 - 1] + at[1:], good), (at, bad)):
+        with pytest.raises(VmlmError) as e:
+            c.attention_tree(q, pos0, None, parent)
+        assert e.value.code == 9
+        out = np.full(q.shape, 3.0, np.float32)
+        with pytest.raises(VmlmError):
+            c.attention_tree(q, pos0, None, parent, out=out)
+    for pos0 in (at, [cap - S] + at[1:], [-1] + at[1:]):
+        check_tree(c.attention_tree(q, pos0, None, good), tree_ref(m, q, pos0, [S] * B, good, 1, hd, 0.125))
+
+
+def test_attention_shares_and_refused_sequences(dev, ops):
+    """On the device, past the guard: the refused sequence's rows stay, the others' are right."""
+    rng = np.random.default_rng(79)
+    B, cap, hd, S = 3, 4096, 64, 4
+    c, m = filled(ops, rng, B, 1, cap, hd, [cap] * B)
+    _, d = device_cache(dev, c)
+    q = rng.standard_normal((B, S, hd), dtype=np.float32)
+    parent = np.array([[-1, 0, 1, 0]] * B, np.int32)
+    parent[1, 3] = 3
+    pos0 = np.array([4090, 1000, 4093], np.int32)  # (the last one's tokens pass the capacity)
+    dq, dp, dt, do = dev.up(q), dev.up(pos0), dev.up(parent), dev.up(np.full(q.shape, 3.0, np.float32))
+    st = dev.stream()
+    dev.sync()
+    dev.check(dev.L.vmlm_hip_attention_tree_kv4(d, dq.ptr, hd, dp.ptr, None, dt.ptr, S, do.ptr, hd, 1, 0.125, None, 0, st))
+    dev.sync()
+    assert dev.L.vmlm_hip_check_guards() == 9
+    out = do.get()
+    assert (out[1:] == 3).all()
+    check_tree(out[:1], tree_ref(m, q[:1], pos0[:1], [S], parent[:1], 1, hd, 0.125))
 
 
 @pytest.mark.parametrize("G", [17, 63])

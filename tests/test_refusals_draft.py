@@ -123,6 +123,23 @@ def test_attention_refused_caches(L):
     assert attend(L, cache(n_kv_heads=0), H=0) == 9
 
 
+def test_attention_sizes_at_their_limits(L):
+    """More rows or heads than a grid takes."""
+    far = dict(k=1 << 40, v=2 << 40, k_meta=3 << 40, v_meta=4 << 40)
+    need = C.c_size_t()
+    for c, H, n in ((dict(batch=64, n_kv_heads=64, cap=32, head_dim=32), 64, 32769),
+                    (dict(batch=4096, n_kv_heads=1, cap=32, head_dim=32), 1024, 33),
+                    (dict(batch=65535, n_kv_heads=33, cap=32, head_dim=32), 33, 1)):
+        c = cache(**far, **c)
+        w = H * 32
+        assert attend(L, c, q=5 << 40, ldq=w, pos0=W, count=None, parent=None, n=n, out=9 << 40, ldo=w, H=H) == 9
+        assert "limit" in message(L) or "2^21" in message(L)
+        assert L.vmlm_hip_attention_tree_kv4_work(c, H, n, C.byref(need)) == 9
+    # what a workspace holds does not grow with the sequences that are not split
+    c = cache(**far, batch=2048, n_kv_heads=32, cap=8192, head_dim=128)
+    assert L.vmlm_hip_attention_tree_kv4_work(c, 256, 64, C.byref(need)) == 0 and 0 < need.value < 64 << 20
+
+
 @pytest.mark.parametrize("empty", [dict(n=0), dict(H=0), dict(c=dict(batch=0))])
 def test_attention_nothing_to_do(L, empty):
     if "c" in empty:
