@@ -43,7 +43,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2m __attribute__((ext_vector_type(2), aligned(4)));
 typedef uint32_t u32x4m __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x4l __attribute__((ext_vector_type(4)));
-typedef int i32x4l __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int TA_W = 4;  // waves of a workgroup
 constexpr float TA_NONE = -3.40282347e38f;  // the maximum of no score yet
@@ -841,23 +841,31 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         }
     }
     __syncthreads();
-    for (int i = tid; i < rows * HD; i += 64 * TA_W) {
-        const int r = i / HD, c = i % HD;
-        float mx = TA_NONE, L = 0.0f, o = 0.0f;
+    for (int i = tid; i < rows * (HD / 4); i += 64 * TA_W) {
+        const int r = i / (HD / 4), c = i % (HD / 4) * 4;
+        float mx = TA_NONE, L = 0.0f, f[TA_W];
 #pragma unroll
         for (int x = 0; x < TA_W; ++x) mx = fmaxf(mx, rm[(x * ROWS + r) * 2]);
 #pragma unroll
         for (int x = 0; x < TA_W; ++x) {
-            const float f = __builtin_amdgcn_exp2f(rm[(x * ROWS + r) * 2] - mx);
-            L = __builtin_fmaf(f, rm[(x * ROWS + r) * 2 + 1], L);
-            o = __builtin_fmaf(f, ((const float *)(lds + M::RO))[(x * ROWS + r) * HD + c], o);
+            f[x] = __builtin_amdgcn_exp2f(rm[(x * ROWS + r) * 2] - mx);
+            L = __builtin_fmaf(f[x], rm[(x * ROWS + r) * 2 + 1], L);
+        }
+        f32x4u o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < TA_W; ++x) {
+            const f32x4l v = *(const f32x4l *)((const float *)(lds + M::RO) + (x * ROWS + r) * HD + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f[x], v[e], o[e]);
         }
         if (shares == 1) {
             const int R = row0 + r;
-            p.out[((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c] = o * TA_UNBASE / L;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = o[e] * TA_UNBASE / L;
+            *(f32x4u *)(p.out + ((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c) = o;
         } else {
             float *pw = p.work + ((size_t)kept * p.tiles + tile) * (ROWS * (HD + 2));
-            pw[r * HD + c] = o;
+            *(f32x4u *)(pw + r * HD + c) = o;
             if (c == 0) {
                 pw[ROWS * HD + 2 * r] = mx;
                 pw[ROWS * HD + 2 * r + 1] = L;
