@@ -660,12 +660,16 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         }
         __builtin_amdgcn_wave_barrier();
         // 6. the running maximum of weight times value
-        // whether query t of the lane sees position at
-        auto sees = [&](int t, int at) {
+        // the block's positions that query t of the lane sees
+        auto sees = [&](int t) {
             const unsigned long long v = mask[t * 16 + col];
-            const int at0 = at - tr.pos0;
-            return p.parent ? at0 < 0 || (at0 < 64 && (v >> (at0 & 63) & 1)) : at <= (int)(uint32_t)v;
+            const int own = tr.pos0 - p0, n = (int)(uint32_t)v - p0;  // the tokens' first; the last seen
+            if (p.parent)
+                return own >= 32 ? ~0u : own < 0 ? (own > -64 ? (uint32_t)(v >> -own) : 0u) : (uint32_t)(v << own) | ((1u << own) - 1);
+            return n >= 31 ? ~0u : n < 0 ? 0u : (2u << n) - 1;
         };
+        // whether the query's scores are in the millions: their rounding is larger than a weight's
+        auto far = [&](int t) { return fabsf(m[t]) >= TA_FAR && m[t] > TA_NONE; };
         float top[MT];
         uint32_t seen = 0;  // a byte a tile
         if (is_shared()) {
@@ -680,14 +684,15 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const int f = fe[t * 16 + col];
+                const uint32_t in8 = edge ? sees(t) >> (8 * j) & 255u : 255u;
+                seen |= in8 << (8 * t);
                 top[t] = TA_NONE;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float y = ldexpf(S[t][i / 4][i % 4], ek[8 * j + i] + f);
                     S[t][i / 4][i % 4] = y;
-                    const bool in = !edge || sees(t, p0 + 8 * j + i);
-                    seen |= (in ? 1u : 0u) << (8 * t + i);
-                    top[t] = in ? fmaxf(top[t], __builtin_fmaf(y, cs, ev[8 * j + i])) : top[t];
+                    const float v = __builtin_fmaf(y, cs, ev[8 * j + i]);
+                    top[t] = fmaxf(top[t], in8 >> i & 1 ? v : TA_NONE);
                 }
                 apart();
             }
@@ -707,17 +712,25 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
                 for (int n = 0; n <= NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) O[t][n][i] *= corr;
-                far_any |= __any(fabsf(to) >= TA_FAR && to > TA_NONE);
+                far_any |= __any(far(t));
             }
         }
         // 7. weights, in S's place
         if (is_shared()) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float base = (float)(ev_run - TA_TOP_E) - (m[t] - TA_BASE);
+                const float v = (float)(ev_run - TA_TOP_E);
+                float f = cq[t], base = v - (m[t] - TA_BASE);
+                if (far_any && far(t)) {  // (the exponents themselves, none above TA_BASE + TA_SLACK)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        S[t][i / 4][i % 4] = __builtin_fmaf(S[t][i / 4][i % 4], f, v) - m[t];
+                    f = 1.0f;
+                    base = TA_BASE;
+                }
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    S[t][i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i / 4][i % 4], cq[t], base));
+                    S[t][i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i / 4][i % 4], f, base));
                 if (!M::ONES) {
                     float sum = 0.0f;
 #pragma unroll
@@ -729,13 +742,12 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const float base = m[t] - TA_BASE;
-                // scores of millions: their rounding is larger than a weight's
-                const bool far = fabsf(m[t]) >= TA_FAR && m[t] > TA_NONE;
+                const bool is_far = far_any && far(t);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float y = S[t][i / 4][i % 4], v = ev[8 * j + i];
-                    float d = __builtin_fmaf(y, cs, v - base);
-                    if (far) d = (__builtin_fmaf(y, cs, v) - m[t]) + TA_BASE;
+                    const float v = ev[8 * j + i];
+                    float d = __builtin_fmaf(S[t][i / 4][i % 4], cs, v - base);
+                    if (is_far) d = (__builtin_fmaf(S[t][i / 4][i % 4], cs, v) - m[t]) + TA_BASE;
                     const float w8 = seen >> (8 * t + i) & 1 ? __builtin_amdgcn_exp2f(d) : 0.0f;
                     S[t][i / 4][i % 4] = w8;
                     l[t] = __builtin_fmaf(w8, iev[8 * j + i], l[t]);
@@ -789,7 +801,7 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
                     const int g = NG == 1 ? 0 : (at >> 5) * (NG / 2) + i;
 #pragma unroll
                     for (int t = 0; t < MT; ++t)
-                        if (sees(t, p0 + (at & 31)) && j == g / 2) {
+                        if ((sees(t) >> (at & 31) & 1) && j == g / 2) {
                             O[t][NT][0] = g % 2 ? O[t][NT][0] : __builtin_nanf("");
                             O[t][NT][2] = g % 2 ? __builtin_nanf("") : O[t][NT][2];
                         }
@@ -806,7 +818,7 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         const Raw raw = next;
         if (blk + TA_W < b1) next.load(p.c, head, blk + TA_W, lane);
         const bool edge = blk >= whole;
-        bool shared = !edge && !far_any;
+        bool shared = !edge;
         if (shared && !shared_meta(raw)) shared = choose(raw) && shared_meta(raw);
         if (!shared) own_meta(raw, blk * KV4_BLOCK, edge);
         block(raw, blk, edge, shared);

@@ -182,6 +182,33 @@ def test_attention_scores_far_from_zero(ops, H, Hkv, hd, n, S, far):
     check_tree(out, exact_ref(m, q, [pos0], parent, Hkv, hd, scale))
 
 
+@pytest.mark.parametrize("far", [2 ** 24, 2 ** 27, 2 ** 40, 2 ** 90])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("H,Hkv,hd,n,S", SHAPES)
+def test_attention_scores_beyond_f32s_steps(ops, H, Hkv, hd, n, S, far, sign):
+    """Scores so large that a step of f32 is more than a weight's exponent: 2^28 and more, whose steps are 32
+    and more, so that what the largest ones' weights are to each other is within a rounding of the
+    score. They are 2^21 and more from the others', which have none: the output lies between the least
+    and the largest of the values at those positions, off by the sums' roundings."""
+    rng = np.random.default_rng(n)
+    q, k, v, parent, pos0 = case(rng, H, Hkv, hd, n, S)
+    q[:], k[:] = 0, 0
+    q[..., 0], q[..., 1] = np.float32(far) * sign, np.float32(far) / 8
+    k[..., 0] = 15
+    k[..., 1] = rng.integers(0, 6, k.shape[:-1])
+    out, m, q, scale = run(ops, q, k, v, parent, pos0, 1.0)
+    assert np.array_equal(m["k"][0, :, :n], k[0].transpose(1, 0, 2))
+    out = out.reshape(S, Hkv, H // Hkv, hd)
+    for t in range(S):
+        see = sees(parent[0], pos0, S, t)
+        for kv in range(Hkv):
+            score = k[0, see, kv, 1]
+            top = see[score == score.max()]
+            x = m["v"][0, kv, top]
+            tol = (96 + n) * U * np.abs(m["v"][0, kv, see]).max()
+            assert (out[t, kv] >= x.min(0) - tol).all() and (out[t, kv] <= x.max(0) + tol).all()
+
+
 @pytest.mark.parametrize("H,Hkv,hd", [(1, 1, 32), (1, 1, 64), (4, 1, 128), (3, 1, 256), (2, 1, 64)])
 def test_attention_every_bit_of_the_weights(ops, H, Hkv, hd):
     """One position has nearly all the weight, and half of its channels hold an exact zero
