@@ -323,16 +323,21 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         share = d.rest / p.c.Hkv;
         kept = d.at + d.rest;
     }
-    // the wave's query rows, loaded before anything is known of the sequence
-    constexpr int CW = (HD + 63) / 64, RW = ROWS / TA_W;
+    // 16 queries a wave, loaded before anything is known of the sequence: lane (column, j) holds
+    // channels CL j .. of its column's
+    constexpr int GL = CL < 32 ? 1 : CL / 32;  // groups of the lane's channels
     const int row0 = tile * ROWS;
-    float x[RW][CW];
+    const bool mine = w < MT;
+    float x[CL];
+    if (mine) {
+        const int R = min(row0 + w * 16 + col, p.S * p.G - 1), t = R / p.G;
+        const float *q = p.q + ((size_t)b * p.S + t) * p.ldq + ((size_t)kvh * p.G + R % p.G) * HD + CL * j;
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        const int R = min(row0 + w + i * TA_W, p.S * p.G - 1), t = R / p.G;
-        const float *q = p.q + ((size_t)b * p.S + t) * p.ldq + ((size_t)kvh * p.G + R % p.G) * HD;
+        for (int c = 0; c < CL; c += 4) {
+            const f32x4u v = *(const f32x4u *)(q + c);
 #pragma unroll
-        for (int c = 0; c < CW; ++c) x[i][c] = q[min(c * 64 + lane, HD - 1)];
+            for (int e = 0; e < 4; ++e) x[c + e] = v[e];
+        }
     }
     const TreeRows tr = tree_rows(p.pos0, p.count, p.parent, p.S, p.c.cap, b, p.guard,
                                   kvh == 0 && tile == 0 && share == 0);
@@ -354,37 +359,44 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     // 1. the queries' operands
     int *fe = (int *)(lds + M::F), *ge = (int *)(lds + M::E);
     unsigned long long *mask = (unsigned long long *)(lds + M::MASK);
-    for (int i = tid; i < MT * 64; i += 64 * TA_W)  // the sums' step: zeros where there is no group
-        *(u32x4 *)(lds + M::Q + ((i >> 6) * M::FR + 2 * KS) * 1024 + (i & 63) * 16) = u32x4{0, 0, 0, 0};
     for (int i = tid; i < TA_W * 64; i += 64 * TA_W)
         *(u32x4 *)(lds + M::WAVE + (i >> 6) * M::WB + (i & 63) * 16) =
             M::ONES && (i & 63) >= 60 ? u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u} : u32x4{0, 0, 0, 0};
     if (tid < 16) ge[tid] = TA_NO_GROUP;
     __syncthreads();
-    int own_e[RW], bad[RW];  // a row's power of two
+    int own_e = 0;  // the query's power of two
+    bool bad = false;
+    auto group_of = [&](int g) { return CL < 32 ? j * CL / 32 : j * GL + g; };  // the lane's g-th
+    if (mine) {
+        float mx[GL], most = 0.0f;
+        int fine = 1;
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        const int r = w + i * TA_W;
-        float mx[CW], most = 0.0f;
-        bad[i] = 0;
+        for (int g = 0; g < GL; ++g) {
+            mx[g] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < CW; ++c) {
-            if (r >= rows || c * 64 + lane >= HD) x[i][c] = 0.0f;
-            mx[c] = ta_swap16(ta_row16(fabsf(x[i][c]), ta_max), ta_max);  // of its 32 channels
-            most = fmaxf(most, mx[c]);
-            bad[i] |= !(fabsf(x[i][c]) <= 3.40282347e38f);
+            for (int c = 0; c < CL / GL; ++c) {
+                float &v = x[g * 32 + c];
+                if (w * 16 + col >= rows) v = 0.0f;
+                mx[g] = fmaxf(mx[g], fabsf(v));
+                fine &= fabsf(v) <= 3.40282347e38f;
+            }
+            if (CL <= 16) mx[g] = ta_swap16(mx[g], ta_max);
+            if (CL <= 8) mx[g] = ta_swap32(mx[g], ta_max);
+            most = fmaxf(most, mx[g]);
         }
-        most = ta_swap32(most, ta_max);
-        bad[i] = __any(bad[i]);
-        own_e[i] = most > 0.0f && !bad[i] ? ilogbf(most) : 0;
-        if (lane == 0) fe[r] = own_e[i] - 8 + p.scale_e;
+        most = ta_swap32(ta_swap16(most, ta_max), ta_max);
+        bad = ta_swap32(ta_swap16(fine ? 0.0f : 1.0f, ta_max), ta_max) > 0.0f;
+        own_e = most > 0.0f && !bad ? ilogbf(most) : 0;
+        if (j == 0) fe[w * 16 + col] = own_e - 8 + p.scale_e;
 #pragma unroll
-        for (int c = 0; c < CW; ++c)
-            if ((lane & 31) == 0 && c * 64 + lane < HD && mx[c] > 0.0f && !bad[i])
-                atomicMax(&ge[c * 2 + lane / 32], ilogbf(mx[c]) - own_e[i]);
+        for (int g = 0; g < GL; ++g) {
+            const float e = mx[g] > 0.0f && !bad ? (float)(ilogbf(mx[g]) - own_e) : (float)TA_NO_GROUP;
+            const float all = ta_row16(e, ta_max);
+            if (col == 0) atomicMax(&ge[group_of(g)], (int)all);
+        }
     }
     if (p.parent) {
-        if (w == 0) {  // ancestors by doubling: of 2, 4, 8 .. tokens at once
+        if (w == TA_W - 1) {  // ancestors by doubling: of 2, 4, 8 .. tokens at once
             int up = tr.parent;
             unsigned long long seen = 1ull << lane;
 #pragma unroll
@@ -407,27 +419,46 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         mask[tid] = (uint32_t)(tr.pos0 + (row0 + min(tid, rows - 1)) / p.G);  // the last position
     }
     __syncthreads();
+    if (mine) {
+        uint8_t *at = lds + M::Q + w * M::FR * 1024 + lane * 16;
+        const Rest rest;
+        float sum[GL];
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        const int r = w + i * TA_W;
-        uint8_t *at = lds + M::Q + (r / 16) * M::FR * 1024 + (r % 16) * 16;
+        for (int g = 0; g < GL; ++g) sum[g] = 0.0f;
 #pragma unroll
-        for (int cc = 0; cc < CW; ++cc) {
-            const int c = cc * 64 + lane, g = min(c / 32, NG - 1);
-            const float y = bad[i] ? __builtin_nanf("") : ldexpf(x[i][cc] * p.sign, 8 - own_e[i] - ge[g]);  // below 2^9
-            const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
-            const float sum = ta_swap16(ta_row16((float)hi + (float)lo, ta_add), ta_add);
-            if (c >= HD) continue;
-            _Float16 *o = (_Float16 *)(at + (2 * (c % CL / 8)) * 1024 + c / CL * 256) + slot8(c % 8);
-            o[0] = hi;
-            o[512] = lo;
-            if ((c & 31) == 0) {
-                const _Float16 sh = (_Float16)sum, sl = (_Float16)(sum - (float)sh);
-                _Float16 *s = (_Float16 *)(at + 2 * KS * 1024 + g / 4 * 256) + g % 4 * 2;
-                s[0] = s[1] = sh;
-                s[256] = s[257] = sl;
+        for (int s = 0; s < KS; ++s) {
+            const int e = 8 - own_e - ge[group_of(s / 4)];
+            _Float16 hi[8], lo[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float y = bad ? __builtin_nanf("") : ldexpf(x[8 * s + c] * p.sign, e);  // below 2^9
+                hi[c] = (_Float16)y;
+                lo[c] = rest(y, hi[c]);
+                sum[CL < 32 ? 0 : s / 4] += (float)hi[c] + (float)lo[c];
             }
+            *(f16x8 *)(at + 2 * s * 1024) = f16x8{hi[0], hi[4], hi[1], hi[5], hi[2], hi[6], hi[3], hi[7]};
+            *(f16x8 *)(at + (2 * s + 1) * 1024) = f16x8{lo[0], lo[4], lo[1], lo[5], lo[2], lo[6], lo[3], lo[7]};
         }
+#pragma unroll
+        for (int g = 0; g < GL; ++g) {
+            if (CL <= 16) sum[g] = ta_swap16(sum[g], ta_add);
+            if (CL <= 8) sum[g] = ta_swap32(sum[g], ta_add);
+        }
+        // the sums' step: of lane j twice the upper terms of groups 4 (j & 1) .. where j < 2, else the lower
+        uint32_t e[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int g = 4 * (j & 1) + i;
+            const int from = col + 16 * (NG == 8 ? (g >> 1) & 3 : NG == 4 ? i : NG == 2 ? (i & 1) * 2 : 0);
+            float v = __shfl(sum[0], from, 64);
+            if (GL == 2) {
+                const float v1 = __shfl(sum[GL - 1], from, 64);
+                v = g & 1 ? v1 : v;
+            }
+            const _Float16 h = (_Float16)v, l = rest(v, h), o = j < 2 ? h : l;
+            if (g < NG) e[i] = __builtin_bit_cast(uint32_t, f16x2{o, o});
+        }
+        *(u32x4 *)(at + 2 * KS * 1024) = u32x4{e[0], e[1], e[2], e[3]};
     }
     __syncthreads();
 
