@@ -176,34 +176,21 @@ struct RawBlock {
     static constexpr int NG = HD / 32, KD = HD / 32, GX = NG < 4 ? NG : 4;
     static constexpr int OWN = HD == 256 ? 2 : 1, VM = NG < 2 ? 1 : NG / 2;
     uint32_t k[2][KD], km[2][GX], own[2][OWN], v[HD / 16], vm[VM];
-    __device__ __forceinline__ void load(const Kv4View &c, size_t head, int blk, int lane) {
+    // (addresses: the same for all lanes, and 32 bits of a lane's own)
+    __device__ __forceinline__ static uint32_t key_row(int r, int x) { return 8 * (r >> 2) + (r & 3) + 4 * x; }
+    __device__ __forceinline__ void load_meta(const Kv4View &c, size_t row0, int lane) {
         const int r = lane & 15, j = lane >> 4;
-        // (addresses: the same for all lanes, and 32 bits of a lane's own)
-        const size_t row0 = head * c.cap + blk * KV4_BLOCK;
-        const uint8_t *kb = c.k + row0 * (HD / 2);
-        const uint32_t *kmb = c.km + row0 * NG;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const uint32_t row = 8 * (r >> 2) + (r & 3) + 4 * x;
-            const uint8_t *kp = kb + (row * (HD / 2) + j * (HD / 8));
-            const uint32_t *mp = kmb + row * NG;
+            const uint32_t *mp = c.km + row0 * NG + key_row(r, x) * NG;
             if constexpr (HD == 32) {
-                k[x][0] = *(const uint32_t *)kp;
                 km[x][0] = own[x][0] = mp[0];
             } else if constexpr (HD == 64) {
-                const u32x2m a = *(const u32x2m *)kp, b = *(const u32x2m *)mp;
-                k[x][0] = a[0];
-                k[x][1] = a[1];
+                const u32x2m b = *(const u32x2m *)mp;
                 km[x][0] = b[0];
                 km[x][1] = b[1];
                 own[x][0] = j < 2 ? b[0] : b[1];
             } else {
-#pragma unroll
-                for (int i = 0; i < KD; i += 4) {
-                    const u32x4m a = *(const u32x4m *)(kp + i * 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) k[x][i + e] = a[e];
-                }
                 const u32x4m b = *(const u32x4m *)(mp + (NG == 8 ? 4 * (j & 1) : 0));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) km[x][e] = b[e];
@@ -211,12 +198,35 @@ struct RawBlock {
                 for (int e = 0; e < OWN; ++e) own[x][e] = mp[j * OWN + e];
             }
         }
-        const uint32_t *vp = (const uint32_t *)(c.v + row0 * (HD / 2));
-#pragma unroll
-        for (int n = 0; n < HD / 16; ++n) v[n] = vp[(uint32_t)((n * 16 + r) * 4 + j)];
         const uint32_t *mp = c.vm + row0 * NG + (uint32_t)((lane & 31) * NG + (lane >> 5) * (NG / 2));
 #pragma unroll
         for (int i = 0; i < VM; ++i) vm[i] = mp[i];
+    }
+    __device__ __forceinline__ void load_k(const Kv4View &c, size_t row0, int lane) {
+        const int r = lane & 15, j = lane >> 4;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint8_t *kp = c.k + row0 * (HD / 2) + (key_row(r, x) * (HD / 2) + j * (HD / 8));
+            if constexpr (HD == 32) {
+                k[x][0] = *(const uint32_t *)kp;
+            } else if constexpr (HD == 64) {
+                const u32x2m a = *(const u32x2m *)kp;
+                k[x][0] = a[0];
+                k[x][1] = a[1];
+            } else {
+#pragma unroll
+                for (int i = 0; i < KD; i += 4) {
+                    const u32x4m a = *(const u32x4m *)(kp + i * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) k[x][i + e] = a[e];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const Kv4View &c, size_t row0, int lane) {
+        const uint32_t *vp = (const uint32_t *)(c.v + row0 * (HD / 2));
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) v[n] = vp[(uint32_t)((n * 16 + (lane & 15)) * 4 + (lane >> 4))];
     }
 };
 
@@ -639,7 +649,7 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
 
     // What follows a block's meta. (One copy of the products for both kinds of blocks: with
     // two, the accumulators took their registers twice.)
-    auto block = [&](const Raw &raw, int blk, bool edge, bool shared) {
+    auto block = [&](Raw &raw, int blk, size_t next, bool edge, bool shared) {
         const int p0 = blk * KV4_BLOCK;
         // (kept from splitting the code after it in two)
         auto is_shared = [&] {
@@ -677,6 +687,7 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
                 for (int i = 0; i < D; ++i) kf[x][o * D + i] = Codes8(raw.k[x][o * D + i], s4, c4).v;
             }
         }
+        raw.load_k(p.c, next, lane);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             apart();
@@ -820,6 +831,7 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
 #pragma unroll
             for (int t = 0; t < MT; ++t) O[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t], O[t][n], 0, 0, 0);
         }
+        raw.load_v(p.c, next, lane);
         // 9. values that are NaN, to the queries that see them: through the middles' sums
         unsigned long long any_nan = 0;
 #pragma unroll
@@ -843,16 +855,22 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     };
 
     const int whole = min(b1, min(zone, last + 1) / KV4_BLOCK);  // blocks that all queries see
-    Raw next;
-    if (b0 + w < b1) next.load(p.c, head, b0 + w, lane);
+    Raw raw;
+    const size_t first = head * p.c.cap;
+    if (b0 + w < b1) {
+        raw.load_meta(p.c, first + (b0 + w) * KV4_BLOCK, lane);
+        raw.load_k(p.c, first + (b0 + w) * KV4_BLOCK, lane);
+        raw.load_v(p.c, first + (b0 + w) * KV4_BLOCK, lane);
+    }
     for (int blk = b0 + w; blk < b1; blk += TA_W) {
-        const Raw raw = next;
-        if (blk + TA_W < b1) next.load(p.c, head, blk + TA_W, lane);
         const bool edge = blk >= whole;
         bool shared = !edge;
         if (shared && !shared_meta(raw)) shared = choose(raw) && shared_meta(raw);
         if (!shared) own_meta(raw, blk * KV4_BLOCK, edge);
-        block(raw, blk, edge, shared);
+        // what comes next into the same registers, as soon as they are read (the last block again at the end)
+        const size_t next = first + (blk + TA_W < b1 ? blk + TA_W : blk) * KV4_BLOCK;
+        raw.load_meta(p.c, next, lane);
+        block(raw, blk, next, edge, shared);
     }
     if (M::ONES) {
 #pragma unroll
