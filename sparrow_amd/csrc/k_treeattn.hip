@@ -147,7 +147,7 @@ __device__ __forceinline__ uint32_t minus24(uint32_t s) {
 __device__ __forceinline__ int slot8(int o) { return o < 4 ? 2 * o : 2 * o - 7; }
 
 // LDS of a workgroup: the queries' operands [tile][step and term, then the sums][lane][8], for each
-// wave its block's V middles as f16 [16][32], scales [8][32] and three numbers for each position, for each
+// wave its block's meta and three numbers for each position (V's middles as f16 [16][32]), for each
 // query its power of two and the tokens it sees, for each group the queries' weight; the waves' results
 // then lie over it all.
 template <int HD, int MT>
@@ -157,8 +157,10 @@ struct TreeLds {
     static constexpr bool ONES = NG < 8;  // the middles' rows leave one for the weights' sum
     static constexpr int Q = 0;
     static constexpr int WAVE = Q + MT * FR * 1024;
-    static constexpr int SC = 1024, N = SC + 512;  // scales [8][32], numbers
-    static constexpr int WB = N + 3 * 128;
+    static constexpr int SC = 1024, N = SC + 512;  // V's scales [8][32], numbers
+    static constexpr int KG = NG > 4 ? 8 : 4;
+    static constexpr int KM = N + 3 * 128, KSC = KM + 32 * KG * 4;  // K's middles [32][KG], scales [group][32]
+    static constexpr int WB = KSC + NG * 64;
     static constexpr int F = WAVE + TA_W * WB;
     static constexpr int MASK = F + MT * 64;  // u64
     static constexpr int E = MASK + MT * 128;
@@ -173,34 +175,26 @@ struct TreeLds {
 // What a wave reads of a block of 32 positions.
 template <int HD>
 struct RawBlock {
-    static constexpr int NG = HD / 32, KD = HD / 32, GX = NG < 4 ? NG : 4;
+    static constexpr int NG = HD / 32, KD = HD / 32;
     static constexpr int OWN = HD == 256 ? 2 : 1, VM = NG < 2 ? 1 : NG / 2;
-    uint32_t k[2][KD], km[2][GX], own[2][OWN], v[HD / 16], vm[VM];
+    uint32_t k[2][KD], v[HD / 16], km[VM], vm[VM];  // meta: of position lane % 32, half of the groups
     // (addresses: the same for all lanes, and 32 bits of a lane's own)
     __device__ __forceinline__ static uint32_t key_row(int r, int x) { return 8 * (r >> 2) + (r & 3) + 4 * x; }
     __device__ __forceinline__ void load_meta(const Kv4View &c, size_t row0, int lane) {
-        const int r = lane & 15, j = lane >> 4;
+        const uint32_t m = (lane & 31) * NG + (lane >> 5) * (NG / 2);
+        const uint32_t *kp = c.km + row0 * NG + m, *vp = c.vm + row0 * NG + m;
+        if constexpr (VM == 1) {
+            km[0] = kp[0];
+            vm[0] = vp[0];
+        } else {
+            typedef uint32_t vec __attribute__((ext_vector_type(VM), aligned(4)));
+            const vec a = *(const vec *)kp, b = *(const vec *)vp;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint32_t *mp = c.km + row0 * NG + key_row(r, x) * NG;
-            if constexpr (HD == 32) {
-                km[x][0] = own[x][0] = mp[0];
-            } else if constexpr (HD == 64) {
-                const u32x2m b = *(const u32x2m *)mp;
-                km[x][0] = b[0];
-                km[x][1] = b[1];
-                own[x][0] = j < 2 ? b[0] : b[1];
-            } else {
-                const u32x4m b = *(const u32x4m *)(mp + (NG == 8 ? 4 * (j & 1) : 0));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) km[x][e] = b[e];
-#pragma unroll
-                for (int e = 0; e < OWN; ++e) own[x][e] = mp[j * OWN + e];
+            for (int i = 0; i < VM; ++i) {
+                km[i] = a[i];
+                vm[i] = b[i];
             }
         }
-        const uint32_t *mp = c.vm + row0 * NG + (uint32_t)((lane & 31) * NG + (lane >> 5) * (NG / 2));
-#pragma unroll
-        for (int i = 0; i < VM; ++i) vm[i] = mp[i];
     }
     __device__ __forceinline__ void load_k(const Kv4View &c, size_t row0, int lane) {
         const int r = lane & 15, j = lane >> 4;
@@ -372,6 +366,9 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     for (int i = tid; i < TA_W * 64; i += 64 * TA_W)
         *(u32x4 *)(lds + M::WAVE + (i >> 6) * M::WB + (i & 63) * 16) =
             M::ONES && (i & 63) >= 60 ? u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u} : u32x4{0, 0, 0, 0};
+    if (NG < 4)  // (no group there)
+        for (int i = tid; i < TA_W * 32; i += 64 * TA_W)
+            *(u32x4 *)(lds + M::WAVE + (i >> 5) * M::WB + M::KM + (i & 31) * 16) = u32x4{0, 0, 0, 0};
     if (tid < 16) ge[tid] = TA_NO_GROUP;
     __syncthreads();
     int own_e = 0;  // the query's power of two
@@ -491,11 +488,10 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     // two: keys stand below 2^ek, values below 2^ev, those of the block that they were taken from with
     // room above. kg and vg bring scales to them, cq scores back.
     int ek_run = 0, ev_run = 0;
-    float kg[Raw::GX], kown[Raw::OWN], vg = 0.0f;
+    constexpr int VM = Raw::VM;
+    float kg[VM], vg = 0.0f;
 #pragma unroll
-    for (int g = 0; g < Raw::GX; ++g) kg[g] = 0.0f;
-#pragma unroll
-    for (int o = 0; o < Raw::OWN; ++o) kown[o] = 0.0f;
+    for (int i = 0; i < VM; ++i) kg[i] = 0.0f;
     bool far_any = false;
 
     // (nothing is moved over it, nor kept in registers for what comes after: fewer of them)
@@ -503,78 +499,63 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // the group of the lane's g-th meta, and of its o-th codes
-    auto meta_group = [&](int g) { return NG == 8 ? 4 * (j & 1) + g : g; };
+    const int lp = lane & 31, hf = lane >> 5;
+    // the group of the lane's i-th meta, and of its o-th K codes
+    auto group = [&](int i) { return NG == 1 ? 0 : hf * VM + i; };
     auto own_group = [&](int o) { return NG == 1 ? 0 : NG == 2 ? j >> 1 : j * Raw::OWN + o; };
 
     // What the products take of a block's meta: middles as two f16 terms, scales.
-    uint32_t middles[2][Raw::GX], vmiddles[Raw::VM];
-    float own[2][Raw::OWN], vscales[Raw::VM];
-    unsigned long long nan_p[Raw::VM];  // lanes whose value's meta is a NaN
+    uint32_t kmid[VM], vmid[VM];
+    float kscale[VM], vscale[VM];
+    unsigned long long nan_p[VM];  // lanes whose value's meta is a NaN
 
     // 2. by the shared powers of two; false where a position is too large for them, or its keys or a
-    // group of its values smaller than 2^-TA_SPAN of them
+    // group of its values smaller than 2^-TA_SPAN of them (zeros lose nothing)
     auto shared_meta = [&](const Raw &raw) {
-        float hi = 0.0f, lo = __builtin_inff();
+        float kmost = 0.0f, hi = 0.0f, lo = __builtin_inff();
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            float most = 0.0f;
-#pragma unroll
-            for (int g = 0; g < Raw::GX; ++g) {
-                const float s = 8.0f * (kv4_scale(raw.km[x][g]) * kg[g]);
-                const float mid = __builtin_fmaf(kv4_min(raw.km[x][g]), kg[g], s);
-                most = fmaxf(most, fmaxf(fabsf(mid), s));
-                middles[x][g] = two_terms(mid, rest);
-            }
-            hi = fmaxf(hi, most);
-            lo = fminf(lo, most);
-#pragma unroll
-            for (int o = 0; o < Raw::OWN; ++o) own[x][o] = kv4_scale(raw.own[x][o]) * kown[o];
-        }
-        float most = 0.0f;
-#pragma unroll
-        for (int i = 0; i < Raw::VM; ++i) {
-            vscales[i] = kv4_scale(raw.vm[i]) * vg;
-            const float mid = __builtin_fmaf(kv4_min(raw.vm[i]), vg, 8.0f * vscales[i]);
-            const float v = fmaxf(fabsf(mid), 8.0f * vscales[i]);
-            most = fmaxf(most, v);
-            lo = fminf(lo, v == 0.0f ? TA_TOP : v);  // (zeros lose nothing)
-            vmiddles[i] = two_terms(mid, rest);
+        for (int i = 0; i < VM; ++i) {
+            kscale[i] = kv4_scale(raw.km[i]) * kg[i];
+            const float k8 = 8.0f * kscale[i], km = __builtin_fmaf(kv4_min(raw.km[i]), kg[i], k8);
+            kmost = fmaxf(kmost, fmaxf(fabsf(km), k8));
+            kmid[i] = two_terms(km, rest);
+            vscale[i] = kv4_scale(raw.vm[i]) * vg;
+            const float v8 = 8.0f * vscale[i], vm = __builtin_fmaf(kv4_min(raw.vm[i]), vg, v8);
+            const float v = fmaxf(fabsf(vm), v8);
+            hi = fmaxf(hi, v);
+            lo = fminf(lo, v == 0.0f ? TA_TOP : v);
+            vmid[i] = two_terms(vm, rest);
             nan_p[i] = 0;
         }
-        return __all(fmaxf(hi, most) < TA_TOP && lo >= TA_TOP / (1 << TA_SPAN));
+        if (NG > 1) kmost = ta_swap32(kmost, ta_max);
+        lo = fminf(lo, kmost == 0.0f && kg[0] > 0.0f ? TA_TOP : kmost);
+        return __all(fmaxf(kmost, hi) < TA_TOP && lo >= TA_TOP / (1 << TA_SPAN));
     };
     // 3. the powers of two of a block whose positions did not suit the ones there were; false
     // where they leave the range that the shared form keeps to
     auto choose = [&](const Raw &raw) {
         int e = -0x1000;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int g = 0; g < Raw::GX; ++g) {
-                const float s = kv4_scale(raw.km[x][g]), mid = __builtin_fmaf(0.125f, kv4_min(raw.km[x][g]), s);
-                e = max(e, exp_of(fmaxf(fabsf(mid), s)) + ge[meta_group(g)]);
-            }
-        const float ke = ta_swap32(ta_swap16(ta_row16((float)e, ta_max), ta_max), ta_max);
         float v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < Raw::VM; ++i) {
-            const float s = kv4_scale(raw.vm[i]);
-            v = fmaxf(v, fmaxf(fabsf(__builtin_fmaf(0.125f, kv4_min(raw.vm[i]), s)), s));
+        for (int i = 0; i < VM; ++i) {
+            const float s = kv4_scale(raw.km[i]), mid = __builtin_fmaf(0.125f, kv4_min(raw.km[i]), s);
+            e = max(e, exp_of(fmaxf(fabsf(mid), s)) + ge[group(i)]);
+            const float sv = kv4_scale(raw.vm[i]);
+            v = fmaxf(v, fmaxf(fabsf(__builtin_fmaf(0.125f, kv4_min(raw.vm[i]), sv)), sv));
         }
+        const float ke = ta_swap32(ta_swap16(ta_row16((float)e, ta_max), ta_max), ta_max);
         v = ta_swap32(ta_swap16(ta_row16(v, ta_max), ta_max), ta_max);
         // (a group's middle / 8 and its scale are below 2^e; 8 times that, with two bits of room)
         const int old = ev_run;
         ek_run = __builtin_amdgcn_readfirstlane((int)ke) + 5;
         ev_run = __builtin_amdgcn_readfirstlane(exp_of(v)) + 5;
         bool fits = ev_run >= -90 && ev_run <= 120 && ek_run >= -90 && ek_run <= 120;
-        auto factor = [&](int g) { return ldexpf(1.0f, ge[g] + TA_TOP_E - ek_run); };
 #pragma unroll
-        for (int g = 0; g < Raw::GX; ++g) kg[g] = NG == 8 ? factor(meta_group(g)) : uniform(factor(g));
-#pragma unroll
-        for (int o = 0; o < Raw::OWN; ++o) kown[o] = factor(own_group(o));
-#pragma unroll
-        for (int g = 0; g < NG; ++g) fits &= ge[g] == TA_NO_GROUP || (ge[g] - ek_run <= 100 && ge[g] - ek_run >= -100);
+        for (int i = 0; i < VM; ++i) {
+            const int g = ge[group(i)], f = g - ek_run;
+            kg[i] = ldexpf(1.0f, f + TA_TOP_E);
+            fits &= g == TA_NO_GROUP || (f <= 100 && f >= -100);
+        }
         vg = uniform(ldexpf(1.0f, TA_TOP_E - ev_run));
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
@@ -590,60 +571,50 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         fits = __all(fits);
         if (!fits) {  // (nothing is shared until the next choice)
 #pragma unroll
-            for (int g = 0; g < Raw::GX; ++g) kg[g] = 0.0f;
+            for (int i = 0; i < VM; ++i) kg[i] = 0.0f;
         }
         return fits;
     };
     // 2'. by a power of two for every position, which the other lanes find in LDS; nothing past
     // the last position
     auto own_meta = [&](const Raw &raw, int p0, bool edge) {
+        const bool in = !edge || p0 + lp <= last;
+        float km[VM], vm[VM], mag = 0.0f;
+        int e = -0x1000;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int at = 8 * (col >> 2) + (col & 3) + 4 * x;
-            const bool in = !edge || p0 + at <= last;
-            float mid[Raw::GX];
-            int e = -0x1000, eg[Raw::GX];
-#pragma unroll
-            for (int g = 0; g < Raw::GX; ++g) {
-                const uint32_t meta = in ? raw.km[x][g] : 0u;
-                const float s = kv4_scale(meta);
-                mid[g] = __builtin_fmaf(0.125f, kv4_min(meta), s);
-                eg[g] = ge[meta_group(g)];
-                e = max(e, exp_of(fmaxf(fabsf(mid[g]), s)) + eg[g]);
-            }
-            if (NG == 8) e = max(e, __shfl_xor(e, 16, 64));
-            e += 3 - TA_TOP_E;
-            if (j == 0) ek[at] = e;
-#pragma unroll
-            for (int g = 0; g < Raw::GX; ++g) middles[x][g] = two_terms(ldexpf(mid[g], eg[g] - e + 3), rest);
-#pragma unroll
-            for (int o = 0; o < Raw::OWN; ++o)
-                own[x][o] = in ? ldexpf(kv4_scale(raw.own[x][o]), ge[own_group(o)] - e) : 0.0f;
-        }
-        float mid[Raw::VM], mag = 0.0f;
-#pragma unroll
-        for (int i = 0; i < Raw::VM; ++i) {
-            const uint32_t meta = !edge || p0 + (lane & 31) <= last ? raw.vm[i] : 0u;
-            vscales[i] = kv4_scale(meta);
-            mid[i] = __builtin_fmaf(0.125f, kv4_min(meta), vscales[i]);
+        for (int i = 0; i < VM; ++i) {
+            const uint32_t mk = in ? raw.km[i] : 0u, mv = in ? raw.vm[i] : 0u;
+            kscale[i] = kv4_scale(mk);
+            km[i] = __builtin_fmaf(0.125f, kv4_min(mk), kscale[i]);
+            e = max(e, exp_of(fmaxf(fabsf(km[i]), kscale[i])) + ge[group(i)]);
+            vscale[i] = kv4_scale(mv);
+            vm[i] = __builtin_fmaf(0.125f, kv4_min(mv), vscale[i]);
             nan_p[i] = 0;
             if (edge) {  // what some queries see and others do not: told at the end
-                const bool bad = !(mid[i] == mid[i]);
+                const bool bad = !(vm[i] == vm[i]);
                 nan_p[i] = __ballot(bad);
-                if (bad) mid[i] = vscales[i] = 0.0f;
+                if (bad) vm[i] = vscale[i] = 0.0f;
             }
-            mag = fmaxf(mag, fmaxf(fabsf(mid[i]), vscales[i]));
+            mag = fmaxf(mag, fmaxf(fabsf(vm[i]), vscale[i]));
         }
-        if (NG > 1) mag = ta_swap32(mag, ta_max);
-        const int e = max(exp_of(mag) + 3 - TA_TOP_E, -105);
+        if (NG > 1) {
+            e = (int)ta_swap32((float)e, ta_max);
+            mag = ta_swap32(mag, ta_max);
+        }
+        e += 3 - TA_TOP_E;
+        const int ve = max(exp_of(mag) + 3 - TA_TOP_E, -105);
 #pragma unroll
-        for (int i = 0; i < Raw::VM; ++i) {
-            vmiddles[i] = two_terms(ldexpf(mid[i], 3 - e), rest);
-            vscales[i] = ldexpf(vscales[i], -e);
+        for (int i = 0; i < VM; ++i) {
+            const int f = ge[group(i)] - e;
+            kmid[i] = two_terms(ldexpf(km[i], f + 3), rest);
+            kscale[i] = ldexpf(kscale[i], f);
+            vmid[i] = two_terms(ldexpf(vm[i], 3 - ve), rest);
+            vscale[i] = ldexpf(vscale[i], -ve);
         }
         if (lane < 32) {
-            ev[lane] = (float)e;
-            iev[lane] = ldexpf(1.0f, -e - TA_BASE);
+            ek[lane] = e;
+            ev[lane] = (float)ve;
+            iev[lane] = ldexpf(1.0f, -ve - TA_BASE);
         }
     };
 
@@ -657,30 +628,34 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
             asm volatile("" : "+s"(v));
             return v != 0;
         };
-        // 4. values' meta, where the lanes that hold their codes find it
+        // 4. the meta, where the lanes that hold the codes find it
         if (NG > 1 || lane < 32) {
             _Float16 *o = (_Float16 *)wl + (lane & 24) + slot8(lane & 7);
 #pragma unroll
-            for (int i = 0; i < Raw::VM; ++i) {
-                const int g = (lane >> 5) * (NG / 2) + i;
-                const f16x2 t = __builtin_bit_cast(f16x2, vmiddles[i]);
+            for (int i = 0; i < VM; ++i) {
+                const int g = group(i);
+                const f16x2 t = __builtin_bit_cast(f16x2, vmid[i]);
                 o[g * 64] = t[0];
                 o[g * 64 + 32] = t[1];
-                o[M::SC / 2 + g * 32] = (_Float16)vscales[i];
+                o[M::SC / 2 + g * 32] = (_Float16)vscale[i];
+                ((uint32_t *)(wl + M::KM))[lp * M::KG + g] = kmid[i];
+                ((_Float16 *)(wl + M::KSC))[g * 32 + lp] = (_Float16)kscale[i];
             }
         }
+        __builtin_amdgcn_wave_barrier();
         // 5. scores: rows of S^T, 4 j' + i of tile x is position 8 j' + 4 x + i
         f32x4 S[MT][2];
         f16x8 kf[2][KS + 1];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            uint32_t ex[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int g = 0; g < Raw::GX; ++g) ex[g] = NG <= 4 && (j & 1) ? 0u : middles[x][g];  // (no group 4 ..)
-            kf[x][KS] = __builtin_bit_cast(f16x8, u32x4{ex[0], ex[1], ex[2], ex[3]});
+            const int at = (int)Raw::key_row(col, x);
+            u32x4 ex = *(const u32x4 *)(wl + M::KM + (at * M::KG + (NG > 4 ? 4 * (j & 1) : 0)) * 4);
+            if (NG <= 4 && (j & 1)) ex = u32x4{0, 0, 0, 0};  // (no group 4 ..)
+            kf[x][KS] = __builtin_bit_cast(f16x8, ex);
 #pragma unroll
             for (int o = 0; o < Raw::OWN; ++o) {
-                const uint32_t sp = f16_pair(own[x][o], own[x][o]), cp = minus24(sp);
+                const _Float16 sk = ((const _Float16 *)(wl + M::KSC))[own_group(o) * 32 + at];
+                const uint32_t sp = __builtin_bit_cast(uint32_t, f16x2{sk, sk}), cp = minus24(sp);
                 const uint32_t s4[4] = {sp, sp, sp, sp}, c4[4] = {cp, cp, cp, cp};
                 constexpr int D = KS / Raw::OWN;
 #pragma unroll
@@ -835,13 +810,13 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         // 9. values that are NaN, to the queries that see them: through the middles' sums
         unsigned long long any_nan = 0;
 #pragma unroll
-        for (int i = 0; i < Raw::VM; ++i) any_nan |= nan_p[i];
+        for (int i = 0; i < VM; ++i) any_nan |= nan_p[i];
         if (any_nan) {
 #pragma unroll
-            for (int i = 0; i < Raw::VM; ++i) {
+            for (int i = 0; i < VM; ++i) {
                 for (unsigned long long left = nan_p[i]; left; left &= left - 1) {
                     const int at = __builtin_ctzll(left);
-                    const int g = NG == 1 ? 0 : (at >> 5) * (NG / 2) + i;
+                    const int g = NG == 1 ? 0 : (at >> 5) * VM + i;
 #pragma unroll
                     for (int t = 0; t < MT; ++t)
                         if ((sees(t) >> (at & 31) & 1) && j == g / 2) {
