@@ -165,8 +165,11 @@ struct TreeLds {
     static constexpr int MASK = F + MT * 64;  // u64
     static constexpr int E = MASK + MT * 128;
     static constexpr int END = E + 64;
-    static constexpr int RO = 0;  // [wave][16 MT][HD], then maxima and sums
-    static constexpr int RM = RO + TA_W * 16 * MT * HD * 4;
+    // [wave][16 MT][channels] (rows of other banks), then maxima and sums; half of the channels at a time
+    // where two workgroups a CU would not fit
+    static constexpr int PARTS = TA_W * 16 * MT * HD * 4 > 72 * 1024 ? 2 : 1, RC = HD / PARTS, RS = RC + 4;
+    static constexpr int RO = 0;
+    static constexpr int RM = RO + TA_W * 16 * MT * RS * 4;
     static constexpr int REND = RM + TA_W * 16 * MT * 8;
     static constexpr int OFF = END > REND ? END : REND;  // [wave][16 MT][8] the middles' sums
     static constexpr int SIZE = OFF + TA_W * 16 * MT * 32;
@@ -862,49 +865,55 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         if (2 * j + 1 < NG) off[(t * 16 + col) * 8 + 2 * j + 1] = O[t][NT][2] + O[t][NT][3];
     }
     __syncthreads();  // the operands are read; the results lie over them
-    float *ro = (float *)(lds + M::RO) + w * ROWS * HD, *rm = (float *)(lds + M::RM);
+    constexpr int RC = M::RC, RS = M::RS, NP = NT / M::PARTS;
+    float *ro = (float *)(lds + M::RO) + w * ROWS * RS, *rm = (float *)(lds + M::RM);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+    for (int part = 0; part < M::PARTS; ++part) {
+        if (part) __syncthreads();
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float mid = off[(t * 16 + col) * 8 + n / 2];
-            *(f32x4l *)(ro + (t * 16 + col) * HD + n * 16 + 4 * j) =
-                f32x4l{O[t][n][0] + mid, O[t][n][1] + mid, O[t][n][2] + mid, O[t][n][3] + mid};
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int n = part * NP + i;
+                const float mid = off[(t * 16 + col) * 8 + n / 2];
+                *(f32x4l *)(ro + (t * 16 + col) * RS + i * 16 + 4 * j) =
+                    f32x4l{O[t][n][0] + mid, O[t][n][1] + mid, O[t][n][2] + mid, O[t][n][3] + mid};
+            }
+            if (j == 0 && part == 0) {
+                rm[(w * ROWS + t * 16 + col) * 2] = m[t];
+                rm[(w * ROWS + t * 16 + col) * 2 + 1] = l[t];
+            }
         }
-        if (j == 0) {
-            rm[(w * ROWS + t * 16 + col) * 2] = m[t];
-            rm[(w * ROWS + t * 16 + col) * 2 + 1] = l[t];
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < rows * (HD / 4); i += 64 * TA_W) {
-        const int r = i / (HD / 4), c = i % (HD / 4) * 4;
-        float mx = TA_NONE, L = 0.0f, f[TA_W];
+        __syncthreads();
+        for (int i = tid; i < rows * (RC / 4); i += 64 * TA_W) {
+            const int r = i / (RC / 4), ci = i % (RC / 4) * 4, c = part * RC + ci;
+            float mx = TA_NONE, L = 0.0f, f[TA_W];
 #pragma unroll
-        for (int x = 0; x < TA_W; ++x) mx = fmaxf(mx, rm[(x * ROWS + r) * 2]);
+            for (int x = 0; x < TA_W; ++x) mx = fmaxf(mx, rm[(x * ROWS + r) * 2]);
 #pragma unroll
-        for (int x = 0; x < TA_W; ++x) {
-            f[x] = __builtin_amdgcn_exp2f(rm[(x * ROWS + r) * 2] - mx);
-            L = __builtin_fmaf(f[x], rm[(x * ROWS + r) * 2 + 1], L);
-        }
-        f32x4u o = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int x = 0; x < TA_W; ++x) {
+                f[x] = __builtin_amdgcn_exp2f(rm[(x * ROWS + r) * 2] - mx);
+                L = __builtin_fmaf(f[x], rm[(x * ROWS + r) * 2 + 1], L);
+            }
+            f32x4u o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int x = 0; x < TA_W; ++x) {
-            const f32x4l v = *(const f32x4l *)((const float *)(lds + M::RO) + (x * ROWS + r) * HD + c);
+            for (int x = 0; x < TA_W; ++x) {
+                const f32x4l v = *(const f32x4l *)((const float *)(lds + M::RO) + (x * ROWS + r) * RS + ci);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f[x], v[e], o[e]);
-        }
-        if (shares == 1) {
-            const int R = row0 + r;
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f[x], v[e], o[e]);
+            }
+            if (shares == 1) {
+                const int R = row0 + r;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = o[e] * TA_UNBASE / L;
-            *(f32x4u *)(p.out + ((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c) = o;
-        } else {
-            float *pw = p.work + ((size_t)kept * p.tiles + tile) * (ROWS * (HD + 2));
-            *(f32x4u *)(pw + r * HD + c) = o;
-            if (c == 0) {
-                pw[ROWS * HD + 2 * r] = mx;
-                pw[ROWS * HD + 2 * r + 1] = L;
+                for (int e = 0; e < 4; ++e) o[e] = o[e] * TA_UNBASE / L;
+                *(f32x4u *)(p.out + ((size_t)b * p.S + R / p.G) * p.ldo + ((size_t)kvh * p.G + R % p.G) * HD + c) = o;
+            } else {
+                float *pw = p.work + ((size_t)kept * p.tiles + tile) * (ROWS * (HD + 2));
+                *(f32x4u *)(pw + r * HD + c) = o;
+                if (c == 0) {
+                    pw[ROWS * HD + 2 * r] = mx;
+                    pw[ROWS * HD + 2 * r + 1] = L;
+                }
             }
         }
     }
