@@ -964,6 +964,9 @@ TreePlan tree_plan(const Kv4View &c, int H, int S) {
     const int most = c.hd <= 64 ? 4 : c.hd == 128 ? 2 : 1;
     TreePlan pl;
     pl.mt = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : most;
+    // (heads of 128: 48 rows fill the registers; 491 us where 32 take 544 with 2 x 2048 tokens of 32 heads over 8
+    // after 2048 positions, but a round of workgroups that is not full costs more)
+    if (c.hd == 128 && (long long)c.B * c.Hkv * ((rows + 47) / 48) >= 1024) pl.mt = 3;
     pl.rows = 16 * pl.mt;
     pl.tiles = (int)((rows + pl.rows - 1) / pl.rows);
     // Workgroups for two a CU, where a sequence's length gives each wave of a share two blocks. Where there are as
@@ -998,6 +1001,7 @@ int launch_hd(const TreeAttnParams &p, const TreePlan &pl, hipStream_t st) {
     if constexpr (HD <= 128) {
         if (pl.mt == 2) return launch_t<HD, 2>(p, pl, st);
     }
+    if constexpr (HD == 128) return launch_t<HD, 3>(p, pl, st);
     if constexpr (HD <= 64) return launch_t<HD, 4>(p, pl, st);
     return VMLM_OK;
 }

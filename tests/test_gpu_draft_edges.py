@@ -366,6 +366,27 @@ def test_attention_many_queries_a_head(ops, G, S, hd):
     check_tree(out, tree_ref(m, q, [90], [S], parent, 1, hd, float(np.float32(hd ** -0.5))))
 
 
+@pytest.mark.parametrize("H,Hkv,hd", [(8, 4, 128), (4, 4, 64), (12, 4, 128), (8, 8, 256)])
+def test_attention_chunks_that_fill_the_card(ops, H, Hkv, hd):
+    """Many tiles of many sequences, of unlike lengths, that end inside a token's heads or behind the last."""
+    rng = np.random.default_rng(H + hd)
+    B, cap, S = 16, 480, 400
+    pos0 = rng.integers(0, 80, B).astype(np.int32)
+    count = rng.integers(1, S + 1, B).astype(np.int32)
+    pos0[3], pos0[5], count[0], count[5], count[7], count[9] = -1, 80, 0, 400, 17, 1
+    c, m = filled(ops, rng, B, Hkv, cap, hd, np.where(pos0 >= 0, pos0 + count, 0))
+    q = rng.standard_normal((B, S, H * hd), dtype=np.float32)
+    out = c.attention_tree(q, pos0, count)
+    scale = float(np.float32(hd ** -0.5))
+    for b in range(B):
+        n = count[b] if pos0[b] >= 0 else 0
+        assert not out[b, n:].any()
+        for t in {0, 11, 15, 16, 23, 24, n // 2, n - 2, n - 1} & set(range(n)):
+            one = {x: y[b:b + 1] for x, y in m.items()}
+            check_tree(out[b:b + 1, t:t + 1],
+                       tree_ref(one, q[b:b + 1, t:t + 1], [pos0[b] + t], [1], None, Hkv, hd, scale))
+
+
 def test_attention_queries_in_the_output(dev, ops):
     """Two calls in a row whose second reads what the first wrote, and an unaligned output."""
     rng = np.random.default_rng(30)
