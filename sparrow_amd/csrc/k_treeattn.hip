@@ -158,7 +158,7 @@ struct TreeLds {
     static constexpr int Q = 0;
     static constexpr int WAVE = Q + MT * FR * 1024;
     static constexpr int SC = 1024, N = SC + 512;  // V's scales [8][32], numbers
-    static constexpr int KG = NG > 4 ? 8 : 4;
+    static constexpr int KG = 8;  // (zeros where there is no group)
     static constexpr int KM = N + 3 * 128, KSC = KM + 32 * KG * 4;  // K's middles [32][KG], scales [group][32]
     static constexpr int WB = KSC + NG * 64;
     static constexpr int F = WAVE + TA_W * WB;
@@ -369,9 +369,9 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     for (int i = tid; i < TA_W * 64; i += 64 * TA_W)
         *(u32x4 *)(lds + M::WAVE + (i >> 6) * M::WB + (i & 63) * 16) =
             M::ONES && (i & 63) >= 60 ? u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u} : u32x4{0, 0, 0, 0};
-    if (NG < 4)  // (no group there)
-        for (int i = tid; i < TA_W * 32; i += 64 * TA_W)
-            *(u32x4 *)(lds + M::WAVE + (i >> 5) * M::WB + M::KM + (i & 31) * 16) = u32x4{0, 0, 0, 0};
+    if (NG < 8)
+        for (int i = tid; i < TA_W * 64; i += 64 * TA_W)
+            *(u32x4 *)(lds + M::WAVE + (i >> 6) * M::WB + M::KM + (i & 63) * 16) = u32x4{0, 0, 0, 0};
     if (tid < 16) ge[tid] = TA_NO_GROUP;
     __syncthreads();
     int own_e = 0;  // the query's power of two
@@ -652,9 +652,7 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int at = (int)Raw::key_row(col, x);
-            u32x4 ex = *(const u32x4 *)(wl + M::KM + (at * M::KG + (NG > 4 ? 4 * (j & 1) : 0)) * 4);
-            if (NG <= 4 && (j & 1)) ex = u32x4{0, 0, 0, 0};  // (no group 4 ..)
-            kf[x][KS] = __builtin_bit_cast(f16x8, ex);
+            kf[x][KS] = *(const f16x8 *)(wl + M::KM + (at * M::KG + 4 * (j & 1)) * 4);
 #pragma unroll
             for (int o = 0; o < Raw::OWN; ++o) {
                 const _Float16 sk = ((const _Float16 *)(wl + M::KSC))[own_group(o) * 32 + at];
@@ -739,18 +737,20 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
         if (is_shared()) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float v = (float)(ev_run - TA_TOP_E);
-                float f = cq[t], base = v - (m[t] - TA_BASE);
-                if (far_any && far(t)) {  // (the exponents themselves, none above TA_BASE + TA_SLACK)
+                const float v = (float)(ev_run - TA_TOP_E), base = v - (m[t] - TA_BASE);
+                if (far_any) {
+                    const bool is_far = far(t);  // (the exponents themselves, none above TA_BASE + TA_SLACK)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float d = __builtin_fmaf(S[t][i / 4][i % 4], cq[t], base);
+                        if (is_far) d = (__builtin_fmaf(S[t][i / 4][i % 4], cq[t], v) - m[t]) + TA_BASE;
+                        S[t][i / 4][i % 4] = __builtin_amdgcn_exp2f(d);
+                    }
+                } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        S[t][i / 4][i % 4] = __builtin_fmaf(S[t][i / 4][i % 4], f, v) - m[t];
-                    f = 1.0f;
-                    base = TA_BASE;
+                        S[t][i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i / 4][i % 4], cq[t], base));
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    S[t][i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i / 4][i % 4], f, base));
                 if (!M::ONES) {
                     float sum = 0.0f;
 #pragma unroll
