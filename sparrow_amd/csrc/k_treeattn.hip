@@ -26,10 +26,10 @@
 // score * log2(e) - maximum is one fused operation that rounds at its own small size.
 // 16-bit terms stand below 2^11 and hold 11 bits down to 2^-14 and steps of 2^-24 below it.
 //
-// Bound by its instructions: with 63 tokens over 65463 positions, 36 heads of 64, 146 us, vector
-// instructions 63 % of the cycles and matrix instructions 28 %, which hardly overlap; 190 MB of cache
-// at 1.3 TB/s. 333 tokens of 3 sequences after 4000 positions, 32 heads over 8 of 128: 189 us, 68 % and 28 %. A
-// wave makes a block's operands for 64 queries (heads up to 64) or 32 (the registers there are).
+// Bound by its instructions: with 63 tokens over 65463 positions, 36 heads of 64, 116 us, vector
+// instructions 62 % of the cycles and matrix instructions 36 %, which do not run beside each other; 190 MB of
+// cache at 1.6 TB/s. 333 tokens of 3 sequences after 4000 positions, 32 heads over 8 of 128: 151 us, 66 % and
+// 34 %. A wave makes a block's operands for 64 queries (heads up to 64), 32 or 48 (128): the registers there are.
 #include <algorithm>
 
 #include "kv4.hpp"
@@ -54,7 +54,7 @@ constexpr int TA_TOP_E = 11, TA_SPAN = 14;
 constexpr float TA_TOP = 1 << TA_TOP_E;
 // A weight is 2^TA_BASE at the maximum that its wave knew when it last raised it, which it
 // does where one is 2^TA_SLACK larger: with 64 queries some maximum grows in nearly every block
-// (63 tokens, 65463 positions, 36 heads of 64: 192 us when each was followed, 158 then).
+// (63 tokens, 65463 positions, 36 heads of 64: 192 us when each was followed, 158 otherwise).
 constexpr int TA_BASE = 9, TA_SLACK = 6;
 constexpr float TA_UNBASE = 1.0f / (1 << TA_BASE);
 constexpr float TA_FAR = 4194304.0f;        // scores whose f32 steps are no longer small
