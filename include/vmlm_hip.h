@@ -449,10 +449,11 @@ int vmlm_hip_rope_qk(float *q_out, size_t ldqo, float *k_out, size_t ldko, const
  * the cache's keys come rotated. S is at most 64 with parents, 65535 without;
  * batch * S * n_heads at most 2^27, batch * n_kv_heads 2^21. A
  * query head with a NaN or an infinity gives NaN, a position with one in its key or value to the queries
- * that see it. Queries and weights are held in 22 bits, and so are a position's keys and values as far as
- * they reach 2^-14 of the largest of its head (of the keys weighed by the queries' groups of 32 channels),
- * smaller ones to 2^-36 of that one: results are off by f32 roundings of the queries times the largest value
- * that a key's 32 channels can hold, and of the weights times the values' likewise. The keys and values
+ * that see it. Queries are held in 22 bits, and so are a position's keys and values as far as they reach
+ * 2^-14 of the largest of its head (of the keys weighed by the queries' groups of 32 channels), smaller
+ * ones to 2^-36 of that one; a position's weight times its largest value likewise in 22 bits, and to 2^-34 of the
+ * largest such product: results are off by f32 roundings of the queries times the largest value that a
+ * key's 32 channels can hold, and of the weights times the values' likewise. The keys and values
  * of tokens that a token does not see change no bit of its result. `work`: vmlm_hip_attention_tree_kv4_work() bytes, 16-byte aligned, used by one
  * call at a time; null: the stream's own workspace, which a call under stream capture may
  * not use (9), since graphs that run at once would share it. */

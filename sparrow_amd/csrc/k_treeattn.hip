@@ -513,7 +513,8 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
     unsigned long long nan_p[VM];  // lanes whose value's meta is a NaN
 
     // 2. by the shared powers of two; false where a position is too large for them, or its keys or a
-    // group of its values smaller than 2^-TA_SPAN of them (zeros lose nothing)
+    // group of its values smaller than 2^-TA_SPAN of them. (Zeros lose nothing; but where all of a position's
+    // values are, its weight would be taken for that of the others' size, and small ones beside it lost.)
     auto shared_meta = [&](const Raw &raw) {
         float kmost = 0.0f, hi = 0.0f, lo = __builtin_inff();
 #pragma unroll
@@ -530,9 +531,12 @@ __global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(
             vmid[i] = two_terms(vm, rest);
             nan_p[i] = 0;
         }
-        if (NG > 1) kmost = ta_swap32(kmost, ta_max);
+        if (NG > 1) {
+            kmost = ta_swap32(kmost, ta_max);
+            hi = ta_swap32(hi, ta_max);
+        }
         lo = fminf(lo, kmost == 0.0f && kg[0] > 0.0f ? TA_TOP : kmost);
-        return __all(fmaxf(kmost, hi) < TA_TOP && lo >= TA_TOP / (1 << TA_SPAN));
+        return __all(fmaxf(kmost, hi) < TA_TOP && lo >= TA_TOP / (1 << TA_SPAN) && hi > 0.0f);
     };
     // 3. the powers of two of a block whose positions did not suit the ones there were; false
     // where they leave the range that the shared form keeps to

@@ -100,6 +100,24 @@ def test_attention_values_of_other_magnitudes(ops, H, Hkv, hd, n, S, times):
     check_tree(out, tree_ref(m, q, [pos0], [S], parent, Hkv, hd, scale))
 
 
+@pytest.mark.parametrize("small", [0.0, 1e-30, 1e-6])
+@pytest.mark.parametrize("H,Hkv,hd,n,S", SHAPES)
+@pytest.mark.parametrize("where", [0, 1, 2])
+def test_attention_weight_on_no_value(ops, H, Hkv, hd, n, S, small, where):
+    """A position with nearly all the weight (e^60 times the others') whose values are 0, or next to it: what the
+    others' weights bring keeps its bits."""
+    rng = np.random.default_rng(n + hd + where)
+    q, k, v, parent, pos0 = case(rng, H, Hkv, hd, n, S)
+    base = rng.standard_normal((Hkv, hd))
+    q = (base[None, None, np.arange(H) // (H // Hkv)] + 0.01 * q).astype(np.float32)
+    scale = float(np.float32(hd ** -0.5))
+    at = [0, pos0 // 2, pos0][where]
+    k[0, at] = 60 / scale * base / (base * base).sum(-1, keepdims=True)
+    v[0, at] *= np.float32(small)
+    out, m, q, scale = run(ops, q, k, v, parent, pos0)
+    check_tree(out, tree_ref(m, q, [pos0], [S], parent, Hkv, hd, scale))
+
+
 @pytest.mark.parametrize("times", [1e4, 1e6, 1e12])
 @pytest.mark.parametrize("H,Hkv,hd,n,S", [s for s in SHAPES if s[2] > 32])
 def test_attention_query_groups_of_other_magnitudes(ops, H, Hkv, hd, n, S, times):
