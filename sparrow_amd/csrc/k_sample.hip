@@ -23,8 +23,8 @@
 // by f32 comparisons, for the tokens to sort. Few rows are cut into slices, which also list the
 // tokens of their first bins, so that the second reading is seldom needed.
 //
-// 512 rows of 122753 (251 MB): 52 us greedy, HBM's rate; 103 with top_k 50 and 124 without a filter, the first
-// reading bound by 25 vector instructions a token and its LDS addition. One row 25 us (35 without a
+// 512 rows of 122753 (251 MB): 52 us greedy, HBM's rate; 102 with top_k 50 and 123 without a filter, the first
+// reading bound by two dozen vector instructions a token and its LDS addition. One row 25 us (35 without a
 // filter): a slice's 9 and its end's 16, latencies.
 #include <algorithm>
 
@@ -79,7 +79,10 @@ struct Place {
         per = PER / (double)t;
         refer(max);
     }
-    __device__ __forceinline__ void refer(float max) { ref = __builtin_floor(-(double)max * per); }
+    __device__ __forceinline__ void refer(float max) {
+        ref = __builtin_floor(-(double)max * per);
+        if (__builtin_fma(-(double)max, per, -ref) < 0.0) ref -= 1.0;  // (the product was rounded up to it)
+    }
     __device__ __forceinline__ bool too_far(float max) const { return !(fabs((double)max * per) < TOO_FAR); }
     // T so small against the logits that only the largest one's equals can have a weight: a
     // larger T that leaves f64 its rests says the same (the next logit is 2^25 bins away)
@@ -88,7 +91,7 @@ struct Place {
         refer(max);
     }
     __device__ __forceinline__ int bin(float l, uint32_t *rest) const {
-        const double y = (-(double)l * per) + (0x1p20 - ref);  // (+inf for a masked one)
+        const double y = __builtin_fma(-(double)l, per, 0x1p20 - ref);  // (+inf for a masked one)
         const unsigned long long b = __builtin_bit_cast(unsigned long long, y);
         *rest = (uint32_t)b;
         return (int)min((uint32_t)(b >> 32) - 0x41300000u, (uint32_t)(BINS - 1));
