@@ -227,12 +227,6 @@ struct RawBlock {
     }
 };
 
-// Waves a SIMD that the registers are held to: one more where they nearly suffice (16 sequences
-// with 32 tokens, heads of 64: 43 us at two, 34 at three).
-constexpr int ta_waves(int hd, int mt) {
-    return mt == 1 ? (hd == 32 ? 5 : hd == 64 ? 4 : 2) : mt == 2 && hd <= 64 ? 3 : 2;
-}
-
 // How the positions are dealt out where there are fewer tiles than the card takes workgroups, or a long
 // sequence among short ones: in proportion to a sequence's blocks, which only the card knows. (One of
 // 32700 positions beside 15 of 600, 8 tokens each: 36 heads of 64 53 us, 311 with shares that the capacity
@@ -304,8 +298,10 @@ __device__ __forceinline__ Dealt deal(const TreeAttnParams &p, int stream, bool 
 }
 
 // A tile of 16 MT (token, head) pairs of one sequence and kv head, and one share of the positions.
+// (Registers for two waves a SIMD: 8 sequences of 16000 positions, 4 heads over each of 4 of 256 and 16 tokens,
+// 121 us, 167 with registers for one.)
 template <int HD, int MT>
-__global__ __launch_bounds__(64 * TA_W, ta_waves(HD, MT)) void tree_attn_kernel(TreeAttnParams p) {
+__global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams p) {
     using M = TreeLds<HD, MT>;
     using Raw = RawBlock<HD>;
     constexpr int NG = HD / 32, KS = HD / 32, NT = HD / 16, CL = HD / 4, ROWS = 16 * MT;
