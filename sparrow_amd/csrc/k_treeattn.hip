@@ -229,8 +229,8 @@ struct RawBlock {
 
 // How the positions are dealt out where there are fewer tiles than the card takes workgroups, or a long
 // sequence among short ones: in proportion to a sequence's blocks, which only the card knows. (One of
-// 32700 positions beside 15 of 600, 8 tokens each: 36 heads of 64 53 us, 311 with shares that the capacity
-// set alike for all; 8 of 128 65 and 141; 16 of 2600, where nothing is gained, 58 and 54, 45 and 45.)
+// 32700 positions beside 15 of 600, 8 tokens each: 36 heads of 64 44 us, 246 with shares that the capacity
+// sets alike for all; 32 heads over 8 of 128 47 and 127. 16 of 2600, where nothing is gained: 48 and 47, 34 and 34.)
 constexpr int TA_SHARES = 64, TA_LEAST = 2 * TA_W;  // at most; blocks of a share
 __device__ __forceinline__ float share_blocks(float blocks, int per) {
     return fmaxf(blocks / (float)per, (float)TA_LEAST);
