@@ -970,7 +970,8 @@ TreePlan tree_plan(const Kv4View &c, int H, int S) {
     pl.rows = 16 * pl.mt;
     pl.tiles = (int)((rows + pl.rows - 1) / pl.rows);
     // Workgroups for two a CU, where a sequence's length gives each wave of a share two blocks. Where there are as
-    // many without shares, only a cache of 8192 positions and more, 120 us of one workgroup.
+    // many without shares, only a cache of 8192 positions and more (16 sequences of 36 heads of 64, 8 tokens: where one
+    // has 8100 positions and 15 have 600, 24 us, 66 without; where all have 600, 20 and 16).
     const size_t pairs = (size_t)c.B * c.Hkv, slots = 512;
     pl.per = pairs * pl.tiles < slots || c.cap >= 8192 ? (int)(slots / pl.tiles) : 0;
     const size_t longest = (size_t)c.cap / KV4_BLOCK / TA_LEAST;  // shares of the longest sequence
