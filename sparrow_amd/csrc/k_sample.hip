@@ -836,7 +836,6 @@ __global__ __launch_bounds__(THREADS, 8) void sample_row_kernel(SampleParams p) 
     for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
     unsigned long long best = 0;  // (without the index where T > 0)
     Place at;
-    bool lost = false;
     for (int first = 0; first < n; first += THREADS * 16) {
         Tokens<THREADS> now;
         now.load(row, first, n);
@@ -866,7 +865,6 @@ __global__ __launch_bounds__(THREADS, 8) void sample_row_kernel(SampleParams p) 
             if (c.t > 0.0f && fabsf(max) <= 3.40282347e38f) {
                 const Place old = at;
                 at = Place(c.t, max);
-                lost |= at.too_far(max);
                 // the bins so far move behind by as many as the largest logit came before
                 const double d = fmin(old.ref - at.ref, (double)BINS);
                 const int by = old.per == 0.0 ? 0 : (int)d;
@@ -889,7 +887,10 @@ __global__ __launch_bounds__(THREADS, 8) void sample_row_kernel(SampleParams p) 
     if (settled(p, r, c, best)) return;
     const float max = of_bits((uint32_t)(best >> 32));
     __syncthreads();
-    if (lost) {
+    // (The last place alone counts. A mask's lowest value may have set one before it that was too far: what
+    // was counted there has moved behind all bins since, or that place is within BINS of the last one's, below
+    // 2^50, where bins and rests are exact.)
+    if (at.too_far(max)) {
         at.widen(max);
         count_row(s, row, n, at);
     }
