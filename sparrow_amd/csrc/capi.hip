@@ -1454,7 +1454,9 @@ static int check_tree_attn(const Kv4View &c, const float *q, size_t ldq, const i
     if (rc || c.B == 0 || S == 0 || H == 0) return rc;
     const size_t rows = (size_t)c.B * S, w = H * c.hd, nb = (size_t)c.B * 4;
     VMLM_GUARD(c.cap > 0, "kv4 tree attention: capacity 0");
-    // (a workgroup of 256 threads for 16 rows and more)
+    // (A workgroup of 256 threads for 16 rows and more, and one of less for each pair of sequence and kv head: 2^23 +
+    // 2^21. Of 9 pairs and more they are rounded up to a multiple of 8: 16 / 9 of 2^23, below the 2^24 that a grid's 2^32 - 1
+    // threads take. Shares add 519 x 512 at most.)
     VMLM_GUARD(rows * H <= (size_t)1 << 27 && (size_t)c.B * c.Hkv <= (size_t)1 << 21,
                "kv4 tree attention: %zu tokens of %zu heads (limit 2^27 together), %d sequences of %d kv heads (2^21)",
                rows, H, c.B, c.Hkv);

@@ -68,6 +68,7 @@ struct TreeAttnParams {
     // tiles of queries; whether positions are dealt out in shares: `per` is the number of workgroups that a
     // tile of all sequences may have, 0 if each takes all of a sequence's
     int tiles, per;
+    int apart;    // a stream's tiles lie so many workgroups apart
     float *out;
     int *dealt;   // [B][2]: where a sequence's shares' results begin, how many shares it has
     float *work;  // [..][tile]: the results, of sequences of more than one share
@@ -308,8 +309,10 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 15, j = lane >> 4;
-    // the tiles that read the same positions lie 8 workgroups apart: on one XCD
-    const int x8 = blockIdx.x / 8, stream = x8 / p.tiles * 8 + (int)(blockIdx.x % 8), tile = x8 % p.tiles;
+    // the tiles that read the same positions lie 8 workgroups apart: on one XCD. Fewer streams than 8 take all XCDs, with
+    // no workgroups that have nothing to do (2048 tokens of 32 heads over one of 64: 86 us, 473 on one XCD).
+    const int x8 = blockIdx.x / p.apart, stream = x8 / p.tiles * p.apart + (int)(blockIdx.x % p.apart),
+              tile = x8 % p.tiles;
     int b, kvh = stream % p.c.Hkv, share = 0, shares = 1, kept = stream;
     if (p.per == 0) {
         b = stream / p.c.Hkv;
@@ -987,7 +990,8 @@ int launch_t(const TreeAttnParams &p, const TreePlan &pl, hipStream_t st) {
     using M = TreeLds<HD, MT>;
     int rc = allow_lds((const void *)tree_attn_kernel<HD, MT>, M::SIZE, M::SIZE);
     if (rc) return rc;
-    tree_attn_kernel<HD, MT><<<(unsigned)((pl.streams + 7) / 8 * 8 * p.tiles), 64 * TA_W, M::SIZE, st>>>(p);
+    const size_t grid = (pl.streams + p.apart - 1) / p.apart * p.apart * p.tiles;
+    tree_attn_kernel<HD, MT><<<(unsigned)grid, 64 * TA_W, M::SIZE, st>>>(p);
     VMLM_HIP_CHECK(hipGetLastError());
     if (p.per == 0) return VMLM_OK;
     tree_merge_kernel<HD><<<dim3((unsigned)(p.tiles * pl.rows), (unsigned)p.c.Hkv, (unsigned)p.c.B),
@@ -1028,6 +1032,7 @@ int launch_tree_attn(const TreeAttnArgs &a, hipStream_t st) {
     p.G = a.H / a.c.Hkv;
     p.tiles = pl.tiles;
     p.per = pl.per;
+    p.apart = (int)std::min(pl.streams, (size_t)8);
     p.out = a.out;
     p.dealt = (int *)a.work;
     p.work = a.work + ((size_t)a.c.B * 2 + 63) / 64 * 64;
