@@ -27,6 +27,7 @@ struct RopeParams {
     const int32_t *pos;
     const double *freq;
     int H, Hkv, hd, rot, units;  // units: of 2 V channels a head, the rotated ones first
+    int y0;                      // of the launch, in workgroups along a row
     float m;
 };
 
@@ -34,7 +35,7 @@ template <int V, bool INTER>
 __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
     typedef float vec __attribute__((ext_vector_type(V), aligned(4)));  // from any float on
     const int row = blockIdx.x;
-    const int id = blockIdx.y * 256 + threadIdx.x;
+    const int id = (p.y0 + blockIdx.y) * 256 + threadIdx.x;
     const int h = id / p.units, u = id % p.units;
     if (h >= p.H + p.Hkv) return;
     const int pos = p.pos[row];
@@ -77,13 +78,17 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
 }
 
 template <int V>
-int launch_t(const RopeParams &p, int rows, bool inter, hipStream_t st) {
-    const dim3 grid((unsigned)rows, cdiv((size_t)(p.H + p.Hkv) * p.units, 256));
-    if (inter)
-        rope_kernel<V, true><<<grid, 256, 0, st>>>(p);
-    else
-        rope_kernel<V, false><<<grid, 256, 0, st>>>(p);
-    VMLM_HIP_CHECK(hipGetLastError());
+int launch_t(RopeParams p, int rows, bool inter, hipStream_t st) {
+    // (a grid has at most 65535 workgroups along y; a row up to 2 x 65535 heads of 510 channels)
+    const int all = (int)cdiv((size_t)(p.H + p.Hkv) * p.units, 256);
+    for (p.y0 = 0; p.y0 < all; p.y0 += 65535) {
+        const dim3 grid((unsigned)rows, (unsigned)std::min(65535, all - p.y0));
+        if (inter)
+            rope_kernel<V, true><<<grid, 256, 0, st>>>(p);
+        else
+            rope_kernel<V, false><<<grid, 256, 0, st>>>(p);
+        VMLM_HIP_CHECK(hipGetLastError());
+    }
     return VMLM_OK;
 }
 
@@ -110,6 +115,7 @@ int launch_rope_qk(const RopeArgs &a, hipStream_t st) {
                            a.hd,
                            a.rot,
                            a.hd / (wide ? 8 : 2),
+                           0,
                            a.m};
         const int rc = wide ? launch_t<4>(p, rows, a.inter, st) : launch_t<1>(p, rows, a.inter, st);
         if (rc) return rc;
