@@ -567,7 +567,10 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
             if (tid + i * THREADS < n) s.list[k[i]] = v[i];
         __syncthreads();
     };
-    // the bin of a rank, and of a mass (the last one that is not empty and starts below it)
+    // The bin of a rank, and of a mass (the last one that is not empty and starts below it; for a mass of 0 the
+    // largest logit's, which is the second one where its rest was rounded up to a whole bin).
+    uint32_t first_rest;
+    const int first_bin = at.bin(max, &first_rest);
     auto bin_of_rank = [&](uint32_t rank) {
         int b = 0;
         for (int step = BINS / 2; step; step /= 2)
@@ -580,7 +583,7 @@ __device__ __forceinline__ void finish(Shared &s, const SampleParams &p, int r, 
             if (with_equal ? s.above[b + step] < m : s.above[b + step] <= m) b += step;
         // (the empty ones behind the last token start at the whole mass)
         while (b > 0 && tokens(b) == 0) --b;
-        return b;
+        return std::max(b, first_bin);
     };
     uint32_t kept = live;
     const bool by_k = c.top_k > 0 && (uint32_t)c.top_k < live;
