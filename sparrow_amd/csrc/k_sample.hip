@@ -460,8 +460,9 @@ __device__ __forceinline__ Found locate(Shared &s, const float *row, int vocab, 
 }
 
 // The smallest logit with exp((l - max) / t) >= min_p in 64 bits: next to where its logarithm puts
-// it, the lanes try the f32 around it.
+// it, the lanes try the f32 around it. (min_p 1: the largest one itself, however many weights beside it are 1 in 64 bits.)
 __device__ __forceinline__ float least_of(float max, float t, float min_p) {
+    if (min_p == 1.0f) return max;
     const float near = (float)fmax((double)max + (double)t * log((double)min_p), -3.40282347e38);
     const uint32_t key = order_bits(near) + (threadIdx.x & 63) - 32u;
     const float l = of_bits(key);

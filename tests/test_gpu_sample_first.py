@@ -37,3 +37,23 @@ def test_sample_next_to_a_bins_border(ops):
             for r in range(40):
                 want, share, near = sample_ref(x[r], u[r], 1.5, k, p, m)
                 assert near < 1e-8 or (token[r] == want and abs(prob[r] - share) <= 2.0 ** -20)
+
+
+@pytest.mark.parametrize("t", [1.0, 1e4, 1e10, 3e38])
+@pytest.mark.parametrize("rows,vocab", [(3, 100), (300, 5000), (3, 40000)])
+def test_sample_min_p_of_one(ops, rows, vocab, t):
+    """The largest logit and its equals, and none of a lesser one, were it a step of f32 below and the weights
+    alike in 64 bits."""
+    rng = np.random.default_rng(vocab)
+    x = (rng.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    for r in range(rows):
+        top = x[r].max() + np.float32(1)
+        at = rng.permutation(vocab)[:80]
+        x[r, at[:3]] = top
+        for i, j in enumerate(at[3:]):
+            x[r, j] = top - (i + 1) * np.spacing(top)
+    u = rng.random(rows, dtype=np.float32)
+    token, prob = ops.sample(x, u, np.float32(t), min_p=1.0)
+    for r in range(rows):
+        equal = np.flatnonzero(x[r] == x[r].max())
+        assert token[r] == equal[int(float(u[r]) * 3)] and abs(prob[r] * 3 - 1) <= 2.0 ** -20
