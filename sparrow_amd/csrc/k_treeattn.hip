@@ -58,6 +58,16 @@ constexpr float TA_TOP = 1 << TA_TOP_E;
 constexpr int TA_BASE = 9, TA_SLACK = 6;
 constexpr float TA_UNBASE = 1.0f / (1 << TA_BASE);
 constexpr float TA_FAR = 4194304.0f;        // scores whose f32 steps are no longer small
+// The weights' sum. A position adds 2^score to it whatever its values; the weight that the products take is that times the
+// value's power of two, so that of positions with scores alike those of small values weigh least. Three ways to sum:
+//  * by the product, whose 16-bit terms end 2^-34 below the largest weight: where values are within 2^TA_SUM16 of the
+//    largest that the wave has met, n of them are off by n 2^-24 at most, as a sum in f32 is;
+//  * of the f32 weights over the values' powers of two: within 2^TA_SUM32, and 2^TA_RISE for values that come after
+//    smaller ones (weights below 2^-126, and sums rescaled by less, are lost; below n 2^-24 of the sum up to there);
+//  * by exponents of the scores alone: beyond, as with zeros among large values. And for blocks that not all queries
+//    see, so that what a query does not see has no say in how its sum is formed.
+// (All scores' exponents alone: 8 more exponentials a tile and block.)
+constexpr int TA_SUM16 = 10, TA_SUM32 = 110, TA_RISE = 85;
 
 struct TreeAttnParams {
     Kv4View c;
@@ -85,6 +95,8 @@ __device__ __forceinline__ float ta_swap32(float v, float (*f)(float, float)) {
     const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return f(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
+// v times 2^e for integers e of any size (the weights' sums go below what a factor can be)
+__device__ __forceinline__ float ta_scale(float v, float e) { return ldexpf(v, (int)fmaxf(e, -1000.0f)); }
 __device__ __forceinline__ float ta_add(float a, float b) { return a + b; }
 __device__ __forceinline__ float ta_max(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float ta_row16(float v, float (*f)(float, float)) {
@@ -117,6 +129,10 @@ __device__ __forceinline__ uint32_t two_terms(float x, const Rest &rest) {
 // A number that is the same in all lanes, in a scalar register.
 __device__ __forceinline__ float uniform(float v) {
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+__device__ __forceinline__ int uniform(int v) {
+    asm volatile("" : "+v"(v));  // (else what comes after it is done before it, in vector registers)
+    return __builtin_amdgcn_readfirstlane(v);
 }
 
 // The exponent e of a magnitude below 2^e (of numbers that are not normal -126).
@@ -165,7 +181,8 @@ struct TreeLds {
     static constexpr int F = WAVE + TA_W * WB;
     static constexpr int MASK = F + MT * 64;  // u64
     static constexpr int E = MASK + MT * 128;
-    static constexpr int END = E + 64;
+    static constexpr int LM = E + 64;
+    static constexpr int END = LM + TA_W * MT * 64;
     // [wave][16 MT][channels] (rows of other banks), then maxima and sums; half of the channels at a time
     // where two workgroups a CU would not fit
     static constexpr int PARTS = TA_W * 16 * MT * HD * 4 > 72 * 1024 ? 2 : 1, RC = HD / PARTS, RS = RC + 4;
@@ -490,6 +507,11 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     // two: keys stand below 2^ek, values below 2^ev, those of the block that they were taken from with
     // room above. kg and vg bring scales to them, cq scores back.
     int ek_run = 0, ev_run = 0;
+    int ev_top = -1000, ev_low = 1000;  // the values' powers of two so far, of what all queries see
+    // The weights' sum by the scores alone from here on (no block is shared then), in units of 2^lm, which is in LDS:
+    // in a register it costs every block.
+    int alone = 0, wide = 0;
+    float *lm = (float *)(lds + M::LM) + w * ROWS;
     constexpr int VM = Raw::VM;
     float kg[VM], vg = 0.0f;
 #pragma unroll
@@ -537,6 +559,28 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         lo = fminf(lo, kmost == 0.0f && kg[0] > 0.0f ? TA_TOP : kmost);
         return __all(fmaxf(kmost, hi) < TA_TOP && lo >= TA_TOP / (1 << TA_SPAN) && hi > 0.0f);
     };
+    // the sums of weights that stand in O, in units of 2^ev, to the others
+    auto join_sums = [&] {
+        if (M::ONES) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                if (j == 3) {
+                    l[t] += ldexpf(O[t][NT][3], TA_TOP_E - ev_run - TA_BASE);
+                    O[t][NT][3] = 0.0f;
+                }
+        }
+    };
+    auto share_nothing = [&] {  // until the next choice
+#pragma unroll
+        for (int i = 0; i < VM; ++i) kg[i] = 0.0f;
+    };
+    auto also = [&](int top, int low) {  // values of these powers of two besides those so far
+        const int rises = top > ev_top;
+        ev_top = max(ev_top, top);
+        ev_low = min(ev_low, low);
+        wide |= (int)(ev_top - ev_low > TA_SUM32) | (rises & (int)(ev_top - ev_low > TA_RISE));
+        wide = uniform(wide);
+    };
     // 3. the powers of two of a block whose positions did not suit the ones there were; false
     // where they leave the range that the shared form keeps to
     auto choose = [&](const Raw &raw) {
@@ -552,7 +596,7 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
         const float ke = ta_swap32(ta_swap16(ta_row16((float)e, ta_max), ta_max), ta_max);
         v = ta_swap32(ta_swap16(ta_row16(v, ta_max), ta_max), ta_max);
         // (a group's middle / 8 and its scale are below 2^e; 8 times that, with two bits of room)
-        const int old = ev_run;
+        join_sums();
         ek_run = __builtin_amdgcn_readfirstlane((int)ke) + 5;
         ev_run = __builtin_amdgcn_readfirstlane(exp_of(v)) + 5;
         bool fits = ev_run >= -90 && ev_run <= 120 && ek_run >= -90 && ek_run <= 120;
@@ -568,17 +612,12 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
             const int f = fe[t * 16 + col] + ek_run - TA_TOP_E;
             cq[t] = ldexpf(cs, f);
             fits &= f <= 100;
-            // the sums of weights that stand in O are in units of 2^ev: to the others
-            if (M::ONES && j == 3) {
-                l[t] += ldexpf(O[t][NT][3], TA_TOP_E - old - TA_BASE);
-                O[t][NT][3] = 0.0f;
-            }
         }
-        fits = __all(fits);
-        if (!fits) {  // (nothing is shared until the next choice)
-#pragma unroll
-            for (int i = 0; i < VM; ++i) kg[i] = 0.0f;
-        }
+        const int at = uniform(ev_run - TA_TOP_E);
+        fits = __all(fits) && (!M::ONES || at >= ev_top - TA_SUM16);
+        if (fits) also(at, at);
+        fits &= wide == 0;
+        if (!fits) share_nothing();
         return fits;
     };
     // 2'. by a power of two for every position, which the other lanes find in LDS; nothing past
@@ -616,6 +655,13 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
             kscale[i] = ldexpf(kscale[i], f);
             vmid[i] = two_terms(ldexpf(vm[i], 3 - ve), rest);
             vscale[i] = ldexpf(vscale[i], -ve);
+        }
+        if (!edge) {
+            const float top = ta_swap16(ta_row16((float)ve, ta_max), ta_max);
+            const float low = ta_swap16(ta_row16((float)-ve, ta_max), ta_max);
+            const int from = ev_low, to = ev_top;
+            also(uniform((int)top), -uniform((int)low));
+            if (ev_top != to || ev_low != from) share_nothing();
         }
         if (lane < 32) {
             ek[lane] = e;
@@ -728,7 +774,7 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
                 // (each query by its own scores: nothing that only others see shows in it)
                 const float to = mx > m[t] + TA_SLACK ? mx : m[t], corr = __builtin_amdgcn_exp2f(m[t] - to);
                 m[t] = to;
-                l[t] *= corr;
+                l[t] *= alone ? 1.0f : corr;
 #pragma unroll
                 for (int n = 0; n <= NT; ++n)
 #pragma unroll
@@ -766,6 +812,24 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
             for (int t = 0; t < MT; ++t) {
                 const float base = m[t] - TA_BASE;
                 const bool is_far = far_any && far(t);
+                if (alone) {
+                    float a = TA_NONE;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        a = fmaxf(a, seen >> (8 * t + i) & 1 ? S[t][i / 4][i % 4] * cs : TA_NONE);
+                    a = __builtin_ceilf(ta_swap32(ta_swap16(a, ta_max), ta_max));
+                    const float old = lm[t * 16 + col], to = a > old + TA_SLACK ? a : old;
+                    l[t] = ta_scale(l[t], old - to);
+                    lm[t * 16 + col] = to;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float v = ev[8 * j + i];
+                        float d = __builtin_fmaf(S[t][i / 4][i % 4], cs, -to);
+                        // (as the weight below is rounded)
+                        if (is_far) d = ((__builtin_fmaf(S[t][i / 4][i % 4], cs, v) - m[t]) - v) + (m[t] - to);
+                        l[t] += __builtin_amdgcn_exp2f(seen >> (8 * t + i) & 1 ? d : -1000.0f);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float v = ev[8 * j + i];
@@ -773,7 +837,10 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
                     if (is_far) d = (__builtin_fmaf(S[t][i / 4][i % 4], cs, v) - m[t]) + TA_BASE;
                     const float w8 = seen >> (8 * t + i) & 1 ? __builtin_amdgcn_exp2f(d) : 0.0f;
                     S[t][i / 4][i % 4] = w8;
-                    l[t] = __builtin_fmaf(w8, iev[8 * j + i], l[t]);
+                }
+                if (!alone) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) l[t] = __builtin_fmaf(S[t][i / 4][i % 4], iev[8 * j + i], l[t]);
                 }
                 apart();
             }
@@ -836,6 +903,7 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     };
 
     const int whole = min(b1, min(zone, last + 1) / KV4_BLOCK);  // blocks that all queries see
+    int share_end = whole;                                       // that may share powers of two
     Raw raw;
     const size_t first = head * p.c.cap;
     if (b0 + w < b1) {
@@ -845,18 +913,28 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
     }
     for (int blk = b0 + w; blk < b1; blk += TA_W) {
         const bool edge = blk >= whole;
-        bool shared = !edge;
+        bool shared = blk < share_end;
         if (shared && !shared_meta(raw)) shared = choose(raw) && shared_meta(raw);
-        if (!shared) own_meta(raw, blk * KV4_BLOCK, edge);
+        if (!shared) {
+            own_meta(raw, blk * KV4_BLOCK, edge);
+            if (!alone && (edge || wide)) {
+                alone = 1;
+                share_end = 0;
+                join_sums();
+#pragma unroll
+                for (int t = 0; t < MT; ++t) lm[t * 16 + col] = m[t];
+            }
+        }
         // what comes next into the same registers, as soon as they are read (the last block again at the end)
         const size_t next = first + (blk + TA_W < b1 ? blk + TA_W : blk) * KV4_BLOCK;
         raw.load_meta(p.c, next, lane);
         block(raw, blk, next, edge, shared);
     }
-    if (M::ONES) {
+    if (alone) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-            if (j == 3) l[t] += ldexpf(O[t][NT][3], TA_TOP_E - ev_run - TA_BASE);
+        for (int t = 0; t < MT; ++t) l[t] = ta_scale(l[t], lm[t * 16 + col] - m[t]);
+    } else {
+        join_sums();
     }
 
     // 10. the waves' results
@@ -896,7 +974,7 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
 #pragma unroll
             for (int x = 0; x < TA_W; ++x) {
                 f[x] = __builtin_amdgcn_exp2f(rm[(x * ROWS + r) * 2] - mx);
-                L = __builtin_fmaf(f[x], rm[(x * ROWS + r) * 2 + 1], L);
+                L += ta_scale(rm[(x * ROWS + r) * 2 + 1], rm[(x * ROWS + r) * 2] - mx);
             }
             f32x4u o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -942,7 +1020,7 @@ __global__ __launch_bounds__(HD < 64 ? 64 : HD) void tree_merge_kernel(TreeAttnP
     if (R >= tr.n * p.G) return;  // (what was read is not this query's)
     const float mx = ta_swap32(ta_swap16(ta_row16(m, ta_max), ta_max), ta_max);
     const float f = lane < shares ? __builtin_amdgcn_exp2f(m - mx) : 0.0f;
-    const float L = wave_sum_dpp(lane < shares ? f * l : 0.0f);
+    const float L = wave_sum_dpp(lane < shares ? ta_scale(l, m - mx) : 0.0f);
     float o = 0.0f;
     for (int s = 0; s < shares; s += 8) {
 #pragma unroll
