@@ -818,15 +818,15 @@ __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams 
                     for (int i = 0; i < 8; ++i)
                         a = fmaxf(a, seen >> (8 * t + i) & 1 ? S[t][i / 4][i % 4] * cs : TA_NONE);
                     a = __builtin_ceilf(ta_swap32(ta_swap16(a, ta_max), ta_max));
-                    const float old = lm[t * 16 + col], to = a > old + TA_SLACK ? a : old;
+                    // (far: the maximum itself, from which the weights are taken; a score's own rounding is another step)
+                    const float old = lm[t * 16 + col], to = is_far ? m[t] : a > old + TA_SLACK ? a : old;
                     l[t] = ta_scale(l[t], old - to);
                     lm[t * 16 + col] = to;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float v = ev[8 * j + i];
                         float d = __builtin_fmaf(S[t][i / 4][i % 4], cs, -to);
-                        // (as the weight below is rounded)
-                        if (is_far) d = ((__builtin_fmaf(S[t][i / 4][i % 4], cs, v) - m[t]) - v) + (m[t] - to);
+                        if (is_far) d = (__builtin_fmaf(S[t][i / 4][i % 4], cs, v) - to) - v;
                         l[t] += __builtin_amdgcn_exp2f(seen >> (8 * t + i) & 1 ? d : -1000.0f);
                     }
                 }

@@ -79,3 +79,62 @@ def test_attention_unseen_large_values_leave_no_trace(ops, hd, H):
         outs.append(c.attention_tree(q, [pos0], None, parent)[0])
     for out in outs[1:]:
         assert np.array_equal(out[[0, 1, 3, 5]], outs[0][[0, 1, 3, 5]])
+
+
+@pytest.mark.parametrize("far", [2.0 ** 12, 2.0 ** 24, 2.0 ** 33, 2.0 ** 60])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 67, 2.0 ** -67])
+@pytest.mark.parametrize("H,Hkv,hd,n,S", SHAPES)
+def test_attention_far_scores_of_some_positions(ops, H, Hkv, hd, n, S, far, sign, size):
+    """Scores far above and below the others' among ordinary ones: what a block of far scores adds to the sum stays
+    finite. Where one of them is the largest score it takes all of the weight; where they are the lowest they have none."""
+    rng = np.random.default_rng(n + S)
+    k, v = rng.standard_normal((2, 1, n + S, Hkv * hd), dtype=np.float32)
+    k[..., ::hd] = 0
+    v *= np.float32(size)
+    at = rng.permutation(n + S)[:6]
+    at[0] = 7
+    k[0, at, ::hd] = (-far if sign < 0 else far) * (1 + np.arange(6, dtype=np.float32)[:, None])
+    k[0, at[:, None], np.arange(Hkv * hd) % hd != 0] = 0
+    q = rng.standard_normal((1, S, H * hd), dtype=np.float32)
+    q[..., ::hd] = 8  # (the far scores are whole numbers: one is larger than the next by far)
+    cap = -(-(n + S) // 32) * 32
+    c, m = ops.Kv4Cache(1, Hkv, cap, hd), new_model(1, Hkv, cap, hd)
+    c.append(k, v, [0])
+    put(m, k[0], v[0], 0, 0, n + S, Hkv)
+    for parent in (None, random_tree(rng, S, "late")[None]):
+        out = c.attention_tree(q, [n], None, parent, scale=0.125)
+        ref, tol, live = tree_ref(m, q, [n], [S], parent, Hkv, hd, 0.125)
+        # a score's error is that of its own size: the far ones' do not matter where they decide alone or not at all
+        u = np.float64(2.0 ** -24)
+        near = np.setdiff1d(np.arange(n + S), at)
+        kmax = np.abs(m["k"][0][:, near]).max()
+        ds = (2 * hd + 48) * u * 0.125 * kmax * np.abs(q[0]).reshape(S, H, hd).sum(-1).max()
+        bound = (2 * (ds + (96 + n + S + 400) * u)) * np.abs(v).max()
+        assert np.isfinite(out).all() and (np.abs(out - ref) <= bound).all(), (np.abs(out - ref) / bound).max()
+
+
+@pytest.mark.parametrize("far", [2.0 ** 20, 2.0 ** 33, 2.0 ** 60])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 67, 2.0 ** -67])
+@pytest.mark.parametrize("H,Hkv,hd,n,S", [(1, 1, 64, 96, 6), (4, 1, 128, 32, 8), (2, 2, 32, 224, 3), (2, 1, 256, 64, 4), (1, 1, 64, 4064, 6)])
+def test_attention_tokens_far_below_the_rest(ops, H, Hkv, hd, n, S, far, size):
+    """Tokens in a block of their own that see themselves and what comes before: their own scores are far
+    below all others, so that they have no weight."""
+    rng = np.random.default_rng(n + S)
+    k, v = rng.standard_normal((2, 1, n + S, Hkv * hd), dtype=np.float32)
+    v[:, n:] *= np.float32(size)
+    k[0, :n, ::hd] = 0
+    k[0, n:] = 0
+    k[0, n:, ::hd] = -far
+    q = rng.standard_normal((1, S, H * hd), dtype=np.float32)
+    q[..., ::hd] = 8
+    cap = n + 32
+    c, m = ops.Kv4Cache(1, Hkv, cap, hd), new_model(1, Hkv, cap, hd)
+    c.append(k, v, [0])
+    put(m, k[0], v[0], 0, 0, n + S, Hkv)
+    parent = np.full((1, S), -1, np.int32)
+    out = c.attention_tree(q, [n], None, parent, scale=0.125)
+    # (nor does the bound take their values in, which could hide a part of the sum)
+    m["v"][:, :, n:] = 0
+    m["vm"][:, :, n:] = 0
+    check_tree(out, tree_ref(m, q, [n], [S], parent, Hkv, hd, 0.125))
