@@ -1499,7 +1499,9 @@ int vmlm_hip_attention_tree_kv4(const vmlm_kv4_cache *cache, const float *q, siz
     int rc = check_kv4(cache, &a.c);
     if (!rc) rc = check_tree_attn(a.c, q, ldq, pos0, count, parent, S, out, ldo, n_heads, scale);
     if (rc || a.c.B == 0 || S == 0 || n_heads == 0) return rc;
-    const size_t wf = tree_attn_work_floats(a.c, (int)n_heads, (int)S);
+    const size_t wf = tree_attn_splits(a.c, (int)n_heads, (int)S)
+                          ? tree_attn_work_floats(a.c, (int)n_heads, (int)S)
+                          : 0;
     if (wf && work) {
         const size_t rows = (size_t)a.c.B * S, w = n_heads * a.c.hd, nb = (size_t)a.c.B * 4;
         VMLM_GUARD(work_bytes >= wf * 4 && ((uintptr_t)work & 15) == 0,

@@ -570,7 +570,7 @@ struct RopeArgs {
 int launch_rope_qk(const RopeArgs &a, hipStream_t st);
 
 // Several tokens a sequence (tree.hpp) over the 4-bit cache (k_treeattn.hip). `work`:
-// tree_attn_work_floats() floats.
+// tree_attn_work_floats() floats, of calls that tree_attn_splits().
 constexpr int TREE_MAX = 64;  // tokens of a tree
 struct TreeAttnArgs {
     Kv4View c;
@@ -583,6 +583,7 @@ struct TreeAttnArgs {
     float *work = nullptr;
 };
 size_t tree_attn_work_floats(const Kv4View &c, int H, int S);
+bool tree_attn_splits(const Kv4View &c, int H, int S);
 int launch_tree_attn(const TreeAttnArgs &a, hipStream_t st);
 
 // The accepted rows of drafted trees to the front, in caches of one shape (k_tree.hip).

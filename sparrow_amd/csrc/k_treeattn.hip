@@ -1052,14 +1052,20 @@ TreePlan tree_plan(const Kv4View &c, int H, int S) {
     pl.tiles = (int)((rows + pl.rows - 1) / pl.rows);
     // Workgroups for two a CU, where a sequence's length gives each wave of a share two blocks. Where there are as
     // many without shares, only a cache of 8192 positions and more (16 sequences of 36 heads of 64, 8 tokens: where one
-    // has 8100 positions and 15 have 600, 24 us, 66 without; where all have 600, 20 and 16).
-    const size_t pairs = (size_t)c.B * c.Hkv, slots = 512;
-    pl.per = pairs * pl.tiles < slots || c.cap >= 8192 ? (int)(slots / pl.tiles) : 0;
+    // has 8100 positions and 15 have 600, 24 us, 66 without; where all have 600, 20 and 16), and only where the workgroups
+    // that each look over all sequences are few beside the positions of one that is long. (4 queries over each kv
+    // head of 64, 4 tokens, all of 600 positions, and one of the whole capacity; us with shares and without:
+    // 512 sequences of 2 kv heads, 8192: 32 and 21, 39 and 64; of 8, 8192: 112 and 72, 115 and 77; 32768: 113 and 73, 120
+    // and 239; 1024 of 2, 8192: 69 and 37, 72 and 65; 32768: 72 and 38, 79 and 235; 16384 of 1 of 32, 8192: 1850 and 87.)
+    const size_t pairs = (size_t)c.B * c.Hkv, groups = pairs * pl.tiles, slots = 512;
+    pl.per = groups < slots || c.cap >= 8192 ? (int)(slots / pl.tiles) : 0;
     const size_t longest = (size_t)c.cap / KV4_BLOCK / TA_LEAST;  // shares of the longest sequence
     if (longest <= 1 || (c.B == 1 && pl.per < 2 * c.Hkv)) pl.per = 0;
+    // (what a workspace is asked for depends on the sequences' number by their table alone)
+    pl.work = pl.per == 0 ? 0 : ((size_t)c.B * 2 + 63) / 64 * 64 + (size_t)pl.per * pl.tiles * pl.rows * (c.hd + 2);
+    if (groups >= slots && (groups > (size_t)c.cap / 8 || c.B > c.cap / 16)) pl.per = 0;
     // (all shares of sequences of more than one are `per` at most; of several sequences each may round up to one)
     pl.streams = pl.per == 0 ? pairs : std::min(c.B == 1 ? (size_t)pl.per : pairs + pl.per, pairs * longest);
-    pl.work = pl.per == 0 ? 0 : ((size_t)c.B * 2 + 63) / 64 * 64 + (size_t)pl.per * pl.tiles * pl.rows * (c.hd + 2);
     return pl;
 }
 
@@ -1095,6 +1101,8 @@ size_t tree_attn_work_floats(const Kv4View &c, int H, int S) {
     if (c.B == 0 || c.Hkv == 0 || c.cap == 0 || H == 0 || S == 0) return 0;
     return tree_plan(c, H, S).work;
 }
+
+bool tree_attn_splits(const Kv4View &c, int H, int S) { return tree_plan(c, H, S).per != 0; }
 
 int launch_tree_attn(const TreeAttnArgs &a, hipStream_t st) {
     const TreePlan pl = tree_plan(a.c, a.H, a.S);

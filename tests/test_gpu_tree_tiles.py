@@ -4,7 +4,7 @@ import ctypes as C
 
 import numpy as np
 import pytest
-from test_gpu_4bit import dev, device_cache, filled, ops  # noqa: F401
+from test_gpu_4bit import dev, device_cache, filled, new_model, ops, put  # noqa: F401
 from test_gpu_draft import check_tree, tree_ref
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +56,21 @@ def test_attention_of_the_most_rows(dev, ops):
     dev.check(dev.L.vmlm_hip_memcpy_d2h(got.ctypes.data, ptrs[1], got.nbytes))
     assert (got[1] == 3).all()
     check_tree(got[None, :1], tree_ref(m, q, [8], [1], None, 1, hd, scale))
+
+
+@pytest.mark.parametrize("B,Hkv,cap", [(513, 1, 8192), (512, 1, 8192), (1100, 1, 8192), (300, 4, 8192)])
+def test_attention_long_caches_of_many_sequences(ops, B, Hkv, cap):
+    """As many sequences as are dealt out by their lengths, and more, a long one among them."""
+    rng = np.random.default_rng(B)
+    hd, S, n = 32, 2, np.full(B, 2)
+    pos0 = rng.integers(0, 40, B).astype(np.int32)
+    pos0[[3, B // 2]], pos0[5] = [1500, 700], -1
+    c, m = ops.Kv4Cache(B, Hkv, cap, hd), new_model(B, Hkv, 1536, hd)
+    k, v = rng.standard_normal((2, B, 1502, Hkv * hd), dtype=np.float32)
+    lens = np.where(pos0 >= 0, pos0 + 2, 0)
+    c.append(k, v, np.zeros(B), lens)
+    for b in range(B):
+        put(m, k[b], v[b], b, 0, lens[b], Hkv)
+    q = rng.standard_normal((B, S, Hkv * hd), dtype=np.float32)
+    out = c.attention_tree(q, pos0, n, out=np.full_like(q, 3.0))
+    check_tree(out, tree_ref(m, q, pos0, n, None, Hkv, hd, float(np.float32(hd ** -0.5))), 3.0)
