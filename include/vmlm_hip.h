@@ -452,11 +452,13 @@ int vmlm_hip_rope_qk(float *q_out, size_t ldqo, float *k_out, size_t ldko, const
  * that see it. Queries are held in 22 bits, and so are a position's keys and values as far as they reach
  * 2^-14 of the largest of its head (of the keys weighed by the queries' groups of 32 channels), smaller
  * ones to 2^-36 of that one; a position's weight times its largest value likewise in 22 bits, and to 2^-34 of the
- * largest such product: results are off by f32 roundings of the queries times the largest value that a
- * key's 32 channels can hold, and of the weights times the values' likewise. The keys and values
- * of tokens that a token does not see change no bit of its result. `work`: vmlm_hip_attention_tree_kv4_work() bytes, 16-byte aligned, used by one
- * call at a time; null: the stream's own workspace, which a call under stream capture may
- * not use (9), since graphs that run at once would share it. */
+ * largest such product (a position of zeros counts as one of 2^-94 there): results are off by f32
+ * roundings of the queries times the largest value that a key's 32 channels can hold, and of the weights
+ * times the values' likewise. The weights' sum takes the scores alone, whatever the values' sizes. The keys
+ * and values of tokens that a token does not see change no bit of its result. `work`:
+ * vmlm_hip_attention_tree_kv4_work() bytes, 16-byte aligned, used by one call at a time; null: the
+ * stream's own workspace, which a call under stream capture may not use where it splits positions (9),
+ * since graphs that run at once would share it. */
 int vmlm_hip_attention_tree_kv4(const vmlm_kv4_cache *cache, const float *q, size_t ldq,
                                 const int32_t *pos0, const int32_t *count, const int32_t *parent,
                                 size_t S, float *out, size_t ldo, size_t n_heads, float scale,
@@ -467,12 +469,14 @@ int vmlm_hip_attention_tree_kv4_work(const vmlm_kv4_cache *cache, size_t n_heads
  * of equal ones the lowest index, have weights exp((l - l_max) / temperature[row]). Kept are
  * the first top_k[row] (<= 0: all), of those the ones before which the weights sum to less than
  * top_p[row] of theirs (>= 1: all; the first one always), of those the ones of at least
- * min_p[row] times the first one's. token[row] is the first whose weight and those before it sum to
- * more than u[row] times the kept ones', prob[row] its share of them. Borders are decided in more
- * than 32 bits (sums to 2^-30 of a weight). temperature 0: the first token, prob 1. u < 0: the row is
- * idle, token and prob stay as they are. A row of which all is -infinity has no token: -1, prob 0;
- * one with a NaN or +infinity: -1, prob NaN. Settings out of range (u >= 1, temperature < 0 or not
- * finite, min_p outside 0 .. 1, NaN) trip the device guard and leave the row as it is. top_k, top_p, min_p and prob may be null.
+ * min_p[row] times the first one's (1: its equals). token[row] is the first whose weight and those
+ * before it sum to more than u[row] times the kept ones', prob[row] its share of them. Weights below 2^-46 of
+ * the first one's count as none; borders are decided in more than 32 bits (sums to 2^-30 of a weight
+ * beside that). A row gives the same alone and among others. temperature 0: the first token, prob 1.
+ * u < 0: the row is idle, token and prob stay as they are. A row of which all is -infinity has no token:
+ * -1, prob 0; one with a NaN or +infinity: -1, prob NaN. Settings out of range (u >= 1, temperature < 0
+ * or not finite, min_p outside 0 .. 1, NaN) trip the device guard and leave the row as it is. top_k,
+ * top_p, min_p and prob may be null.
  * vocab is below 2^20, rows at most 2^20. `work` as above. */
 int vmlm_hip_sample(const float *logits, size_t ld, const float *u, const float *temperature,
                     const int32_t *top_k, const float *top_p, const float *min_p, size_t rows,

@@ -7,7 +7,7 @@
 //
 // A thread turns V neighbouring pairs of a head (16-byte loads where rot and the head allow
 // V = 4). Bound by the rows' bytes, read once and written once: 2048 rows of 32 + 8 heads of 128,
-// half of each turned, 84 MB in 16.8 us (5.0 TB/s); one row of 36 + 36 heads of 64 5.2 us, a
+// half of each turned, 84 MB in 16.0 us (5.2 TB/s); one row of 36 + 36 heads of 64 5.2 us, a
 // launch.
 //
 // Angles: pos * freq / 2 pi is formed in 64 bits and its whole turns dropped there; a

@@ -11,7 +11,7 @@
 // (the k-th token, the mass p, the token drawn) is answered by the bins' counts and masses
 // down to one bin. Where the bins up to the last one that can matter hold few tokens, those are
 // gathered and sorted together; else one bin is, for each question. 2048 bins from the largest logit's
-// reach weights of 2^-46; what lies behind has none.
+// reach weights of 2^-46; what lies behind counts as none (a million tokens of that are 2^-26 of the first).
 //
 // Next to a border between two tokens 32 bits are too few: with 122753 tokens of like weight
 // a sum off by 2^-24 takes the neighbour's token once in 50 rows. So l / T is formed in 64 bits, and a
@@ -19,11 +19,13 @@
 // integer in units of 2^-30: a bin's sum of d and its count are one 64-bit atomic add in
 // LDS, whose order changes nothing. A token's bin and rest depend on its logit and T alone.
 //
-// A row is read once for its bins (a larger logit than those before moves them along), and once more,
-// by f32 comparisons, for the tokens to sort. Few rows are cut into slices, which also list the
-// tokens of their first bins, so that the second reading is seldom needed.
+// A row is read once for its bins (a larger logit than those before moves them along), and as a rule once more,
+// by f32 comparisons, for the tokens to sort. Where a bin that a question ends in holds more tokens than are sorted at
+// once, as in flat rows and those of few values, it is narrowed by two readings a time, for each such question, and min_p
+// may count its tokens in one of its own. Few rows are cut into slices, which also list the tokens of their first bins, so
+// that the second reading is seldom needed.
 //
-// 512 rows of 122753 (251 MB): 52 us greedy, HBM's rate; 102 with top_k 50 and 123 without a filter, the first
+// 512 rows of 122753 (251 MB): 52 us greedy, HBM's rate; 98 with top_k 50 and 118 without a filter, the first
 // reading bound by two dozen vector instructions a token and its LDS addition. One row 25 us (35 without a
 // filter): a slice's 9 and its end's 16, latencies.
 #include <algorithm>
@@ -830,7 +832,9 @@ __device__ __forceinline__ void count_row(Shared &s, const float *row, int n, co
     __syncthreads();
 }
 
-// A workgroup a row; two of them on a CU.
+// A workgroup a row; two of them on a CU, though 38 vector registers are spilled for that (in the gathers, the scans and the
+// decisions; the first reading is free of it): 512 rows of 122753 with mixed settings 115 us, 141 with registers
+// enough for one alone. (The last kernel of slices, one a CU, spills 12.)
 __global__ __launch_bounds__(THREADS, 8) void sample_row_kernel(SampleParams p) {
     __shared__ Shared s;
     const int r = blockIdx.x, tid = threadIdx.x, n = p.vocab;
@@ -1041,7 +1045,9 @@ __global__ __launch_bounds__(THREADS) void sample_finish_kernel(SampleParams p, 
 }
 
 // Slices where a row is long and rows do not fill the chip by themselves: two launches and
-// the bins' way through memory cost more than a row's own workgroup does from there on.
+// the bins' way through memory cost more than a row's own workgroup does from there on. (us with top_k 50 in slices and not:
+// a row of 16384 21 and 16, of 30000 21 both, 40000 22 and 26, 122753 25 and 50; 32 of 122753 31 and 52, 64 of 40000 25
+// and 27. Beyond: 200 of 30000 33 and 24, but 64 of 122753 38 and 54: the longest rows would still gain.)
 int slices_of(int rows, int vocab) {
     const int n = (vocab + SLICE - 1) / SLICE;
     return n >= 4 && (long long)rows * n <= 512 ? n : 0;

@@ -9,8 +9,8 @@
 // wait for another's: one launch for up to 16 caches. A row's source never lies before it
 // (path[i] >= i), but it may be another's target, so all sources are read, into
 // registers (K, meta) and LDS (V: its codes are packed along positions), before the first
-// target is written. Bound by latencies: 8 tokens, 2 caches of 36 heads of 64 3.8 us; 16 trees of up to
-// 63, 4 such caches 9.8 us.
+// target is written. Bound by latencies: 8 tokens, 2 caches of 36 heads of 64 3.9 us; 16 trees of up to
+// 63, 4 such caches 9.3 us.
 #include <algorithm>
 
 #include "kv4.hpp"

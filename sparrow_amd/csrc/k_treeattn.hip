@@ -26,9 +26,9 @@
 // score * log2(e) - maximum is one fused operation that rounds at its own small size.
 // 16-bit terms stand below 2^11 and hold 11 bits down to 2^-14 and steps of 2^-24 below it.
 //
-// Bound by its instructions: with 63 tokens over 65463 positions, 36 heads of 64, 116 us, vector
-// instructions 62 % of the cycles and matrix instructions 36 %, which do not run beside each other; 190 MB of
-// cache at 1.6 TB/s. 333 tokens of 3 sequences after 4000 positions, 32 heads over 8 of 128: 151 us, 66 % and
+// Bound by its instructions: with 63 tokens over 65463 positions, 36 heads of 64, 117 us, vector
+// instructions 59 % of the cycles and matrix instructions 37 %, which do not run beside each other; 190 MB of
+// cache at 1.6 TB/s. 333 tokens of 3 sequences after 4000 positions, 32 heads over 8 of 128: 156 us, 64 % and
 // 34 %. A wave makes a block's operands for 64 queries (heads up to 64), 32 or 48 (128): the registers there are.
 #include <algorithm>
 
@@ -249,7 +249,10 @@ struct RawBlock {
 // sequence among short ones: in proportion to a sequence's blocks, which only the card knows. (One of
 // 32700 positions beside 15 of 600, 8 tokens each: 36 heads of 64 44 us, 246 with shares that the capacity
 // sets alike for all; 32 heads over 8 of 128 47 and 127. 16 of 2600, where nothing is gained: 48 and 47, 34 and 34.)
-constexpr int TA_SHARES = 64, TA_LEAST = 2 * TA_W;  // at most; blocks of a share
+// At most (a lane of the merging wave each; 8 tokens over 65000 positions, 4 heads over one of 64: 25 us, 32 with 32 shares);
+// blocks of a share (us with 4, 8 and 16: 8 tokens over 1000 positions, 36 heads of 64 11.3, 11.3, 13.1, over 600 11.3,
+// 12.2, 12.5; 4 sequences of 2000, 8 heads over 2 of 128 19.0, 19.1, 24.0).
+constexpr int TA_SHARES = 64, TA_LEAST = 2 * TA_W;
 __device__ __forceinline__ float share_blocks(float blocks, int per) {
     return fmaxf(blocks / (float)per, (float)TA_LEAST);
 }
@@ -317,7 +320,7 @@ __device__ __forceinline__ Dealt deal(const TreeAttnParams &p, int stream, bool 
 
 // A tile of 16 MT (token, head) pairs of one sequence and kv head, and one share of the positions.
 // (Registers for two waves a SIMD: 8 sequences of 16000 positions, 4 heads over each of 4 of 256 and 16 tokens,
-// 121 us, 167 with registers for one.)
+// 121 us, 167 with registers for one. <128, 3> spills 5 and <256, 1> 3, two of which the products read.)
 template <int HD, int MT>
 __global__ __launch_bounds__(64 * TA_W, 2) void tree_attn_kernel(TreeAttnParams p) {
     using M = TreeLds<HD, MT>;
@@ -1044,9 +1047,14 @@ TreePlan tree_plan(const Kv4View &c, int H, int S) {
     const long long rows = (long long)S * (H / c.Hkv);
     const int most = c.hd <= 64 ? 4 : c.hd == 128 ? 2 : 1;
     TreePlan pl;
+    // Rows of a tile (us with 16, 32 and 64; 16 sequences of 960 positions, 36 heads of 64: 16 tokens 21.7, 28.0, 50.8; 32
+    // 32.4, 29.3, 52.1; 64 53, 48, 56; one of 65000: 24 tokens 100, 76, 113; 40 167, 137, 114. The widest, for what is
+    // read often, costs a sixth after short contexts. Heads of 128, with 16 and 32: 8 sequences of 16000, 4 heads over
+    // each of 8: 3 tokens 43, 55; 8 74, 58; 16 133, 99.)
     pl.mt = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : most;
-    // (heads of 128: 48 rows fill the registers; 491 us where 32 take 544 with 2 x 2048 tokens of 32 heads over 8
-    // after 2048 positions, but a round of workgroups that is not full costs more)
+    // Heads of 128: 48 rows fill the registers, but a round of workgroups that is not full costs more (us with 48 and 32,
+    // 4 heads over each of 8: 2 x 2048 tokens after 2048 positions 507 and 547, 4 x 400 184 and 189, 2 x 1024 242 both; below
+    // the limit 4 x 300 146 and 138, 3 x 333 after 4000 201 and 186, 512 of one 80 and 62).
     if (c.hd == 128 && (long long)c.B * c.Hkv * ((rows + 47) / 48) >= 1024) pl.mt = 3;
     pl.rows = 16 * pl.mt;
     pl.tiles = (int)((rows + pl.rows - 1) / pl.rows);
