@@ -22,7 +22,8 @@
 // A row is read once for its bins (a larger logit than those before moves them along), and as a rule once more,
 // by f32 comparisons, for the tokens to sort. Where a bin that a question ends in holds more tokens than are sorted at
 // once, as in flat rows and those of few values, it is narrowed by two readings a time, for each such question, and min_p
-// may count its tokens in one of its own. Few rows are cut into slices, which also list the tokens of their first bins, so
+// may count its tokens in one of its own (a row of 122753 within a hundredth of each other 0.5 ms, of equal logits 0.8, with
+// top_k and top_p 2.4; 512 of them 1.1, 1.7 and 4.8). Few rows are cut into slices, which also list the tokens of their first bins, so
 // that the second reading is seldom needed.
 //
 // 512 rows of 122753 (251 MB): 52 us greedy, HBM's rate; 98 with top_k 50 and 118 without a filter, the first
