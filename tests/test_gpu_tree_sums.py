@@ -105,7 +105,9 @@ def test_attention_far_scores_of_some_positions(ops, H, Hkv, hd, n, S, far, sign
     for parent in (None, random_tree(rng, S, "late")[None]):
         out = c.attention_tree(q, [n], None, parent, scale=0.125)
         ref, tol, live = tree_ref(m, q, [n], [S], parent, Hkv, hd, 0.125)
-        # a score's error is that of its own size: the far ones' do not matter where they decide alone or not at all
+        # The bound of tree_ref with the largest ds of the ordinary positions in place of each one's, and t at most 100
+        # (what lies further off has a weight below 2^-144): a far score's own error decides nothing, since the far
+        # ones are whole steps apart from each other and from the rest.
         u = np.float64(2.0 ** -24)
         near = np.setdiff1d(np.arange(n + S), at)
         kmax = np.abs(m["k"][0][:, near]).max()
